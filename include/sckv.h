@@ -337,6 +337,108 @@ SCKV_API size_t sckv_o_proj_workspace_bytes(const sckv_pool* pool,
                      int n_tokens, int in_features, int out_features);
 
 /* ========================================================================== */
+/* Speculative decoding: a tree of drafted tokens per sequence (no reference  */
+/* counterpart: the reference decodes one token per request and step)         */
+/* ========================================================================== */
+/* A step checks n nodes per sequence at once. Node i's K/V row is appended to
+ * slot ctx + i (ctx committed tokens); its rotary position is its own
+ * (ctx + depth). Then every node attends to the committed tokens and to the
+ * nodes its mask names, the logits choose the accepted path, and the path's
+ * rows move to slots ctx, ctx + 1, ... */
+
+/* Attention of a tree's nodes: row (token t = cu_q[b] + i, q head hq) of out =
+ * softmax(scale * q . K^T) V over keys 0 .. ctx_lens[b] - 1 of sequence b and
+ * the keys ctx_lens[b] + j whose bit j % 64 of
+ * tree_mask[t * mask_words + j / 64] is set (j < the sequence's nodes; later
+ * bits are ignored). A row that sees no key gives zeros.
+ * q / out : [n_tokens][num_q_heads][head_dim] of q_dtype / out_dtype (F16 /
+ *           BF16 / F32); q enters the products rounded to the pool's 16-bit
+ *           type (f16 for one-byte pools). BF16 pools need bf16 q.
+ * cu_q    : int32 [n_seqs + 1] device, non-decreasing; at most 64 * mask_words
+ *           nodes per sequence, mask_words 1 .. 4.
+ * ctx_lens: int32 [n_seqs] device, committed tokens (>= 0) before the nodes.
+ * Rows of `out` that belong to no sequence stay as they are, and so do those
+ * of a sequence whose offsets, context or node count is out of range
+ * (reported in the status word, kernel id 18). All pool types, any group size
+ * num_q_heads / num_kv_heads; head_dim 128, else SCKV_ERR_UNSUPPORTED. fp32
+ * accumulation. workspace: sckv_tree_attn_workspace_bytes(...) bytes of device
+ * memory, 16-byte aligned, not shared by calls that overlap on the GPU. */
+SCKV_API int sckv_tree_attn(sckv_pool* pool, int layer, const void* q, int q_dtype,
+                   int num_q_heads, int n_seqs, int n_tokens,
+                   const int32_t* cu_q, const int32_t* ctx_lens,
+                   const int32_t* block_table, int64_t bt_stride,
+                   int max_blocks, const uint64_t* tree_mask, int mask_words,
+                   float scale, void* out, int out_dtype, void* workspace,
+                   size_t workspace_bytes, void* stream);
+SCKV_API size_t sckv_tree_attn_workspace_bytes(const sckv_pool* pool, int n_tokens,
+                   int num_q_heads);
+
+/* Per-head RMSNorm of q and k (optional), rotary positions with several axes,
+ * then the K/V append of sckv_append for one layer. Frequency i turns by
+ * positions[axis_map[i]][t] / rope_scaling * inv_freq[i] (formed in 64 bits),
+ * so a token's rotary position is independent of its slot start_pos[b] + i:
+ * tree nodes rotate by depth, image and video tokens by (time, height, width).
+ * q, k, v : rows [heads][128] of token t at t * q_stride / k_stride / v_stride
+ *           elements (heads packed; the strides let the three be slices of one
+ *           projection), 16-byte aligned. q_out [n_tokens][num_q_heads][128].
+ * q_norm_w / k_norm_w : fp16 [128] or NULL.
+ * positions : int32 [n_axes] rows of pos_stride elements; axis_map int32 [64],
+ *           entries 0 .. n_axes - 1 (others are reported and read as 0).
+ * All pool types. int8 rows are quantised as sckv_append_rope does; FP8 pools
+ * stage the rotated k in fp16 (workspace) and fold K and V into the pages in a
+ * second launch. Tokens outside cu_tokens[0] .. cu_tokens[n_seqs] - 1 are
+ * skipped. head_dim 128. */
+SCKV_API int sckv_append_rope_axes(sckv_pool* pool, int layer, const void* q,
+                   int64_t q_stride, void* q_out, int num_q_heads, int q_dtype,
+                   int q_out_dtype, const void* k, int64_t k_stride,
+                   const void* v, int64_t v_stride, int src_dtype,
+                   const void* q_norm_w, const void* k_norm_w, float eps,
+                   const float* inv_freq, float rope_scaling,
+                   const int32_t* positions, int64_t pos_stride, int n_axes,
+                   const int32_t* axis_map, int n_seqs, int n_tokens,
+                   const int32_t* cu_tokens, const int32_t* start_pos,
+                   const int32_t* block_table, int64_t bt_stride,
+                   int max_blocks, void* workspace, size_t workspace_bytes,
+                   void* stream);
+/* Workspace of sckv_append_rope_axes (0 unless the pool is FP8). */
+SCKV_API size_t sckv_append_rope_axes_workspace_bytes(const sckv_pool* pool, int n_tokens);
+
+/* Move accepted rows: for j < n_keep[b], the K and V rows (and scales) of
+ * position ctx_lens[b] + path[b * max_path + j] of sequence b become those of
+ * position ctx_lens[b] + j, in layers layer0 .. layer0 + n_layers - 1. path is
+ * strictly increasing (a node comes after its parent) and stays inside the
+ * block table; a sequence that breaks this, or whose n_keep is not in
+ * 0 .. max_path, is reported (kernel id 20) and left as it is. FP8 pools: rows
+ * from another page enter as an append of their values would (the page scale
+ * grows to max|x| / 448, rows already there are re-encoded). The pages rows
+ * move into must belong to this sequence alone. Page bookkeeping is the
+ * caller's. */
+SCKV_API int sckv_compact_tree(sckv_pool* pool, int layer0, int n_layers,
+                   int n_seqs, const int32_t* path, int max_path,
+                   const int32_t* n_keep, const int32_t* ctx_lens,
+                   const int32_t* block_table, int64_t bt_stride,
+                   int max_blocks, void* stream);
+
+/* Greedy choice of the accepted path. Node i of sequence b is row
+ * t = cu_tokens[b] + i of logits [n_tokens] rows of `vocab` values, ld
+ * elements apart (F16 / BF16 / F32); node 0 is the root. From the root, the
+ * walk goes to the first later node j with parents[j] == current node (index
+ * within the sequence) and tokens[j] == argmax(logits of the current node)
+ * (lowest index of equal values; NaN counts as the largest), until there is
+ * none or max_path nodes are taken.
+ * path [n_seqs][max_path]: the nodes, then -1; n_keep [n_seqs]: how many (0
+ * for a sequence without nodes, or with more than 1024, which is reported:
+ * kernel id 19); next_token [n_seqs]: the argmax of the last node, -1 if none.
+ * All int32, device. */
+SCKV_API int sckv_verify_tree(sckv_pool* pool, const void* logits, int logits_dtype,
+                   int64_t ld, int n_tokens, int vocab, const int32_t* tokens,
+                   const int32_t* parents, const int32_t* cu_tokens, int n_seqs,
+                   int max_path, int32_t* path, int32_t* n_keep,
+                   int32_t* next_token, void* workspace, size_t workspace_bytes,
+                   void* stream);
+SCKV_API size_t sckv_verify_tree_workspace_bytes(const sckv_pool* pool, int n_tokens, int vocab);
+
+/* ========================================================================== */
 /* KV-head-sharded output exchange (no reference counterpart: the reference  */
 /* has no multi-process code; this is the optional layout of a multi-GPU box) */
 /* ========================================================================== */

@@ -10,9 +10,10 @@ from .arena import PagedKVArena
 from .attention_layer import PagedAttentionLayer
 from .kv_index import KVPrefixIndex
 from .paged_cache import DecodeStepGraph, PagedKVCache
-from .pool import KVPool, rope_inv_freq
+from .pool import KVPool, rope_axis_map, rope_inv_freq
 from .prefix_cache import NativeKVPrefixCache, PagedKVStats, chain_merkle_prefix_hash
 from .scheduler import ContinuousBatchScheduler, PagedDecoderModel, PrefixPageIndex
+from .tree import PromptLookupDrafter, TreeDrafter, tree_mask
 
 __all__ = [
     "ContinuousBatchScheduler",
@@ -29,6 +30,10 @@ __all__ = [
     "SCKVBoundsError",
     "SCKVError",
     "SCKVPoolExhausted",
+    "PromptLookupDrafter",
+    "TreeDrafter",
     "chain_merkle_prefix_hash",
+    "rope_axis_map",
     "rope_inv_freq",
+    "tree_mask",
 ]

@@ -100,6 +100,21 @@ _SIGNATURES = [
     ("sckv_decode_attn_noalloc", c_int,
      [c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int64, c_int, c_void_p, c_int, c_float, c_void_p, c_int,
       c_int, c_void_p]),
+    ("sckv_tree_attn", c_int,
+     [c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p,
+      c_int, c_float, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    ("sckv_tree_attn_workspace_bytes", c_size_t, [c_void_p, c_int, c_int]),
+    ("sckv_append_rope_axes", c_int,
+     [c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_int,
+      c_void_p, c_void_p, c_float, c_void_p, c_float, c_void_p, c_int64, c_int, c_void_p, c_int, c_int, c_void_p,
+      c_void_p, c_void_p, c_int64, c_int, c_void_p, c_size_t, c_void_p]),
+    ("sckv_append_rope_axes_workspace_bytes", c_size_t, [c_void_p, c_int]),
+    ("sckv_compact_tree", c_int,
+     [c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
+    ("sckv_verify_tree", c_int,
+     [c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p,
+      c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    ("sckv_verify_tree_workspace_bytes", c_size_t, [c_void_p, c_int, c_int]),
     ("sckv_alloc_reset", c_int, [c_void_p, c_void_p]),
     ("sckv_alloc_pages", c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     ("sckv_free_pages", c_int, [c_void_p, c_void_p, c_int, c_void_p]),

@@ -124,3 +124,27 @@ class PagedAttentionLayer:
                                  q_out_dtype=torch.float32, max_blocks=c.max_blocks)
         attn = c.decode_attention(layer, q, n_rows, scale=self.scale, out_dtype=torch.float32)
         return self.pool.o_proj(attn, w_o, out_dtype=out_dtype)
+
+    def tree(self, layer: int, x: torch.Tensor, positions: torch.Tensor, tree_mask: torch.Tensor,
+             cu_tokens: torch.Tensor, ctx_lens: torch.Tensor, w_q: torch.Tensor, w_k: torch.Tensor,
+             w_v: torch.Tensor, w_o: torch.Tensor, q_norm_w: Optional[torch.Tensor] = None,
+             k_norm_w: Optional[torch.Tensor] = None, axis_map: Optional[torch.Tensor] = None,
+             out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The nodes of a tree step opened with `PagedKVCache.begin_tree` (which
+        gives cu_tokens and ctx_lens): x [total, hidden] at rotary positions
+        `positions` (int32 [total], or [axes, total] with an axis_map) -> the
+        layer output [total, hidden_out]. Projections, norms + rotation +
+        append, attention under the tree's masks, o_proj. Per-head norms only."""
+        c, pool = self.cache, self.pool
+        d = c.head_dim
+        q = pool.o_proj(x, w_q).view(x.shape[0], -1, d)
+        k = pool.o_proj(x, w_k).view(x.shape[0], -1, d)
+        v = pool.o_proj(x, w_v).view(x.shape[0], -1, d)
+        if axis_map is None:
+            axis_map = torch.zeros(d // 2, dtype=torch.int32, device=c.device)
+        q_dt = torch.bfloat16 if pool.kv_dtype == "bf16" else torch.float32
+        q = c.append_tree_rope(layer, q, k, v, positions, axis_map, cu_tokens, ctx_lens, self.inv_freq,
+                               rope_scaling=self.rope_scaling, q_norm_w=q_norm_w, k_norm_w=k_norm_w,
+                               eps=self.rms_eps, q_out_dtype=q_dt)
+        attn = c.tree_attention(layer, q, cu_tokens, ctx_lens, tree_mask, scale=self.scale, out_dtype=torch.float32)
+        return pool.o_proj(attn, w_o, out_dtype=out_dtype)

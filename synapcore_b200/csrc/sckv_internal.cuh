@@ -32,6 +32,10 @@ enum SckvKernelId : int32_t {
   KID_QKV = 14,
   KID_SELFTEST = 15,
   KID_EXCHANGE = 16,
+  KID_ROPE_AXES = 17,
+  KID_TREE_ATTN = 18,
+  KID_VERIFY = 19,
+  KID_COMPACT = 20,
 };
 
 // Allocator control words (int64, device).

@@ -1,0 +1,660 @@
+// Operators of a speculative decoding step around its attention: q/k norm +
+// rotary positions with several axes + K/V append, the move of the accepted
+// rows next to the committed ones, and the choice of the accepted path from
+// the logits.
+#include <math.h>
+
+#include "sckv_geo.cuh"
+
+using namespace sckv_geo;
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// QK-norm + rotary positions with several axes + append, one layer.
+//
+//   x' = x / sqrt(mean(x^2) + eps) * w                    (q and k, when w is given)
+//   a_i = pos[axis[i]][t] / scaling * inv_freq[i],        i < D / 2
+//   out = [x1 cos a - x2 sin a, x2 cos a + x1 sin a]      (halves of x')
+//
+// A token's rotary positions are independent of its page slot: the nodes of a
+// drafted tree sit in consecutive slots but rotate by depth, and image tokens
+// rotate by (time, height, width).
+//
+// Bound by HBM: (Hq + 2 Hkv) rows read and written once. Eight lanes own a
+// head row, each 8 dims of the first half and their 8 partners of the second
+// (two 16-byte loads and stores per 16-bit row, rotation without exchange, a
+// norm of three shuffles); a CTA takes `tpb` tokens so their angles are
+// computed once for all heads. The angle is formed and reduced to [-pi, pi] in
+// 64 bits (a far position times a frequency near 1 has no useful fp32 bits
+// left after the reduction); sin and cos then run in fp32.
+// ---------------------------------------------------------------------------
+constexpr int kRopeThreads = 256;
+constexpr int kRopeD = 128;
+constexpr int kRopeTokens = 4;  // most tokens of one CTA
+
+struct RopeAxes {
+  Geo g;
+  int layer;
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_stride, k_stride, v_stride;  // elements between tokens
+  int q_dtype, src_dtype;
+  void* q_out;
+  int q_out_dtype;
+  __half* k_stage;  // FP8 pools: rotated k [n_tokens][H][D], appended by the next launch
+  const __half* q_w;
+  const __half* k_w;
+  float eps;
+  const float* inv_freq;
+  double inv_scaling;
+  const int32_t* positions;
+  int64_t pos_stride;
+  int n_axes;
+  const int32_t* axis_map;
+  int hq, n_seqs, n_tokens, tpb;
+  const int32_t* cu;
+  const int32_t* start_pos;
+  const int32_t* bt;
+  int64_t bt_stride;
+  int max_blocks;
+};
+
+// Sum and max over the 8 lanes that own a row (`m`: their lanes).
+__device__ __forceinline__ float row_sum(float v, unsigned m) {
+  v += __shfl_xor_sync(m, v, 1);
+  v += __shfl_xor_sync(m, v, 2);
+  return v + __shfl_xor_sync(m, v, 4);
+}
+__device__ __forceinline__ float row_max(float v, unsigned m) {
+  v = fmaxf(v, __shfl_xor_sync(m, v, 1));
+  v = fmaxf(v, __shfl_xor_sync(m, v, 2));
+  return fmaxf(v, __shfl_xor_sync(m, v, 4));
+}
+
+__device__ __forceinline__ void store8(void* dst, int64_t idx, int dtype, const float (&v)[8]) {
+  if (dtype == SCKV_DTYPE_F32) {
+    float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(dst) + idx);
+    o[0] = make_float4(v[0], v[1], v[2], v[3]);
+    o[1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    store8_16(dst, idx, dtype, v);
+  }
+}
+
+// One K or V row into its int8 page slot as the arena stores its fp16 pages:
+// the fp16 value, quantised per row (s = max(max|x| / 127, 1e-7), fp16 scale).
+__device__ __forceinline__ void store_row8_int8(const Geo& g, int layer, int64_t page, int kv, int h, int slot, int l8,
+                                                unsigned m, const float (&a)[8], const float (&b)[8]) {
+  float x[16], top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x[i] = __half2float(__float2half_rn(a[i]));
+    x[8 + i] = __half2float(__float2half_rn(b[i]));
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(x[i]));
+  const float s = fmaxf(row_max(top, m) / 127.0f, 1e-7f);
+  int8_t* dst = reinterpret_cast<int8_t*>(g.data) + row_off(g, layer, page, kv, h, slot);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    union {
+      int8_t c[8];
+      uint2 w;
+    } u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      u.c[i] = static_cast<int8_t>(fminf(fmaxf(rintf(x[8 * half + i] / s), -127.0f), 127.0f));
+    *reinterpret_cast<uint2*>(dst + half * (kRopeD / 2) + 8 * l8) = u.w;
+  }
+  if (l8 == 0)
+    reinterpret_cast<__half*>(g.scales)[int8_scale_idx(g, layer, page, kv, h, slot)] = __float2half_rn(s);
+}
+
+__global__ void __launch_bounds__(kRopeThreads) rope_axes_kernel(const RopeAxes p) {
+  __shared__ float s_cos[kRopeTokens * (kRopeD / 2)], s_sin[kRopeTokens * (kRopeD / 2)];
+  __shared__ int64_t s_page[kRopeTokens];
+  __shared__ int s_slot[kRopeTokens];  // -1: not a token of any sequence
+  const int t0 = blockIdx.x * p.tpb;
+  const int nt = min(p.tpb, p.n_tokens - t0);
+  for (int i = threadIdx.x; i < nt * (kRopeD / 2); i += kRopeThreads) {
+    const int t = t0 + i / (kRopeD / 2), f = i % (kRopeD / 2);
+    int axis = __ldg(p.axis_map + f);
+    if (axis < 0 || axis >= p.n_axes) {
+      if (blockIdx.x == 0) sckv_report(p.g.status, SCKV_ERR_BOUNDS, axis, KID_ROPE_AXES);
+      axis = 0;
+    }
+    const double a = (double)__ldg(p.positions + axis * p.pos_stride + t) * p.inv_scaling * (double)__ldg(p.inv_freq + f);
+    const double r = a - 6.283185307179586 * rint(a * 0.15915494309189535);
+    sincosf((float)r, &s_sin[i], &s_cos[i]);
+  }
+  if (threadIdx.x < nt) {
+    const int t = t0 + threadIdx.x;
+    int slot = -1;
+    int64_t page = -1;
+    if (t >= __ldg(p.cu) && t < __ldg(p.cu + p.n_seqs)) {
+      const int b = sckv_find_seq(p.cu, p.n_seqs, t);
+      const int pos = __ldg(p.start_pos + b) + (t - __ldg(p.cu + b));
+      page = resolve_page(p.g, p.bt, p.bt_stride, p.max_blocks, b, pos, KID_ROPE_AXES);
+      slot = page >= 0 ? pos % SCKV_PAGE_TOKENS : 0;
+    }
+    s_page[threadIdx.x] = page;
+    s_slot[threadIdx.x] = slot;
+  }
+  __syncthreads();
+  const int l8 = threadIdx.x & 7;
+  const unsigned m = 0xffu << (threadIdx.x & 24);
+  const int H = p.g.H, rows = p.hq + 2 * H;
+  for (int r = threadIdx.x >> 3; r < nt * rows; r += kRopeThreads / 8) {
+    const int tt = r / rows, hr = r - tt * rows;
+    const int64_t page = s_page[tt];
+    const int slot = s_slot[tt];
+    if (slot < 0) continue;
+    const int t = t0 + tt;
+    const int kind = hr < p.hq ? 0 : hr < p.hq + H ? 1 : 2;  // q, k, v
+    const int h = kind == 0 ? hr : kind == 1 ? hr - p.hq : hr - p.hq - H;
+    if (kind != 0 && page < 0) continue;
+    const void* src = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
+    const int64_t stride = kind == 0 ? p.q_stride : kind == 1 ? p.k_stride : p.v_stride;
+    const int dt = kind == 0 ? p.q_dtype : p.src_dtype;
+    const int64_t base = t * stride + (int64_t)h * kRopeD + 8 * l8;
+    float a[8], b[8];
+    load8(src, base, dt, a);
+    load8(src, base + kRopeD / 2, dt, b);
+    if (kind < 2) {
+      const __half* w = kind == 0 ? p.q_w : p.k_w;
+      if (w != nullptr) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
+        const float inv = 1.f / sqrtf(row_sum(ss, m) * (1.f / kRopeD) + p.eps);
+        float wa[8], wb[8];
+        load8(w, 8 * l8, SCKV_DTYPE_F16, wa);
+        load8(w, kRopeD / 2 + 8 * l8, SCKV_DTYPE_F16, wb);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          a[i] = a[i] * inv * wa[i];
+          b[i] = b[i] * inv * wb[i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int f = tt * (kRopeD / 2) + 8 * l8 + i;
+        const float c = s_cos[f], s = s_sin[f];
+        const float x = a[i], y = b[i];
+        a[i] = x * c - y * s;
+        b[i] = y * c + x * s;
+      }
+    }
+    if (kind == 0) {
+      const int64_t o = ((int64_t)t * p.hq + h) * kRopeD + 8 * l8;
+      store8(p.q_out, o, p.q_out_dtype, a);
+      store8(p.q_out, o + kRopeD / 2, p.q_out_dtype, b);
+    } else if (p.g.dtype == SCKV_DTYPE_INT8) {
+      store_row8_int8(p.g, p.layer, page, kind - 1, h, slot, l8, m, a, b);
+    } else if (p.g.dtype == SCKV_DTYPE_FP8_E4M3) {
+      if (kind == 1) {
+        const int64_t o = ((int64_t)t * H + h) * kRopeD + 8 * l8;
+        store8_16(p.k_stage, o, SCKV_DTYPE_F16, a);
+        store8_16(p.k_stage, o + kRopeD / 2, SCKV_DTYPE_F16, b);
+      }
+    } else {
+      const int64_t o = row_off(p.g, p.layer, page, kind - 1, h, slot) + 8 * l8;
+      store8_16(p.g.data, o, p.g.dtype, a);
+      store8_16(p.g.data, o + kRopeD / 2, p.g.dtype, b);
+    }
+  }
+}
+
+// FP8 pools, second launch: one warp per (sequence, K|V, head) folds the new
+// rows into its pages (page scales span 16 tokens, so a row cannot be stored
+// by itself). K comes from the rotated fp16 rows, V from its source.
+__global__ void rope_axes_fp8_kernel(const RopeAxes p) {
+  const int units = p.n_seqs * 2 * p.g.H;
+  const int u = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  if (u >= units) return;
+  const int h = u % p.g.H, kv = (u / p.g.H) & 1, b = u / (2 * p.g.H);
+  const int c0 = __ldg(p.cu), cn = min(__ldg(p.cu + p.n_seqs), p.n_tokens);
+  const int t_first = max(__ldg(p.cu + b), max(c0, 0)), t_end = min(__ldg(p.cu + b + 1), cn);
+  const int64_t stride = kv ? p.v_stride : (int64_t)p.g.H * kRopeD;
+  for (int t = t_first; t < t_end;) {
+    const int pos = __ldg(p.start_pos + b) + (t - __ldg(p.cu + b));
+    const int slot0 = pos >= 0 ? pos % SCKV_PAGE_TOKENS : 0;
+    const int n_new = min(t_end - t, SCKV_PAGE_TOKENS - slot0);
+    const int64_t page = resolve_page(p.g, p.bt, p.bt_stride, p.max_blocks, b, pos, KID_ROPE_AXES);
+    if (page >= 0)
+      fp8_page_head_update(p.g, p.layer, page, kv, h, slot0, n_new, kv ? p.v : (const void*)p.k_stage,
+                           (int64_t)t * stride + (int64_t)h * kRopeD, stride, kv ? p.src_dtype : SCKV_DTYPE_F16);
+    t += n_new;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Accepted rows: row ctx + path[j] of a sequence moves to row ctx + j, j <
+// n_keep, in every layer, K and V (with the int8 scales). path increases, so
+// path[j] >= j: rows only move down, and a row is read before anything lands
+// on it when destinations are taken in order.
+//
+// Bound by HBM (each moved row read and written once). One warp owns
+// (sequence, layer, K|V, head) and takes one destination page at a time: all
+// of its loads are issued, then its stores, 16 bytes a lane. Rows that stay
+// where they are are not touched.
+//
+// FP8: a page-head has one scale for its 16 rows. Rows that come from other
+// pages are values code * s_src; the destination's scale grows to
+// max(s, max|value| / 448) as an append's does, and the rows it already held
+// are re-encoded when it grew. A destination page is only a source for rows
+// of itself and of earlier pages, so scales are read before they change.
+// ---------------------------------------------------------------------------
+constexpr int kCompactWarps = 8;
+
+struct Compact {
+  Geo g;
+  int layer0, n_layers, n_seqs, max_path;
+  const int32_t* path;  // [n_seqs][max_path]
+  const int32_t* n_keep;
+  const int32_t* ctx;
+  const int32_t* bt;
+  int64_t bt_stride;
+  int max_blocks;
+};
+
+template <bool kFP8>
+__global__ void __launch_bounds__(kCompactWarps * 32) compact_kernel(const Compact p) {
+  const Geo& g = p.g;
+  const int lane = threadIdx.x & 31;
+  const int64_t units = (int64_t)p.n_seqs * p.n_layers * 2 * g.H;
+  int64_t u = (int64_t)blockIdx.x * kCompactWarps + (threadIdx.x >> 5);
+  if (u >= units) return;
+  const int h = (int)(u % g.H);
+  u /= g.H;
+  const int kv = (int)(u & 1);
+  u >>= 1;
+  const int l = (int)(u % p.n_layers), b = (int)(u / p.n_layers);
+  const int layer = p.layer0 + l;
+  const bool reporter = l == 0 && kv == 0 && h == 0 && lane == 0;
+  const int keep = __ldg(p.n_keep + b), ctx = __ldg(p.ctx + b);
+  const int32_t* path = p.path + (int64_t)b * p.max_path;
+  const int cap = p.max_blocks * SCKV_PAGE_TOKENS;
+  if (keep < 0 || keep > p.max_path || ctx < 0 || ctx > cap) {
+    if (reporter) sckv_report(g.status, SCKV_ERR_BOUNDS, b, KID_COMPACT);
+    return;
+  }
+  // the path increases and stays inside the table; rows 0 .. j0 - 1 do not move
+  bool bad = false;
+  int j0 = keep;
+  for (int j = lane; j < keep; j += 32) {
+    const int pj = __ldg(path + j), before = j > 0 ? __ldg(path + j - 1) : -1;
+    bad |= pj <= before || pj >= cap - ctx;
+    if (pj != j) j0 = min(j0, j);
+  }
+  if (__any_sync(0xffffffffu, bad)) {
+    if (reporter) sckv_report(g.status, SCKV_ERR_BOUNDS, b, KID_COMPACT);
+    return;
+  }
+  j0 = __reduce_min_sync(0xffffffffu, j0);
+  if (j0 >= keep) return;
+  const int32_t* bt = p.bt + (int64_t)b * p.bt_stride;
+  const int eb = g.dtype == SCKV_DTYPE_F16 || g.dtype == SCKV_DTYPE_BF16 ? 2 : 1;
+  const int cpr = g.D * eb / 16;  // 16-byte chunks of a row
+  uint8_t* data = reinterpret_cast<uint8_t*>(g.data);
+  float* fscale = reinterpret_cast<float*>(g.scales);
+  __half* hscale = reinterpret_cast<__half*>(g.scales);
+  for (int blk = (ctx + j0) / SCKV_PAGE_TOKENS; blk <= (ctx + keep - 1) / SCKV_PAGE_TOKENS; ++blk) {
+    const int32_t dpage = __ldg(bt + blk);
+    if (dpage < 0 || dpage >= g.P) {
+      if (reporter) sckv_report(g.status, SCKV_ERR_BOUNDS, dpage, KID_COMPACT);
+      continue;
+    }
+    const int first = blk * SCKV_PAGE_TOKENS - ctx;  // path index of slot 0
+    // byte offset of the row that slot `s` takes over, -1 if it keeps its own; its page through *from
+    auto source = [&](int s, int32_t* from) -> int64_t {
+      const int j = first + s;
+      if (j < j0 || j >= keep) return -1;
+      const int pos = ctx + __ldg(path + j);
+      const int32_t page = __ldg(bt + pos / SCKV_PAGE_TOKENS);
+      if (page < 0 || page >= g.P) {
+        if (reporter) sckv_report(g.status, SCKV_ERR_BOUNDS, page, KID_COMPACT);
+        return -1;
+      }
+      *from = page;
+      return row_off(g, layer, page, kv, h, pos % SCKV_PAGE_TOKENS) * eb;
+    };
+    const int64_t dst0 = row_off(g, layer, dpage, kv, h, 0) * eb;
+    constexpr int kBatch = 8;
+    if constexpr (!kFP8) {
+      for (int i0 = 0; i0 < SCKV_PAGE_TOKENS * cpr; i0 += 32 * kBatch) {
+        uint4 r[kBatch];
+        bool mv[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const int i = i0 + 32 * k + lane;
+          int32_t from;
+          const int64_t off = i < SCKV_PAGE_TOKENS * cpr ? source(i / cpr, &from) : -1;
+          mv[k] = off >= 0;
+          if (mv[k]) r[k] = *reinterpret_cast<const uint4*>(data + off + (i % cpr) * 16);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+          if (mv[k]) *reinterpret_cast<uint4*>(data + dst0 + (int64_t)(i0 + 32 * k + lane) * 16) = r[k];
+      }
+      if (g.dtype == SCKV_DTYPE_INT8) {
+        const int s = lane & 15, j = first + s;
+        const bool mine = lane < SCKV_PAGE_TOKENS && j >= j0 && j < keep;
+        __half sc = __float2half_rn(0.f);
+        bool have = false;
+        if (mine) {
+          const int pos = ctx + __ldg(path + j);
+          const int32_t page = __ldg(bt + pos / SCKV_PAGE_TOKENS);
+          have = page >= 0 && page < g.P;
+          if (have) sc = hscale[int8_scale_idx(g, layer, page, kv, h, pos % SCKV_PAGE_TOKENS)];
+        }
+        __syncwarp();
+        if (have) hscale[int8_scale_idx(g, layer, dpage, kv, h, s)] = sc;
+      }
+    } else {
+      const float s_dst = fscale[fp8_scale_idx(g, layer, dpage, kv, h)];
+      // pass 1: the largest value that comes from another page
+      float top = 0.f;
+      for (int i = lane; i < SCKV_PAGE_TOKENS * cpr; i += 32) {
+        int32_t from = dpage;
+        const int64_t off = source(i / cpr, &from);
+        if (off < 0 || from == dpage) continue;
+        const float sc = fscale[fp8_scale_idx(g, layer, from, kv, h)];
+        const uint4 w = *reinterpret_cast<const uint4*>(data + off + (i % cpr) * 16);
+        const uint8_t* c = reinterpret_cast<const uint8_t*>(&w);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(sckv_fp8_to_float(c[e]) * sc));
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float s_new = fmaxf(s_dst, top / 448.0f);
+      // pass 2: rows in order, 32 / cpr of them at a time (loads before stores)
+      for (int i0 = 0; i0 < SCKV_PAGE_TOKENS * cpr; i0 += 32) {
+        const int i = i0 + lane;
+        int32_t from = dpage;
+        int64_t off = i < SCKV_PAGE_TOKENS * cpr ? source(i / cpr, &from) : -1;
+        bool store = off >= 0;
+        off += (i % cpr) * 16;
+        if (!store && i < SCKV_PAGE_TOKENS * cpr && first + i / cpr < j0 && s_new > s_dst) {
+          off = dst0 + (int64_t)i * 16;  // a row that stays: re-encoded under the grown scale
+          from = dpage;
+          store = true;
+        }
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        if (store) {
+          w = *reinterpret_cast<const uint4*>(data + off);
+          const float sc = from == dpage ? s_dst : fscale[fp8_scale_idx(g, layer, from, kv, h)];
+          if (sc != s_new) {
+            uint8_t* c = reinterpret_cast<uint8_t*>(&w);
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              c[e] = s_new > 0.f ? sckv_float_to_fp8(sckv_fp8_to_float(c[e]) * sc / s_new) : (uint8_t)0;
+          }
+        }
+        __syncwarp();
+        if (store) *reinterpret_cast<uint4*>(data + dst0 + (int64_t)i * 16) = w;
+      }
+      __syncwarp();
+      if (lane == 0 && s_new > s_dst) fscale[fp8_scale_idx(g, layer, dpage, kv, h)] = s_new;
+    }
+    __syncwarp();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Greedy check of a drafted tree: t_i = argmax_v logits[i][v] (the lowest
+// index of equal values; NaN counts as the largest, as torch.argmax has it),
+// then from node 0 on the child whose token is t of its parent, the first of
+// equals, until there is none. Bound by HBM (the logits, read once): rows are
+// cut into `chunks` so that few rows still fill the GPU, every CTA leaves its
+// chunk's best as one 64-bit word (ordered value, then the complement of the
+// index), and one warp per sequence joins them and walks.
+// ---------------------------------------------------------------------------
+constexpr int kVerifyThreads = 256;
+constexpr int kVerifyMaxNodes = 1024;
+
+// Larger value, then lower index <-> larger word.
+__device__ __forceinline__ unsigned long long rank_word(float x, uint32_t idx) {
+  x += 0.f;  // -0 counts as 0
+  uint32_t b = __float_as_uint(x);
+  b = x != x ? 0xffffffffu : (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  return ((unsigned long long)b << 32) | (uint32_t)~idx;
+}
+
+template <int DT>
+__device__ __forceinline__ float logit_at(const void* base, int64_t i) {
+  if (DT == SCKV_DTYPE_F32) return reinterpret_cast<const float*>(base)[i];
+  if (DT == SCKV_DTYPE_F16) return __half2float(reinterpret_cast<const __half*>(base)[i]);
+  return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(base)[i]);
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kVerifyThreads) verify_argmax_kernel(const void* logits, int64_t ld, int vocab,
+                                                                       int chunks, unsigned long long* best) {
+  const int row = blockIdx.x / chunks, c = blockIdx.x - row * chunks;
+  const int64_t per = ((int64_t)vocab + chunks - 1) / chunks;
+  const int lo = (int)min((int64_t)vocab, c * per), hi = (int)min((int64_t)vocab, (c + 1) * per);
+  const int64_t base = row * ld;
+  unsigned long long w = 0;
+  for (int i = lo + threadIdx.x; i < hi; i += kVerifyThreads) {
+    const unsigned long long x = rank_word(logit_at<DT>(logits, base + i), (uint32_t)i);
+    w = x > w ? x : w;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const unsigned long long x = __shfl_xor_sync(0xffffffffu, w, o);
+    w = x > w ? x : w;
+  }
+  __shared__ unsigned long long s[kVerifyThreads / 32];
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = w;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int i = 1; i < kVerifyThreads / 32; ++i) w = s[i] > w ? s[i] : w;
+    best[blockIdx.x] = w;
+  }
+}
+
+__global__ void verify_walk_kernel(const unsigned long long* best, int chunks, const int32_t* tokens,
+                                   const int32_t* parents, const int32_t* cu, int n_tokens, int max_path,
+                                   int32_t* path, int32_t* n_keep, int32_t* next, int32_t* status) {
+  __shared__ int32_t s_best[kVerifyMaxNodes];
+  const int b = blockIdx.x, lane = threadIdx.x;
+  const int t0 = __ldg(cu + b), n = __ldg(cu + b + 1) - t0;
+  int32_t* out = path + (int64_t)b * max_path;
+  const bool ok = t0 >= 0 && n >= 0 && n <= kVerifyMaxNodes && t0 + n <= n_tokens;
+  if (!ok && lane == 0) sckv_report(status, SCKV_ERR_BOUNDS, b, KID_VERIFY);
+  int keep = 0, token = -1;
+  if (ok && n > 0) {
+    for (int i = lane; i < n; i += 32) {
+      unsigned long long w = 0;
+      for (int c = 0; c < chunks; ++c) {
+        const unsigned long long x = best[(int64_t)(t0 + i) * chunks + c];
+        w = x > w ? x : w;
+      }
+      s_best[i] = (int32_t)~(uint32_t)w;
+    }
+    __syncwarp();
+    int cur = 0;
+    if (lane == 0) out[0] = 0;
+    keep = 1;
+    token = s_best[0];
+    while (keep < max_path) {
+      // the first later node that hangs on `cur` and carries its token
+      int child = -1;
+      for (int j0 = cur + 1; j0 < n && child < 0; j0 += 32) {
+        const int j = j0 + lane;
+        const bool hit = j < n && __ldg(parents + t0 + j) == cur && __ldg(tokens + t0 + j) == token;
+        const unsigned m = __ballot_sync(0xffffffffu, hit);
+        if (m) child = j0 + __ffs(m) - 1;
+      }
+      if (child < 0) break;
+      if (lane == 0) out[keep] = child;
+      ++keep;
+      cur = child;
+      token = s_best[cur];
+    }
+  }
+  for (int j = keep + lane; j < max_path; j += 32) out[j] = -1;
+  if (lane == 0) {
+    n_keep[b] = keep;
+    next[b] = token;
+  }
+}
+
+// Cuts per row so that the argmax pass has a few CTAs per SM.
+int verify_chunks(int num_sms, int n_tokens, int vocab) {
+  const int most = (vocab + 2047) / 2048;  // at least 2048 logits a CTA
+  int c = (8 * num_sms + n_tokens - 1) / n_tokens;
+  if (c > most) c = most;
+  return c < 1 ? 1 : c;
+}
+
+}  // namespace
+
+extern "C" size_t sckv_append_rope_axes_workspace_bytes(const sckv_pool* p, int n_tokens) {
+  if (p == nullptr || n_tokens <= 0 || p->kv_dtype != SCKV_DTYPE_FP8_E4M3) return 0;
+  return (size_t)n_tokens * p->num_kv_heads * p->head_dim * 2;
+}
+
+extern "C" int sckv_append_rope_axes(sckv_pool* p, int layer, const void* q, int64_t q_stride, void* q_out,
+                                     int num_q_heads, int q_dtype, int q_out_dtype, const void* k, int64_t k_stride,
+                                     const void* v, int64_t v_stride, int src_dtype, const void* q_norm_w,
+                                     const void* k_norm_w, float eps, const float* inv_freq, float rope_scaling,
+                                     const int32_t* positions, int64_t pos_stride, int n_axes,
+                                     const int32_t* axis_map, int n_seqs, int n_tokens, const int32_t* cu_tokens,
+                                     const int32_t* start_pos, const int32_t* block_table, int64_t bt_stride,
+                                     int max_blocks, void* workspace, size_t workspace_bytes, void* stream) {
+  if (p == nullptr || layer < 0 || layer >= p->num_layers || n_seqs < 0 || n_tokens < 0 || num_q_heads <= 0 ||
+      n_axes <= 0)
+    return SCKV_ERR_INVALID_ARG;
+  if (p->head_dim != kRopeD) return SCKV_ERR_UNSUPPORTED;
+  if (!is_src_dtype(src_dtype) || !is_src_dtype(q_dtype) || !is_src_dtype(q_out_dtype)) return SCKV_ERR_INVALID_ARG;
+  if (!(rope_scaling > 0.f) || !(eps >= 0.f)) return SCKV_ERR_INVALID_ARG;
+  if (n_seqs == 0 || n_tokens == 0) return SCKV_OK;
+  if (!q || !q_out || !k || !v || !inv_freq || !positions || !axis_map || !cu_tokens || !start_pos || !block_table ||
+      bt_stride < max_blocks || max_blocks <= 0)
+    return SCKV_ERR_INVALID_ARG;
+  if (q_stride < (int64_t)num_q_heads * kRopeD || k_stride < (int64_t)p->num_kv_heads * kRopeD ||
+      v_stride < (int64_t)p->num_kv_heads * kRopeD)
+    return SCKV_ERR_INVALID_ARG;
+  const int64_t qe = q_dtype == SCKV_DTYPE_F32 ? 4 : 2, se = src_dtype == SCKV_DTYPE_F32 ? 4 : 2;
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+        reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(q_norm_w) |
+        reinterpret_cast<uintptr_t>(k_norm_w) | reinterpret_cast<uintptr_t>(workspace)) & 15) ||
+      ((q_stride * qe) & 15) || ((k_stride * se) & 15) || ((v_stride * se) & 15))
+    return SCKV_ERR_ALIGNMENT;
+  const size_t need = sckv_append_rope_axes_workspace_bytes(p, n_tokens);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return SCKV_ERR_INVALID_ARG;
+  RopeAxes a{};
+  a.g = geo_of(p);
+  a.layer = layer;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.q_stride = q_stride;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.q_dtype = q_dtype;
+  a.src_dtype = src_dtype;
+  a.q_out = q_out;
+  a.q_out_dtype = q_out_dtype;
+  a.k_stage = reinterpret_cast<__half*>(workspace);
+  a.q_w = reinterpret_cast<const __half*>(q_norm_w);
+  a.k_w = reinterpret_cast<const __half*>(k_norm_w);
+  a.eps = eps;
+  a.inv_freq = inv_freq;
+  a.inv_scaling = 1.0 / (double)rope_scaling;
+  a.positions = positions;
+  a.pos_stride = pos_stride;
+  a.n_axes = n_axes;
+  a.axis_map = axis_map;
+  a.hq = num_q_heads;
+  a.n_seqs = n_seqs;
+  a.n_tokens = n_tokens;
+  a.tpb = 1;
+  a.cu = cu_tokens;
+  a.start_pos = start_pos;
+  a.bt = block_table;
+  a.bt_stride = bt_stride;
+  a.max_blocks = max_blocks;
+  SCKV_DEVICE_GUARD(p->device);
+  cudaStream_t s = as_stream(stream);
+  rope_axes_kernel<<<(n_tokens + a.tpb - 1) / a.tpb, kRopeThreads, 0, s>>>(a);
+  SCKV_LAUNCH_CHECK();
+  if (p->kv_dtype == SCKV_DTYPE_FP8_E4M3) {
+    const int64_t units = (int64_t)n_seqs * 2 * p->num_kv_heads;
+    rope_axes_fp8_kernel<<<(unsigned)((units + 3) / 4), 128, 0, s>>>(a);
+    SCKV_LAUNCH_CHECK();
+  }
+  return SCKV_OK;
+}
+
+extern "C" int sckv_compact_tree(sckv_pool* p, int layer0, int n_layers, int n_seqs, const int32_t* path, int max_path,
+                                 const int32_t* n_keep, const int32_t* ctx_lens, const int32_t* block_table,
+                                 int64_t bt_stride, int max_blocks, void* stream) {
+  if (p == nullptr || layer0 < 0 || n_layers <= 0 || layer0 + n_layers > p->num_layers || n_seqs < 0 || max_path < 0)
+    return SCKV_ERR_INVALID_ARG;
+  if (n_seqs == 0 || max_path == 0) return SCKV_OK;
+  if (!path || !n_keep || !ctx_lens || !block_table || bt_stride < max_blocks || max_blocks <= 0)
+    return SCKV_ERR_INVALID_ARG;
+  Compact c{geo_of(p), layer0, n_layers, n_seqs, max_path, path, n_keep, ctx_lens, block_table, bt_stride, max_blocks};
+  const int64_t blocks = ((int64_t)n_seqs * n_layers * 2 * p->num_kv_heads + kCompactWarps - 1) / kCompactWarps;
+  if (blocks > INT32_MAX) return SCKV_ERR_INVALID_ARG;
+  SCKV_DEVICE_GUARD(p->device);
+  if (p->kv_dtype == SCKV_DTYPE_FP8_E4M3)
+    compact_kernel<true><<<(unsigned)blocks, kCompactWarps * 32, 0, as_stream(stream)>>>(c);
+  else
+    compact_kernel<false><<<(unsigned)blocks, kCompactWarps * 32, 0, as_stream(stream)>>>(c);
+  SCKV_LAUNCH_CHECK();
+  return SCKV_OK;
+}
+
+extern "C" size_t sckv_verify_tree_workspace_bytes(const sckv_pool* p, int n_tokens, int vocab) {
+  if (p == nullptr || n_tokens <= 0 || vocab <= 0) return 0;
+  return (size_t)n_tokens * verify_chunks(p->num_sms, n_tokens, vocab) * sizeof(unsigned long long);
+}
+
+extern "C" int sckv_verify_tree(sckv_pool* p, const void* logits, int logits_dtype, int64_t ld, int n_tokens, int vocab,
+                                const int32_t* tokens, const int32_t* parents, const int32_t* cu_tokens, int n_seqs,
+                                int max_path, int32_t* path, int32_t* n_keep, int32_t* next_token, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+  if (p == nullptr || !is_src_dtype(logits_dtype) || n_tokens < 0 || vocab <= 0 || ld < vocab || n_seqs < 0 ||
+      max_path <= 0)
+    return SCKV_ERR_INVALID_ARG;
+  if (n_seqs == 0) return SCKV_OK;
+  if (!cu_tokens || !path || !n_keep || !next_token) return SCKV_ERR_INVALID_ARG;
+  if (n_tokens > 0 && (!logits || !tokens || !parents)) return SCKV_ERR_INVALID_ARG;
+  const size_t need = sckv_verify_tree_workspace_bytes(p, n_tokens, vocab);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return SCKV_ERR_INVALID_ARG;
+  if (reinterpret_cast<uintptr_t>(workspace) & 7) return SCKV_ERR_ALIGNMENT;
+  const size_t el = logits_dtype == SCKV_DTYPE_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(logits) & (el - 1)) return SCKV_ERR_ALIGNMENT;
+  SCKV_DEVICE_GUARD(p->device);
+  cudaStream_t s = as_stream(stream);
+  unsigned long long* best = reinterpret_cast<unsigned long long*>(workspace);
+  int chunks = 1;
+  if (n_tokens > 0) {
+    chunks = verify_chunks(p->num_sms, n_tokens, vocab);
+    const int64_t blocks = (int64_t)n_tokens * chunks;
+    if (blocks > INT32_MAX) return SCKV_ERR_INVALID_ARG;
+    switch (logits_dtype) {
+      case SCKV_DTYPE_F32:
+        verify_argmax_kernel<SCKV_DTYPE_F32><<<(unsigned)blocks, kVerifyThreads, 0, s>>>(logits, ld, vocab, chunks, best);
+        break;
+      case SCKV_DTYPE_F16:
+        verify_argmax_kernel<SCKV_DTYPE_F16><<<(unsigned)blocks, kVerifyThreads, 0, s>>>(logits, ld, vocab, chunks, best);
+        break;
+      default:
+        verify_argmax_kernel<SCKV_DTYPE_BF16><<<(unsigned)blocks, kVerifyThreads, 0, s>>>(logits, ld, vocab, chunks, best);
+    }
+    SCKV_LAUNCH_CHECK();
+  }
+  verify_walk_kernel<<<n_seqs, 32, 0, s>>>(best, chunks, tokens, parents, cu_tokens, n_tokens, max_path, path, n_keep,
+                                           next_token, p->status);
+  SCKV_LAUNCH_CHECK();
+  return SCKV_OK;
+}

@@ -23,6 +23,7 @@ import torch
 
 from . import _native as N
 from .pool import KVPool, PAGE_TOKENS, to_device
+from .tree import MAX_TREE_NODES
 
 
 def _ceil_div(a: int, b: int) -> int:
@@ -55,6 +56,7 @@ class PagedKVCache:
         self.row_of: Dict[Hashable, int] = {}  # sequence id -> row
         self.seq_at: List[Hashable] = []       # row -> sequence id
         self._arange = torch.arange(self.max_seqs + 1, dtype=torch.int32, device=self.device)
+        self._tree: Optional[List[int]] = None  # nodes per row of a tree step between begin_tree and commit_tree
 
     # ------------------------------------------------------------------ rows
     @property
@@ -83,6 +85,7 @@ class PagedKVCache:
     def remove_sequence(self, seq_id: Hashable, keep_cached: bool = False) -> None:
         """Drop the sequence's pins on its pages (shared pages survive for their
         other holders) and compact the rows."""
+        self._no_tree()
         r = self.row_of.pop(seq_id)
         n = self._pages_of(r)
         if n:
@@ -103,6 +106,7 @@ class PagedKVCache:
     def remove_sequences(self, seq_ids: Sequence[Hashable], keep_cached: bool = False) -> None:
         """remove_sequence for several sequences with one release launch (the
         pins of all their pages are dropped together, in the order given)."""
+        self._no_tree()
         seq_ids = list(seq_ids)
         if not seq_ids:
             return
@@ -123,6 +127,7 @@ class PagedKVCache:
 
     def move_to_row(self, seq_id: Hashable, row: int) -> None:
         """Swap two live rows (used to keep decode-phase sequences first)."""
+        self._no_tree()
         r = self.row_of[seq_id]
         if r == row:
             return
@@ -151,6 +156,7 @@ class PagedKVCache:
     # -------------------------------------------------------------- prefill
     def _grow(self, r: int, n_new: int) -> None:
         """Allocate (pinned) pages so row r can hold n_new more tokens."""
+        self._no_tree()
         have = self._pages_of(r)
         need = _ceil_div(self.lengths[r] + n_new, PAGE_TOKENS)
         if need > self.max_blocks:
@@ -189,6 +195,7 @@ class PagedKVCache:
     def _grow_rows(self, r0: int, n_new: Sequence[int]) -> None:
         """Pinned pages for rows r0.. so each can hold n_new[i] more tokens:
         one allocation launch and one block-table scatter for all rows."""
+        self._no_tree()
         rows, cols = [], []
         for i, t in enumerate(n_new):
             r = r0 + i
@@ -354,6 +361,7 @@ class PagedKVCache:
     def decode_reserve(self, n_rows: int) -> None:
         """One new token for rows 0..n_rows-1: pages for those crossing a page
         boundary are allocated on the device, lengths advance by one."""
+        self._no_tree()
         self.pool.reserve_decode(self.block_table, self.ctx_lens, n_seqs=n_rows, max_blocks=self.max_blocks)
         for r in range(n_rows):
             self.lengths[r] += 1
@@ -381,10 +389,93 @@ class PagedKVCache:
                                             scale=scale, out=out, out_dtype=out_dtype, max_blocks=self.max_blocks,
                                             chunk_pages=self.chunk_pages, workspace=workspace)
 
+    # ------------------------------------------------------ tree decoding
+    def _no_tree(self) -> None:
+        if self._tree is not None:
+            raise RuntimeError("a tree step is open: commit_tree first")
+
+    def begin_tree(self, n_nodes: Sequence[int]) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Open a step that checks a tree of n_nodes[r] drafted tokens on each
+        of rows 0..len(n_nodes)-1: pages for all of them are reserved, the
+        lengths stay. Returns the device int32 cu_tokens [n + 1] and the
+        committed lengths [n] that the step's calls take. Closed by
+        commit_tree; until then the rows cannot change otherwise."""
+        nodes = [int(n) for n in n_nodes]
+        if not 0 < len(nodes) <= self.n_live or min(nodes) < 0:
+            raise ValueError("begin_tree needs one node count >= 0 for each of rows 0..n-1")
+        if max(nodes) > MAX_TREE_NODES:
+            raise ValueError(f"a tree has more than {MAX_TREE_NODES} nodes")
+        self._grow_rows(0, nodes)
+        self._tree = nodes
+        cu = [0]
+        for n in nodes:
+            cu.append(cu[-1] + n)
+        meta = to_device(cu + self.lengths[:len(nodes)], torch.int32, self.device)
+        return meta[:len(cu)], meta[len(cu):]
+
+    def _open_tree(self) -> int:
+        if self._tree is None:
+            raise RuntimeError("no tree step is open: begin_tree first")
+        return len(self._tree)
+
+    def append_tree(self, layer: int, k: torch.Tensor, v: torch.Tensor, cu_tokens: torch.Tensor,
+                    ctx_lens: torch.Tensor) -> None:
+        """One layer's K/V rows of the nodes, k, v [total, Hkv, D] as they are
+        cached (rotated already), at slots length + node."""
+        n = self._open_tree()
+        self.pool.append(k, v, cu_tokens, ctx_lens, self.block_table[:n], layer0=layer, max_blocks=self.max_blocks)
+
+    def append_tree_rope(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                         positions: torch.Tensor, axis_map: torch.Tensor, cu_tokens: torch.Tensor,
+                         ctx_lens: torch.Tensor, inv_freq: torch.Tensor, **kw) -> torch.Tensor:
+        """append_tree from the projections: norms and rotary positions of the
+        nodes first (KVPool.append_rope_axes, whose keywords it takes);
+        returns the rotated q."""
+        n = self._open_tree()
+        return self.pool.append_rope_axes(layer, q, k, v, positions, axis_map, cu_tokens, ctx_lens,
+                                          self.block_table[:n], inv_freq, max_blocks=self.max_blocks, **kw)
+
+    def tree_attention(self, layer: int, q: torch.Tensor, cu_tokens: torch.Tensor, ctx_lens: torch.Tensor,
+                       tree_mask: torch.Tensor, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                       out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        """Attention of the nodes, q [total, Hq, D], over their rows' committed
+        tokens and the nodes of their masks (KVPool.tree_attn)."""
+        n = self._open_tree()
+        return self.pool.tree_attn(layer, q, cu_tokens, ctx_lens, self.block_table[:n], tree_mask, scale=scale,
+                                   out=out, out_dtype=out_dtype, max_blocks=self.max_blocks)
+
+    def commit_tree(self, path: torch.Tensor, n_keep: torch.Tensor, keep: Sequence[int]) -> None:
+        """Close a tree step: the rows of each sequence's accepted path (path
+        [n, P] and n_keep [n], int32 on the device, as verify_tree gives them)
+        move next to its committed ones, the lengths advance by keep[r] (the
+        same counts on the host; 0 drops the whole tree) and the pages past
+        them are released."""
+        n = self._open_tree()
+        kept = [int(c) for c in keep]
+        if len(kept) != n or path.dim() != 2 or path.shape[0] != n or n_keep.numel() != n:
+            raise ValueError("one path, n_keep and keep per row of the step")
+        if any(not 0 <= c <= min(m, path.shape[1]) for c, m in zip(kept, self._tree)):
+            raise ValueError("a row cannot keep more tokens than its tree or its path has")
+        old = to_device(self.lengths[:n], torch.int32, self.device)
+        self.pool.compact_tree(self.block_table[:n], old, path, n_keep, max_blocks=self.max_blocks)
+        rows, cols = [], []
+        for r, (c, m) in enumerate(zip(kept, self._tree)):
+            first, end = _ceil_div(self.lengths[r] + c, PAGE_TOKENS), _ceil_div(self.lengths[r] + m, PAGE_TOKENS)
+            rows.extend([r] * (end - first))
+            cols.extend(range(first, end))
+            self.lengths[r] += c
+        self._tree = None
+        if rows:
+            at = to_device([rows, cols], torch.int64, self.device)
+            self.pool.release_pages(self.block_table[at[0], at[1]])
+            self.block_table[at[0], at[1]] = -1
+        self.ctx_lens[:n].copy_(to_device(self.lengths[:n], torch.int32, self.device))
+
     # ------------------------------------------------------ sharing / fork
     def share_prefix(self, seq_id: Hashable, page_ids: Sequence[int]) -> None:
         """Start an empty sequence with full prefix pages held elsewhere (a
         prefix-cache hit): its block table points at them and pins them."""
+        self._no_tree()
         r = self.row_of[seq_id]
         if self.lengths[r] != 0:
             raise ValueError("share_prefix needs an empty sequence")
@@ -400,6 +491,7 @@ class PagedKVCache:
     def fork(self, src_id: Hashable, dst_id: Hashable) -> int:
         """Copy-on-write fork: full pages are shared (pinned once more), the
         partially filled last page is copied to a fresh page."""
+        self._no_tree()
         rs = self.row_of[src_id]
         rd = self.add_sequence(dst_id)
         n_tok = self.lengths[rs]
@@ -485,6 +577,7 @@ class DecodeStepGraph:
 
     def replay(self) -> torch.Tensor:
         """Run the captured step on the current stream; returns `out`."""
+        self.cache._no_tree()
         if self.cache.n_live < self.n_rows:
             raise RuntimeError("fewer live sequences than the captured batch")
         self.graph.replay()

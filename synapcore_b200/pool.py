@@ -12,7 +12,8 @@ same 16-token slot in every layer, as the reference's all-layer page does
 from __future__ import annotations
 
 import ctypes
-from typing import Dict, Optional, Tuple
+from contextlib import nullcontext
+from typing import Dict, Optional, Sequence, Tuple
 
 import torch
 
@@ -49,6 +50,26 @@ def rope_inv_freq(theta: float, head_dim: int, device: Optional[torch.device] = 
 
     inv = 1.0 / (float(theta) ** (np.arange(0, head_dim, 2, dtype=np.float32) / float(head_dim)))
     return torch.from_numpy(np.asarray(inv, dtype=np.float32)).to(device if device is not None else "cpu")
+
+
+def rope_axis_map(sections: Sequence[int], interleaved: bool = False,
+                  device: Optional[torch.device] = None) -> torch.Tensor:
+    """Which position axis each rotary frequency turns by, int32
+    [sum(sections)], for KVPool.append_rope_axes. sections[a] frequencies
+    belong to axis a, in runs (the first sections[0] to axis 0, and so on) or,
+    interleaved, in turn: frequency i to axis i mod A while that axis has
+    frequencies left, else to axis 0."""
+    sec = [int(n) for n in sections]
+    if not sec or min(sec) < 0 or sum(sec) == 0:
+        raise ValueError("sections must be non-negative counts, not all zero")
+    A, total = len(sec), sum(sec)
+    if interleaved:
+        axes = [i % A if i // A < sec[i % A] else 0 for i in range(total)]
+        if [axes.count(a) for a in range(A)] != sec:
+            raise ValueError(f"sections {sec} cannot be interleaved: axis 0 must have the most frequencies")
+    else:
+        axes = [a for a, n in enumerate(sec) for _ in range(n)]
+    return torch.tensor(axes, dtype=torch.int32, device=device if device is not None else "cpu")
 
 
 def _stream_ptr(stream: Optional[torch.cuda.Stream]) -> int:
@@ -568,6 +589,213 @@ class KVPool:
                                            torch_dtype_code(out.dtype), _stream_ptr(stream)),
                 "sckv_prefill_attn")
         return out
+
+    # ------------------------------------------------- speculative decoding
+    def _stream_scope(self, stream: Optional[torch.cuda.Stream]):
+        """Temporaries of a call on `stream` belong to that stream."""
+        return nullcontext() if stream is None else torch.cuda.stream(stream)
+
+    def _here(self, stream: Optional[torch.cuda.Stream]) -> int:
+        return (stream if stream is not None else torch.cuda.current_stream(self.device)).cuda_stream
+
+    def _table(self, block_table: torch.Tensor, n_seqs: int, max_blocks: Optional[int]) -> Tuple[torch.Tensor, int]:
+        bt = block_table if block_table.dim() == 2 else block_table.view(1, -1)
+        mb = bt.shape[1] if max_blocks is None else int(max_blocks)
+        _need(bt, "block_table", self.device, torch.int32, contiguous=False)
+        if bt.shape[0] < n_seqs or mb > bt.shape[1] or (mb > 1 and bt.stride(1) != 1) or \
+                (n_seqs > 1 and bt.stride(0) < mb):
+            raise ValueError("block_table must be [>= n_seqs, >= max_blocks] rows with unit column stride")
+        return bt, mb
+
+    def tree_attn(self, layer: int, q: torch.Tensor, cu_q: torch.Tensor, ctx_lens: torch.Tensor,
+                  block_table: torch.Tensor, tree_mask: torch.Tensor, scale: Optional[float] = None,
+                  out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                  max_blocks: Optional[int] = None, workspace: Optional[torch.Tensor] = None,
+                  stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+        """Attention of drafted trees: node i of sequence b (row cu_q[b] + i of
+        q [n_tokens, Hq, D], its K/V appended at slot ctx_lens[b] + i) over the
+        ctx_lens[b] committed tokens and the nodes j whose bit is set in its
+        mask, tree_mask int64 [n_tokens, W] (bit j % 64 of word j / 64; W <= 4,
+        at most 64 W nodes per sequence; synapcore_b200.tree_mask builds it
+        from parent indices). Returns out [n_tokens, Hq, D]; rows that see
+        nothing are 0, rows of no sequence stay as they are in `out`.
+        workspace: as decode_attn's, of tree_attn_workspace_bytes bytes."""
+        if q.dim() != 3 or q.shape[2] != self.head_dim or q.shape[1] % self.num_kv_heads != 0 or q.shape[1] == 0:
+            raise ValueError(f"q must be [n_tokens, k*{self.num_kv_heads}, {self.head_dim}]")
+        if not 0 <= layer < self.num_layers:
+            raise ValueError("layer out of range")
+        n_tok, hq, d = q.shape
+        n_seqs = cu_q.numel() - 1
+        mask = tree_mask if tree_mask.dim() == 2 else tree_mask.view(-1, 1)
+        if mask.shape[0] != n_tok or not 1 <= mask.shape[1] <= 4:
+            raise ValueError("tree_mask must be [n_tokens, 1 to 4]")
+        _need(cu_q, "cu_q", self.device, torch.int32, 1)
+        _need(ctx_lens, "ctx_lens", self.device, torch.int32, n_seqs)
+        _need(mask, "tree_mask", self.device, torch.int64)
+        bt, mb = self._table(block_table, n_seqs, max_blocks)
+        scale = float(d) ** -0.5 if scale is None else float(scale)
+        if not 0.0 < scale < float("inf"):
+            raise ValueError("scale must be positive")
+        with self._stream_scope(stream):
+            q = q.contiguous()
+            _need(q, "q", self.device)
+            if out is None:
+                out = torch.empty((n_tok, hq, d), dtype=out_dtype or q.dtype, device=self.device)
+            else:
+                _need(out, "out", self.device)
+                if tuple(out.shape) != (n_tok, hq, d):
+                    raise ValueError("out must have q's shape")
+            need = self.tree_attn_workspace_bytes(n_tok, hq)
+            if workspace is not None:
+                _need(workspace, "workspace", self.device, torch.uint8, min_numel=need)
+            else:
+                workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=self.device)
+            N.check(self.lib.sckv_tree_attn(self.handle, layer, q.data_ptr(), torch_dtype_code(q.dtype), hq, n_seqs,
+                                            n_tok, cu_q.data_ptr(), ctx_lens.data_ptr(), bt.data_ptr(), bt.stride(0),
+                                            mb, mask.data_ptr(), mask.shape[1], scale, out.data_ptr(),
+                                            torch_dtype_code(out.dtype), workspace.data_ptr(), workspace.numel(),
+                                            self._here(stream)),
+                    "sckv_tree_attn")
+        return out
+
+    def tree_attn_workspace_bytes(self, n_tokens: int, num_q_heads: int) -> int:
+        return int(self.lib.sckv_tree_attn_workspace_bytes(self.handle, n_tokens, num_q_heads))
+
+    @staticmethod
+    def _head_rows(t: torch.Tensor) -> torch.Tensor:
+        """[T, H, D] with packed heads and 16-byte aligned tokens: t itself (a
+        slice of a wider projection, say), or a contiguous copy."""
+        T, H, D = t.shape
+        packed = t.stride(2) == 1 and (H == 1 or t.stride(1) == D)
+        el = t.element_size()
+        if packed and (T <= 1 or (t.stride(0) >= H * D and t.stride(0) * el % 16 == 0)) and t.data_ptr() % 16 == 0:
+            return t
+        return t.contiguous()
+
+    def append_rope_axes(self, layer: int, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
+                         positions: torch.Tensor, axis_map: torch.Tensor, cu_tokens: torch.Tensor,
+                         start_pos: torch.Tensor, block_table: torch.Tensor, inv_freq: torch.Tensor,
+                         rope_scaling: float = 1.0, q_norm_w: Optional[torch.Tensor] = None,
+                         k_norm_w: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                         q_out: Optional[torch.Tensor] = None, q_out_dtype: Optional[torch.dtype] = None,
+                         max_blocks: Optional[int] = None, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+        """append_rope with positions of their own: rotary frequency i of token
+        t turns by positions[axis_map[i], t] (int32 [A, n_tokens]; axis_map
+        int32 [D / 2], see rope_axis_map), while its K/V row goes to slot
+        start_pos[b] + i. For image and video tokens (time, height, width) and
+        for tree nodes, whose position is their depth. q [n_tokens, Hq, D],
+        k_new / v_new [n_tokens, Hkv, D] may be slices of one projection
+        (heads packed); per-head norms (fp16 weights of D elements) only.
+        Returns the rotated q. Every pool type."""
+        if q.dim() != 3 or k_new.dim() != 3 or v_new.dim() != 3:
+            raise ValueError("q, k_new and v_new must be [n_tokens, heads, D]")
+        nt, hq, d = q.shape
+        n_seqs = cu_tokens.numel() - 1
+        if d != self.head_dim or tuple(k_new.shape) != (nt, self.num_kv_heads, d) or k_new.shape != v_new.shape:
+            raise ValueError("q must be [n_tokens, Hq, D] and k_new / v_new [n_tokens, Hkv, D]")
+        if k_new.dtype != v_new.dtype:
+            raise TypeError("k_new and v_new must have the same dtype")
+        if not 0 <= layer < self.num_layers:
+            raise ValueError("layer out of range")
+        pos = positions if positions.dim() == 2 else positions.view(1, -1)
+        _need(pos, "positions", self.device, torch.int32, contiguous=False)
+        if pos.shape[1] != nt or pos.shape[0] < 1:
+            raise ValueError("positions must be [axes, n_tokens]")
+        _need(axis_map, "axis_map", self.device, torch.int32)
+        if axis_map.numel() != d // 2:
+            raise ValueError("axis_map must have D / 2 entries")
+        _need(inv_freq, "inv_freq", self.device, torch.float32, d // 2)
+        _need(cu_tokens, "cu_tokens", self.device, torch.int32, 1)
+        _need(start_pos, "start_pos", self.device, torch.int32, n_seqs)
+        bt, mb = self._table(block_table, n_seqs, max_blocks)
+        for name, w in (("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w)):
+            if w is not None:
+                _need(w, name, self.device, torch.float16)
+                if w.numel() != d:
+                    raise ValueError(f"{name} must have D elements (a norm of each head)")
+        for name, t in (("q", q), ("k_new", k_new), ("v_new", v_new)):
+            _need(t, name, self.device, contiguous=False)
+        with self._stream_scope(stream):
+            q, k_new, v_new = self._head_rows(q), self._head_rows(k_new), self._head_rows(v_new)
+            if pos.stride(1) != 1 and nt > 1:
+                pos = pos.contiguous()
+            if q_out is None:
+                q_out = torch.empty((nt, hq, d), dtype=q_out_dtype or q.dtype, device=self.device)
+            else:
+                _need(q_out, "q_out", self.device)
+                if tuple(q_out.shape) != (nt, hq, d):
+                    raise ValueError("q_out must have q's shape")
+            need = int(self.lib.sckv_append_rope_axes_workspace_bytes(self.handle, nt))
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+            stride = lambda t: max(t.stride(0), t.shape[1] * d) if nt > 1 else t.shape[1] * d  # noqa: E731
+            N.check(self.lib.sckv_append_rope_axes(
+                self.handle, layer, q.data_ptr(), stride(q), q_out.data_ptr(), hq, torch_dtype_code(q.dtype),
+                torch_dtype_code(q_out.dtype), k_new.data_ptr(), stride(k_new), v_new.data_ptr(), stride(v_new),
+                torch_dtype_code(k_new.dtype), _ptr(q_norm_w), _ptr(k_norm_w), float(eps), inv_freq.data_ptr(),
+                float(rope_scaling), pos.data_ptr(), pos.stride(0) if pos.shape[0] > 1 else nt, pos.shape[0],
+                axis_map.data_ptr(), n_seqs, nt, cu_tokens.data_ptr(), start_pos.data_ptr(), bt.data_ptr(),
+                bt.stride(0), mb, _ptr(ws), need, self._here(stream)),
+                "sckv_append_rope_axes")
+        return q_out
+
+    def compact_tree(self, block_table: torch.Tensor, ctx_lens: torch.Tensor, path: torch.Tensor,
+                     n_keep: torch.Tensor, layer0: int = 0, n_layers: Optional[int] = None,
+                     max_blocks: Optional[int] = None, stream: Optional[torch.cuda.Stream] = None) -> None:
+        """Move accepted rows: position ctx_lens[b] + path[b, j] becomes
+        position ctx_lens[b] + j for j < n_keep[b], K and V, in layers layer0
+        .. layer0 + n_layers - 1 (default: all). path int32 [n_seqs, P],
+        strictly increasing along a row up to n_keep[b] (verify_tree's)."""
+        if path.dim() != 2:
+            raise ValueError("path must be [n_seqs, max_path]")
+        n_seqs = path.shape[0]
+        nl = self.num_layers - layer0 if n_layers is None else int(n_layers)
+        if layer0 < 0 or nl <= 0 or layer0 + nl > self.num_layers:
+            raise ValueError("compact_tree layers out of range")
+        _need(path, "path", self.device, torch.int32)
+        _need(n_keep, "n_keep", self.device, torch.int32, n_seqs)
+        _need(ctx_lens, "ctx_lens", self.device, torch.int32, n_seqs)
+        bt, mb = self._table(block_table, n_seqs, max_blocks)
+        N.check(self.lib.sckv_compact_tree(self.handle, layer0, nl, n_seqs, path.data_ptr(), path.shape[1],
+                                           n_keep.data_ptr(), ctx_lens.data_ptr(), bt.data_ptr(), bt.stride(0), mb,
+                                           self._here(stream)),
+                "sckv_compact_tree")
+
+    def verify_tree(self, logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, cu_tokens: torch.Tensor,
+                    max_path: Optional[int] = None, stream: Optional[torch.cuda.Stream] = None
+                    ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Greedy choice of the accepted path of each sequence's tree: logits
+        [n_tokens, vocab] of the nodes, their tokens and parents (index within
+        the sequence, node 0 the root), all int32 [n_tokens]. Returns
+        (path [n_seqs, max_path] padded with -1, n_keep [n_seqs], next_token
+        [n_seqs]), int32: from the root, on to the first child that carries
+        the argmax of its parent's logits; next_token is the last node's
+        argmax. max_path (default: n_tokens) bounds a path's length."""
+        if logits.dim() != 2 or logits.shape[1] == 0:
+            raise ValueError("logits must be [n_tokens, vocab]")
+        nt, vocab = logits.shape
+        n_seqs = cu_tokens.numel() - 1
+        mp = max(1, nt) if max_path is None else int(max_path)
+        if mp < 1:
+            raise ValueError("max_path must be at least 1")
+        _need(logits, "logits", self.device, contiguous=False)
+        _need(tokens, "tokens", self.device, torch.int32, nt)
+        _need(parents, "parents", self.device, torch.int32, nt)
+        _need(cu_tokens, "cu_tokens", self.device, torch.int32, 1)
+        with self._stream_scope(stream):
+            if (vocab > 1 and logits.stride(1) != 1) or (nt > 1 and logits.stride(0) < vocab):
+                logits = logits.contiguous()
+            out = torch.empty(n_seqs * (mp + 2), dtype=torch.int32, device=self.device)
+            path, keep, nxt = out[:n_seqs * mp].view(n_seqs, mp), out[n_seqs * mp:n_seqs * (mp + 1)], \
+                out[n_seqs * (mp + 1):]
+            need = int(self.lib.sckv_verify_tree_workspace_bytes(self.handle, nt, vocab))
+            ws = torch.empty(max(need, 8), dtype=torch.uint8, device=self.device)
+            N.check(self.lib.sckv_verify_tree(self.handle, logits.data_ptr(), torch_dtype_code(logits.dtype),
+                                              logits.stride(0) if nt > 1 else vocab, nt, vocab, tokens.data_ptr(),
+                                              parents.data_ptr(), cu_tokens.data_ptr(), n_seqs, mp, path.data_ptr(),
+                                              keep.data_ptr(), nxt.data_ptr(), ws.data_ptr(), ws.numel(),
+                                              self._here(stream)),
+                    "sckv_verify_tree")
+        return path, keep, nxt
 
     # ---------------------------------------------------------------- kernel 5
     def alloc_reset(self, stream: Optional[torch.cuda.Stream] = None) -> None:

@@ -34,6 +34,7 @@ import torch
 
 from .paged_cache import PAGE_TOKENS, PagedKVCache
 from .pool import to_device
+from .tree import MAX_TREE_NODES, TreeDrafter, tree_mask
 
 
 class PagedDecoderModel(Protocol):
@@ -69,6 +70,7 @@ class BatchStepResult(TypedDict):
     naive_expert_calls_without_sharing: int
     expert_dedup_savings_pct: float
     step_latency_ms: float
+    accepted_tokens: Dict[str, List[int]]  # with a drafter: every token a request emitted in the step
 
 
 class BatchSchedulerMetrics(TypedDict):
@@ -263,13 +265,21 @@ class ContinuousBatchScheduler:
     the host and cannot be captured). The first step at a batch size runs
     eagerly and is then captured; later ones copy their token ids and
     positions into the graph's inputs and replay it. Row moves and page
-    reservation stay outside the graph."""
+    reservation stay outside the graph.
+
+    drafter (a TreeDrafter) makes decode steps speculative: each request's
+    last token and the drafter's proposals form a tree whose nodes run through
+    the model together (attn_in sees their positions), the accepted path's
+    tokens and the one after it are emitted, and the other nodes' rows are
+    dropped. The tokens are those of one-by-one greedy decoding, up to the
+    rounding of a differently batched pass; a step's accepted_tokens lists
+    them (emitted_tokens has the last). Not together with capture_decode."""
 
     def __init__(self, model, cache=None, max_batch_size: int = 8,
                  prefix_index: Optional[PrefixPageIndex] = None, eos_token_id: Optional[int] = None,
                  attn_scale: Optional[float] = None, *, max_context: int = 4096, max_pages: Optional[int] = None,
                  device=None, compute_dtype: torch.dtype = torch.float64, keep_finished_cached: bool = False,
-                 capture_decode: bool = False):
+                 capture_decode: bool = False, drafter: Optional[TreeDrafter] = None):
         if isinstance(cache, int) and not isinstance(cache, bool):
             max_batch_size, cache = cache, None  # ContinuousBatchScheduler(engine, 4)
         self.engine = None
@@ -305,7 +315,12 @@ class ContinuousBatchScheduler:
         self._dispatch0 = self._dispatch_counts()
         if capture_decode and self.engine is not None:
             raise ValueError("capture_decode needs a model whose decode step is device work only")
+        if capture_decode and drafter is not None:
+            raise ValueError("capture_decode and drafter exclude each other")
         self.capture_decode = bool(capture_decode)
+        self.drafter = drafter
+        self.drafted_tokens = 0   # proposed so far
+        self.accepted_drafts = 0  # of them accepted
         # (batch size, layers) -> (graph, token ids, positions, logits, next ids)
         self._decode_graphs: Dict[tuple, tuple] = {}
 
@@ -482,6 +497,66 @@ class ContinuousBatchScheduler:
             self._emit(req, logits_host[r] if logits_host is not None else logits[r], int(out[r]))
         return out
 
+    def _draft(self, req: BatchRequestState) -> tuple:
+        """(tokens, parents) of a request's tree, its last token the root."""
+        length = self.cache.length(req.request_id)
+        room = min(MAX_TREE_NODES, self.cache.max_blocks * PAGE_TOKENS - length) - 1
+        room = min(room, req.max_new_tokens - len(req.generated_ids) - 1)
+        toks, par = [], []
+        if room > 0:
+            toks, par = self.drafter.propose(req.prompt_ids + req.generated_ids, room)
+            toks, par = [int(t) for t in toks], [int(p) for p in par]
+            if len(toks) != len(par) or len(toks) > room or any(not -1 <= p < i for i, p in enumerate(par)):
+                raise ValueError("a drafter returns at most max_nodes tokens, each with a parent before it")
+        return [req.generated_ids[-1]] + toks, [-1] + [p + 1 for p in par]
+
+    def _decode_tree(self, reqs: List[BatchRequestState], n_layers: int) -> List[List[int]]:
+        """One speculative step: the tokens that each request emits."""
+        cache, B = self.cache, len(reqs)
+        trees = [self._draft(req) for req in reqs]
+        for r, req in enumerate(reqs):
+            cache.move_to_row(req.request_id, r)
+        n = [len(t) for t, _ in trees]
+        mask, depth = tree_mask([p for _, p in trees])
+        first = [req.pos_offset for req, k in zip(reqs, n) for _ in range(k)]
+        meta = to_device([[t for ts, _ in trees for t in ts], [p for _, ps in trees for p in ps],
+                          [a + d for a, d in zip(first, depth.tolist())]], torch.int64, self.device)
+        small = meta[:2].to(torch.int32)
+        mask = to_device(mask, torch.int64, self.device)
+        cu, ctx = cache.begin_tree(n)
+
+        def attend(l, q, k, v):
+            cache.append_tree(l, k, v, cu, ctx)
+            return cache.tree_attention(l, q, cu, ctx, mask, scale=self.attn_scale, out_dtype=torch.float32)
+
+        try:
+            logits = self.model.logits(self._layers(self.model.embed(meta[0]), meta[2], attend, n_layers))
+            path, keep, nxt = cache.pool.verify_tree(logits, small[0], small[1], cu, max_path=max(n))
+            host = torch.cat([path, keep[:, None], nxt[:, None]], dim=1).tolist()
+        except BaseException:
+            none = torch.zeros(B, dtype=torch.int32, device=self.device)
+            cache.commit_tree(none[:, None], none, [0] * B)  # the rows as they were
+            raise
+        cache.commit_tree(path, keep, [h[-2] for h in host])
+        logits_host = logits.cpu().numpy() if self.engine is not None else logits
+        out: List[List[int]] = []
+        at = 0
+        for req, (toks, _), h in zip(reqs, trees, host):
+            nodes, after = h[:h[-2]], h[-1]
+            req.pos_offset += len(nodes)
+            self.drafted_tokens += len(toks) - 1
+            self.accepted_drafts += len(nodes) - 1
+            said = []
+            for i, node in enumerate(nodes):
+                tok = toks[nodes[i + 1]] if i + 1 < len(nodes) else after
+                said.append(int(tok))
+                self._emit(req, logits_host[at + node], int(tok))
+                if req.is_finished:
+                    break
+            out.append(said)
+            at += len(toks)
+        return out
+
     # --------------------------------------------------------------- steps
     def step_batch(self, max_layers: Optional[int] = None) -> Optional[BatchStepResult]:
         """engine/scheduler.py:311-380: admitted requests prefill (here as one
@@ -507,8 +582,14 @@ class ContinuousBatchScheduler:
                 if req.is_finished:
                     completed.append(req.request_id)
         d1 = self._dispatch_counts()
+        accepted = {rid: [tok] for rid, tok in emitted.items()}
         if decode_reqs:
-            toks = self._decode(decode_reqs, n_layers)
+            if self.drafter is not None:
+                said = self._decode_tree(decode_reqs, n_layers)
+                accepted.update((req.request_id, s) for req, s in zip(decode_reqs, said))
+                toks = [s[-1] for s in said]
+            else:
+                toks = self._decode(decode_reqs, n_layers)
             for req, tok in zip(decode_reqs, toks):
                 emitted[req.request_id] = int(tok)
                 if req.is_finished:
@@ -524,7 +605,7 @@ class ContinuousBatchScheduler:
         self.elapsed_ms += ms
         uniq, naive = d2[0] - d1[0], d2[1] - d1[1]  # the decode batch's (engine/scheduler.py:361-366)
         del d0
-        return {
+        res: BatchStepResult = {
             "step_idx": self.step_counter,
             "batch_size": len(active_ids),
             "active_request_ids": active_ids,
@@ -536,6 +617,9 @@ class ContinuousBatchScheduler:
             "expert_dedup_savings_pct": round(100.0 * (1.0 - uniq / max(1, naive)), 2) if naive > 0 else 0.0,
             "step_latency_ms": round(ms, 3),
         }
+        if self.drafter is not None:
+            res["accepted_tokens"] = accepted
+        return res
 
     def run_until_complete(self, max_layers: Optional[int] = None) -> List[BatchStepResult]:
         steps = []

@@ -99,6 +99,9 @@ struct sckv_pool {
   // A third map with one-head, K-or-V boxes (tensor-memory prefill).
   alignas(64) unsigned char tmap_kv2[128];
   int tmap2_ready;
+  // A fourth map with whole 16-bit page-heads in 8-row groups (tree attention).
+  alignas(64) unsigned char tmap_tree[128];
+  int tmap_tree_ready;
 };
 
 // KV-head-sharded output exchange between the ranks of one box (one process

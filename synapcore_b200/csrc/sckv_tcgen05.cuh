@@ -6,6 +6,7 @@
 #include <cuda.h>
 
 #include "sckv_internal.cuh"
+#include "sckv_mma_common.cuh"
 
 namespace sckv_tc {
 
@@ -115,6 +116,86 @@ __device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
 
 __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t cols) {
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
+
+}  // namespace sckv_tc
+
+namespace sckv_tc {
+
+using sckv_mma::pack2;
+
+// 8 query values (dims d..d+7 of one row) as packed f16 / bf16 pairs.
+template <bool kBF16>
+__device__ __forceinline__ uint4 load_q8(const void* q, int64_t idx, int dtype) {
+  if (dtype == (kBF16 ? SCKV_DTYPE_BF16 : SCKV_DTYPE_F16))
+    return *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(q) + idx);
+  float v[8];
+  if (dtype == SCKV_DTYPE_F32) {
+    const float4 a = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(q) + idx);
+    const float4 b = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(q) + idx + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+    // the other 16-bit type: one 16-byte load, converted in registers (the
+    // values are exact in fp32, so the MMA type sees them rounded once)
+    const uint4 raw = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(q) + idx);
+    const uint32_t w4[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (dtype == SCKV_DTYPE_BF16) {
+        v[2 * i] = __uint_as_float(w4[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w4[i] & 0xFFFF0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w4[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+      }
+    }
+  }
+  uint4 r;
+  r.x = pack2<kBF16>(v[0], v[1]);
+  r.y = pack2<kBF16>(v[2], v[3]);
+  r.z = pack2<kBF16>(v[4], v[5]);
+  r.w = pack2<kBF16>(v[6], v[7]);
+  return r;
+}
+
+// sm_100 arithmetic the softmax threads use to save issue slots: a 3-input
+// max, and packed pairs of fp32 values (two independent round-to-nearest
+// fp32 operations per instruction, the same results as two scalar ones).
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t f32x2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void f32x2_split(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// a packed pair times a packed factor, rounded to a 16-bit pair
+template <bool kBF16>
+__device__ __forceinline__ uint32_t mul_pack2(float x, float y, uint64_t f2) {
+  float a, b;
+  f32x2_split(mul_f32x2(f32x2(x, y), f2), a, b);
+  return pack2<kBF16>(a, b);
 }
 
 }  // namespace sckv_tc

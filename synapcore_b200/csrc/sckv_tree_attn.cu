@@ -1,24 +1,117 @@
-// Attention of a tree of drafted tokens over a paged cache.
+// Attention of a tree of drafted tokens over a paged cache, on the
+// 5th-generation tensor cores (tcgen05.mma, accumulators in tensor memory).
 //
 // Node i of sequence b is the query of rows (i, head); its own K/V row sits in
-// slot ctx_lens[b] + i. It sees the sequence's ctx_lens[b] committed tokens and
-// the nodes j whose bit is set in its mask:
+// slot ctx_lens[b] + i. It sees the ctx_lens[b] committed tokens and the nodes
+// j whose bit is set in its mask:
 //
-//   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j - m)
+//   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^(scale_log2 q . k_j - m)
 //
-// One CTA per (node, q head); its four warps take every fourth key with an
-// online softmax each (4 dims a lane) and merge at the end.
+// with a running reference m (one pass over K and V).
+//
+// Work. The rows of a kv head are its (node, q head of the group) pairs. A
+// group of rows is up to 256 of them: one or two 128-row query tiles over
+// the sequence's key tiles of 64 keys (4 pages). The key tiles of all (sequence, kv head,
+// row group) items form one line that the CTAs share out evenly (one
+// persistent CTA per SM), so that few sequences, long ones and ragged batches
+// all keep every SM on HBM. An item that a border cuts leaves unnormalised
+// partials (at most two per CTA) that a second kernel joins.
+//
+// With one query tile (at most 128 rows) the two softmax warpgroups take
+// alternate key tiles, each with its own reference, sum and O accumulator,
+// joined at the end of the item: four S buffers are in flight and a tile has
+// twice its own time for its softmax. With two query tiles each warpgroup owns
+// one and both use every K/V tile.
+//
+// 16 warps (a warp runs on SM sub-partition warp % 4):
+//   warps 0, 2   TMA producers. 16-bit pools: K, V; one 4 KiB box per
+//                page-head, which a rank-5 view of the pool lays out as 8-row
+//                groups [rows 0-7 | 8-15][dims 0-63 | 64-127], so that groups
+//                of consecutive pages have one stride. One-byte pools: pages
+//                0-1, 2-3 of the tile, K and V of a page in one 4 KiB box into
+//                a staging ring, plus the tile's scales (warp 0).
+//   warps 3, 13-15  one-byte pools: decode staged codes into the f16 rings.
+//                int8 codes times their token's fp16 scale (the rounding that
+//                the cache's values have); e4m3 codes exactly, their page's
+//                scales go to the scores (K) and to P (V).
+//   warp 1       one thread issues every MMA and commit.
+//   warps 4-11   softmax, one thread per query row; they also load Q and
+//                write the results.
+//
+// P is held as 2^6 times the weight, so that f16's smallest step is 2^-31 of
+// a weight of 1 (m is stale by at most 2^8: P <= 2^14); e4m3 pages multiply it
+// by their V scale over a reference that has seen the largest one. bf16 pools
+// split P into bf16 hi + lo parts (rounding 2^-16); f16 P rounds by 2^-11 at
+// most, as the 16-bit output does. Sums, references and O are fp32.
+//
+// Rows of K/V tiles past the sequence's last node hold anything: their scores
+// are masked and their V rows zeroed. A node's V that is not finite must not
+// reach rows that do not see it (0 x NaN): such elements are zeroed in the
+// tile and added to the rows that see them at the end.
+#include <cuda.h>
 #include <math.h>
 
 #include "sckv_geo.cuh"
+#include "sckv_mma_common.cuh"
+#include "sckv_tcgen05.cuh"
 
 using namespace sckv_geo;
+using namespace sckv_mma;
+using namespace sckv_tc;
 
 namespace {
 
 constexpr int kHD = 128;
-constexpr int kWarps = 4;
 constexpr int kMaskWordsMax = 4;
+constexpr int kMaxSeqs = 2048;
+constexpr int kRows = 128;                     // rows of a query tile (UMMA M)
+constexpr int kKeys = 64;                      // keys of a K/V tile
+constexpr int kTilePages = kKeys / SCKV_PAGE_TOKENS;
+constexpr int kThreadsTree = 512;
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kColS = 0;                  // S[w][b] at 64 (2 w + b)
+constexpr uint32_t kColO = 256;                // O[w] at 256 + 128 w
+constexpr int kWarpProdA = 0, kWarpMma = 1, kWarpProdB = 2;
+constexpr int kQHalf = kRows * 128;            // one 64-dim half of a query tile: 16 KiB
+constexpr int kQTile = 2 * kQHalf;
+constexpr int kPageTile = 4096;                // one page-head in f16 / bf16
+constexpr int kSlot = kTilePages * kPageTile;  // a K (or V) tile: 16 KiB
+constexpr int kScaleSlots = 16;                // tiles whose scales are kept (more than both rings together)
+constexpr int kMinShare = 2;                   // key tiles a CTA takes at least
+
+template <int KVDT>
+struct TreeCfg {
+  static constexpr bool kFP8 = KVDT == SCKV_DTYPE_FP8_E4M3, kINT8 = KVDT == SCKV_DTYPE_INT8;
+  static constexpr bool kB8 = kFP8 || kINT8;
+  static constexpr bool kBF16 = KVDT == SCKV_DTYPE_BF16;
+  static constexpr int kStages = kB8 ? 3 : 4;         // K and V tiles in the MMA's type
+  static constexpr int kStaging = kB8 ? 3 : 0;        // staged one-byte tiles (K and V)
+  // PV of tile j goes out after S of tile j + kLag (one query tile; 1 with two): at most the spare S buffers, and
+  // below kStages, so that the V tile which shared a slot with tile j was complete before S(j): a softmax warp's
+  // parity wait on v_full then cannot be met by an older phase
+  static constexpr int kLag = kB8 ? 2 : 3;
+  static_assert(kLag < kStages && kLag <= 3, "V slots and S buffers cover the lag");
+  static constexpr int kOffK = 2 * kQTile;
+  static constexpr int kOffV = kOffK + kStages * kSlot;
+  static constexpr int kOffStage = kOffV + kStages * kSlot;
+  static constexpr int kOffScale = kOffStage + kStaging * kSlot;
+  static constexpr int kOffBar = kOffScale + (kB8 ? kScaleSlots * 256 : 0);
+  static constexpr int kNumBars = 4 * kStages + 12 + 4 + 2 * kStaging;
+  static constexpr int kOffMl = kOffBar + ((kNumBars * 8 + 15) / 16) * 16;  // float2 [2][128]: m, l of a row
+  static constexpr int kOffVref = kOffMl + 2 * kRows * 8;                   // float [2]
+  static constexpr int kOffBad = kOffVref + 16;                             // u64 [2][4]: nodes whose V is not finite
+  static constexpr int kOffTmem = kOffBad + 64;
+  static constexpr int kOffAbort = kOffTmem + 4;
+  static constexpr int kOffPartial = kOffTmem + 16;                         // int [kThreadsTree]
+  static constexpr int kOffCum = kOffPartial + kThreadsTree * 4;            // int [n_seqs + 1]
+  static constexpr int kFixedSmem = 1024 + kOffCum + 4;                     // + 4 n_seqs
+  static_assert(kStages + (kB8 ? kStaging : 0) < kScaleSlots, "scale slots outlive their tiles");
+};
+
+// What the joining kernel needs of a CTA whose first item began in an earlier one and ends in it.
+struct JoinHead {
+  int n_parts, c0, slot0, rows, row0, q_base, h, pad;
+};
 
 struct TreeParams {
   Geo g;
@@ -31,99 +124,969 @@ struct TreeParams {
   int64_t bt_stride;
   const unsigned long long* mask;
   int mask_words;
-  int max_blocks, n_seqs, n_tokens, hq;
+  int max_blocks, n_seqs, n_tokens, hq, G;
   int q_dtype, out_dtype;
   float scale_log2;
+  // workspace: JoinHead [grid], then per CTA two slots of float4 [32][part_rows] (O by 4 dims and row)
+  // and float2 [part_rows] (m, l)
+  JoinHead* heads;
+  float* parts;
+  int part_rows;
 };
 
-__device__ __forceinline__ void load_row4(const Geo& g, int layer, int64_t page, int kv, int h, int slot, int lane,
-                                          float (&x)[4]) {
-  const int64_t o = row_off(g, layer, page, kv, h, slot) + 4 * lane;
-  if (g.dtype == SCKV_DTYPE_INT8) {
-    const float s = __half2float(reinterpret_cast<const __half*>(g.scales)[int8_scale_idx(g, layer, page, kv, h, slot)]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      x[i] = __half2float(__float2half_rn((float)reinterpret_cast<const int8_t*>(g.data)[o + i] * s));
-  } else if (g.dtype == SCKV_DTYPE_FP8_E4M3) {
-    const float s = reinterpret_cast<const float*>(g.scales)[fp8_scale_idx(g, layer, page, kv, h)];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = sckv_fp8_to_float(reinterpret_cast<const uint8_t*>(g.data)[o + i]) * s;
+__device__ __forceinline__ int64_t slot_floats(int part_rows) { return (int64_t)part_rows * (kHD + 2); }
+
+// Geometry of one sequence: nodes, committed tokens, key tiles, row groups; false (all zero) if out of range.
+__device__ __forceinline__ bool tree_seq(const TreeParams& p, int s, int& n, int& ctx, int& kt, int& groups) {
+  const int t0 = __ldg(p.cu_q + s), t1 = __ldg(p.cu_q + s + 1);
+  ctx = __ldg(p.ctx_lens + s);
+  const int cap = p.max_blocks * SCKV_PAGE_TOKENS;
+  n = t1 - t0;
+  const bool ok = t0 >= 0 && t1 >= t0 && t1 <= p.n_tokens && n <= 64 * p.mask_words && ctx >= 0 && ctx <= cap - n;
+  if (!ok) n = ctx = 0;
+  kt = n > 0 ? (ctx + n + kKeys - 1) / kKeys : 0;
+  groups = (n * p.G + 2 * kRows - 1) / (2 * kRows);
+  return ok;
+}
+
+// A CTA's walk over its share of the line of key tiles, one item (or part of one) at a time.
+struct TreeWalk {
+  int seq, t, t1;
+};
+struct TreeSeg {
+  int seq, h, n, ctx, L;
+  int kt, ka, nk;         // the item's key tiles; first one here and how many
+  int row0, rows, nq;     // first row of the group, rows of it, query tiles (1 or 2)
+  int q_base, pages;      // first token; pages of the sequence
+};
+
+__device__ __forceinline__ bool tree_next(const TreeParams& p, const int* cum, TreeWalk& w, TreeSeg& s) {
+  if (w.t >= w.t1) return false;
+  while (cum[w.seq + 1] <= w.t) ++w.seq;
+  int groups;
+  tree_seq(p, w.seq, s.n, s.ctx, s.kt, groups);
+  const int rem = w.t - cum[w.seq];
+  const int item = rem / s.kt;
+  s.seq = w.seq;
+  s.ka = rem - item * s.kt;
+  s.nk = min(s.kt - s.ka, w.t1 - w.t);
+  s.h = item / groups;
+  s.row0 = (item - s.h * groups) * 2 * kRows;
+  s.rows = min(2 * kRows, s.n * p.G - s.row0);
+  s.nq = s.rows > kRows ? 2 : 1;
+  s.L = s.ctx + s.n;
+  s.pages = (s.L + SCKV_PAGE_TOKENS - 1) / SCKV_PAGE_TOKENS;
+  s.q_base = __ldg(p.cu_q + s.seq);
+  w.t += s.nk;
+  return true;
+}
+
+// The CTA (of n) whose share of `total` tiles holds tile t; shares begin at total * c / n.
+__device__ __forceinline__ int tree_owner(int t, int total, int n) {
+  return (int)((((int64_t)t + 1) * n - 1) / total);
+}
+__device__ __forceinline__ int tree_begin(int c, int total, int n) { return (int)((int64_t)total * c / n); }
+
+// 64 bits from bit `off` of a row's view of keys ctx + i: ones for committed tokens (i < 0), the mask for nodes
+// i < n, zeros after.
+__device__ __forceinline__ unsigned long long tree_window(const unsigned long long* words, int n_words, int n,
+                                                          int off) {
+  if (off <= -64) return ~0ull;
+  auto word = [&](int i) -> unsigned long long {
+    if (i >= n_words || 64 * i >= n) return 0ull;
+    const unsigned long long live = n - 64 * i >= 64 ? ~0ull : (1ull << (n - 64 * i)) - 1;
+    return __ldg(words + i) & live;
+  };
+  if (off < 0) return ((1ull << -off) - 1) | (word(0) << -off);
+  const int i = off >> 6, sh = off & 63;
+  return sh ? (word(i) >> sh) | (word(i + 1) << (64 - sh)) : word(i);
+}
+
+// Element (node's row, dim) of V as the cache stands for it.
+__device__ float tree_v(const Geo& g, int layer, int64_t page, int h, int slot, int d) {
+  const int64_t o = row_off(g, layer, page, 1, h, slot) + d;
+  if (g.dtype == SCKV_DTYPE_INT8)
+    return __half2float(__hmul(__float2half_rn((float)reinterpret_cast<const int8_t*>(g.data)[o]),
+                               reinterpret_cast<const __half*>(g.scales)[int8_scale_idx(g, layer, page, 1, h, slot)]));
+  if (g.dtype == SCKV_DTYPE_FP8_E4M3)
+    return sckv_fp8_to_float(reinterpret_cast<const uint8_t*>(g.data)[o]) *
+           reinterpret_cast<const float*>(g.scales)[fp8_scale_idx(g, layer, page, 1, h)];
+  return sckv_load_as_float(g.data, o, g.dtype);
+}
+
+__device__ __forceinline__ void tree_store4(void* dst, int64_t idx, int dtype, float a, float b, float c, float d) {
+  if (dtype == SCKV_DTYPE_F32) {
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(dst) + idx) = make_float4(a, b, c, d);
   } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = sckv_load_as_float(g.data, o + i, g.dtype);
+    const uint2 v = dtype == SCKV_DTYPE_BF16 ? make_uint2(pack2<true>(a, b), pack2<true>(c, d))
+                                             : make_uint2(pack2<false>(a, b), pack2<false>(c, d));
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(dst) + idx) = v;
   }
 }
 
-__global__ void __launch_bounds__(kWarps * 32) tree_attn_simple_kernel(const TreeParams p) {
-  const int t = blockIdx.x / p.hq, head = blockIdx.x - t * p.hq;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (t < __ldg(p.cu_q) || t >= __ldg(p.cu_q + p.n_seqs)) return;
-  const int b = sckv_find_seq(p.cu_q, p.n_seqs, t);
-  const int t0 = __ldg(p.cu_q + b), n = __ldg(p.cu_q + b + 1) - t0, ctx = __ldg(p.ctx_lens + b);
-  const int cap = p.max_blocks * SCKV_PAGE_TOKENS;
-  if (t0 < 0 || ctx < 0 || n < 0 || t0 + n > p.n_tokens || n > 64 * p.mask_words || ctx > cap - n) {
-    if (threadIdx.x == 0) sckv_report(p.g.status, SCKV_ERR_BOUNDS, b, KID_TREE_ATTN);
-    return;
-  }
-  const int h = head / (p.hq / p.g.H);
-  float q[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
-  const int64_t row = ((int64_t)t * p.hq + head) * kHD;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) q[i] = sckv_load_as_float(p.q, row + 4 * lane + i, p.q_dtype) * p.scale_log2;
-  float m = -INFINITY, l = 0.f;
-  const int32_t* bt = p.bt + (int64_t)b * p.bt_stride;
-  for (int k = warp; k < ctx + n; k += kWarps) {
-    if (k >= ctx) {
-      const int j = k - ctx;
-      if (!((p.mask[(int64_t)t * p.mask_words + (j >> 6)] >> (j & 63)) & 1)) continue;
+template <int KVDT>
+__global__ void __launch_bounds__(kThreadsTree, 1)
+    tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap tmap) {
+  using C = TreeCfg<KVDT>;
+  constexpr bool kBF16 = C::kBF16;
+  constexpr int kStages = C::kStages;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + C::kOffBar);
+  uint64_t* k_full = bars;                   // [S] K tile in shared memory
+  uint64_t* k_empty = k_full + kStages;      // [S] the S products that read it finished (commit)
+  uint64_t* v_full = k_empty + kStages;      // [S] V tile in shared memory
+  uint64_t* v_empty = v_full + kStages;      // [S] the PV products that read it finished (commit)
+  uint64_t* s_full = v_empty + kStages;      // [w][2] S in tensor memory (commit)
+  uint64_t* p_full = s_full + 4;             // [w][2] P in tensor memory, V tile fixed (one arrival per warp)
+  uint64_t* pv_done = p_full + 4;            // [w][2] PV finished (commit)
+  uint64_t* o_empty = pv_done + 4;           // the item's O was read (one arrival per softmax warp)
+  uint64_t* q_full = o_empty + 1;            // the item's Q is in shared memory (one arrival per softmax warp)
+  uint64_t* mma_done = q_full + 1;           // every issued MMA finished
+  uint64_t* o_full = mma_done + 1;           // the item's sums are written and its O is complete (one arrival per softmax warp)
+  uint64_t* st_full = o_full + 1;            // one-byte pools: [SS] staged tile landed, its scales are written
+  uint64_t* st_empty = st_full + C::kStaging;  // [SS] decoded (one arrival per decoding warp)
+  float2* s_ml = reinterpret_cast<float2*>(base + C::kOffMl);
+  float* s_vref = reinterpret_cast<float*>(base + C::kOffVref);
+  unsigned long long* s_bad = reinterpret_cast<unsigned long long*>(base + C::kOffBad);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + C::kOffTmem);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(base + C::kOffAbort);
+  int* partial = reinterpret_cast<int*>(base + C::kOffPartial);
+  int* cum = reinterpret_cast<int*>(base + C::kOffCum);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  pdl_trigger();
+  // ---- key tiles per sequence, prefix-summed by the whole CTA
+  {
+    const int per = (p.n_seqs + kThreadsTree - 1) / kThreadsTree;
+    const int s0 = min(p.n_seqs, (int)threadIdx.x * per), s1 = min(p.n_seqs, s0 + per);
+    int local = 0, n, ctx, kt, groups;
+    for (int s = s0; s < s1; ++s) {
+      if (!tree_seq(p, s, n, ctx, kt, groups) && blockIdx.x == 0)
+        sckv_report(p.g.status, SCKV_ERR_BOUNDS, s, KID_TREE_ATTN);
+      local += kt * groups * p.g.H;
     }
-    int32_t page = __ldg(bt + k / SCKV_PAGE_TOKENS);
-    if (page < 0 || page >= p.g.P) {
-      if (lane == 0) sckv_report(p.g.status, SCKV_ERR_BOUNDS, page, KID_TREE_ATTN);
-      page = 0;
+    // inclusive scan within each warp, then over the warps
+    int x = local;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
     }
-    float x[4];
-    load_row4(p.g, p.layer, page, 0, h, k % SCKV_PAGE_TOKENS, lane, x);
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s = fmaf(q[i], x[i], s);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const float mn = fmaxf(m, s);
-    const float alpha = exp2f(m - mn), w = exp2f(s - mn);
-    m = mn;
-    l = fmaf(l, alpha, w);
-    load_row4(p.g, p.layer, page, 1, h, k % SCKV_PAGE_TOKENS, lane, x);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = fmaf(acc[i], alpha, w * x[i]);
+    if (lane == 31) partial[warp] = x;
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < C::kNumBars; ++i) {
+        uint64_t* bar = &bars[i];
+        uint32_t count = 1;
+        if (C::kB8 && ((bar >= k_full && bar < k_full + kStages) || (bar >= v_full && bar < v_full + kStages))) count = 2;
+        if (bar >= p_full && bar < p_full + 4) count = 4;
+        if (bar == o_empty || bar == q_full || bar == o_full) count = 8;
+        if (C::kB8 && bar >= st_full && bar < st_full + C::kStaging) count = 2;
+        if (C::kB8 && bar >= st_empty && bar < st_empty + C::kStaging) count = 4;
+        mbar_init(bar, count);
+      }
+      for (int i = 0; i < 2 * kMaskWordsMax; ++i) s_bad[i] = 0;
+      *abort_flag = 0;
+      fence_mbar_init();
+    }
+    if (warp == kWarpMma) tmem_alloc(tmem_slot, kTmemCols);
+    __syncthreads();
+    int before = 0;
+    for (int i = 0; i < warp; ++i) before += partial[i];
+    int run = before + x - local;
+    for (int s = s0; s < s1; ++s) {
+      cum[s] = run;
+      tree_seq(p, s, n, ctx, kt, groups);
+      run += kt * groups * p.g.H;
+    }
+    if (threadIdx.x == kThreadsTree - 1) cum[p.n_seqs] = before + x;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
   }
-  __shared__ float s_acc[kWarps][kHD], s_m[kWarps], s_l[kWarps];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) s_acc[warp][4 * lane + i] = acc[i];
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
+  const uint32_t tmem = *tmem_slot;
+  const int total = cum[p.n_seqs];
+  // CTAs that take a share: no fewer than kMinShare tiles each
+  const int n_cta = max(1, min((int)gridDim.x, total / kMinShare));
+  TreeWalk walk{0, 0, 0};
+  if ((int)blockIdx.x < n_cta && total > 0) {
+    walk.t = tree_begin(blockIdx.x, total, n_cta);
+    walk.t1 = tree_begin(blockIdx.x + 1, total, n_cta);
+    int lo = 0, hi = p.n_seqs - 1;
+    while (lo < hi) {  // the last sequence that begins at or before t
+      const int mid = (lo + hi + 1) >> 1;
+      if (cum[mid] <= walk.t) lo = mid; else hi = mid - 1;
+    }
+    walk.seq = lo;
   }
+  if (threadIdx.x == 0) {
+    JoinHead hd{};
+    TreeWalk w = walk;
+    TreeSeg s;
+    if (tree_next(p, cum, w, s) && s.ka > 0 && s.ka + s.nk == s.kt) {
+      const int first = walk.t - s.ka;  // the item's first tile
+      hd.c0 = tree_owner(first, total, n_cta);
+      hd.slot0 = tree_begin(hd.c0, total, n_cta) == first ? 0 : 1;
+      hd.n_parts = (int)blockIdx.x - hd.c0 + 1;
+      hd.rows = s.rows;
+      hd.row0 = s.row0;
+      hd.q_base = s.q_base;
+      hd.h = s.h;
+    }
+    p.heads[blockIdx.x] = hd;
+  }
+
+  const int64_t layer_base = (int64_t)p.layer * p.g.P;
+  if (warp == kWarpProdA || warp == kWarpProdB) {
+    // ------------------------------------------------------------ producers
+    const int part = warp == kWarpProdB ? 1 : 0;  // 16-bit: V; one-byte: pages 2, 3
+    if (lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap)) : "memory");
+    TreeSeg s;
+    int g = 0;
+    bool aborted = false;
+    if constexpr (!C::kB8) {
+      if (lane == 0) {
+        uint64_t* fulls = part ? v_full : k_full;
+        uint64_t* empties = part ? v_empty : k_empty;
+        uint8_t* ring = base + (part ? C::kOffV : C::kOffK);
+        while (!aborted && tree_next(p, cum, walk, s)) {
+          const int32_t* bt_row = p.bt + (int64_t)s.seq * p.bt_stride;
+          int ids[kTilePages], nxt[kTilePages];
+          auto fetch = [&](int j, int (&v)[kTilePages]) {
+#pragma unroll
+            for (int i = 0; i < kTilePages; ++i) {
+              const int blk = j * kTilePages + i;
+              v[i] = blk < s.pages ? __ldg(bt_row + blk) : 0;
+            }
+          };
+          fetch(s.ka, nxt);
+          for (int j = s.ka; j < s.ka + s.nk; ++j, ++g) {
+#pragma unroll
+            for (int i = 0; i < kTilePages; ++i) ids[i] = nxt[i];
+            if (j + 1 < s.ka + s.nk) fetch(j + 1, nxt);
+            const int st = g % kStages;
+            if (g >= kStages &&
+                (*abort_flag || !mbar_wait_bounded(&empties[st], ((g / kStages) - 1) & 1, SCKV_WAIT_LIMIT_NS))) {
+              aborted = true;
+              break;
+            }
+            const int np = min(kTilePages, s.pages - j * kTilePages);
+            mbar_arrive_expect_tx(&fulls[st], (uint32_t)np * kPageTile);
+            const uint32_t dst = smem_u32(ring + st * kSlot);
+#pragma unroll
+            for (int i = 0; i < kTilePages; ++i) {
+              if (i >= np) break;
+              int page = ids[i];
+              if (page < 0 || page >= p.g.P) {
+                sckv_report(p.g.status, SCKV_ERR_BOUNDS, page, KID_TREE_ATTN);
+                page = 0;
+              }
+              const int slab = (int)(((layer_base + page) * 2 + part) * p.g.H + s.h);
+              tma_load_5d(dst + i * kPageTile, &tmap, 0, 0, 0, 0, slab, &fulls[st]);
+            }
+          }
+        }
+        // nothing of ours may still be landing when the CTA retires
+        for (int t = g > kStages ? g - kStages : 0; t < g; ++t)
+          mbar_wait_bounded(&fulls[t % kStages], (t / kStages) & 1, SCKV_WAIT_LIMIT_NS);
+      }
+    } else {
+      // scales: FP8 lanes 0-7 one fp32 each (K, V of 4 pages); int8 every lane four tokens' fp16
+      const int skv = C::kFP8 ? (lane >> 2) & 1 : lane >> 4;
+      const int spg = C::kFP8 ? lane & 3 : (lane >> 2) & 3;
+      const bool has_scale = part == 0 && (C::kINT8 || lane < 8);
+      while (!aborted && tree_next(p, cum, walk, s)) {
+        const int32_t* bt_row = p.bt + (int64_t)s.seq * p.bt_stride;
+        const int je = s.ka + s.nk;
+        auto fetch = [&](int blk) -> int {
+          int page = blk < s.pages ? __ldg(bt_row + blk) : -1;
+          return blk < s.pages && (page < 0 || page >= p.g.P) ? 0 : page;
+        };
+        // FP8: a page past the last node scales by 1 (K, masked anyway) and 0 (V)
+        auto load_scale = [&](int page) -> uint2 {
+          uint2 r = make_uint2(C::kFP8 && skv == 0 ? 0x3f800000u : 0u, 0u);
+          if (page < 0) return r;
+          if (C::kFP8) {
+            const float f = __ldg(reinterpret_cast<const float*>(p.g.scales) + ((layer_base + page) * 2 + skv) * p.g.H + s.h);
+            r.x = __float_as_uint(skv == 0 ? fmaxf(f, 1e-30f) : f);  // (never 0: it multiplies masked scores, -inf)
+            if (f != f) r.x = __float_as_uint(f);
+          } else {
+            r = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const __half*>(p.g.scales) +
+                                                     (((layer_base + page) * 2 + skv) * p.g.H + s.h) * 16) + (lane & 3));
+          }
+          return r;
+        };
+        uint2 sc = make_uint2(0u, 0u);
+        int sid = -1;
+        if (has_scale) {
+          sc = load_scale(fetch(s.ka * kTilePages + spg));
+          if (s.nk > 1) sid = fetch((s.ka + 1) * kTilePages + spg);
+        }
+        int nid[2] = {0, 0};
+        auto fetch_ids = [&](int j) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int blk = j * kTilePages + 2 * part + i;
+            nid[i] = blk < s.pages ? __ldg(bt_row + blk) : 0;
+          }
+        };
+        if (lane == 0) fetch_ids(s.ka);
+        for (int j = s.ka; j < je; ++j, ++g) {
+          const int st = g % C::kStaging;
+          const int ab = __shfl_sync(0xffffffffu, *abort_flag, 0);
+          if (g >= C::kStaging && (ab || !warp_wait(&st_empty[st], ((g / C::kStaging) - 1) & 1))) {
+            aborted = true;
+            break;
+          }
+          if (has_scale) {
+            uint8_t* slot = base + C::kOffScale + (g % kScaleSlots) * 256;
+            if (C::kFP8) reinterpret_cast<uint32_t*>(slot)[lane] = sc.x;
+            else reinterpret_cast<uint2*>(slot)[lane] = sc;
+            if (j + 1 < je) {
+              sc = load_scale(sid);
+              if (j + 2 < je) sid = fetch((j + 2) * kTilePages + spg);
+            }
+          }
+          __syncwarp();
+          if (lane == 0) {
+            const int ids[2] = {nid[0], nid[1]};
+            if (j + 1 < je) fetch_ids(j + 1);
+            const int np = max(0, min(2, s.pages - j * kTilePages - 2 * part));
+            mbar_arrive_expect_tx(&st_full[st], (uint32_t)np * 4096u);
+            const uint32_t dst = smem_u32(base + C::kOffStage + st * kSlot + 2 * part * 4096);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              if (i >= np) break;
+              int page = ids[i];
+              if (page < 0 || page >= p.g.P) {
+                sckv_report(p.g.status, SCKV_ERR_BOUNDS, page, KID_TREE_ATTN);
+                page = 0;
+              }
+              tma_load_5d(dst + i * 4096, &tmap, 0, 0, s.h, 0, (int)(layer_base + page), &st_full[st]);
+            }
+          }
+          __syncwarp();
+        }
+      }
+      if (lane == 0)
+        for (int t = g > C::kStaging ? g - C::kStaging : 0; t < g; ++t)
+          mbar_wait_bounded(&st_full[t % C::kStaging], (t / C::kStaging) & 1, SCKV_WAIT_LIMIT_NS);
+    }
+    if (aborted && lane == 0) {
+      if (!*abort_flag) sckv_report(p.g.status, SCKV_ERR_TIMEOUT, blockIdx.x, KID_TREE_ATTN);
+      *abort_flag = 1;
+    }
+  } else if (C::kB8 && (warp == 3 || warp >= 13)) {
+    // ------------------------------------------------------------ decoding of one-byte pages
+    // Warp `role` decodes pages 2 (role & 1), + 1 of K (role < 2) or V. Lane
+    // (quarter, rowbit, c): rows r and r ^ 5 of a quarter's eight lanes keep both the
+    // swizzled 16-byte reads and the two 16-byte writes free of bank conflicts.
+    const int role = warp == 3 ? 0 : warp - 12;
+    const int kv = role >> 1, part = role & 1;
+    uint64_t* fulls = kv ? v_full : k_full;
+    uint64_t* empties = kv ? v_empty : k_empty;
+    uint8_t* ring = base + (kv ? C::kOffV : C::kOffK);
+    const int qt = lane >> 3;
+    const int r8 = (lane & 4) ? qt ^ 5 : qt;  // row of the 8-row group
+    TreeSeg s;
+    int g = 0;
+    bool aborted = false;
+    while (!aborted && tree_next(p, cum, walk, s)) {
+      for (int j = s.ka; j < s.ka + s.nk; ++j, ++g) {
+        const int ss = g % C::kStaging, st = g % kStages;
+        const int ab = __shfl_sync(0xffffffffu, *abort_flag, 0);
+        if (ab || !warp_wait(&st_full[ss], (g / C::kStaging) & 1) ||
+            (g >= kStages && !warp_wait(&empties[st], ((g / kStages) - 1) & 1))) {
+          aborted = true;
+          break;
+        }
+        const int np = max(0, min(2, s.pages - j * kTilePages - 2 * part));
+        const __half* tok = reinterpret_cast<const __half*>(base + C::kOffScale + (g % kScaleSlots) * 256) + kv * 64;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (i >= np) break;
+          const int pg = 2 * part + i;
+          const uint8_t* src = base + C::kOffStage + ss * kSlot + pg * 4096 + kv * 2048;
+          uint8_t* dst = ring + st * kSlot + pg * kPageTile;
+#pragma unroll
+          for (int sub = 0; sub < 2; ++sub) {
+            const int row = sub * 8 + r8;
+            const __half2 s2 = C::kINT8 ? __half2half2(tok[pg * SCKV_PAGE_TOKENS + row]) : __half2half2(__half(1.f));
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const int c8 = half * 4 + (lane & 3);  // 16 codes: dims 16 c8 ..
+              const uint4 w = *reinterpret_cast<const uint4*>(src + row * 128 + ((c8 ^ r8) << 4));
+              const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+              uint32_t o[8];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                cvt_b8x4<KVDT>(ws[e], o[2 * e], o[2 * e + 1]);
+                if (C::kINT8) {
+#pragma unroll
+                  for (int k = 0; k < 2; ++k) {
+                    const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&o[2 * e + k]), s2);
+                    o[2 * e + k] = *reinterpret_cast<const uint32_t*>(&x);
+                  }
+                }
+              }
+              uint8_t* d = dst + sub * 2048 + half * 1024 + r8 * 128;
+              const int c = 2 * (lane & 3);
+              *reinterpret_cast<uint4*>(d + ((c ^ r8) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+              *reinterpret_cast<uint4*>(d + (((c + 1) ^ r8) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+            }
+          }
+        }
+        fence_proxy_async_smem();  // read by the tensor cores
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&fulls[st]);
+          mbar_arrive(&st_empty[ss]);
+        }
+      }
+    }
+    if (aborted && lane == 0) {
+      if (!*abort_flag) sckv_report(p.g.status, SCKV_ERR_TIMEOUT, blockIdx.x, KID_TREE_ATTN);
+      *abort_flag = 1;
+    }
+  } else if (warp == kWarpMma && lane == 0) {
+    // ------------------------------------------------------------ MMA issuer
+    auto wait1 = [&](uint64_t* bar, uint32_t parity) -> bool {
+      return mbar_wait_bounded(bar, parity, SCKV_WAIT_LIMIT_NS);
+    };
+    constexpr uint32_t kIdescS = instr_desc_f16(kBF16, kKeys, false);
+    constexpr uint32_t kIdescPV = instr_desc_f16(kBF16, kHD, true);
+    const uint64_t q_desc0 = smem_desc_sw128(smem_u32(base), 16, 1024);
+    const uint64_t k_desc0 = smem_desc_sw128(smem_u32(base + C::kOffK), 16, 2048);
+    const uint64_t v_desc0 = smem_desc_sw128(smem_u32(base + C::kOffV), 1024, 2048);
+    TreeSeg s;
+    bool ok = true;
+    int gt = 0;              // key tiles of earlier items
+    int gw[2] = {0, 0};      // S tiles of each warpgroup in earlier items
+    for (int k = 0; ok && tree_next(p, cum, walk, s); ++k) {
+      if (*abort_flag || !wait1(q_full, k & 1)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const bool two = s.nq == 2;
+      const int lag = two ? 1 : C::kLag;
+      for (int jj = 0; jj < s.nk + lag; ++jj) {
+        if (jj < s.nk) {
+          const int gj = gt + jj, st = gj % kStages;
+          if (*abort_flag || !wait1(&k_full[st], (gj / kStages) & 1)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t k_desc = desc_advance(k_desc0, (uint32_t)(st * kSlot));
+          const int w0 = two ? 0 : jj & 1;
+          const int i0 = two ? jj : jj >> 1;
+          const uint32_t s0 = tmem + kColS + (uint32_t)((2 * w0 + ((gw[w0] + i0) & 1)) * kKeys);
+          const uint32_t s1 = tmem + kColS + (uint32_t)((2 + ((gw[1] + jj) & 1)) * kKeys);
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks) {
+            const int half = ks >> 2, kk = ks & 3;
+            const uint64_t bdesc = desc_advance(k_desc, (uint32_t)(half * 1024 + kk * 32));
+            umma_ss(s0, desc_advance(q_desc0, (uint32_t)(half * kQHalf + kk * 32)), bdesc, kIdescS, ks > 0);
+            if (two)
+              umma_ss(s1, desc_advance(q_desc0, (uint32_t)(kQTile + half * kQHalf + kk * 32)), bdesc, kIdescS, ks > 0);
+          }
+          umma_commit(&s_full[2 * w0 + ((gw[w0] + i0) & 1)]);
+          if (two) umma_commit(&s_full[2 + ((gw[1] + jj) & 1)]);
+          umma_commit(&k_empty[st]);
+        }
+        const int pj = jj - lag;  // the tile whose PV goes out now
+        if (pj >= 0) {
+          const int gj = gt + pj, st = gj % kStages;
+          const int w0 = two ? 0 : pj & 1;
+          const int i0 = two ? pj : pj >> 1;
+          const int a0 = gw[w0] + i0, a1 = gw[1] + pj;
+          if (!wait1(&v_full[st], (gj / kStages) & 1) || !wait1(&p_full[2 * w0 + (a0 & 1)], (a0 >> 1) & 1) ||
+              (two && !wait1(&p_full[2 + (a1 & 1)], (a1 >> 1) & 1)) ||
+              (i0 == 0 && k > 0 && !wait1(o_empty, (k - 1) & 1))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t v_desc = desc_advance(v_desc0, (uint32_t)(st * kSlot));
+          const uint32_t p0 = tmem + kColS + (uint32_t)((2 * w0 + (a0 & 1)) * kKeys);
+          const uint32_t p1 = tmem + kColS + (uint32_t)((2 + (a1 & 1)) * kKeys);
+          const uint32_t o0 = tmem + kColO + (uint32_t)(w0 * kHD), o1 = tmem + kColO + (uint32_t)kHD;
+#pragma unroll
+          for (int pg = 0; pg < kTilePages; ++pg) {
+            // B = V rows of page pg: 128 dims in two 64-dim halves (LBO), 16 keys in two 8-row groups (SBO)
+            const uint64_t bdesc = desc_advance(v_desc, (uint32_t)(pg * kPageTile));
+            const uint32_t acc = (i0 > 0 || pg > 0) ? 1u : 0u;
+            umma_ts(o0, p0 + (uint32_t)(pg * 8), bdesc, kIdescPV, acc);
+            if (two) umma_ts(o1, p1 + (uint32_t)(pg * 8), bdesc, kIdescPV, acc);
+            if (kBF16) {
+              umma_ts(o0, p0 + (uint32_t)(pg * 8 + 32), bdesc, kIdescPV, 1u);
+              if (two) umma_ts(o1, p1 + (uint32_t)(pg * 8 + 32), bdesc, kIdescPV, 1u);
+            }
+          }
+          umma_commit(&pv_done[2 * w0 + (a0 & 1)]);
+          if (two) umma_commit(&pv_done[2 + (a1 & 1)]);
+          umma_commit(&v_empty[st]);
+        }
+      }
+      if (!ok) break;
+      gt += s.nk;
+      gw[0] += two ? s.nk : (s.nk + 1) >> 1;
+      gw[1] += two ? s.nk : s.nk >> 1;
+    }
+    if (!ok) {
+      if (!*abort_flag) sckv_report(p.g.status, SCKV_ERR_TIMEOUT, blockIdx.x, KID_TREE_ATTN);
+      *abort_flag = 1;
+    }
+    umma_commit(mma_done);  // every MMA above has finished before the tensor memory is released
+    wait1(mma_done, 0);
+  } else if (warp >= 4 && warp < 12) {
+    // ------------------------------------------------------------ softmax, Q, results
+    const int w = (warp - 4) >> 2;     // warpgroup
+    const int quad = warp & 3;         // tensor memory lanes 32 quad ..
+    const int row = quad * 32 + lane;  // query row of the tile = tensor memory lane
+    const int tid = threadIdx.x - 128; // 0 .. 255
+    const uint32_t t_row = tmem + ((uint32_t)(quad * 32) << 16);
+    const uint32_t col_s = kColS + (uint32_t)(2 * w * kKeys);
+    const uint32_t col_o = kColO + (uint32_t)(w * kHD);
+    uint64_t* my_s_full = s_full + 2 * w;
+    uint64_t* my_p_full = p_full + 2 * w;
+    uint64_t* my_pv_done = pv_done + 2 * w;
+    // Q rows of an item into shared memory (128-byte swizzled, K-major): with one
+    // query tile all 256 threads load it, with two each warpgroup its own.
+    // Rows past the last keep what they have: no other row sees it.
+    auto load_q = [&](const TreeSeg& s) {
+      const int n_it = s.nq == 2 ? 16 : 8, step = s.nq == 2 ? 128 : 256;
+      const int t = s.nq == 2 ? tid & 127 : tid;
+      const int tile_row0 = s.nq == 2 ? w * kRows : 0;
+      uint8_t* q_tile = base + (s.nq == 2 ? w * kQTile : 0);
+      const int64_t q0 = (int64_t)s.q_base * p.hq + (int64_t)s.h * p.G;
+#pragma unroll 1
+      for (int b8 = 0; b8 < n_it; b8 += 8) {
+        uint4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int c = t + (b8 + i) * step;
+          const int r = tile_row0 + (c >> 4);
+          if (r < s.rows) {
+            const int rr = s.row0 + r, node = rr / p.G;
+            v[i] = load_q8<kBF16>(p.q, (q0 + (int64_t)node * p.hq + (rr - node * p.G)) * kHD + (c & 15) * 8, p.q_dtype);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int c = t + (b8 + i) * step;
+          const int r = c >> 4, half = (c >> 3) & 1, ch = c & 7;
+          if (tile_row0 + r < s.rows)
+            *reinterpret_cast<uint4*>(q_tile + half * kQHalf + r * 128 + ((ch ^ (r & 7)) << 4)) = v[i];
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    };
+    bool ok = true;
+    int g = 0;   // S tiles of this warpgroup in earlier items
+    int gt = 0;  // key tiles of earlier items
+    TreeSeg s;
+    bool more = tree_next(p, cum, walk, s);
+    if (more) load_q(s);
+    for (int k = 0; ok && more; ++k) {
+      const bool two = s.nq == 2;
+      const int r_in = (two ? w * kRows : 0) + row;  // row of the group
+      const bool valid = r_in < s.rows;
+      const int node = (s.row0 + r_in) / p.G;
+      const int head = s.h * p.G + (s.row0 + r_in) - node * p.G;
+      const unsigned long long* mask = p.mask + (int64_t)(s.q_base + (valid ? node : 0)) * p.mask_words;
+      const bool live = __any_sync(0xffffffffu, valid);
+      const int n = two ? s.nk : (s.nk + 1 - w) >> 1;
+      unsigned long long* bad = s_bad + (k & 1) * kMaskWordsMax;
+      float m = -INFINITY, l = 0.f;
+      float vref = 0.f;  // FP8: the V scale that O counts in
+      for (int i = 0; i < n; ++i) {
+        const int jj = two ? i : 2 * i + w;
+        const int gj = g + i, b = gj & 1;
+        const int st = (gt + jj) % kStages;
+        const int key0 = (s.ka + jj) * kKeys;
+        const bool tail = key0 + kKeys > s.ctx;
+        if (*abort_flag || !warp_wait(&my_s_full[b], (gj >> 1) & 1)) {
+          ok = false;
+          break;
+        }
+        // the V tile of S(g) cannot be replaced before P(g) is written, so this wait is for its own phase
+        if ((tail || C::kFP8) && !warp_wait(&v_full[st], ((gt + jj) / kStages) & 1)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (live) {
+          float sv[kKeys];
+          {
+            uint32_t r0[32], r1[32];
+            tmem_ld32(t_row + col_s + b * kKeys, r0);
+            tmem_ld32(t_row + col_s + b * kKeys + 32, r1);
+            tc_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+              sv[c] = __uint_as_float(r0[c]);
+              sv[32 + c] = __uint_as_float(r1[c]);
+            }
+          }
+          if (tail) {
+            const unsigned long long win = valid ? tree_window(mask, p.mask_words, s.n, key0 - s.ctx) : 0ull;
+#pragma unroll
+            for (int c = 0; c < kKeys; ++c) sv[c] = ((win >> c) & 1) ? sv[c] : -INFINITY;
+          }
+          float ks[kTilePages], vs[kTilePages];
+          if (C::kFP8) {
+            const float4* sc = reinterpret_cast<const float4*>(base + C::kOffScale + ((gt + jj) % kScaleSlots) * 256);
+            const float4 a = sc[0], c = sc[1];
+            ks[0] = a.x * p.scale_log2; ks[1] = a.y * p.scale_log2; ks[2] = a.z * p.scale_log2; ks[3] = a.w * p.scale_log2;
+            vs[0] = c.x; vs[1] = c.y; vs[2] = c.z; vs[3] = c.w;
+          } else {
+#pragma unroll
+            for (int q = 0; q < kTilePages; ++q) ks[q] = p.scale_log2;
+          }
+          // the row's largest score; the scale is positive
+          float pm = -INFINITY;
+          if (C::kFP8) {
+#pragma unroll
+            for (int q = 0; q < kTilePages; ++q) {
+              float x = -INFINITY;
+#pragma unroll
+              for (int c = 0; c < 16; c += 2) x = fmax3(x, sv[16 * q + c], sv[16 * q + c + 1]);
+              pm = fmaxf(pm, x * ks[q]);
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < kKeys; c += 2) pm = fmax3(pm, sv[c], sv[c + 1]);
+            pm *= p.scale_log2;
+          }
+          // stale reference: it moves when a tile exceeds it by more than 2^8
+          float alpha = 1.f;
+          bool rescale = false;
+          if (pm > m + 8.f) {
+            if (m != -INFINITY) {
+              alpha = ex2_approx(m - pm);
+              rescale = true;
+            }
+            m = pm;
+            l *= alpha;
+          }
+          float inv_vref = 0.f;
+          if (C::kFP8) {
+            const float vm = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+            if (vm > vref) {  // (the same for the whole warpgroup) twice the largest: growth below 2 needs no rescale
+              if (vref > 0.f) {
+                alpha *= vref / (2.f * vm);
+                rescale = true;
+              }
+              vref = 2.f * vm;
+            }
+            inv_vref = vref > 0.f ? 1.f / vref : 0.f;
+          }
+          if (__any_sync(0xffffffffu, rescale) && i > 0) {
+            // O holds PV of this item's earlier tiles: wait for the last, then scale this warp's rows
+            if (!warp_wait(&my_pv_done[(gj - 1) & 1], ((gj - 1) >> 1) & 1)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+#pragma unroll 1
+            for (int cc = 0; cc < 4; ++cc) {
+              uint32_t r[32];
+              tmem_ld32(t_row + col_o + cc * 32, r);
+              tc_wait_ld();
+#pragma unroll
+              for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * alpha);
+              tmem_st32(t_row + col_o + cc * 32, r);
+            }
+            tc_wait_st();
+          }
+          {
+            uint32_t ph[32], plo[32];
+            // 2^6 times the weight; a row that sees no key yet (m = -inf) has every score -inf: 2^-inf = 0
+            const float mm = (m == -INFINITY) ? 0.f : m - 6.f;
+            const uint64_t negm2 = f32x2(-mm, -mm);
+            const uint64_t minus1 = f32x2(-1.f, -1.f);
+            uint64_t ls2 = f32x2(0.f, 0.f);
+#pragma unroll
+            for (int q = 0; q < kTilePages; ++q) {
+              const uint64_t scale2 = f32x2(ks[q], ks[q]);
+              uint64_t v2 = 0;
+              if (C::kFP8) v2 = f32x2(vs[q] * inv_vref, vs[q] * inv_vref);
+#pragma unroll
+              for (int c = 8 * q; c < 8 * q + 8; ++c) {
+                float x0, x1;
+                f32x2_split(fma_f32x2(f32x2(sv[2 * c], sv[2 * c + 1]), scale2, negm2), x0, x1);
+                const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+                ls2 = add_f32x2(ls2, f32x2(p0, p1));
+                ph[c] = C::kFP8 ? mul_pack2<false>(p0, p1, v2) : pack2<kBF16>(p0, p1);
+                if (kBF16) {
+                  // lo = p - bf16(p), exact
+                  const uint64_t hi2 = f32x2(__uint_as_float(ph[c] << 16), __uint_as_float(ph[c] & 0xFFFF0000u));
+                  float l0, l1;
+                  f32x2_split(fma_f32x2(hi2, minus1, f32x2(p0, p1)), l0, l1);
+                  plo[c] = pack2<true>(l0, l1);
+                }
+              }
+            }
+            float ls0, ls1;
+            f32x2_split(ls2, ls0, ls1);
+            tmem_st32(t_row + col_s + b * kKeys, ph);
+            if (kBF16) tmem_st32(t_row + col_s + b * kKeys + 32, plo);
+            l += ls0 + ls1;
+            tc_wait_st();
+          }
+        }
+        if (tail && (!two || w == 0)) {
+          // V rows past the last node become 0, and so does what is not finite in a node's row (noted)
+          uint8_t* vt = base + C::kOffV + st * kSlot;
+          const int r0 = max(0, s.ctx - key0);
+          for (int c = row; c < (kKeys - r0) * 16; c += 128) {
+            const int r = r0 + (c >> 4), ch = c & 15;
+            const int key = key0 + r;
+            uint4* cell = reinterpret_cast<uint4*>(vt + (r >> 4) * kPageTile + ((r >> 3) & 1) * 2048 + (ch >> 3) * 1024 +
+                                                   (r & 7) * 128 + (((ch & 7) ^ (r & 7)) << 4));
+            if (key >= s.L) {
+              *cell = make_uint4(0u, 0u, 0u, 0u);
+            } else {
+              constexpr uint32_t kExp = kBF16 ? 0x7F80u : 0x7C00u;
+              uint4 x = *cell;
+              uint32_t* xs = &x.x;
+              bool hit = false;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if ((xs[e] & kExp) == kExp) { xs[e] &= 0xFFFF0000u; hit = true; }
+                if ((xs[e] & (kExp << 16)) == (kExp << 16)) { xs[e] &= 0x0000FFFFu; hit = true; }
+              }
+              if (hit) {
+                *cell = x;
+                atomicOr(bad + ((key - s.ctx) >> 6), 1ull << ((key - s.ctx) & 63));
+              }
+            }
+          }
+          fence_proxy_async_smem();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&my_p_full[b]);
+      }
+      if (!ok) break;
+      // ---- the item's result, once this warpgroup's last PV finished
+      const int glast = g + n - 1;
+      if (n > 0 && !warp_wait(&my_pv_done[glast & 1], (glast >> 1) & 1)) {
+        ok = false;
+        break;
+      }
+      // (idle warps of a half-empty tile have the same reference V scale as the others: rows they hold are not written)
+      s_ml[w * kRows + row] = make_float2(m, l);
+      if (row == 0) s_vref[w] = C::kFP8 ? vref : 1.f;
+      // both warpgroups' O are complete and every S product has finished (a bounded wait, not a named barrier: a
+      // warp that gave up must not leave the others waiting)
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(o_full);
+      if (!warp_wait(o_full, k & 1)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      // one query tile: O[0] and O[1] join, warpgroup w writes dims 64 w ..; two: its own rows
+      const bool join = !two && s.nk > 1;
+      float f0, f1 = 0.f, M, Lsum;
+      if (two) {
+        M = m;
+        Lsum = l;
+        f0 = C::kFP8 ? vref : 1.f;
+      } else {
+        const float2 a = s_ml[row], c = join ? s_ml[kRows + row] : make_float2(-INFINITY, 0.f);
+        M = fmaxf(a.x, c.x);
+        const float e0 = a.x == -INFINITY ? 1.f : ex2_approx(a.x - M);
+        const float e1 = c.x == -INFINITY ? 1.f : ex2_approx(c.x - M);
+        Lsum = a.y * e0 + (join ? c.y * e1 : 0.f);
+        f0 = e0 * s_vref[0];
+        f1 = join ? e1 * s_vref[1] : 0.f;
+      }
+      const bool full = s.nk == s.kt;
+      if (full) {
+        const float inv = Lsum == 0.f ? 0.f : 1.f / Lsum;  // no key seen: zeros; NaN stays NaN
+        f0 *= inv;
+        f1 *= inv;
+      }
+      const int d0 = two ? 0 : 64 * w, nd = two ? kHD : 64;
+      const int64_t obase = ((int64_t)(s.q_base + node) * p.hq + head) * kHD;
+      float* part = p.parts + (int64_t)(2 * blockIdx.x + (k > 0 ? 1 : 0)) * slot_floats(p.part_rows);
+      if (live) {
+#pragma unroll 1
+        for (int cc = 0; cc < nd; cc += 32) {
+          uint32_t r[32], r1[32];
+          tmem_ld32(t_row + kColO + (two ? w * kHD : 0) + d0 + cc, r);
+          if (join) tmem_ld32(t_row + kColO + kHD + d0 + cc, r1);
+          tc_wait_ld();
+          if (valid) {
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+              float x[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                x[e] = __uint_as_float(r[c + e]) * f0;
+                if (join) x[e] = fmaf(__uint_as_float(r1[c + e]), f1, x[e]);
+              }
+              if (full)
+                tree_store4(p.out, obase + d0 + cc + c, p.out_dtype, x[0], x[1], x[2], x[3]);
+              else
+                reinterpret_cast<float4*>(part)[(int64_t)((d0 + cc + c) >> 2) * p.part_rows + r_in] =
+                    make_float4(x[0], x[1], x[2], x[3]);
+            }
+          }
+          __syncwarp();
+        }
+        if (!full && valid && (two || w == 0))
+          reinterpret_cast<float2*>(part + (int64_t)p.part_rows * kHD)[r_in] = make_float2(M, Lsum);
+        // what is not finite in the V of nodes this row sees
+        if (valid) {
+#pragma unroll 1
+          for (int wd = 0; wd < p.mask_words; ++wd) {
+            unsigned long long hit = bad[wd];
+            if (hit) hit &= tree_window(mask, p.mask_words, s.n, 64 * wd);
+#pragma unroll 1
+            for (; hit; hit &= hit - 1) {
+              const int pos = s.ctx + 64 * wd + __ffsll((long long)hit) - 1;
+              int page = __ldg(p.bt + (int64_t)s.seq * p.bt_stride + pos / SCKV_PAGE_TOKENS);
+              if (page < 0 || page >= p.g.P) page = 0;
+#pragma unroll 1
+              for (int d = d0; d < d0 + nd; ++d) {
+                const float v = tree_v(p.g, p.layer, page, s.h, pos % SCKV_PAGE_TOKENS, d);
+                if (isfinite(v)) continue;
+                if (full) {
+                  sckv_store_from_float(p.out, obase + d, p.out_dtype,
+                                        sckv_load_as_float(p.out, obase + d, p.out_dtype) + v);
+                } else {
+                  part[((int64_t)(d >> 2) * p.part_rows + r_in) * 4 + (d & 3)] += v;
+                }
+              }
+            }
+          }
+        }
+      }
+      // the other flags were last read in the item before and are next set in the one after
+      if (tid < kMaskWordsMax) s_bad[((k + 1) & 1) * kMaskWordsMax + tid] = 0;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(o_empty);
+      g += n;
+      gt += s.nk;
+      more = tree_next(p, cum, walk, s);
+      if (more) load_q(s);
+    }
+    if (!ok) {
+      if (lane == 0 && !*abort_flag) sckv_report(p.g.status, SCKV_ERR_TIMEOUT, blockIdx.x, KID_TREE_ATTN);
+      if (lane == 0) *abort_flag = 1;
+    }
+  }
+  if (warp == kWarpMma) __syncwarp();
+  tc_fence_before();
   __syncthreads();
-  const int d = threadIdx.x;
-  float M = -INFINITY, L = 0.f, O = 0.f;
-  for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w]);
-  for (int w = 0; w < kWarps; ++w) {
-    if (s_m[w] == -INFINITY) continue;
-    const float e = exp2f(s_m[w] - M);
-    L = fmaf(s_l[w], e, L);
-    O = fmaf(s_acc[w][d], e, O);
+  if (warp == kWarpMma) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
   }
-  sckv_store_from_float(p.out, row + d, p.out_dtype, L == 0.f ? 0.f : O / L)  /* NaN stays NaN */;
+}
+
+// Joins the partials of items that CTA borders cut: block (c, 32 rows) takes
+// the item that ends in CTA c's first segment, thread (row, 16 dims).
+__global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
+  pdl_wait();
+  const JoinHead hd = p.heads[blockIdx.x];
+  const int r = blockIdx.y * 32 + (threadIdx.x & 31), dg = threadIdx.x >> 5;
+  if (r >= hd.rows || hd.n_parts == 0) return;
+  auto slot = [&](int i) { return p.parts + (int64_t)(2 * (hd.c0 + i) + (i == 0 ? hd.slot0 : 0)) * slot_floats(p.part_rows); };
+  auto ml = [&](int i) { return reinterpret_cast<const float2*>(slot(i) + (int64_t)p.part_rows * kHD)[r]; };
+  float M = -INFINITY;
+  for (int i = 0; i < hd.n_parts; ++i) M = fmaxf(M, ml(i).x);
+  float L = 0.f, x[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) x[e] = 0.f;
+  for (int i = 0; i < hd.n_parts; ++i) {
+    const float2 a = ml(i);
+    const float f = a.x == -INFINITY ? 1.f : ex2_approx(a.x - M);
+    L = fmaf(a.y, f, L);
+    const float4* o = reinterpret_cast<const float4*>(slot(i));
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float4 v = o[(int64_t)(4 * dg + c) * p.part_rows + r];
+      x[4 * c] = fmaf(v.x, f, x[4 * c]);
+      x[4 * c + 1] = fmaf(v.y, f, x[4 * c + 1]);
+      x[4 * c + 2] = fmaf(v.z, f, x[4 * c + 2]);
+      x[4 * c + 3] = fmaf(v.w, f, x[4 * c + 3]);
+    }
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const int rr = hd.row0 + r, node = rr / p.G;
+  const int64_t o = ((int64_t)(hd.q_base + node) * p.hq + hd.h * p.G + (rr - node * p.G)) * kHD + 16 * dg;
+#pragma unroll
+  for (int c = 0; c < 16; c += 4)
+    tree_store4(p.out, o + c, p.out_dtype, x[c] * inv, x[c + 1] * inv, x[c + 2] * inv, x[c + 3] * inv);
+}
+
+// Rank-5 view of a 16-bit pool whose boxes are whole page-heads in 8-row
+// groups: dims {64 of the head dim, 8 tokens, 2 halves of the head dim, 2
+// groups of tokens, (slab, K|V, head)}, 128-byte swizzle.
+int ensure_tree_tmap(sckv_pool* p) {
+  if (p->tmap_tree_ready) return SCKV_OK;
+  PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
+  if (encode == nullptr)
+    return sckv_record_error(__FILE__, __LINE__, "cudaGetDriverEntryPoint", "cuTensorMapEncodeTiled not found");
+  const cuuint64_t dims[5] = {64, 8, 2, 2, (cuuint64_t)p->num_layers * (cuuint64_t)p->max_pages * 2 * p->num_kv_heads};
+  const cuuint64_t strides[4] = {256, 128, 2048, 4096};
+  const cuuint32_t box[5] = {64, 8, 2, 2, 1};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  const CUresult r = encode(reinterpret_cast<CUtensorMap*>(p->tmap_tree), CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, p->data, dims,
+                            strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    char what[64];
+    snprintf(what, sizeof what, "CUresult %d", (int)r);
+    return sckv_record_error(__FILE__, __LINE__, "cuTensorMapEncodeTiled", what);
+  }
+  p->tmap_tree_ready = 1;
+  return SCKV_OK;
+}
+
+// Rows of a partial slot: a group's rows, at most.
+int tree_part_rows(int n_tokens, int mask_words, int G) {
+  const int64_t rows = (int64_t)(n_tokens < 64 * mask_words ? n_tokens : 64 * mask_words) * G;
+  return rows > kRows ? 2 * kRows : kRows;
+}
+
+size_t tree_head_bytes(const sckv_pool* p) { return ((size_t)p->num_sms * sizeof(JoinHead) + 255) / 256 * 256; }
+
+template <int KVDT>
+int launch_tree(sckv_pool* p, const TreeParams& t, cudaStream_t stream) {
+  using C = TreeCfg<KVDT>;
+  const int rc = C::kB8 ? ensure_tmap(p, 1, p->tmap_kv1, &p->tmap1_ready) : ensure_tree_tmap(p);
+  if (rc != SCKV_OK) return rc;
+  const CUtensorMap* map = reinterpret_cast<const CUtensorMap*>(C::kB8 ? p->tmap_kv1 : p->tmap_tree);
+  auto kern = tree_attn_kernel<KVDT>;
+  const int smem = C::kFixedSmem + 4 * t.n_seqs;
+  static_assert(C::kFixedSmem + 4 * kMaxSeqs <= 227 * 1024, "shared memory of the largest batch");
+  SCKV_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  kern<<<p->num_sms, kThreadsTree, smem, stream>>>(t, *map);
+  SCKV_LAUNCH_CHECK();
+  SCKV_CUDA_CHECK(sckv_launch_pdl(tree_join_kernel, dim3(p->num_sms, t.part_rows / 32), dim3(256), 0, stream, t));
+  SCKV_LAUNCH_CHECK();
+  return SCKV_OK;
 }
 
 }  // namespace
 
 extern "C" size_t sckv_tree_attn_workspace_bytes(const sckv_pool* p, int n_tokens, int num_q_heads) {
-  (void)p;
-  (void)n_tokens;
-  (void)num_q_heads;
-  return 0;
+  if (p == nullptr || n_tokens <= 0 || num_q_heads <= 0) return 0;
+  const int rows = tree_part_rows(n_tokens, kMaskWordsMax, num_q_heads / p->num_kv_heads);
+  return tree_head_bytes(p) + (size_t)p->num_sms * 2 * rows * (kHD + 2) * sizeof(float);
 }
 
 extern "C" int sckv_tree_attn(sckv_pool* p, int layer, const void* q, int q_dtype, int num_q_heads, int n_seqs,
@@ -143,8 +1106,15 @@ extern "C" int sckv_tree_attn(sckv_pool* p, int layer, const void* q, int q_dtyp
     return SCKV_ERR_INVALID_ARG;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15)
     return SCKV_ERR_ALIGNMENT;
-  const size_t need = sckv_tree_attn_workspace_bytes(p, n_tokens, num_q_heads);
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return SCKV_ERR_INVALID_ARG;
+  if (workspace == nullptr || workspace_bytes < sckv_tree_attn_workspace_bytes(p, n_tokens, num_q_heads))
+    return SCKV_ERR_INVALID_ARG;
+  const int G = num_q_heads / p->num_kv_heads;
+  // tile and box numbers are 32-bit
+  const int64_t groups = ((int64_t)(n_tokens < 64 * mask_words ? n_tokens : 64 * mask_words) * G + 2 * kRows - 1) / (2 * kRows);
+  if (n_seqs > kMaxSeqs || max_blocks > INT32_MAX / SCKV_PAGE_TOKENS ||
+      (int64_t)n_seqs * (max_blocks / kTilePages + 1) * groups * p->num_kv_heads > INT32_MAX ||
+      (int64_t)p->num_layers * p->max_pages * 2 * p->num_kv_heads > INT32_MAX)
+    return SCKV_ERR_UNSUPPORTED;
   TreeParams t{};
   t.g = geo_of(p);
   t.layer = layer;
@@ -160,13 +1130,20 @@ extern "C" int sckv_tree_attn(sckv_pool* p, int layer, const void* q, int q_dtyp
   t.n_seqs = n_seqs;
   t.n_tokens = n_tokens;
   t.hq = num_q_heads;
+  t.G = G;
   t.q_dtype = q_dtype;
   t.out_dtype = out_dtype;
   t.scale_log2 = scale * 1.4426950408889634f;
-  const int64_t blocks = (int64_t)n_tokens * num_q_heads;
-  if (blocks > INT32_MAX) return SCKV_ERR_INVALID_ARG;
+  t.heads = reinterpret_cast<JoinHead*>(workspace);
+  t.parts = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + tree_head_bytes(p));
+  t.part_rows = tree_part_rows(n_tokens, mask_words, G);
   SCKV_DEVICE_GUARD(p->device);
-  tree_attn_simple_kernel<<<(unsigned)blocks, kWarps * 32, 0, as_stream(stream)>>>(t);
-  SCKV_LAUNCH_CHECK();
-  return SCKV_OK;
+  cudaStream_t s = as_stream(stream);
+  switch (p->kv_dtype) {
+    case SCKV_DTYPE_F16: return launch_tree<SCKV_DTYPE_F16>(p, t, s);
+    case SCKV_DTYPE_BF16: return launch_tree<SCKV_DTYPE_BF16>(p, t, s);
+    case SCKV_DTYPE_INT8: return launch_tree<SCKV_DTYPE_INT8>(p, t, s);
+    case SCKV_DTYPE_FP8_E4M3: return launch_tree<SCKV_DTYPE_FP8_E4M3>(p, t, s);
+    default: return SCKV_ERR_UNSUPPORTED;
+  }
 }

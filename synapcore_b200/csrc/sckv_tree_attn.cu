@@ -224,6 +224,20 @@ __device__ __forceinline__ void tree_store4(void* dst, int64_t idx, int dtype, f
   }
 }
 
+// Every lane of the warp waits; the result is the same on all lanes.
+__device__ __forceinline__ bool warp_wait_polled(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait_polled(bar, parity, SCKV_WAIT_LIMIT_NS));
+}
+
+// 1 on one lane of the (converged) warp.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ void reg_give() { asm volatile("setmaxnreg.dec.sync.aligned.u32 80;"); }
+
 template <int KVDT>
 __global__ void __launch_bounds__(kThreadsTree, 1)
     tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap tmap) {
@@ -339,8 +353,12 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
   }
 
   const int64_t layer_base = (int64_t)p.layer * p.g.P;
+  // Registers: 128 a thread at launch; the softmax warpgroups take 176 for a row's 64 scores and their P, the two
+  // others give theirs up (256 x 80 + 256 x 176 = 512 x 128). Each role does it in its own branch, so that the
+  // compiler knows the count of every region.
   if (warp == kWarpProdA || warp == kWarpProdB) {
     // ------------------------------------------------------------ producers
+    reg_give();
     const int part = warp == kWarpProdB ? 1 : 0;  // 16-bit: V; one-byte: pages 2, 3
     if (lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap)) : "memory");
     TreeSeg s;
@@ -368,7 +386,7 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
             if (j + 1 < s.ka + s.nk) fetch(j + 1, nxt);
             const int st = g % kStages;
             if (g >= kStages &&
-                (*abort_flag || !mbar_wait_bounded(&empties[st], ((g / kStages) - 1) & 1, SCKV_WAIT_LIMIT_NS))) {
+                (*abort_flag || !mbar_wait_polled(&empties[st], ((g / kStages) - 1) & 1, SCKV_WAIT_LIMIT_NS))) {
               aborted = true;
               break;
             }
@@ -390,7 +408,7 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
         }
         // nothing of ours may still be landing when the CTA retires
         for (int t = g > kStages ? g - kStages : 0; t < g; ++t)
-          mbar_wait_bounded(&fulls[t % kStages], (t / kStages) & 1, SCKV_WAIT_LIMIT_NS);
+          mbar_wait_polled(&fulls[t % kStages], (t / kStages) & 1, SCKV_WAIT_LIMIT_NS);
       }
     } else {
       // scales: FP8 lanes 0-7 one fp32 each (K, V of 4 pages); int8 every lane four tokens' fp16
@@ -436,7 +454,7 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
         for (int j = s.ka; j < je; ++j, ++g) {
           const int st = g % C::kStaging;
           const int ab = __shfl_sync(0xffffffffu, *abort_flag, 0);
-          if (g >= C::kStaging && (ab || !warp_wait(&st_empty[st], ((g / C::kStaging) - 1) & 1))) {
+          if (g >= C::kStaging && (ab || !warp_wait_polled(&st_empty[st], ((g / C::kStaging) - 1) & 1))) {
             aborted = true;
             break;
           }
@@ -472,7 +490,7 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
       }
       if (lane == 0)
         for (int t = g > C::kStaging ? g - C::kStaging : 0; t < g; ++t)
-          mbar_wait_bounded(&st_full[t % C::kStaging], (t / C::kStaging) & 1, SCKV_WAIT_LIMIT_NS);
+          mbar_wait_polled(&st_full[t % C::kStaging], (t / C::kStaging) & 1, SCKV_WAIT_LIMIT_NS);
     }
     if (aborted && lane == 0) {
       if (!*abort_flag) sckv_report(p.g.status, SCKV_ERR_TIMEOUT, blockIdx.x, KID_TREE_ATTN);
@@ -483,6 +501,7 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
     // Warp `role` decodes pages 2 (role & 1), + 1 of K (role < 2) or V. Lane
     // (quarter, rowbit, c): rows r and r ^ 5 of a quarter's eight lanes keep both the
     // swizzled 16-byte reads and the two 16-byte writes free of bank conflicts.
+    reg_give();
     const int role = warp == 3 ? 0 : warp - 12;
     const int kv = role >> 1, part = role & 1;
     uint64_t* fulls = kv ? v_full : k_full;
@@ -497,8 +516,8 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
       for (int j = s.ka; j < s.ka + s.nk; ++j, ++g) {
         const int ss = g % C::kStaging, st = g % kStages;
         const int ab = __shfl_sync(0xffffffffu, *abort_flag, 0);
-        if (ab || !warp_wait(&st_full[ss], (g / C::kStaging) & 1) ||
-            (g >= kStages && !warp_wait(&empties[st], ((g / kStages) - 1) & 1))) {
+        if (ab || !warp_wait_polled(&st_full[ss], (g / C::kStaging) & 1) ||
+            (g >= kStages && !warp_wait_polled(&empties[st], ((g / kStages) - 1) & 1))) {
           aborted = true;
           break;
         }
@@ -550,10 +569,12 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
       if (!*abort_flag) sckv_report(p.g.status, SCKV_ERR_TIMEOUT, blockIdx.x, KID_TREE_ATTN);
       *abort_flag = 1;
     }
-  } else if (warp == kWarpMma && lane == 0) {
+  } else if (warp == kWarpMma) {
     // ------------------------------------------------------------ MMA issuer
+    reg_give();
+    const uint32_t el = elect_one();
     auto wait1 = [&](uint64_t* bar, uint32_t parity) -> bool {
-      return mbar_wait_bounded(bar, parity, SCKV_WAIT_LIMIT_NS);
+      return warp_wait_polled(bar, parity);
     };
     constexpr uint32_t kIdescS = instr_desc_f16(kBF16, kKeys, false);
     constexpr uint32_t kIdescPV = instr_desc_f16(kBF16, kHD, true);
@@ -585,6 +606,7 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
           const int i0 = two ? jj : jj >> 1;
           const uint32_t s0 = tmem + kColS + (uint32_t)((2 * w0 + ((gw[w0] + i0) & 1)) * kKeys);
           const uint32_t s1 = tmem + kColS + (uint32_t)((2 + ((gw[1] + jj) & 1)) * kKeys);
+          if (el) {
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks) {
             const int half = ks >> 2, kk = ks & 3;
@@ -596,6 +618,8 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
           umma_commit(&s_full[2 * w0 + ((gw[w0] + i0) & 1)]);
           if (two) umma_commit(&s_full[2 + ((gw[1] + jj) & 1)]);
           umma_commit(&k_empty[st]);
+          }
+          __syncwarp();
         }
         const int pj = jj - lag;  // the tile whose PV goes out now
         if (pj >= 0) {
@@ -614,6 +638,7 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
           const uint32_t p0 = tmem + kColS + (uint32_t)((2 * w0 + (a0 & 1)) * kKeys);
           const uint32_t p1 = tmem + kColS + (uint32_t)((2 + (a1 & 1)) * kKeys);
           const uint32_t o0 = tmem + kColO + (uint32_t)(w0 * kHD), o1 = tmem + kColO + (uint32_t)kHD;
+          if (el) {
 #pragma unroll
           for (int pg = 0; pg < kTilePages; ++pg) {
             // B = V rows of page pg: 128 dims in two 64-dim halves (LBO), 16 keys in two 8-row groups (SBO)
@@ -629,6 +654,8 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
           umma_commit(&pv_done[2 * w0 + (a0 & 1)]);
           if (two) umma_commit(&pv_done[2 + (a1 & 1)]);
           umma_commit(&v_empty[st]);
+          }
+          __syncwarp();
         }
       }
       if (!ok) break;
@@ -637,13 +664,15 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
       gw[1] += two ? s.nk : s.nk >> 1;
     }
     if (!ok) {
-      if (!*abort_flag) sckv_report(p.g.status, SCKV_ERR_TIMEOUT, blockIdx.x, KID_TREE_ATTN);
-      *abort_flag = 1;
+      if (lane == 0 && !*abort_flag) sckv_report(p.g.status, SCKV_ERR_TIMEOUT, blockIdx.x, KID_TREE_ATTN);
+      if (lane == 0) *abort_flag = 1;
     }
-    umma_commit(mma_done);  // every MMA above has finished before the tensor memory is released
+    if (el) umma_commit(mma_done);  // every MMA above has finished before the tensor memory is released
+    __syncwarp();
     wait1(mma_done, 0);
   } else if (warp >= 4 && warp < 12) {
     // ------------------------------------------------------------ softmax, Q, results
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     const int w = (warp - 4) >> 2;     // warpgroup
     const int quad = warp & 3;         // tensor memory lanes 32 quad ..
     const int row = quad * 32 + lane;  // query row of the tile = tensor memory lane
@@ -711,12 +740,12 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
         const int st = (gt + jj) % kStages;
         const int key0 = (s.ka + jj) * kKeys;
         const bool tail = key0 + kKeys > s.ctx;
-        if (*abort_flag || !warp_wait(&my_s_full[b], (gj >> 1) & 1)) {
+        if (*abort_flag || !warp_wait_polled(&my_s_full[b], (gj >> 1) & 1)) {
           ok = false;
           break;
         }
         // the V tile of S(g) cannot be replaced before P(g) is written, so this wait is for its own phase
-        if ((tail || C::kFP8) && !warp_wait(&v_full[st], ((gt + jj) / kStages) & 1)) {
+        if ((tail || C::kFP8) && !warp_wait_polled(&v_full[st], ((gt + jj) / kStages) & 1)) {
           ok = false;
           break;
         }
@@ -789,7 +818,7 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
           }
           if (__any_sync(0xffffffffu, rescale) && i > 0) {
             // O holds PV of this item's earlier tiles: wait for the last, then scale this warp's rows
-            if (!warp_wait(&my_pv_done[(gj - 1) & 1], ((gj - 1) >> 1) & 1)) {
+            if (!warp_wait_polled(&my_pv_done[(gj - 1) & 1], ((gj - 1) >> 1) & 1)) {
               ok = false;
               break;
             }
@@ -877,7 +906,7 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
       if (!ok) break;
       // ---- the item's result, once this warpgroup's last PV finished
       const int glast = g + n - 1;
-      if (n > 0 && !warp_wait(&my_pv_done[glast & 1], (glast >> 1) & 1)) {
+      if (n > 0 && !warp_wait_polled(&my_pv_done[glast & 1], (glast >> 1) & 1)) {
         ok = false;
         break;
       }
@@ -889,7 +918,7 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_full);
-      if (!warp_wait(o_full, k & 1)) {
+      if (!warp_wait_polled(o_full, k & 1)) {
         ok = false;
         break;
       }
@@ -986,8 +1015,10 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
       if (lane == 0 && !*abort_flag) sckv_report(p.g.status, SCKV_ERR_TIMEOUT, blockIdx.x, KID_TREE_ATTN);
       if (lane == 0) *abort_flag = 1;
     }
+  } else {
+    reg_give();
   }
-  if (warp == kWarpMma) __syncwarp();
+  if (warp < 4 || warp >= 12) __syncwarp();
   tc_fence_before();
   __syncthreads();
   if (warp == kWarpMma) {

@@ -9,32 +9,35 @@
 //
 // with a running reference m (one pass over K and V).
 //
-// Work. The rows of a kv head are its (node, q head of the group) pairs. A
-// group of rows is up to 256 of them: one or two 128-row query tiles over
-// the sequence's key tiles of 64 keys (4 pages). The key tiles of all (sequence, kv head,
-// row group) items form one line that the CTAs share out evenly (one
-// persistent CTA per SM), so that few sequences, long ones and ragged batches
-// all keep every SM on HBM. An item that a border cuts leaves unnormalised
-// partials (at most two per CTA) that a second kernel joins.
+// Work. The rows of a kv head are its (node, q head of the group) pairs, in
+// groups of up to two query tiles of 128 rows (one for one-byte pools), over
+// the sequence's key tiles of 128 keys (8 pages). The key tiles of all
+// (sequence, kv head, row group) items form one line that the CTAs share out
+// evenly (one persistent CTA per SM), so that few sequences, long ones and
+// ragged batches all keep every SM on HBM. An item that a border cuts leaves
+// unnormalised partials (at most two per CTA) that a second kernel joins.
 //
-// With one query tile (at most 128 rows) the two softmax warpgroups take
-// alternate key tiles, each with its own reference, sum and O accumulator,
-// joined at the end of the item: four S buffers are in flight and a tile has
-// twice its own time for its softmax. With two query tiles each warpgroup owns
-// one and both use every K/V tile.
+// With one query tile the two softmax warpgroups take a half of 64 keys of
+// every tile each, with their own reference, sum and O accumulator, joined
+// at the end of the item; S has two buffers, so the next tile's scores are
+// made while this one's are weighed. With two query tiles each warpgroup owns one and
+// both use every K/V tile. Either way a tile costs 8 MMAs of 128 x 128 x 16 for
+// S per query tile and 8 for P V (16 with P in two parts): narrower S
+// products (64 keys) take the same time each, limited by their operands'
+// shared-memory reads (measured 60 - 150 cycles against 64).
 //
 // 16 warps (a warp runs on SM sub-partition warp % 4):
 //   warps 0, 2   TMA producers. 16-bit pools: K, V; one 4 KiB box per
 //                page-head, which a rank-5 view of the pool lays out as 8-row
 //                groups [rows 0-7 | 8-15][dims 0-63 | 64-127], so that groups
 //                of consecutive pages have one stride. One-byte pools: pages
-//                0-1, 2-3 of the tile, K and V of a page in one 4 KiB box into
-//                a staging ring, plus the tile's scales (warp 0).
+//                0-1, 2-3 of each half tile, K and V of a page in one 4 KiB
+//                box into a staging ring, plus int8 scales (warp 0).
 //   warps 3, 13-15  one-byte pools: decode staged codes into the f16 rings.
 //                int8 codes times their token's fp16 scale (the rounding that
 //                the cache's values have); e4m3 codes exactly, their page's
 //                scales go to the scores (K) and to P (V).
-//   warp 1       one thread issues every MMA and commit.
+//   warp 1       issues every MMA and commit from one elected lane.
 //   warps 4-11   softmax, one thread per query row; they also load Q and
 //                write the results.
 //
@@ -65,38 +68,36 @@ constexpr int kHD = 128;
 constexpr int kMaskWordsMax = 4;
 constexpr int kMaxSeqs = 2048;
 constexpr int kRows = 128;                     // rows of a query tile (UMMA M)
-constexpr int kKeys = 64;                      // keys of a K/V tile
-constexpr int kTilePages = kKeys / SCKV_PAGE_TOKENS;
+constexpr int kHalf = 64;                      // keys of half a K/V tile
+constexpr int kKeys = 2 * kHalf;               // keys of a K/V tile
+constexpr int kHalfPages = kHalf / SCKV_PAGE_TOKENS;
+constexpr int kTilePages = 2 * kHalfPages;
 constexpr int kThreadsTree = 512;
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kColS = 0;                  // S[w][b] at 64 (2 w + b)
+constexpr uint32_t kColS = 0;                  // S[x] at 128 x
 constexpr uint32_t kColO = 256;                // O[w] at 256 + 128 w
 constexpr int kWarpProdA = 0, kWarpMma = 1, kWarpProdB = 2;
 constexpr int kQHalf = kRows * 128;            // one 64-dim half of a query tile: 16 KiB
 constexpr int kQTile = 2 * kQHalf;
 constexpr int kPageTile = 4096;                // one page-head in f16 / bf16
-constexpr int kSlot = kTilePages * kPageTile;  // a K (or V) tile: 16 KiB
-constexpr int kScaleSlots = 16;                // tiles whose scales are kept (more than both rings together)
-constexpr int kMinShare = 2;                   // key tiles a CTA takes at least
+constexpr int kHalfSlot = kHalfPages * kPageTile;
+constexpr int kSlot = 2 * kHalfSlot;           // a K (or V) tile: 32 KiB
+constexpr int kStages = 2;                     // K and V tiles in the MMA's type
+constexpr int kScaleSlots = 16;                // int8: half tiles whose scales are kept
 
 template <int KVDT>
 struct TreeCfg {
   static constexpr bool kFP8 = KVDT == SCKV_DTYPE_FP8_E4M3, kINT8 = KVDT == SCKV_DTYPE_INT8;
   static constexpr bool kB8 = kFP8 || kINT8;
   static constexpr bool kBF16 = KVDT == SCKV_DTYPE_BF16;
-  static constexpr int kStages = kB8 ? 3 : 4;         // K and V tiles in the MMA's type
-  static constexpr int kStaging = kB8 ? 3 : 0;        // staged one-byte tiles (K and V)
-  // PV of tile j goes out after S of tile j + kLag (one query tile; 1 with two): at most the spare S buffers, and
-  // below kStages, so that the V tile which shared a slot with tile j was complete before S(j): a softmax warp's
-  // parity wait on v_full then cannot be met by an older phase
-  static constexpr int kLag = kB8 ? 2 : 3;
-  static_assert(kLag < kStages && kLag <= 3, "V slots and S buffers cover the lag");
-  static constexpr int kOffK = 2 * kQTile;
+  static constexpr int kQTiles = kB8 ? 1 : 2;
+  static constexpr int kStaging = kB8 ? 3 : 0;        // staged half tiles of codes (K and V)
+  static constexpr int kOffK = kQTiles * kQTile;
   static constexpr int kOffV = kOffK + kStages * kSlot;
   static constexpr int kOffStage = kOffV + kStages * kSlot;
-  static constexpr int kOffScale = kOffStage + kStaging * kSlot;
-  static constexpr int kOffBar = kOffScale + (kB8 ? kScaleSlots * 256 : 0);
-  static constexpr int kNumBars = 4 * kStages + 12 + 4 + 2 * kStaging;
+  static constexpr int kOffScale = kOffStage + kStaging * kHalfSlot;
+  static constexpr int kOffBar = kOffScale + (kINT8 ? kScaleSlots * 256 : 0);
+  static constexpr int kNumBars = 4 * kStages + 6 + 4 + 2 * kStaging;
   static constexpr int kOffMl = kOffBar + ((kNumBars * 8 + 15) / 16) * 16;  // float2 [2][128]: m, l of a row
   static constexpr int kOffVref = kOffMl + 2 * kRows * 8;                   // float [2]
   static constexpr int kOffBad = kOffVref + 16;                             // u64 [2][4]: nodes whose V is not finite
@@ -105,7 +106,7 @@ struct TreeCfg {
   static constexpr int kOffPartial = kOffTmem + 16;                         // int [kThreadsTree]
   static constexpr int kOffCum = kOffPartial + kThreadsTree * 4;            // int [n_seqs + 1]
   static constexpr int kFixedSmem = 1024 + kOffCum + 4;                     // + 4 n_seqs
-  static_assert(kStages + (kB8 ? kStaging : 0) < kScaleSlots, "scale slots outlive their tiles");
+  static_assert(2 * kStages + kStaging < kScaleSlots, "scale slots outlive their half tiles");
 };
 
 // What the joining kernel needs of a CTA whose first item began in an earlier one and ends in it.
@@ -125,6 +126,7 @@ struct TreeParams {
   const unsigned long long* mask;
   int mask_words;
   int max_blocks, n_seqs, n_tokens, hq, G;
+  int group_rows;  // rows of a row group: 256, one-byte pools 128
   int q_dtype, out_dtype;
   float scale_log2;
   // workspace: JoinHead [grid], then per CTA two slots of float4 [32][part_rows] (O by 4 dims and row)
@@ -145,7 +147,7 @@ __device__ __forceinline__ bool tree_seq(const TreeParams& p, int s, int& n, int
   const bool ok = t0 >= 0 && t1 >= t0 && t1 <= p.n_tokens && n <= 64 * p.mask_words && ctx >= 0 && ctx <= cap - n;
   if (!ok) n = ctx = 0;
   kt = n > 0 ? (ctx + n + kKeys - 1) / kKeys : 0;
-  groups = (n * p.G + 2 * kRows - 1) / (2 * kRows);
+  groups = (n * p.G + p.group_rows - 1) / p.group_rows;
   return ok;
 }
 
@@ -171,8 +173,8 @@ __device__ __forceinline__ bool tree_next(const TreeParams& p, const int* cum, T
   s.ka = rem - item * s.kt;
   s.nk = min(s.kt - s.ka, w.t1 - w.t);
   s.h = item / groups;
-  s.row0 = (item - s.h * groups) * 2 * kRows;
-  s.rows = min(2 * kRows, s.n * p.G - s.row0);
+  s.row0 = (item - s.h * groups) * p.group_rows;
+  s.rows = min(p.group_rows, s.n * p.G - s.row0);
   s.nq = s.rows > kRows ? 2 : 1;
   s.L = s.ctx + s.n;
   s.pages = (s.L + SCKV_PAGE_TOKENS - 1) / SCKV_PAGE_TOKENS;
@@ -229,6 +231,20 @@ __device__ __forceinline__ bool warp_wait_polled(uint64_t* bar, uint32_t parity)
   return __all_sync(0xffffffffu, mbar_wait_polled(bar, parity, SCKV_WAIT_LIMIT_NS));
 }
 
+// 16 columns of this thread's tensor memory lane.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory");
+}
+
 // 1 on one lane of the (converged) warp.
 __device__ __forceinline__ uint32_t elect_one() {
   uint32_t r;
@@ -243,7 +259,6 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
     tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap tmap) {
   using C = TreeCfg<KVDT>;
   constexpr bool kBF16 = C::kBF16;
-  constexpr int kStages = C::kStages;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + C::kOffBar);
@@ -251,14 +266,15 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
   uint64_t* k_empty = k_full + kStages;      // [S] the S products that read it finished (commit)
   uint64_t* v_full = k_empty + kStages;      // [S] V tile in shared memory
   uint64_t* v_empty = v_full + kStages;      // [S] the PV products that read it finished (commit)
-  uint64_t* s_full = v_empty + kStages;      // [w][2] S in tensor memory (commit)
-  uint64_t* p_full = s_full + 4;             // [w][2] P in tensor memory, V tile fixed (one arrival per warp)
-  uint64_t* pv_done = p_full + 4;            // [w][2] PV finished (commit)
-  uint64_t* o_empty = pv_done + 4;           // the item's O was read (one arrival per softmax warp)
+  // set x: one query tile: tile i of the item uses set i & 1; two: query tile w uses set w for every tile
+  uint64_t* s_full = v_empty + kStages;      // [x] S in tensor memory (commit)
+  uint64_t* p_full = s_full + 2;             // [x] P in tensor memory, V tile fixed (8 arrivals)
+  uint64_t* pv_done = p_full + 2;            // [x] PV finished (commit)
+  uint64_t* o_empty = pv_done + 2;           // the item's O was read (one arrival per softmax warp)
   uint64_t* q_full = o_empty + 1;            // the item's Q is in shared memory (one arrival per softmax warp)
   uint64_t* mma_done = q_full + 1;           // every issued MMA finished
   uint64_t* o_full = mma_done + 1;           // the item's sums are written and its O is complete (one arrival per softmax warp)
-  uint64_t* st_full = o_full + 1;            // one-byte pools: [SS] staged tile landed, its scales are written
+  uint64_t* st_full = o_full + 1;            // one-byte pools: [SS] staged half tile landed, its scales are written
   uint64_t* st_empty = st_full + C::kStaging;  // [SS] decoded (one arrival per decoding warp)
   float2* s_ml = reinterpret_cast<float2*>(base + C::kOffMl);
   float* s_vref = reinterpret_cast<float*>(base + C::kOffVref);
@@ -294,8 +310,8 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
       for (int i = 0; i < C::kNumBars; ++i) {
         uint64_t* bar = &bars[i];
         uint32_t count = 1;
-        if (C::kB8 && ((bar >= k_full && bar < k_full + kStages) || (bar >= v_full && bar < v_full + kStages))) count = 2;
-        if (bar >= p_full && bar < p_full + 4) count = 4;
+        if (C::kB8 && ((bar >= k_full && bar < k_full + kStages) || (bar >= v_full && bar < v_full + kStages))) count = 4;
+        if (bar >= p_full && bar < p_full + 2) count = 8;
         if (bar == o_empty || bar == q_full || bar == o_full) count = 8;
         if (C::kB8 && bar >= st_full && bar < st_full + C::kStaging) count = 2;
         if (C::kB8 && bar >= st_empty && bar < st_empty + C::kStaging) count = 4;
@@ -322,8 +338,8 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
   }
   const uint32_t tmem = *tmem_slot;
   const int total = cum[p.n_seqs];
-  // CTAs that take a share: no fewer than kMinShare tiles each
-  const int n_cta = max(1, min((int)gridDim.x, total / kMinShare));
+  // CTAs that take a share
+  const int n_cta = max(1, min((int)gridDim.x, total));
   TreeWalk walk{0, 0, 0};
   if ((int)blockIdx.x < n_cta && total > 0) {
     walk.t = tree_begin(blockIdx.x, total, n_cta);
@@ -359,7 +375,7 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
   if (warp == kWarpProdA || warp == kWarpProdB) {
     // ------------------------------------------------------------ producers
     reg_give();
-    const int part = warp == kWarpProdB ? 1 : 0;  // 16-bit: V; one-byte: pages 2, 3
+    const int part = warp == kWarpProdB ? 1 : 0;  // 16-bit: V; one-byte: pages 2, 3 of a half tile
     if (lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap)) : "memory");
     TreeSeg s;
     int g = 0;
@@ -371,7 +387,7 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
         uint8_t* ring = base + (part ? C::kOffV : C::kOffK);
         while (!aborted && tree_next(p, cum, walk, s)) {
           const int32_t* bt_row = p.bt + (int64_t)s.seq * p.bt_stride;
-          int ids[kTilePages], nxt[kTilePages];
+          int ids[kTilePages], nxt[kTilePages];  // page ids, fetched one tile ahead
           auto fetch = [&](int j, int (&v)[kTilePages]) {
 #pragma unroll
             for (int i = 0; i < kTilePages; ++i) {
@@ -411,47 +427,37 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
           mbar_wait_polled(&fulls[t % kStages], (t / kStages) & 1, SCKV_WAIT_LIMIT_NS);
       }
     } else {
-      // scales: FP8 lanes 0-7 one fp32 each (K, V of 4 pages); int8 every lane four tokens' fp16
-      const int skv = C::kFP8 ? (lane >> 2) & 1 : lane >> 4;
-      const int spg = C::kFP8 ? lane & 3 : (lane >> 2) & 3;
-      const bool has_scale = part == 0 && (C::kINT8 || lane < 8);
+      // int8 scales of a half tile: four tokens' fp16 per lane (K, V; 4 pages; 4 x 4 tokens)
+      const int skv = lane >> 4, spg = (lane >> 2) & 3;
+      const bool has_scale = C::kINT8 && part == 0;
       while (!aborted && tree_next(p, cum, walk, s)) {
         const int32_t* bt_row = p.bt + (int64_t)s.seq * p.bt_stride;
-        const int je = s.ka + s.nk;
+        const int je = 2 * (s.ka + s.nk);
         auto fetch = [&](int blk) -> int {
-          int page = blk < s.pages ? __ldg(bt_row + blk) : -1;
+          const int page = blk < s.pages ? __ldg(bt_row + blk) : -1;
           return blk < s.pages && (page < 0 || page >= p.g.P) ? 0 : page;
         };
-        // FP8: a page past the last node scales by 1 (K, masked anyway) and 0 (V)
         auto load_scale = [&](int page) -> uint2 {
-          uint2 r = make_uint2(C::kFP8 && skv == 0 ? 0x3f800000u : 0u, 0u);
-          if (page < 0) return r;
-          if (C::kFP8) {
-            const float f = __ldg(reinterpret_cast<const float*>(p.g.scales) + ((layer_base + page) * 2 + skv) * p.g.H + s.h);
-            r.x = __float_as_uint(skv == 0 ? fmaxf(f, 1e-30f) : f);  // (never 0: it multiplies masked scores, -inf)
-            if (f != f) r.x = __float_as_uint(f);
-          } else {
-            r = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const __half*>(p.g.scales) +
-                                                     (((layer_base + page) * 2 + skv) * p.g.H + s.h) * 16) + (lane & 3));
-          }
-          return r;
+          if (page < 0) return make_uint2(0u, 0u);
+          return __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const __half*>(p.g.scales) +
+                                                      (((layer_base + page) * 2 + skv) * p.g.H + s.h) * 16) + (lane & 3));
         };
         uint2 sc = make_uint2(0u, 0u);
         int sid = -1;
         if (has_scale) {
-          sc = load_scale(fetch(s.ka * kTilePages + spg));
-          if (s.nk > 1) sid = fetch((s.ka + 1) * kTilePages + spg);
+          sc = load_scale(fetch(2 * s.ka * kHalfPages + spg));
+          sid = fetch((2 * s.ka + 1) * kHalfPages + spg);
         }
         int nid[2] = {0, 0};
         auto fetch_ids = [&](int j) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const int blk = j * kTilePages + 2 * part + i;
+            const int blk = j * kHalfPages + 2 * part + i;
             nid[i] = blk < s.pages ? __ldg(bt_row + blk) : 0;
           }
         };
-        if (lane == 0) fetch_ids(s.ka);
-        for (int j = s.ka; j < je; ++j, ++g) {
+        if (lane == 0) fetch_ids(2 * s.ka);
+        for (int j = 2 * s.ka; j < je; ++j, ++g) {
           const int st = g % C::kStaging;
           const int ab = __shfl_sync(0xffffffffu, *abort_flag, 0);
           if (g >= C::kStaging && (ab || !warp_wait_polled(&st_empty[st], ((g / C::kStaging) - 1) & 1))) {
@@ -459,21 +465,19 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
             break;
           }
           if (has_scale) {
-            uint8_t* slot = base + C::kOffScale + (g % kScaleSlots) * 256;
-            if (C::kFP8) reinterpret_cast<uint32_t*>(slot)[lane] = sc.x;
-            else reinterpret_cast<uint2*>(slot)[lane] = sc;
+            reinterpret_cast<uint2*>(base + C::kOffScale + (g % kScaleSlots) * 256)[lane] = sc;
             if (j + 1 < je) {
               sc = load_scale(sid);
-              if (j + 2 < je) sid = fetch((j + 2) * kTilePages + spg);
+              if (j + 2 < je) sid = fetch((j + 2) * kHalfPages + spg);
             }
           }
           __syncwarp();
           if (lane == 0) {
             const int ids[2] = {nid[0], nid[1]};
             if (j + 1 < je) fetch_ids(j + 1);
-            const int np = max(0, min(2, s.pages - j * kTilePages - 2 * part));
+            const int np = max(0, min(2, s.pages - j * kHalfPages - 2 * part));
             mbar_arrive_expect_tx(&st_full[st], (uint32_t)np * 4096u);
-            const uint32_t dst = smem_u32(base + C::kOffStage + st * kSlot + 2 * part * 4096);
+            const uint32_t dst = smem_u32(base + C::kOffStage + st * kHalfSlot + 2 * part * 4096);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               if (i >= np) break;
@@ -498,178 +502,189 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
     }
   } else if (C::kB8 && (warp == 3 || warp >= 13)) {
     // ------------------------------------------------------------ decoding of one-byte pages
-    // Warp `role` decodes pages 2 (role & 1), + 1 of K (role < 2) or V. Lane
+    // Warp `role` decodes pages 2 (role & 1), + 1 of K (role < 2) or V of each half tile. Lane
     // (quarter, rowbit, c): rows r and r ^ 5 of a quarter's eight lanes keep both the
     // swizzled 16-byte reads and the two 16-byte writes free of bank conflicts.
     reg_give();
-    const int role = warp == 3 ? 0 : warp - 12;
-    const int kv = role >> 1, part = role & 1;
-    uint64_t* fulls = kv ? v_full : k_full;
-    uint64_t* empties = kv ? v_empty : k_empty;
-    uint8_t* ring = base + (kv ? C::kOffV : C::kOffK);
-    const int qt = lane >> 3;
-    const int r8 = (lane & 4) ? qt ^ 5 : qt;  // row of the 8-row group
-    TreeSeg s;
-    int g = 0;
-    bool aborted = false;
-    while (!aborted && tree_next(p, cum, walk, s)) {
-      for (int j = s.ka; j < s.ka + s.nk; ++j, ++g) {
-        const int ss = g % C::kStaging, st = g % kStages;
-        const int ab = __shfl_sync(0xffffffffu, *abort_flag, 0);
-        if (ab || !warp_wait_polled(&st_full[ss], (g / C::kStaging) & 1) ||
-            (g >= kStages && !warp_wait_polled(&empties[st], ((g / kStages) - 1) & 1))) {
-          aborted = true;
-          break;
-        }
-        const int np = max(0, min(2, s.pages - j * kTilePages - 2 * part));
-        const __half* tok = reinterpret_cast<const __half*>(base + C::kOffScale + (g % kScaleSlots) * 256) + kv * 64;
+    if constexpr (C::kB8) {
+      const int role = warp == 3 ? 0 : warp - 12;
+      const int kv = role >> 1, part = role & 1;
+      uint64_t* fulls = kv ? v_full : k_full;
+      uint64_t* empties = kv ? v_empty : k_empty;
+      uint8_t* ring = base + (kv ? C::kOffV : C::kOffK);
+      const int qt = lane >> 3;
+      const int r8 = (lane & 4) ? qt ^ 5 : qt;  // row of the 8-row group
+      TreeSeg s;
+      int g = 0;  // half tiles
+      bool aborted = false;
+      while (!aborted && tree_next(p, cum, walk, s)) {
+        for (int j = 2 * s.ka; j < 2 * (s.ka + s.nk); ++j, ++g) {
+          const int ss = g % C::kStaging, gt = g >> 1, st = gt % kStages;
+          const int ab = __shfl_sync(0xffffffffu, *abort_flag, 0);
+          if (ab || !warp_wait_polled(&st_full[ss], (g / C::kStaging) & 1) ||
+              ((g & 1) == 0 && gt >= kStages && !warp_wait_polled(&empties[st], ((gt / kStages) - 1) & 1))) {
+            aborted = true;
+            break;
+          }
+          const int np = max(0, min(2, s.pages - j * kHalfPages - 2 * part));
+          const __half* tok = reinterpret_cast<const __half*>(base + C::kOffScale + (g % kScaleSlots) * 256) + kv * 64;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (i >= np) break;
-          const int pg = 2 * part + i;
-          const uint8_t* src = base + C::kOffStage + ss * kSlot + pg * 4096 + kv * 2048;
-          uint8_t* dst = ring + st * kSlot + pg * kPageTile;
+          for (int i = 0; i < 2; ++i) {
+            if (i >= np) break;
+            const int pg = 2 * part + i;
+            const uint8_t* src = base + C::kOffStage + ss * kHalfSlot + pg * 4096 + kv * 2048;
+            uint8_t* dst = ring + st * kSlot + (g & 1) * kHalfSlot + pg * kPageTile;
 #pragma unroll
-          for (int sub = 0; sub < 2; ++sub) {
-            const int row = sub * 8 + r8;
-            const __half2 s2 = C::kINT8 ? __half2half2(tok[pg * SCKV_PAGE_TOKENS + row]) : __half2half2(__half(1.f));
+            for (int sub = 0; sub < 2; ++sub) {
+              const int row = sub * 8 + r8;
+              __half2 s2 = __half2half2(__half(1.f));
+              if (C::kINT8) s2 = __half2half2(tok[pg * SCKV_PAGE_TOKENS + row]);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const int c8 = half * 4 + (lane & 3);  // 16 codes: dims 16 c8 ..
-              const uint4 w = *reinterpret_cast<const uint4*>(src + row * 128 + ((c8 ^ r8) << 4));
-              const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-              uint32_t o[8];
+              for (int half = 0; half < 2; ++half) {
+                const int c8 = half * 4 + (lane & 3);  // 16 codes: dims 16 c8 ..
+                const uint4 w = *reinterpret_cast<const uint4*>(src + row * 128 + ((c8 ^ r8) << 4));
+                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+                uint32_t o[8];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                cvt_b8x4<KVDT>(ws[e], o[2 * e], o[2 * e + 1]);
-                if (C::kINT8) {
+                for (int e = 0; e < 4; ++e) {
+                  cvt_b8x4<KVDT>(ws[e], o[2 * e], o[2 * e + 1]);
+                  if (C::kINT8) {
 #pragma unroll
-                  for (int k = 0; k < 2; ++k) {
-                    const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&o[2 * e + k]), s2);
-                    o[2 * e + k] = *reinterpret_cast<const uint32_t*>(&x);
+                    for (int k = 0; k < 2; ++k) {
+                      const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&o[2 * e + k]), s2);
+                      o[2 * e + k] = *reinterpret_cast<const uint32_t*>(&x);
+                    }
                   }
                 }
+                uint8_t* d = dst + sub * 2048 + half * 1024 + r8 * 128;
+                const int c = 2 * (lane & 3);
+                *reinterpret_cast<uint4*>(d + ((c ^ r8) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+                *reinterpret_cast<uint4*>(d + (((c + 1) ^ r8) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
               }
-              uint8_t* d = dst + sub * 2048 + half * 1024 + r8 * 128;
-              const int c = 2 * (lane & 3);
-              *reinterpret_cast<uint4*>(d + ((c ^ r8) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-              *reinterpret_cast<uint4*>(d + (((c + 1) ^ r8) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
             }
           }
-        }
-        fence_proxy_async_smem();  // read by the tensor cores
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&fulls[st]);
-          mbar_arrive(&st_empty[ss]);
+          fence_proxy_async_smem();  // read by the tensor cores
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&fulls[st]);
+            mbar_arrive(&st_empty[ss]);
+          }
         }
       }
-    }
-    if (aborted && lane == 0) {
-      if (!*abort_flag) sckv_report(p.g.status, SCKV_ERR_TIMEOUT, blockIdx.x, KID_TREE_ATTN);
-      *abort_flag = 1;
+      if (aborted && lane == 0) {
+        if (!*abort_flag) sckv_report(p.g.status, SCKV_ERR_TIMEOUT, blockIdx.x, KID_TREE_ATTN);
+        *abort_flag = 1;
+      }
     }
   } else if (warp == kWarpMma) {
     // ------------------------------------------------------------ MMA issuer
+    // The whole warp walks and waits, one elected lane issues (a role on one lane alone measured 1.3 x slower).
     reg_give();
     const uint32_t el = elect_one();
-    auto wait1 = [&](uint64_t* bar, uint32_t parity) -> bool {
-      return warp_wait_polled(bar, parity);
-    };
     constexpr uint32_t kIdescS = instr_desc_f16(kBF16, kKeys, false);
     constexpr uint32_t kIdescPV = instr_desc_f16(kBF16, kHD, true);
     const uint64_t q_desc0 = smem_desc_sw128(smem_u32(base), 16, 1024);
     const uint64_t k_desc0 = smem_desc_sw128(smem_u32(base + C::kOffK), 16, 2048);
     const uint64_t v_desc0 = smem_desc_sw128(smem_u32(base + C::kOffV), 1024, 2048);
+    // S[x] = Q tile w . K of slot st
+    auto issue_s = [&](int x, int w, int st) {
+      const uint64_t qd = desc_advance(q_desc0, (uint32_t)(w * kQTile));
+      const uint64_t kd = desc_advance(k_desc0, (uint32_t)(st * kSlot));
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) {
+        const int half = ks >> 2, kk = ks & 3;
+        umma_ss(tmem + kColS + (uint32_t)(x * kKeys), desc_advance(qd, (uint32_t)(half * kQHalf + kk * 32)),
+                desc_advance(kd, (uint32_t)(half * 1024 + kk * 32)), kIdescS, ks > 0);
+      }
+      umma_commit(&s_full[x]);
+    };
+    // O[w] (+)= P[x], half h . V of slot st, half h
+    auto issue_pv = [&](int x, int h, int w, int st, bool first) {
+      const uint64_t vd = desc_advance(v_desc0, (uint32_t)(st * kSlot + h * kHalfSlot));
+      const uint32_t pa = tmem + kColS + (uint32_t)(x * kKeys + h * kHalf), o = tmem + kColO + (uint32_t)(w * kHD);
+#pragma unroll
+      for (int pg = 0; pg < kHalfPages; ++pg) {
+        // B = V rows of page pg: 128 dims in two 64-dim halves (LBO), 16 keys in two 8-row groups (SBO)
+        const uint64_t bdesc = desc_advance(vd, (uint32_t)(pg * kPageTile));
+        umma_ts(o, pa + (uint32_t)(pg * 8), bdesc, kIdescPV, (!first || pg > 0) ? 1u : 0u);
+        if (kBF16) umma_ts(o, pa + (uint32_t)(pg * 8 + 32), bdesc, kIdescPV, 1u);
+      }
+    };
     TreeSeg s;
     bool ok = true;
-    int gt = 0;              // key tiles of earlier items
-    int gw[2] = {0, 0};      // S tiles of each warpgroup in earlier items
+    int gt = 0;              // tiles of earlier items
+    int cnt[2] = {0, 0};     // uses of each set in earlier items
     for (int k = 0; ok && tree_next(p, cum, walk, s); ++k) {
-      if (*abort_flag || !wait1(q_full, k & 1)) {
+      if (*abort_flag || !warp_wait_polled(q_full, k & 1)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      const bool two = s.nq == 2;
-      const int lag = two ? 1 : C::kLag;
-      for (int jj = 0; jj < s.nk + lag; ++jj) {
-        if (jj < s.nk) {
-          const int gj = gt + jj, st = gj % kStages;
-          if (*abort_flag || !wait1(&k_full[st], (gj / kStages) & 1)) {
+      const bool two = C::kQTiles == 2 && s.nq == 2;
+      for (int i = 0; ok && i <= s.nk; ++i) {
+        const int g = gt + i, st = g % kStages;
+        if (i < s.nk) {
+          if (*abort_flag || !warp_wait_polled(&k_full[st], (g / kStages) & 1)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint64_t k_desc = desc_advance(k_desc0, (uint32_t)(st * kSlot));
-          const int w0 = two ? 0 : jj & 1;
-          const int i0 = two ? jj : jj >> 1;
-          const uint32_t s0 = tmem + kColS + (uint32_t)((2 * w0 + ((gw[w0] + i0) & 1)) * kKeys);
-          const uint32_t s1 = tmem + kColS + (uint32_t)((2 + ((gw[1] + jj) & 1)) * kKeys);
-          if (el) {
-#pragma unroll
-          for (int ks = 0; ks < 8; ++ks) {
-            const int half = ks >> 2, kk = ks & 3;
-            const uint64_t bdesc = desc_advance(k_desc, (uint32_t)(half * 1024 + kk * 32));
-            umma_ss(s0, desc_advance(q_desc0, (uint32_t)(half * kQHalf + kk * 32)), bdesc, kIdescS, ks > 0);
-            if (two)
-              umma_ss(s1, desc_advance(q_desc0, (uint32_t)(kQTile + half * kQHalf + kk * 32)), bdesc, kIdescS, ks > 0);
-          }
-          umma_commit(&s_full[2 * w0 + ((gw[w0] + i0) & 1)]);
-          if (two) umma_commit(&s_full[2 + ((gw[1] + jj) & 1)]);
-          umma_commit(&k_empty[st]);
-          }
-          __syncwarp();
-        }
-        const int pj = jj - lag;  // the tile whose PV goes out now
-        if (pj >= 0) {
-          const int gj = gt + pj, st = gj % kStages;
-          const int w0 = two ? 0 : pj & 1;
-          const int i0 = two ? pj : pj >> 1;
-          const int a0 = gw[w0] + i0, a1 = gw[1] + pj;
-          if (!wait1(&v_full[st], (gj / kStages) & 1) || !wait1(&p_full[2 * w0 + (a0 & 1)], (a0 >> 1) & 1) ||
-              (two && !wait1(&p_full[2 + (a1 & 1)], (a1 >> 1) & 1)) ||
-              (i0 == 0 && k > 0 && !wait1(o_empty, (k - 1) & 1))) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint64_t v_desc = desc_advance(v_desc0, (uint32_t)(st * kSlot));
-          const uint32_t p0 = tmem + kColS + (uint32_t)((2 * w0 + (a0 & 1)) * kKeys);
-          const uint32_t p1 = tmem + kColS + (uint32_t)((2 + (a1 & 1)) * kKeys);
-          const uint32_t o0 = tmem + kColO + (uint32_t)(w0 * kHD), o1 = tmem + kColO + (uint32_t)kHD;
-          if (el) {
-#pragma unroll
-          for (int pg = 0; pg < kTilePages; ++pg) {
-            // B = V rows of page pg: 128 dims in two 64-dim halves (LBO), 16 keys in two 8-row groups (SBO)
-            const uint64_t bdesc = desc_advance(v_desc, (uint32_t)(pg * kPageTile));
-            const uint32_t acc = (i0 > 0 || pg > 0) ? 1u : 0u;
-            umma_ts(o0, p0 + (uint32_t)(pg * 8), bdesc, kIdescPV, acc);
-            if (two) umma_ts(o1, p1 + (uint32_t)(pg * 8), bdesc, kIdescPV, acc);
-            if (kBF16) {
-              umma_ts(o0, p0 + (uint32_t)(pg * 8 + 32), bdesc, kIdescPV, 1u);
-              if (two) umma_ts(o1, p1 + (uint32_t)(pg * 8 + 32), bdesc, kIdescPV, 1u);
+          if (!two) {
+            if (el) {
+              issue_s(i & 1, 0, st);
+              umma_commit(&k_empty[st]);
             }
+            __syncwarp();
           }
-          umma_commit(&pv_done[2 * w0 + (a0 & 1)]);
-          if (two) umma_commit(&pv_done[2 + (a1 & 1)]);
-          umma_commit(&v_empty[st]);
-          }
-          __syncwarp();
         }
+        // PV of tile u = i - 1; with two query tiles S(i) of each follows its PV into the same columns
+        const int u = i - 1, gu = g - 1, su = (g + kStages - 1) % kStages;
+        if (u >= 0 && (!warp_wait_polled(&v_full[su], (gu / kStages) & 1) ||
+                       (u == 0 && k > 0 && !warp_wait_polled(o_empty, (k - 1) & 1)))) {
+          ok = false;
+          break;
+        }
+        const bool both = (s.ka + u) * kKeys + kHalf < s.L;  // the tile's second half holds keys
+        for (int w = 0; w < (two ? 2 : 1); ++w) {
+          if (u >= 0) {
+            const int x = two ? w : u & 1;
+            const int use = cnt[x] + (two ? u : u >> 1);
+            if (!warp_wait_polled(&p_full[x], use & 1)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            if (el) {
+              issue_pv(x, 0, w, su, u == 0);
+              if (both) issue_pv(x, 1, two ? w : 1, su, !two && u == 0);
+              umma_commit(&pv_done[x]);
+            }
+            __syncwarp();
+          }
+          if (two && i < s.nk) {
+            if (el) issue_s(w, w, st);
+            __syncwarp();
+          }
+        }
+        if (!ok) break;
+        if (el) {
+          if (two && i < s.nk) umma_commit(&k_empty[st]);
+          if (u >= 0) umma_commit(&v_empty[su]);
+        }
+        __syncwarp();
       }
       if (!ok) break;
       gt += s.nk;
-      gw[0] += two ? s.nk : (s.nk + 1) >> 1;
-      gw[1] += two ? s.nk : s.nk >> 1;
+      cnt[0] += two ? s.nk : (s.nk + 1) >> 1;
+      cnt[1] += two ? s.nk : s.nk >> 1;
     }
-    if (!ok) {
-      if (lane == 0 && !*abort_flag) sckv_report(p.g.status, SCKV_ERR_TIMEOUT, blockIdx.x, KID_TREE_ATTN);
-      if (lane == 0) *abort_flag = 1;
+    if (!ok && lane == 0) {
+      if (!*abort_flag) sckv_report(p.g.status, SCKV_ERR_TIMEOUT, blockIdx.x, KID_TREE_ATTN);
+      *abort_flag = 1;
     }
     if (el) umma_commit(mma_done);  // every MMA above has finished before the tensor memory is released
     __syncwarp();
-    wait1(mma_done, 0);
+    warp_wait_polled(mma_done, 0);
   } else if (warp >= 4 && warp < 12) {
     // ------------------------------------------------------------ softmax, Q, results
     asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
@@ -678,19 +693,16 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
     const int row = quad * 32 + lane;  // query row of the tile = tensor memory lane
     const int tid = threadIdx.x - 128; // 0 .. 255
     const uint32_t t_row = tmem + ((uint32_t)(quad * 32) << 16);
-    const uint32_t col_s = kColS + (uint32_t)(2 * w * kKeys);
     const uint32_t col_o = kColO + (uint32_t)(w * kHD);
-    uint64_t* my_s_full = s_full + 2 * w;
-    uint64_t* my_p_full = p_full + 2 * w;
-    uint64_t* my_pv_done = pv_done + 2 * w;
     // Q rows of an item into shared memory (128-byte swizzled, K-major): with one
     // query tile all 256 threads load it, with two each warpgroup its own.
     // Rows past the last keep what they have: no other row sees it.
     auto load_q = [&](const TreeSeg& s) {
-      const int n_it = s.nq == 2 ? 16 : 8, step = s.nq == 2 ? 128 : 256;
-      const int t = s.nq == 2 ? tid & 127 : tid;
-      const int tile_row0 = s.nq == 2 ? w * kRows : 0;
-      uint8_t* q_tile = base + (s.nq == 2 ? w * kQTile : 0);
+      const bool two = C::kQTiles == 2 && s.nq == 2;
+      const int n_it = two ? 16 : 8, step = two ? 128 : 256;
+      const int t = two ? tid & 127 : tid;
+      const int tile_row0 = two ? w * kRows : 0;
+      uint8_t* q_tile = base + (two ? w * kQTile : 0);
       const int64_t q0 = (int64_t)s.q_base * p.hq + (int64_t)s.h * p.G;
 #pragma unroll 1
       for (int b8 = 0; b8 < n_it; b8 += 8) {
@@ -717,81 +729,111 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
       if (lane == 0) mbar_arrive(q_full);
     };
     bool ok = true;
-    int g = 0;   // S tiles of this warpgroup in earlier items
-    int gt = 0;  // key tiles of earlier items
+    int gt = 0;           // tiles of earlier items
+    int cnt[2] = {0, 0};  // uses of each set in earlier items
     TreeSeg s;
     bool more = tree_next(p, cum, walk, s);
     if (more) load_q(s);
     for (int k = 0; ok && more; ++k) {
-      const bool two = s.nq == 2;
+      const bool two = C::kQTiles == 2 && s.nq == 2;
       const int r_in = (two ? w * kRows : 0) + row;  // row of the group
       const bool valid = r_in < s.rows;
       const int node = (s.row0 + r_in) / p.G;
       const int head = s.h * p.G + (s.row0 + r_in) - node * p.G;
       const unsigned long long* mask = p.mask + (int64_t)(s.q_base + (valid ? node : 0)) * p.mask_words;
       const bool live = __any_sync(0xffffffffu, valid);
-      const int n = two ? s.nk : (s.nk + 1 - w) >> 1;
       unsigned long long* bad = s_bad + (k & 1) * kMaskWordsMax;
       float m = -INFINITY, l = 0.f;
       float vref = 0.f;  // FP8: the V scale that O counts in
-      for (int i = 0; i < n; ++i) {
-        const int jj = two ? i : 2 * i + w;
-        const int gj = g + i, b = gj & 1;
-        const int st = (gt + jj) % kStages;
-        const int key0 = (s.ka + jj) * kKeys;
-        const bool tail = key0 + kKeys > s.ctx;
-        if (*abort_flag || !warp_wait_polled(&my_s_full[b], (gj >> 1) & 1)) {
-          ok = false;
-          break;
+      // FP8: lanes 0-3 the K, 4-7 the V scales of this warpgroup's four pages of a tile, loaded one tile ahead,
+      // their page ids two. A page past the last node scales by 1 (K, masked anyway) and 0 (V).
+      const int32_t* bt_row = p.bt + (int64_t)s.seq * p.bt_stride;
+      auto scale_id = [&](int i) -> int {
+        const int blk = (2 * (s.ka + i) + w) * kHalfPages + (lane & 3);
+        if (lane >= 8 || i >= s.nk || blk >= s.pages) return -1;
+        const int page = __ldg(bt_row + blk);
+        return page < 0 || page >= p.g.P ? 0 : page;
+      };
+      auto scale_of = [&](int page) -> float {
+        if (page < 0) return (lane & 4) ? 0.f : 1.f;
+        const float f = __ldg(reinterpret_cast<const float*>(p.g.scales) +
+                              ((layer_base + page) * 2 + ((lane >> 2) & 1)) * p.g.H + s.h);
+        // (a K scale of 0 would turn masked scores, -inf, into NaN)
+        return (lane & 4) || f != f ? f : fmaxf(f, 1e-30f);
+      };
+      float sc_now = 0.f, sc_next = 0.f;
+      int sc_id = -1;
+      if (C::kFP8) {
+        sc_next = scale_of(scale_id(0));
+        sc_id = scale_id(1);
+      }
+      for (int i = 0; i < s.nk; ++i) {
+        const int x = two ? w : i & 1;
+        const int use = cnt[x] + (two ? i : i >> 1);
+        const int st = (gt + i) % kStages;
+        const int key0 = (s.ka + i) * kKeys;
+        const bool both = key0 + kHalf < s.L;
+        // this warpgroup's halves: one query tile: half w; two: both
+        const int h0 = two ? 0 : w, nh = two ? (both ? 2 : 1) : (w == 0 || both ? 1 : 0);
+        if (C::kFP8) {
+          sc_now = sc_next;
+          sc_next = scale_of(sc_id);
+          sc_id = scale_id(i + 2);
         }
-        // the V tile of S(g) cannot be replaced before P(g) is written, so this wait is for its own phase
-        if ((tail || C::kFP8) && !warp_wait_polled(&v_full[st], ((gt + jj) / kStages) & 1)) {
+        if (*abort_flag || !warp_wait_polled(&s_full[x], use & 1)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        if (live) {
-          float sv[kKeys];
-          {
+        const uint32_t col_s = kColS + (uint32_t)(x * kKeys);
+        if (live && nh > 0) {
+          float sv[kHalf];
+          auto load_half = [&](int h) {
             uint32_t r0[32], r1[32];
-            tmem_ld32(t_row + col_s + b * kKeys, r0);
-            tmem_ld32(t_row + col_s + b * kKeys + 32, r1);
+            tmem_ld32(t_row + col_s + h * kHalf, r0);
+            tmem_ld32(t_row + col_s + h * kHalf + 32, r1);
             tc_wait_ld();
 #pragma unroll
             for (int c = 0; c < 32; ++c) {
               sv[c] = __uint_as_float(r0[c]);
               sv[32 + c] = __uint_as_float(r1[c]);
             }
-          }
-          if (tail) {
-            const unsigned long long win = valid ? tree_window(mask, p.mask_words, s.n, key0 - s.ctx) : 0ull;
+            const int off = key0 + h * kHalf - s.ctx;
+            if (off + kHalf > 0) {
+              const unsigned long long win = valid ? tree_window(mask, p.mask_words, s.n, off) : 0ull;
+              const uint32_t lo = (uint32_t)win, hi = (uint32_t)(win >> 32);
 #pragma unroll
-            for (int c = 0; c < kKeys; ++c) sv[c] = ((win >> c) & 1) ? sv[c] : -INFINITY;
-          }
-          float ks[kTilePages], vs[kTilePages];
-          if (C::kFP8) {
-            const float4* sc = reinterpret_cast<const float4*>(base + C::kOffScale + ((gt + jj) % kScaleSlots) * 256);
-            const float4 a = sc[0], c = sc[1];
-            ks[0] = a.x * p.scale_log2; ks[1] = a.y * p.scale_log2; ks[2] = a.z * p.scale_log2; ks[3] = a.w * p.scale_log2;
-            vs[0] = c.x; vs[1] = c.y; vs[2] = c.z; vs[3] = c.w;
-          } else {
+              for (int c = 0; c < 32; ++c) {
+                sv[c] = (lo >> c) & 1 ? sv[c] : -INFINITY;
+                sv[32 + c] = (hi >> c) & 1 ? sv[32 + c] : -INFINITY;
+              }
+            }
+          };
+          float ks[kHalfPages], vs[kHalfPages];
 #pragma unroll
-            for (int q = 0; q < kTilePages; ++q) ks[q] = p.scale_log2;
+          for (int q = 0; q < kHalfPages; ++q) {
+            ks[q] = p.scale_log2;
+            if (C::kFP8) {
+              ks[q] *= __shfl_sync(0xffffffffu, sc_now, q);
+              vs[q] = __shfl_sync(0xffffffffu, sc_now, 4 + q);
+            }
           }
           // the row's largest score; the scale is positive
           float pm = -INFINITY;
-          if (C::kFP8) {
+#pragma unroll 1
+          for (int hh = 0; hh < nh; ++hh) {
+            load_half(h0 + hh);
+            float x4[4];  // (four short chains; FP8: one per page)
 #pragma unroll
-            for (int q = 0; q < kTilePages; ++q) {
-              float x = -INFINITY;
+            for (int q = 0; q < 4; ++q) {
+              x4[q] = sv[16 * q];
 #pragma unroll
-              for (int c = 0; c < 16; c += 2) x = fmax3(x, sv[16 * q + c], sv[16 * q + c + 1]);
-              pm = fmaxf(pm, x * ks[q]);
+              for (int c = 1; c < 15; c += 2) x4[q] = fmax3(x4[q], sv[16 * q + c], sv[16 * q + c + 1]);
+              x4[q] = fmaxf(x4[q], sv[16 * q + 15]);
+              if (C::kFP8) x4[q] *= ks[q];
             }
-          } else {
-#pragma unroll
-            for (int c = 0; c < kKeys; c += 2) pm = fmax3(pm, sv[c], sv[c + 1]);
-            pm *= p.scale_log2;
+            const float t = fmaxf(fmaxf(x4[0], x4[1]), fmaxf(x4[2], x4[3]));
+            pm = fmaxf(pm, C::kFP8 ? t : t * p.scale_log2);
           }
           // stale reference: it moves when a tile exceeds it by more than 2^8
           float alpha = 1.f;
@@ -814,11 +856,13 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
               }
               vref = 2.f * vm;
             }
-            inv_vref = vref > 0.f ? 1.f / vref : 0.f;
+            inv_vref = vref > 0.f ? __frcp_rn(vref) : 0.f;
           }
           if (__any_sync(0xffffffffu, rescale) && i > 0) {
             // O holds PV of this item's earlier tiles: wait for the last, then scale this warp's rows
-            if (!warp_wait_polled(&my_pv_done[(gj - 1) & 1], ((gj - 1) >> 1) & 1)) {
+            const int xp = two ? w : (i - 1) & 1;
+            const int usep = cnt[xp] + (two ? i - 1 : (i - 1) >> 1);
+            if (!warp_wait_polled(&pv_done[xp], usep & 1)) {
               ok = false;
               break;
             }
@@ -833,48 +877,63 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
               tmem_st32(t_row + col_o + cc * 32, r);
             }
             tc_wait_st();
+            // (the scores' registers were given up for this)
+            load_half(h0 + nh - 1);
           }
-          {
-            uint32_t ph[32], plo[32];
-            // 2^6 times the weight; a row that sees no key yet (m = -inf) has every score -inf: 2^-inf = 0
-            const float mm = (m == -INFINITY) ? 0.f : m - 6.f;
-            const uint64_t negm2 = f32x2(-mm, -mm);
+          // 2^6 times the weight; a row that sees no key yet (m = -inf) has every score -inf: 2^-inf = 0
+          const float mm = (m == -INFINITY) ? 0.f : m - 6.f;
+          const uint64_t negm2 = f32x2(-mm, -mm);
+          uint64_t ls2 = f32x2(0.f, 0.f);
+#pragma unroll 1
+          for (int hh = nh - 1; hh >= 0; --hh) {
+            if (hh < nh - 1) load_half(h0 + hh);
             const uint64_t minus1 = f32x2(-1.f, -1.f);
-            uint64_t ls2 = f32x2(0.f, 0.f);
 #pragma unroll
-            for (int q = 0; q < kTilePages; ++q) {
-              const uint64_t scale2 = f32x2(ks[q], ks[q]);
-              uint64_t v2 = 0;
-              if (C::kFP8) v2 = f32x2(vs[q] * inv_vref, vs[q] * inv_vref);
+            for (int q2 = 0; q2 < kHalfPages; q2 += 2) {  // 32 keys at a time
+              uint32_t ph[16], plo[16];
 #pragma unroll
-              for (int c = 8 * q; c < 8 * q + 8; ++c) {
-                float x0, x1;
-                f32x2_split(fma_f32x2(f32x2(sv[2 * c], sv[2 * c + 1]), scale2, negm2), x0, x1);
-                const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-                ls2 = add_f32x2(ls2, f32x2(p0, p1));
-                ph[c] = C::kFP8 ? mul_pack2<false>(p0, p1, v2) : pack2<kBF16>(p0, p1);
-                if (kBF16) {
-                  // lo = p - bf16(p), exact
-                  const uint64_t hi2 = f32x2(__uint_as_float(ph[c] << 16), __uint_as_float(ph[c] & 0xFFFF0000u));
-                  float l0, l1;
-                  f32x2_split(fma_f32x2(hi2, minus1, f32x2(p0, p1)), l0, l1);
-                  plo[c] = pack2<true>(l0, l1);
+              for (int q = q2; q < q2 + 2; ++q) {
+                const uint64_t scale2 = f32x2(ks[q], ks[q]);
+                uint64_t v2 = 0;
+                if (C::kFP8) v2 = f32x2(vs[q] * inv_vref, vs[q] * inv_vref);
+#pragma unroll
+                for (int c = 8 * q; c < 8 * q + 8; ++c) {
+                  const int d = c - 8 * q2;
+                  float x0, x1;
+                  f32x2_split(fma_f32x2(f32x2(sv[2 * c], sv[2 * c + 1]), scale2, negm2), x0, x1);
+                  const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+                  ls2 = add_f32x2(ls2, f32x2(p0, p1));
+                  ph[d] = C::kFP8 ? mul_pack2<false>(p0, p1, v2) : pack2<kBF16>(p0, p1);
+                  if (kBF16) {
+                    // lo = p - bf16(p), exact
+                    const uint64_t hi2 = f32x2(__uint_as_float(ph[d] << 16), __uint_as_float(ph[d] & 0xFFFF0000u));
+                    float l0, l1;
+                    f32x2_split(fma_f32x2(hi2, minus1, f32x2(p0, p1)), l0, l1);
+                    plo[d] = pack2<true>(l0, l1);
+                  }
                 }
               }
+              const uint32_t pc = t_row + col_s + (h0 + hh) * kHalf + 8 * q2;
+              tmem_st16(pc, ph);
+              if (kBF16) tmem_st16(pc + 32, plo);
             }
-            float ls0, ls1;
-            f32x2_split(ls2, ls0, ls1);
-            tmem_st32(t_row + col_s + b * kKeys, ph);
-            if (kBF16) tmem_st32(t_row + col_s + b * kKeys + 32, plo);
-            l += ls0 + ls1;
-            tc_wait_st();
           }
+          float ls0, ls1;
+          f32x2_split(ls2, ls0, ls1);
+          l += ls0 + ls1;
+          tc_wait_st();
         }
-        if (tail && (!two || w == 0)) {
-          // V rows past the last node become 0, and so does what is not finite in a node's row (noted)
+        if (key0 + kKeys > s.ctx && (!two || w == 0)) {
+          // V rows past the last node become 0, and so does what is not finite in a node's row (noted). The V tile of
+          // S(i) cannot be replaced before P(i) is written, and the one before it in this slot was complete before S(i)
+          // (its PV went out earlier): the wait is for this tile's phase.
+          if (!warp_wait_polled(&v_full[st], ((gt + i) / kStages) & 1)) {
+            ok = false;
+            break;
+          }
           uint8_t* vt = base + C::kOffV + st * kSlot;
-          const int r0 = max(0, s.ctx - key0);
-          for (int c = row; c < (kKeys - r0) * 16; c += 128) {
+          const int r0 = max(h0 * kHalf, s.ctx - key0), r1 = (h0 + nh) * kHalf;
+          for (int c = row; c < (r1 - r0) * 16; c += 128) {
             const int r = r0 + (c >> 4), ch = c & 15;
             const int key = key0 + r;
             uint4* cell = reinterpret_cast<uint4*>(vt + (r >> 4) * kPageTile + ((r >> 3) & 1) * 2048 + (ch >> 3) * 1024 +
@@ -883,8 +942,8 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
               *cell = make_uint4(0u, 0u, 0u, 0u);
             } else {
               constexpr uint32_t kExp = kBF16 ? 0x7F80u : 0x7C00u;
-              uint4 x = *cell;
-              uint32_t* xs = &x.x;
+              uint4 xv = *cell;
+              uint32_t xs[4] = {xv.x, xv.y, xv.z, xv.w};
               bool hit = false;
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
@@ -892,7 +951,7 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
                 if ((xs[e] & (kExp << 16)) == (kExp << 16)) { xs[e] &= 0x0000FFFFu; hit = true; }
               }
               if (hit) {
-                *cell = x;
+                *cell = make_uint4(xs[0], xs[1], xs[2], xs[3]);
                 atomicOr(bad + ((key - s.ctx) >> 6), 1ull << ((key - s.ctx) & 63));
               }
             }
@@ -901,14 +960,17 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&my_p_full[b]);
+        if (lane == 0) mbar_arrive_n(&p_full[x], two ? 2 : 1);  // 8 arrivals either way
       }
       if (!ok) break;
-      // ---- the item's result, once this warpgroup's last PV finished
-      const int glast = g + n - 1;
-      if (n > 0 && !warp_wait_polled(&my_pv_done[glast & 1], (glast >> 1) & 1)) {
-        ok = false;
-        break;
+      // ---- the item's result, once its last PV finished
+      {
+        const int i = s.nk - 1, x = two ? w : i & 1;
+        const int use = cnt[x] + (two ? i : i >> 1);
+        if (!warp_wait_polled(&pv_done[x], use & 1)) {
+          ok = false;
+          break;
+        }
       }
       // (idle warps of a half-empty tile have the same reference V scale as the others: rows they hold are not written)
       s_ml[w * kRows + row] = make_float2(m, l);
@@ -924,7 +986,7 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
       }
       tc_fence_after();
       // one query tile: O[0] and O[1] join, warpgroup w writes dims 64 w ..; two: its own rows
-      const bool join = !two && s.nk > 1;
+      const bool join = !two && s.ka * kKeys + kHalf < s.L;  // a second half held keys
       float f0, f1 = 0.f, M, Lsum;
       if (two) {
         M = m;
@@ -1006,8 +1068,9 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_empty);
-      g += n;
       gt += s.nk;
+      cnt[0] += two ? s.nk : (s.nk + 1) >> 1;
+      cnt[1] += two ? s.nk : s.nk >> 1;
       more = tree_next(p, cum, walk, s);
       if (more) load_q(s);
     }
@@ -1088,9 +1151,11 @@ int ensure_tree_tmap(sckv_pool* p) {
 }
 
 // Rows of a partial slot: a group's rows, at most.
-int tree_part_rows(int n_tokens, int mask_words, int G) {
+int tree_group_rows(const sckv_pool* p) { return sckv_elem_bytes(p->kv_dtype) == 1 ? kRows : 2 * kRows; }
+
+int tree_part_rows(const sckv_pool* p, int n_tokens, int mask_words, int G) {
   const int64_t rows = (int64_t)(n_tokens < 64 * mask_words ? n_tokens : 64 * mask_words) * G;
-  return rows > kRows ? 2 * kRows : kRows;
+  return rows > kRows ? tree_group_rows(p) : kRows;
 }
 
 size_t tree_head_bytes(const sckv_pool* p) { return ((size_t)p->num_sms * sizeof(JoinHead) + 255) / 256 * 256; }
@@ -1116,7 +1181,7 @@ int launch_tree(sckv_pool* p, const TreeParams& t, cudaStream_t stream) {
 
 extern "C" size_t sckv_tree_attn_workspace_bytes(const sckv_pool* p, int n_tokens, int num_q_heads) {
   if (p == nullptr || n_tokens <= 0 || num_q_heads <= 0) return 0;
-  const int rows = tree_part_rows(n_tokens, kMaskWordsMax, num_q_heads / p->num_kv_heads);
+  const int rows = tree_part_rows(p, n_tokens, kMaskWordsMax, num_q_heads / p->num_kv_heads);
   return tree_head_bytes(p) + (size_t)p->num_sms * 2 * rows * (kHD + 2) * sizeof(float);
 }
 
@@ -1141,7 +1206,7 @@ extern "C" int sckv_tree_attn(sckv_pool* p, int layer, const void* q, int q_dtyp
     return SCKV_ERR_INVALID_ARG;
   const int G = num_q_heads / p->num_kv_heads;
   // tile and box numbers are 32-bit
-  const int64_t groups = ((int64_t)(n_tokens < 64 * mask_words ? n_tokens : 64 * mask_words) * G + 2 * kRows - 1) / (2 * kRows);
+  const int64_t groups = ((int64_t)(n_tokens < 64 * mask_words ? n_tokens : 64 * mask_words) * G + kRows - 1) / kRows;
   if (n_seqs > kMaxSeqs || max_blocks > INT32_MAX / SCKV_PAGE_TOKENS ||
       (int64_t)n_seqs * (max_blocks / kTilePages + 1) * groups * p->num_kv_heads > INT32_MAX ||
       (int64_t)p->num_layers * p->max_pages * 2 * p->num_kv_heads > INT32_MAX)
@@ -1167,7 +1232,8 @@ extern "C" int sckv_tree_attn(sckv_pool* p, int layer, const void* q, int q_dtyp
   t.scale_log2 = scale * 1.4426950408889634f;
   t.heads = reinterpret_cast<JoinHead*>(workspace);
   t.parts = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + tree_head_bytes(p));
-  t.part_rows = tree_part_rows(n_tokens, mask_words, G);
+  t.group_rows = tree_group_rows(p);
+  t.part_rows = tree_part_rows(p, n_tokens, mask_words, G);
   SCKV_DEVICE_GUARD(p->device);
   cudaStream_t s = as_stream(stream);
   switch (p->kv_dtype) {

@@ -21,7 +21,11 @@
 // every tile each, with their own reference, sum and O accumulator, joined
 // at the end of the item; S has two buffers, so the next tile's scores are
 // made while this one's are weighed. With two query tiles each warpgroup owns one and
-// both use every K/V tile. Either way a tile costs 8 MMAs of 128 x 128 x 16 for
+// both use every K/V tile. An item of at most 64 (32) rows fills the query
+// tile with 2 (4) copies of them, and each copy weighs only its 32 (16) keys
+// of the half (P is 0 elsewhere): the lanes of tensor memory that would be
+// idle share the softmax, whose time per tile falls accordingly, and the
+// copies' sums and O are joined like those of the warpgroups. Either way a tile costs 8 MMAs of 128 x 128 x 16 for
 // S per query tile and 8 for P V (16 with P in two parts): narrower S
 // products (64 keys) take the same time each, limited by their operands'
 // shared-memory reads (measured 60 - 150 cycles against 64).
@@ -53,6 +57,7 @@
 // tile and added to the rows that see them at the end.
 #include <cuda.h>
 #include <math.h>
+#include <type_traits>
 
 #include "sckv_geo.cuh"
 #include "sckv_mma_common.cuh"
@@ -97,10 +102,10 @@ struct TreeCfg {
   static constexpr int kOffStage = kOffV + kStages * kSlot;
   static constexpr int kOffScale = kOffStage + kStaging * kHalfSlot;
   static constexpr int kOffBar = kOffScale + (kINT8 ? kScaleSlots * 256 : 0);
-  static constexpr int kNumBars = 4 * kStages + 6 + 4 + 2 * kStaging;
+  static constexpr int kNumBars = 4 * kStages + 6 + 7 + 2 * kStaging;
   static constexpr int kOffMl = kOffBar + ((kNumBars * 8 + 15) / 16) * 16;  // float2 [2][128]: m, l of a row
-  static constexpr int kOffVref = kOffMl + 2 * kRows * 8;                   // float [2]
-  static constexpr int kOffBad = kOffVref + 16;                             // u64 [2][4]: nodes whose V is not finite
+  static constexpr int kOffVref = kOffMl + 2 * kRows * 8;                   // float [2][4]: V scale of a warp's O
+  static constexpr int kOffBad = kOffVref + 32;                             // u64 [2][4]: nodes whose V is not finite
   static constexpr int kOffTmem = kOffBad + 64;
   static constexpr int kOffAbort = kOffTmem + 4;
   static constexpr int kOffPartial = kOffTmem + 16;                         // int [kThreadsTree]
@@ -159,6 +164,7 @@ struct TreeSeg {
   int seq, h, n, ctx, L;
   int kt, ka, nk;         // the item's key tiles; first one here and how many
   int row0, rows, nq;     // first row of the group, rows of it, query tiles (1 or 2)
+  int copies;             // copies of the rows in the query tile (1, 2, 4)
   int q_base, pages;      // first token; pages of the sequence
 };
 
@@ -176,6 +182,7 @@ __device__ __forceinline__ bool tree_next(const TreeParams& p, const int* cum, T
   s.row0 = (item - s.h * groups) * p.group_rows;
   s.rows = min(p.group_rows, s.n * p.G - s.row0);
   s.nq = s.rows > kRows ? 2 : 1;
+  s.copies = s.rows <= kRows / 4 ? 4 : s.rows <= kRows / 2 ? 2 : 1;
   s.L = s.ctx + s.n;
   s.pages = (s.L + SCKV_PAGE_TOKENS - 1) / SCKV_PAGE_TOKENS;
   s.q_base = __ldg(p.cu_q + s.seq);
@@ -231,14 +238,19 @@ __device__ __forceinline__ bool warp_wait_polled(uint64_t* bar, uint32_t parity)
   return __all_sync(0xffffffffu, mbar_wait_polled(bar, parity, SCKV_WAIT_LIMIT_NS));
 }
 
-// 16 columns of this thread's tensor memory lane.
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+// 8 / 16 columns of this thread's tensor memory lane.
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
 }
 
 __device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
@@ -274,7 +286,9 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
   uint64_t* q_full = o_empty + 1;            // the item's Q is in shared memory (one arrival per softmax warp)
   uint64_t* mma_done = q_full + 1;           // every issued MMA finished
   uint64_t* o_full = mma_done + 1;           // the item's sums are written and its O is complete (one arrival per softmax warp)
-  uint64_t* st_full = o_full + 1;            // one-byte pools: [SS] staged half tile landed, its scales are written
+  uint64_t* x_full = o_full + 1;             // [w] a piece of O is in the exchange buffer (one arrival per warp of w)
+  uint64_t* x_done = x_full + 2;             // the exchange buffer was read (one arrival per softmax warp)
+  uint64_t* st_full = x_done + 1;            // one-byte pools: [SS] staged half tile landed, its scales are written
   uint64_t* st_empty = st_full + C::kStaging;  // [SS] decoded (one arrival per decoding warp)
   float2* s_ml = reinterpret_cast<float2*>(base + C::kOffMl);
   float* s_vref = reinterpret_cast<float*>(base + C::kOffVref);
@@ -312,7 +326,8 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
         uint32_t count = 1;
         if (C::kB8 && ((bar >= k_full && bar < k_full + kStages) || (bar >= v_full && bar < v_full + kStages))) count = 4;
         if (bar >= p_full && bar < p_full + 2) count = 8;
-        if (bar == o_empty || bar == q_full || bar == o_full) count = 8;
+        if (bar == o_empty || bar == q_full || bar == o_full || bar == x_done) count = 8;
+        if (bar == x_full || bar == x_full + 1) count = 4;
         if (C::kB8 && bar >= st_full && bar < st_full + C::kStaging) count = 2;
         if (C::kB8 && bar >= st_empty && bar < st_empty + C::kStaging) count = 4;
         mbar_init(bar, count);
@@ -721,7 +736,8 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
           const int c = t + (b8 + i) * step;
           const int r = c >> 4, half = (c >> 3) & 1, ch = c & 7;
           if (tile_row0 + r < s.rows)
-            *reinterpret_cast<uint4*>(q_tile + half * kQHalf + r * 128 + ((ch ^ (r & 7)) << 4)) = v[i];
+            for (int e = 0; e < kRows; e += kRows / s.copies)
+              *reinterpret_cast<uint4*>(q_tile + half * kQHalf + (r + e) * 128 + ((ch ^ (r & 7)) << 4)) = v[i];
         }
       }
       fence_proxy_async_smem();
@@ -734,9 +750,15 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
     TreeSeg s;
     bool more = tree_next(p, cum, walk, s);
     if (more) load_q(s);
-    for (int k = 0; ok && more; ++k) {
-      const bool two = C::kQTiles == 2 && s.nq == 2;
-      const int r_in = (two ? w * kRows : 0) + row;  // row of the group
+    int xchg = 0;  // uses of the exchange buffer
+    // One item (or part of one); false if a wait ran out. kTwo: two query tiles; kCopies: copies of the rows.
+    auto run_item = [&](auto two_c, auto copies_c, const int k) -> bool {
+      constexpr bool two = decltype(two_c)::value;
+      constexpr int R = decltype(copies_c)::value;
+      constexpr int kCols = kHalf / R;       // keys of a half that this thread weighs
+      constexpr int kPg = kCols / SCKV_PAGE_TOKENS;
+      const int copy = row / (kRows / R);
+      const int r_in = (two ? w * kRows : 0) + (row & (kRows / R - 1));  // row of the group
       const bool valid = r_in < s.rows;
       const int node = (s.row0 + r_in) / p.G;
       const int head = s.h * p.G + (s.row0 + r_in) - node * p.G;
@@ -744,7 +766,7 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
       const bool live = __any_sync(0xffffffffu, valid);
       unsigned long long* bad = s_bad + (k & 1) * kMaskWordsMax;
       float m = -INFINITY, l = 0.f;
-      float vref = 0.f;  // FP8: the V scale that O counts in
+      float vref = 0.f;  // FP8: the V scale that this warp's O counts in
       // FP8: lanes 0-3 the K, 4-7 the V scales of this warpgroup's four pages of a tile, loaded one tile ahead,
       // their page ids two. A page past the last node scales by 1 (K, masked anyway) and 0 (V).
       const int32_t* bt_row = p.bt + (int64_t)s.seq * p.bt_stride;
@@ -761,111 +783,114 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
         // (a K scale of 0 would turn masked scores, -inf, into NaN)
         return (lane & 4) || f != f ? f : fmaxf(f, 1e-30f);
       };
-      float sc_now = 0.f, sc_next = 0.f;
+      float sc_next = 0.f;
       int sc_id = -1;
       if (C::kFP8) {
         sc_next = scale_of(scale_id(0));
         sc_id = scale_id(1);
       }
+#pragma unroll 1
       for (int i = 0; i < s.nk; ++i) {
         const int x = two ? w : i & 1;
         const int use = cnt[x] + (two ? i : i >> 1);
-        const int st = (gt + i) % kStages;
         const int key0 = (s.ka + i) * kKeys;
         const bool both = key0 + kHalf < s.L;
         // this warpgroup's halves: one query tile: half w; two: both
         const int h0 = two ? 0 : w, nh = two ? (both ? 2 : 1) : (w == 0 || both ? 1 : 0);
+        // (what does not need the scores comes before the wait for them)
+        float ks[kPg], vs[kPg];
+        float alpha = 1.f, inv_vref = 0.f;
+        bool rescale = false;
+#pragma unroll
+        for (int q = 0; q < kPg; ++q) ks[q] = p.scale_log2;
         if (C::kFP8) {
-          sc_now = sc_next;
+          const float sc_now = sc_next;
           sc_next = scale_of(sc_id);
           sc_id = scale_id(i + 2);
-        }
-        if (*abort_flag || !warp_wait_polled(&s_full[x], use & 1)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t col_s = kColS + (uint32_t)(x * kKeys);
-        if (live && nh > 0) {
-          float sv[kHalf];
-          auto load_half = [&](int h) {
-            uint32_t r0[32], r1[32];
-            tmem_ld32(t_row + col_s + h * kHalf, r0);
-            tmem_ld32(t_row + col_s + h * kHalf + 32, r1);
-            tc_wait_ld();
+          float vm = 0.f;
 #pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              sv[c] = __uint_as_float(r0[c]);
-              sv[32 + c] = __uint_as_float(r1[c]);
+          for (int q = 0; q < kPg; ++q) {
+            ks[q] *= __shfl_sync(0xffffffffu, sc_now, copy * kPg + q);
+            vs[q] = __shfl_sync(0xffffffffu, sc_now, 4 + copy * kPg + q);
+            vm = fmaxf(vm, vs[q]);
+          }
+          if (vm > vref) {  // (the same for the whole warp) twice the largest: growth below 2 needs no rescale
+            if (vref > 0.f) {
+              alpha = vref / (2.f * vm);
+              rescale = true;
             }
-            const int off = key0 + h * kHalf - s.ctx;
-            if (off + kHalf > 0) {
+            vref = 2.f * vm;
+          }
+          inv_vref = vref > 0.f ? __frcp_rn(vref) : 0.f;
+        }
+        if (*abort_flag || !warp_wait_polled(&s_full[x], use & 1)) return false;
+        tc_fence_after();
+        const uint32_t col_s = t_row + kColS + (uint32_t)(x * kKeys);
+        if (live && nh > 0) {
+          float sv[kCols];
+          auto load_half = [&](int h) {
+            if constexpr (kCols == 64) {
+              uint32_t r0[32], r1[32];
+              tmem_ld32(col_s + h * kHalf, r0);
+              tmem_ld32(col_s + h * kHalf + 32, r1);
+              tc_wait_ld();
+#pragma unroll
+              for (int c = 0; c < 32; ++c) {
+                sv[c] = __uint_as_float(r0[c]);
+                sv[32 + c] = __uint_as_float(r1[c]);
+              }
+            } else if constexpr (kCols == 32) {
+              uint32_t r0[32];
+              tmem_ld32(col_s + h * kHalf + copy * 32, r0);
+              tc_wait_ld();
+#pragma unroll
+              for (int c = 0; c < 32; ++c) sv[c] = __uint_as_float(r0[c]);
+            } else {
+              uint32_t r0[16];
+              tmem_ld16(col_s + h * kHalf + copy * 16, r0);
+              tc_wait_ld();
+#pragma unroll
+              for (int c = 0; c < 16; ++c) sv[c] = __uint_as_float(r0[c]);
+            }
+            const int off = key0 + h * kHalf + copy * kCols - s.ctx;
+            if (off + kCols > 0) {
               const unsigned long long win = valid ? tree_window(mask, p.mask_words, s.n, off) : 0ull;
               const uint32_t lo = (uint32_t)win, hi = (uint32_t)(win >> 32);
 #pragma unroll
-              for (int c = 0; c < 32; ++c) {
-                sv[c] = (lo >> c) & 1 ? sv[c] : -INFINITY;
-                sv[32 + c] = (hi >> c) & 1 ? sv[32 + c] : -INFINITY;
-              }
+              for (int c = 0; c < kCols; ++c) sv[c] = ((c < 32 ? lo : hi) >> (c & 31)) & 1 ? sv[c] : -INFINITY;
             }
           };
-          float ks[kHalfPages], vs[kHalfPages];
-#pragma unroll
-          for (int q = 0; q < kHalfPages; ++q) {
-            ks[q] = p.scale_log2;
-            if (C::kFP8) {
-              ks[q] *= __shfl_sync(0xffffffffu, sc_now, q);
-              vs[q] = __shfl_sync(0xffffffffu, sc_now, 4 + q);
-            }
-          }
           // the row's largest score; the scale is positive
           float pm = -INFINITY;
 #pragma unroll 1
           for (int hh = 0; hh < nh; ++hh) {
             load_half(h0 + hh);
-            float x4[4];  // (four short chains; FP8: one per page)
+            float t = -INFINITY;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              x4[q] = sv[16 * q];
+            for (int q = 0; q < kPg; ++q) {  // (a short chain per page)
+              float y = sv[16 * q];
 #pragma unroll
-              for (int c = 1; c < 15; c += 2) x4[q] = fmax3(x4[q], sv[16 * q + c], sv[16 * q + c + 1]);
-              x4[q] = fmaxf(x4[q], sv[16 * q + 15]);
-              if (C::kFP8) x4[q] *= ks[q];
+              for (int c = 1; c < 15; c += 2) y = fmax3(y, sv[16 * q + c], sv[16 * q + c + 1]);
+              y = fmaxf(y, sv[16 * q + 15]);
+              t = fmaxf(t, y * ks[q]);
             }
-            const float t = fmaxf(fmaxf(x4[0], x4[1]), fmaxf(x4[2], x4[3]));
-            pm = fmaxf(pm, C::kFP8 ? t : t * p.scale_log2);
+            pm = fmaxf(pm, t);
           }
           // stale reference: it moves when a tile exceeds it by more than 2^8
-          float alpha = 1.f;
-          bool rescale = false;
           if (pm > m + 8.f) {
             if (m != -INFINITY) {
-              alpha = ex2_approx(m - pm);
+              const float e = ex2_approx(m - pm);
+              alpha *= e;
+              l *= e;
               rescale = true;
             }
             m = pm;
-            l *= alpha;
-          }
-          float inv_vref = 0.f;
-          if (C::kFP8) {
-            const float vm = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
-            if (vm > vref) {  // (the same for the whole warpgroup) twice the largest: growth below 2 needs no rescale
-              if (vref > 0.f) {
-                alpha *= vref / (2.f * vm);
-                rescale = true;
-              }
-              vref = 2.f * vm;
-            }
-            inv_vref = vref > 0.f ? __frcp_rn(vref) : 0.f;
           }
           if (__any_sync(0xffffffffu, rescale) && i > 0) {
             // O holds PV of this item's earlier tiles: wait for the last, then scale this warp's rows
             const int xp = two ? w : (i - 1) & 1;
             const int usep = cnt[xp] + (two ? i - 1 : (i - 1) >> 1);
-            if (!warp_wait_polled(&pv_done[xp], usep & 1)) {
-              ok = false;
-              break;
-            }
+            if (!warp_wait_polled(&pv_done[xp], usep & 1)) return false;
             tc_fence_after();
 #pragma unroll 1
             for (int cc = 0; cc < 4; ++cc) {
@@ -882,40 +907,44 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
           }
           // 2^6 times the weight; a row that sees no key yet (m = -inf) has every score -inf: 2^-inf = 0
           const float mm = (m == -INFINITY) ? 0.f : m - 6.f;
-          const uint64_t negm2 = f32x2(-mm, -mm);
+          const uint64_t negm2 = f32x2(-mm, -mm), minus1 = f32x2(-1.f, -1.f);
           uint64_t ls2 = f32x2(0.f, 0.f);
 #pragma unroll 1
           for (int hh = nh - 1; hh >= 0; --hh) {
-            if (hh < nh - 1) load_half(h0 + hh);
-            const uint64_t minus1 = f32x2(-1.f, -1.f);
+            if (two && hh < nh - 1) load_half(h0 + hh);
+            const uint32_t pc = col_s + (h0 + hh) * kHalf;
 #pragma unroll
-            for (int q2 = 0; q2 < kHalfPages; q2 += 2) {  // 32 keys at a time
-              uint32_t ph[16], plo[16];
+            for (int q = 0; q < kPg; ++q) {  // a page (16 keys) at a time
+              uint32_t ph[8], plo[8];
+              const uint64_t scale2 = f32x2(ks[q], ks[q]);
+              uint64_t v2 = 0;
+              if (C::kFP8) v2 = f32x2(vs[q] * inv_vref, vs[q] * inv_vref);
 #pragma unroll
-              for (int q = q2; q < q2 + 2; ++q) {
-                const uint64_t scale2 = f32x2(ks[q], ks[q]);
-                uint64_t v2 = 0;
-                if (C::kFP8) v2 = f32x2(vs[q] * inv_vref, vs[q] * inv_vref);
-#pragma unroll
-                for (int c = 8 * q; c < 8 * q + 8; ++c) {
-                  const int d = c - 8 * q2;
-                  float x0, x1;
-                  f32x2_split(fma_f32x2(f32x2(sv[2 * c], sv[2 * c + 1]), scale2, negm2), x0, x1);
-                  const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-                  ls2 = add_f32x2(ls2, f32x2(p0, p1));
-                  ph[d] = C::kFP8 ? mul_pack2<false>(p0, p1, v2) : pack2<kBF16>(p0, p1);
-                  if (kBF16) {
-                    // lo = p - bf16(p), exact
-                    const uint64_t hi2 = f32x2(__uint_as_float(ph[d] << 16), __uint_as_float(ph[d] & 0xFFFF0000u));
-                    float l0, l1;
-                    f32x2_split(fma_f32x2(hi2, minus1, f32x2(p0, p1)), l0, l1);
-                    plo[d] = pack2<true>(l0, l1);
-                  }
+              for (int d = 0; d < 8; ++d) {
+                float x0, x1;
+                f32x2_split(fma_f32x2(f32x2(sv[16 * q + 2 * d], sv[16 * q + 2 * d + 1]), scale2, negm2), x0, x1);
+                const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+                ls2 = add_f32x2(ls2, f32x2(p0, p1));
+                ph[d] = C::kFP8 ? mul_pack2<false>(p0, p1, v2) : pack2<kBF16>(p0, p1);
+                if (kBF16) {
+                  // lo = p - bf16(p), exact
+                  const uint64_t hi2 = f32x2(__uint_as_float(ph[d] << 16), __uint_as_float(ph[d] & 0xFFFF0000u));
+                  float l0, l1;
+                  f32x2_split(fma_f32x2(hi2, minus1, f32x2(p0, p1)), l0, l1);
+                  plo[d] = pack2<true>(l0, l1);
                 }
               }
-              const uint32_t pc = t_row + col_s + (h0 + hh) * kHalf + 8 * q2;
-              tmem_st16(pc, ph);
-              if (kBF16) tmem_st16(pc + 32, plo);
+              tmem_st8(pc + 8 * (copy * kPg + q), ph);
+              if (kBF16) tmem_st8(pc + 32 + 8 * (copy * kPg + q), plo);
+            }
+            if constexpr (R > 1) {  // the keys of the other copies
+              const uint32_t z[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+#pragma unroll
+              for (int q = 0; q < kHalfPages - kPg; ++q) {
+                const int pg = q < copy * kPg ? q : q + kPg;
+                tmem_st8(pc + 8 * pg, z);
+                if (kBF16) tmem_st8(pc + 32 + 8 * pg, z);
+              }
             }
           }
           float ls0, ls1;
@@ -927,12 +956,11 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
           // V rows past the last node become 0, and so does what is not finite in a node's row (noted). The V tile of
           // S(i) cannot be replaced before P(i) is written, and the one before it in this slot was complete before S(i)
           // (its PV went out earlier): the wait is for this tile's phase.
-          if (!warp_wait_polled(&v_full[st], ((gt + i) / kStages) & 1)) {
-            ok = false;
-            break;
-          }
+          const int st = (gt + i) % kStages;
+          if (!warp_wait_polled(&v_full[st], ((gt + i) / kStages) & 1)) return false;
           uint8_t* vt = base + C::kOffV + st * kSlot;
           const int r0 = max(h0 * kHalf, s.ctx - key0), r1 = (h0 + nh) * kHalf;
+#pragma unroll 1
           for (int c = row; c < (r1 - r0) * 16; c += 128) {
             const int r = r0 + (c >> 4), ch = c & 15;
             const int key = key0 + r;
@@ -962,45 +990,45 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive_n(&p_full[x], two ? 2 : 1);  // 8 arrivals either way
       }
-      if (!ok) break;
       // ---- the item's result, once its last PV finished
       {
         const int i = s.nk - 1, x = two ? w : i & 1;
         const int use = cnt[x] + (two ? i : i >> 1);
-        if (!warp_wait_polled(&pv_done[x], use & 1)) {
-          ok = false;
-          break;
-        }
+        if (!warp_wait_polled(&pv_done[x], use & 1)) return false;
       }
-      // (idle warps of a half-empty tile have the same reference V scale as the others: rows they hold are not written)
       s_ml[w * kRows + row] = make_float2(m, l);
-      if (row == 0) s_vref[w] = C::kFP8 ? vref : 1.f;
+      if (lane == 0) s_vref[w * 4 + quad] = C::kFP8 ? vref : 1.f;
       // both warpgroups' O are complete and every S product has finished (a bounded wait, not a named barrier: a
       // warp that gave up must not leave the others waiting)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_full);
-      if (!warp_wait_polled(o_full, k & 1)) {
-        ok = false;
-        break;
-      }
+      if (!warp_wait_polled(o_full, k & 1)) return false;
       tc_fence_after();
-      // one query tile: O[0] and O[1] join, warpgroup w writes dims 64 w ..; two: its own rows
+      // one query tile: O[0] and O[1] (and the copies) join, warpgroup w writes dims 64 w ..; two: its own rows
       const bool join = !two && s.ka * kKeys + kHalf < s.L;  // a second half held keys
-      float f0, f1 = 0.f, M, Lsum;
-      if (two) {
-        M = m;
-        Lsum = l;
-        f0 = C::kFP8 ? vref : 1.f;
-      } else {
-        const float2 a = s_ml[row], c = join ? s_ml[kRows + row] : make_float2(-INFINITY, 0.f);
-        M = fmaxf(a.x, c.x);
-        const float e0 = a.x == -INFINITY ? 1.f : ex2_approx(a.x - M);
-        const float e1 = c.x == -INFINITY ? 1.f : ex2_approx(c.x - M);
-        Lsum = a.y * e0 + (join ? c.y * e1 : 0.f);
-        f0 = e0 * s_vref[0];
-        f1 = join ? e1 * s_vref[1] : 0.f;
+      float f0 = 1.f, f1 = 0.f, M = m, Lsum = l;
+      if constexpr (!two) {
+        M = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < R; ++e) {
+          const int o = (row & (kRows / R - 1)) + e * (kRows / R);
+          M = fmaxf(M, s_ml[o].x);
+          if (join) M = fmaxf(M, s_ml[kRows + o].x);
+        }
+        auto weight = [&](float mx) { return mx == -INFINITY ? 1.f : ex2_approx(mx - M); };
+        Lsum = 0.f;
+#pragma unroll
+        for (int e = 0; e < R; ++e) {
+          const int o = (row & (kRows / R - 1)) + e * (kRows / R);
+          Lsum = fmaf(s_ml[o].y, weight(s_ml[o].x), Lsum);
+          if (join) Lsum = fmaf(s_ml[kRows + o].y, weight(s_ml[kRows + o].x), Lsum);
+        }
+        f0 = weight(s_ml[row].x);
+        if (join) f1 = weight(s_ml[kRows + row].x);
       }
+      f0 *= s_vref[two ? w * 4 + quad : quad];
+      f1 *= s_vref[4 + quad];
       const bool full = s.nk == s.kt;
       if (full) {
         const float inv = Lsum == 0.f ? 0.f : 1.f / Lsum;  // no key seen: zeros; NaN stays NaN
@@ -1010,59 +1038,120 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
       const int d0 = two ? 0 : 64 * w, nd = two ? kHD : 64;
       const int64_t obase = ((int64_t)(s.q_base + node) * p.hq + head) * kHD;
       float* part = p.parts + (int64_t)(2 * blockIdx.x + (k > 0 ? 1 : 0)) * slot_floats(p.part_rows);
-      if (live) {
+      auto put4 = [&](int d, float a, float b, float c, float e) {
+        if (full)
+          tree_store4(p.out, obase + d, p.out_dtype, a, b, c, e);
+        else
+          reinterpret_cast<float4*>(part)[(int64_t)(d >> 2) * p.part_rows + r_in] = make_float4(a, b, c, e);
+      };
+      // f(word, pos): the nodes that this row sees and whose V is not finite somewhere, by their position
+      auto each_bad = [&](auto f) {
+#pragma unroll 1
+        for (int wd = 0; wd < p.mask_words; ++wd) {
+          unsigned long long hit = bad[wd];
+          if (hit) hit &= tree_window(mask, p.mask_words, s.n, 64 * wd);
+#pragma unroll 1
+          for (; hit; hit &= hit - 1) {
+            const int pos = s.ctx + 64 * wd + __ffsll((long long)hit) - 1;
+            int page = __ldg(bt_row + pos / SCKV_PAGE_TOKENS);
+            if (page < 0 || page >= p.g.P) page = 0;
+            f(page, pos % SCKV_PAGE_TOKENS);
+          }
+        }
+      };
+      // this thread's merged O, 32 dims from d0 + cc
+      auto merged = [&](int cc, float (&y)[32]) {
+        uint32_t r[32];
+        tmem_ld32(t_row + kColO + (two ? w * kHD : 0) + d0 + cc, r);
+        tc_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 32; ++c) y[c] = __uint_as_float(r[c]) * f0;
+        if (join) {
+          tmem_ld32(t_row + kColO + kHD + d0 + cc, r);
+          tc_wait_ld();
+#pragma unroll
+          for (int c = 0; c < 32; ++c) y[c] = fmaf(__uint_as_float(r[c]), f1, y[c]);
+        }
+      };
+      if constexpr (R == 1) {
+        if (live) {
+#pragma unroll 1
+          for (int cc = 0; cc < nd; cc += 32) {
+            float y[32];
+            merged(cc, y);
+            if (valid) {
+#pragma unroll
+              for (int c = 0; c < 32; c += 4) put4(d0 + cc + c, y[c], y[c + 1], y[c + 2], y[c + 3]);
+            }
+            __syncwarp();
+          }
+          if (valid) {
+            each_bad([&](int page, int slot) {
+#pragma unroll 1
+              for (int d = d0; d < d0 + nd; ++d) {
+                const float v = tree_v(p.g, p.layer, page, s.h, slot, d);
+                if (isfinite(v)) continue;
+                if (full)
+                  sckv_store_from_float(p.out, obase + d, p.out_dtype,
+                                        sckv_load_as_float(p.out, obase + d, p.out_dtype) + v);
+                else
+                  part[((int64_t)(d >> 2) * p.part_rows + r_in) * 4 + (d & 3)] += v;
+              }
+            });
+          }
+        }
+      } else {
+        // the copies' rows are added up through the (now idle) Q tile, 32 dims of each warpgroup at a time:
+        // [w][row] of 128 bytes, 16-byte chunks swizzled by the row
+        float* xb = reinterpret_cast<float*>(base) + w * kRows * 32;
 #pragma unroll 1
         for (int cc = 0; cc < nd; cc += 32) {
-          uint32_t r[32], r1[32];
-          tmem_ld32(t_row + kColO + (two ? w * kHD : 0) + d0 + cc, r);
-          if (join) tmem_ld32(t_row + kColO + kHD + d0 + cc, r1);
-          tc_wait_ld();
-          if (valid) {
+          {
+            float y[32];
+            merged(cc, y);
+            float4* mine = reinterpret_cast<float4*>(xb + row * 32);
 #pragma unroll
-            for (int c = 0; c < 32; c += 4) {
-              float x[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                x[e] = __uint_as_float(r[c + e]) * f0;
-                if (join) x[e] = fmaf(__uint_as_float(r1[c + e]), f1, x[e]);
+            for (int j = 0; j < 8; ++j)
+              mine[j ^ (row & 7)] = valid ? make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3])
+                                          : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+          if (valid && copy == 0) {
+            each_bad([&](int page, int slot) {
+#pragma unroll 1
+              for (int d = 0; d < 32; ++d) {
+                const float v = tree_v(p.g, p.layer, page, s.h, slot, d0 + cc + d);
+                if (!isfinite(v)) xb[row * 32 + (((d >> 2) ^ (row & 7)) << 2) + (d & 3)] += v;
               }
-              if (full)
-                tree_store4(p.out, obase + d0 + cc + c, p.out_dtype, x[0], x[1], x[2], x[3]);
-              else
-                reinterpret_cast<float4*>(part)[(int64_t)((d0 + cc + c) >> 2) * p.part_rows + r_in] =
-                    make_float4(x[0], x[1], x[2], x[3]);
+            });
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&x_full[w]);
+          if (!warp_wait_polled(&x_full[w], xchg & 1)) return false;
+          if (valid) {
+            const int sub = row & (kRows / R - 1);
+#pragma unroll
+            for (int jj = 0; jj < 8 / R; ++jj) {
+              const int j = copy * (8 / R) + jj;
+              float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+              for (int e = 0; e < R; ++e) {
+                const float4 b4 = reinterpret_cast<const float4*>(xb + (sub + e * (kRows / R)) * 32)[j ^ (sub & 7)];
+                a.x += b4.x;
+                a.y += b4.y;
+                a.z += b4.z;
+                a.w += b4.w;
+              }
+              put4(d0 + cc + 4 * j, a.x, a.y, a.z, a.w);
             }
           }
           __syncwarp();
-        }
-        if (!full && valid && (two || w == 0))
-          reinterpret_cast<float2*>(part + (int64_t)p.part_rows * kHD)[r_in] = make_float2(M, Lsum);
-        // what is not finite in the V of nodes this row sees
-        if (valid) {
-#pragma unroll 1
-          for (int wd = 0; wd < p.mask_words; ++wd) {
-            unsigned long long hit = bad[wd];
-            if (hit) hit &= tree_window(mask, p.mask_words, s.n, 64 * wd);
-#pragma unroll 1
-            for (; hit; hit &= hit - 1) {
-              const int pos = s.ctx + 64 * wd + __ffsll((long long)hit) - 1;
-              int page = __ldg(p.bt + (int64_t)s.seq * p.bt_stride + pos / SCKV_PAGE_TOKENS);
-              if (page < 0 || page >= p.g.P) page = 0;
-#pragma unroll 1
-              for (int d = d0; d < d0 + nd; ++d) {
-                const float v = tree_v(p.g, p.layer, page, s.h, pos % SCKV_PAGE_TOKENS, d);
-                if (isfinite(v)) continue;
-                if (full) {
-                  sckv_store_from_float(p.out, obase + d, p.out_dtype,
-                                        sckv_load_as_float(p.out, obase + d, p.out_dtype) + v);
-                } else {
-                  part[((int64_t)(d >> 2) * p.part_rows + r_in) * 4 + (d & 3)] += v;
-                }
-              }
-            }
-          }
+          if (lane == 0) mbar_arrive(x_done);
+          if (!warp_wait_polled(x_done, xchg & 1)) return false;
+          ++xchg;
         }
       }
+      if (!full && valid && copy == 0 && (two || w == 0))
+        reinterpret_cast<float2*>(part + (int64_t)p.part_rows * kHD)[r_in] = make_float2(M, Lsum);
       // the other flags were last read in the item before and are next set in the one after
       if (tid < kMaskWordsMax) s_bad[((k + 1) & 1) * kMaskWordsMax + tid] = 0;
       tc_fence_before();
@@ -1071,6 +1160,14 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
       gt += s.nk;
       cnt[0] += two ? s.nk : (s.nk + 1) >> 1;
       cnt[1] += two ? s.nk : s.nk >> 1;
+      return true;
+    };
+    for (int k = 0; ok && more; ++k) {
+      if (C::kQTiles == 2 && s.nq == 2) ok = run_item(std::integral_constant<bool, C::kQTiles == 2>{}, std::integral_constant<int, 1>{}, k);
+      else if (s.copies == 1) ok = run_item(std::false_type{}, std::integral_constant<int, 1>{}, k);
+      else if (s.copies == 2) ok = run_item(std::false_type{}, std::integral_constant<int, 2>{}, k);
+      else ok = run_item(std::false_type{}, std::integral_constant<int, 4>{}, k);
+      if (!ok) break;
       more = tree_next(p, cum, walk, s);
       if (more) load_q(s);
     }

@@ -257,33 +257,6 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   }
 }
 
-__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
-// The same bound for waits that are mostly short: a plain test first, and the
-// global timer read once per 64 polls.
-__device__ __forceinline__ bool mbar_wait_polled(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
-  if (mbar_test_wait(bar, parity)) return true;
-  uint64_t t0 = 0;
-  while (true) {
-#pragma unroll 1
-    for (int i = 0; i < 64; ++i)
-      if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t = globaltimer_ns();
-    if (t0 == 0) t0 = t;
-    else if (t - t0 > limit_ns) return false;
-  }
-}
-
 // Global -> shared bulk copy completing on an mbarrier (bytes % 16 == 0,
 // both addresses 16-byte aligned).
 __device__ __forceinline__ void bulk_g2s(void* dst_smem, const void* src_gmem, uint32_t bytes,

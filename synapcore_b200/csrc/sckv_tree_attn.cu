@@ -17,36 +17,36 @@
 // ragged batches all keep every SM on HBM. An item that a border cuts leaves
 // unnormalised partials (at most two per CTA) that a second kernel joins.
 //
-// With one query tile (Q in tensor memory, S with two buffers) one softmax
-// warpgroup weighs every key tile while the tensor cores make the next one's
-// scores; in one-byte pools the other warpgroup decodes pages. An item of at
-// most 64 (32) rows fills the query tile with 2 (4) copies of them, and each
-// copy weighs only its 64 (32) keys of the tile (P is 0 elsewhere): the lanes of
-// tensor memory that would be idle share the softmax, and the copies' sums and
-// O are joined at the end of the item. With two query tiles (Q in shared
-// memory) each has a warpgroup, and both use every K/V tile. A tile costs 8
-// MMAs of 128 x 128 x 16 for S per query tile and 8 for P V (16 with P in two
-// parts): narrower S products (64 keys) take the same time each, limited by
-// their operands' shared-memory reads (measured 60 - 150 cycles against 64).
+// With one query tile the two softmax warpgroups take a half of 64 keys of
+// every tile each, with their own reference, sum and O accumulator, joined
+// at the end of the item; S has two buffers, so the next tile's scores are
+// made while this one's are weighed. With two query tiles each warpgroup owns one and
+// both use every K/V tile. An item of at most 64 (32) rows fills the query
+// tile with 2 (4) copies of them, and each copy weighs only its 32 (16) keys
+// of the half (P is 0 elsewhere): the lanes of tensor memory that would be
+// idle share the softmax, whose time per tile falls accordingly, and the
+// copies' sums and O are joined like those of the warpgroups. Either way a tile costs 8 MMAs of 128 x 128 x 16 for
+// S per query tile and 8 for P V (16 with P in two parts): narrower S
+// products (64 keys) take the same time each, limited by their operands'
+// shared-memory reads (measured 60 - 150 cycles against 64).
 //
 // 16 warps (a warp runs on SM sub-partition warp % 4):
-//   warps 0, 2   TMA producers. 16-bit pools: K, V; one 4 KiB box per
+//   warps 0, 2   producers. 16-bit pools: K, V by TMA; one 4 KiB box per
 //                page-head, which a rank-5 view of the pool lays out as 8-row
 //                groups [rows 0-7 | 8-15][dims 0-63 | 64-127], so that groups
-//                of consecutive pages have one stride. One-byte pools: pages
-//                0-1, 2-3 of each half tile, K and V of a page in one 4 KiB
-//                box into a staging ring, plus int8 scales (warp 0).
+//                of consecutive pages have one stride. One-byte pools: K and
+//                V of a page in one 4 KiB box into a staging ring, half a tile
+//                at a time; the scales.
+//   warps 3, 13-19  one-byte pools (20 warps): decode a staged page-head each
+//                into the f16 rings. int8 codes times their token's fp16 scale (the rounding that
+//                the cache's values have); e4m3 codes exactly, their page's
+//                scales go to the scores (K) and to P (V).
 //   warps 1, 12  issue the MMAs and commits, from one elected lane each: S, and
 //                P V (a wait takes ~250 cycles, beside the other's products);
 //                with two query tiles warp 1 all of them, each query tile's S
 //                behind its P V.
-//   warps 4-7    softmax of query tile 0, one thread per query row; they also
-//                load Q and write the results.
-//   warps 8-11   16-bit pools: the same for query tile 1.
-//   warps 3, 8-11, 13-15  one-byte pools: decode a staged page-head each into
-//                the f16 rings. int8 codes times their token's fp16 scale (the
-//                rounding that the cache's values have); e4m3 codes exactly,
-//                their page's scales go to the scores (K) and to P (V).
+//   warps 4-11   softmax, one thread per query row; they also load Q and
+//                write the results.
 //
 // P is held as 2^6 times the weight, so that f16's smallest step is 2^-31 of
 // a weight of 1 (m is stale by at most 2^8: P <= 2^14); e4m3 pages multiply it
@@ -80,39 +80,43 @@ constexpr int kHalf = 64;                      // keys of half a K/V tile
 constexpr int kKeys = 2 * kHalf;               // keys of a K/V tile
 constexpr int kHalfPages = kHalf / SCKV_PAGE_TOKENS;
 constexpr int kTilePages = 2 * kHalfPages;
-constexpr int kThreadsTree = 512;
+constexpr int kMaxWarps = 20;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColS = 0;                  // S[x] at 128 x
 constexpr uint32_t kColO = 256;                // O[w] at 256 + 128 w
-constexpr uint32_t kColQ = 384;                // Q of an item with one query tile: 64 columns
 constexpr int kWarpProdA = 0, kWarpMma = 1, kWarpProdB = 2, kWarpMma2 = 12;
 constexpr int kQHalf = kRows * 128;            // one 64-dim half of a query tile: 16 KiB
 constexpr int kQTile = 2 * kQHalf;
 constexpr int kPageTile = 4096;                // one page-head in f16 / bf16
 constexpr int kHalfSlot = kHalfPages * kPageTile;
 constexpr int kSlot = 2 * kHalfSlot;           // a K (or V) tile: 32 KiB
-constexpr int kMaxStages = 3;                  // K and V tiles in the MMA's type (2 beside Q in shared memory or staging)
-constexpr int kOffStage = 4 * kSlot;           // one-byte pools: K ring, V ring (2 tiles each), staging
-constexpr int kScaleSlots = 16;                // int8: half tiles whose scales are kept
+constexpr int kStages = 2;                     // K and V tiles in the MMA's type
+constexpr int kScaleSlots = 16;                // one-byte pools: half tiles whose scales are kept
 
 template <int KVDT>
 struct TreeCfg {
   static constexpr bool kFP8 = KVDT == SCKV_DTYPE_FP8_E4M3, kINT8 = KVDT == SCKV_DTYPE_INT8;
   static constexpr bool kB8 = kFP8 || kINT8;
   static constexpr bool kBF16 = KVDT == SCKV_DTYPE_BF16;
-  static constexpr int kStaging = kB8 ? 4 : 0;        // staged half tiles of codes (K and V)
-  static constexpr int kOffXchg = 6 * kSlot;          // [128 rows] of 32 fp32: copies' O, piece by piece
-  static constexpr int kOffScale = kOffXchg + kRows * 128;
-  static constexpr int kOffBar = kOffScale + (kINT8 ? kScaleSlots * 256 : 0);
-  static constexpr int kNumBars = 4 * kMaxStages + 6 + 6 + 2 * kStaging;
-  static constexpr int kOffMl = kOffBar + ((kNumBars * 8 + 15) / 16) * 16;  // float2 [128]: m, l of a row
-  static constexpr int kOffBad = kOffMl + kRows * 8;                        // u64 [2][4]: nodes whose V is not finite
+  static constexpr int kThreads = kB8 ? 640 : 512;
+  static constexpr int kSoftRegs = kB8 ? 128 : 176, kGiveRegs = kB8 ? 72 : 80;  // registers after the roles split
+  static constexpr int kQTiles = kB8 ? 1 : 2;
+  static constexpr int kStaging = kB8 ? 3 : 0;        // staged half tiles of codes (K and V)
+  static constexpr int kOffK = kQTiles * kQTile;
+  static constexpr int kOffV = kOffK + kStages * kSlot;
+  static constexpr int kOffStage = kOffV + kStages * kSlot;
+  static constexpr int kOffScale = kOffStage + kStaging * kHalfSlot;
+  static constexpr int kOffBar = kOffScale + (kB8 ? kScaleSlots * 256 : 0);
+  static constexpr int kNumBars = 4 * kStages + 6 + 6 + 2 * kStaging;
+  static constexpr int kOffMl = kOffBar + ((kNumBars * 8 + 15) / 16) * 16;  // float2 [2][128]: m, l of a row
+  static constexpr int kOffVref = kOffMl + 2 * kRows * 8;                   // float [2][4]: V scale of a warp's O
+  static constexpr int kOffBad = kOffVref + 32;                             // u64 [2][4]: nodes whose V is not finite
   static constexpr int kOffTmem = kOffBad + 64;
   static constexpr int kOffAbort = kOffTmem + 4;
   static constexpr int kOffPartial = kOffTmem + 16;                         // int [warps]
-  static constexpr int kOffCum = kOffPartial + kThreadsTree / 32 * 4;       // int [n_seqs + 1]
+  static constexpr int kOffCum = kOffPartial + kMaxWarps * 4;               // int [n_seqs + 1]
   static constexpr int kFixedSmem = 1024 + kOffCum + 4;                     // + 4 n_seqs
-  static_assert(2 * 2 + kStaging < kScaleSlots, "scale slots outlive their half tiles");
+  static_assert(2 * kStages + kStaging < kScaleSlots, "scale slots outlive their half tiles");
 };
 
 // What the joining kernel needs of a CTA whose first item began in an earlier one and ends in it.
@@ -234,17 +238,83 @@ __device__ __forceinline__ void tree_store4(void* dst, int64_t idx, int dtype, f
   }
 }
 
+// Barriers by their shared-memory address.
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded by SCKV_WAIT_LIMIT_NS; a plain test first (most waits are short), the global timer once per 64 polls.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+  if (bar_test(bar, parity)) return true;
+  uint64_t t0 = 0;
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (bar_try(bar, parity)) return true;
+    const uint64_t t = globaltimer_ns();
+    if (t0 == 0) t0 = t;
+    else if (t - t0 > SCKV_WAIT_LIMIT_NS) return false;
+  }
+}
 // Every lane of the warp waits; the result is the same on all lanes.
-__device__ __forceinline__ bool warp_wait_polled(uint64_t* bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, mbar_wait_polled(bar, parity, SCKV_WAIT_LIMIT_NS));
+__device__ __forceinline__ bool warp_wait_bar(uint32_t bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, bar_wait(bar, parity));
+}
+// 5-D tiled TMA load.
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x0, int x1, int x2, int x3, int x4,
+                                         uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
+      "%6}], [%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x0), "r"(x1), "r"(x2), "r"(x3), "r"(x4), "r"(bar)
+      : "memory");
 }
 
-// 8 columns of this thread's tensor memory lane.
+// 8 / 16 columns of this thread's tensor memory lane.
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
                "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+__device__ __forceinline__ void bar_arrive_n(uint32_t bar, uint32_t n) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n) : "memory");
+}
+
 // 1 on one lane of the (converged) warp.
 __device__ __forceinline__ uint32_t elect_one() {
   uint32_t r;
@@ -252,33 +322,38 @@ __device__ __forceinline__ uint32_t elect_one() {
   return r;
 }
 
-__device__ __forceinline__ void reg_give() { asm volatile("setmaxnreg.dec.sync.aligned.u32 80;"); }
+template <int N>
+__device__ __forceinline__ void reg_give() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 template <int KVDT>
-__global__ void __launch_bounds__(kThreadsTree, 1)
+__global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
     tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap tmap) {
   using C = TreeCfg<KVDT>;
   constexpr bool kBF16 = C::kBF16;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(base + C::kOffBar);
-  uint64_t* k_full = bars;                      // [S] K tile in shared memory
-  uint64_t* k_empty = k_full + kMaxStages;      // [S] the S products that read it finished (commit)
-  uint64_t* v_full = k_empty + kMaxStages;      // [S] V tile in shared memory
-  uint64_t* v_empty = v_full + kMaxStages;      // [S] the PV products that read it finished (commit)
+  // barriers, as shared-memory addresses (8 bytes each)
+  const uint32_t bar0 = smem_u32(base + C::kOffBar);
+  const uint32_t k_full = bar0;                   // [S] K tile in shared memory
+  const uint32_t k_empty = k_full + 8 * kStages;      // [S] the S products that read it finished (commit)
+  const uint32_t v_full = k_empty + 8 * kStages;      // [S] V tile in shared memory
+  const uint32_t v_empty = v_full + 8 * kStages;      // [S] the PV products that read it finished (commit)
   // set x: one query tile: tile i of the item uses set i & 1; two: query tile w uses set w for every tile
-  uint64_t* s_full = v_empty + kMaxStages;      // [x] S in tensor memory (commit)
-  uint64_t* p_full = s_full + 2;                // [x] P in tensor memory, V tile fixed (one arrival per warp)
-  uint64_t* pv_done = p_full + 2;               // [x] PV finished (commit)
-  // [w] Q of query tile w is in place (w = 1: items with two), and its warpgroup read the O of its item before (4 arrivals)
-  uint64_t* q_full = pv_done + 2;
-  uint64_t* o1_free = q_full + 2;               // O[1] of an item with two query tiles was read (4 arrivals)
-  uint64_t* x_full = o1_free + 1;               // a piece of the copies' O is in the exchange buffer (4 arrivals) ...
-  uint64_t* x_done = x_full + 1;                // ... and was read (4 arrivals)
-  uint64_t* mma_done = x_done + 1;              // every issued MMA finished (2 commits)
-  uint64_t* st_full = mma_done + 1;             // one-byte pools: [SS] staged half tile landed, its scales are written
-  uint64_t* st_empty = st_full + C::kStaging;   // [SS] decoded (one arrival per decoding warp)
+  const uint32_t s_full = v_empty + 8 * kStages;      // [x] S in tensor memory (commit)
+  const uint32_t p_full = s_full + 8 * 2;             // [x] P in tensor memory, V tile fixed (8 arrivals)
+  const uint32_t pv_done = p_full + 8 * 2;            // [x] PV finished (commit)
+  // the item's Q is in shared memory and the O of the item before was read (one arrival per softmax warp)
+  const uint32_t q_full = pv_done + 8 * 2;
+  const uint32_t mma_done = q_full + 8 * 1;           // every issued MMA finished
+  const uint32_t o_full = mma_done + 8 * 1;           // the item's sums are written and its O is complete (one arrival per softmax warp)
+  const uint32_t x_full = o_full + 8 * 1;             // [w] a piece of O is in the exchange buffer (one arrival per warp of w)
+  const uint32_t x_done = x_full + 8 * 2;             // the exchange buffer was read (one arrival per softmax warp)
+  const uint32_t st_full = x_done + 8 * 1;            // one-byte pools: [SS] staged half tile landed, its scales are written
+  const uint32_t st_empty = st_full + 8 * C::kStaging;  // [SS] decoded (one arrival per decoding warp)
   float2* s_ml = reinterpret_cast<float2*>(base + C::kOffMl);
+  float* s_vref = reinterpret_cast<float*>(base + C::kOffVref);
   unsigned long long* s_bad = reinterpret_cast<unsigned long long*>(base + C::kOffBad);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + C::kOffTmem);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(base + C::kOffAbort);
@@ -289,18 +364,15 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
   const int lane = threadIdx.x & 31;
 
   pdl_trigger();
-  bool has_two;  // an item with two query tiles: Q takes 64 KiB of shared memory, the rings hold 2 tiles instead of 3
   // ---- key tiles per sequence, prefix-summed by the whole CTA
   {
-    const int per = (p.n_seqs + kThreadsTree - 1) / kThreadsTree;
+    const int per = (p.n_seqs + C::kThreads - 1) / C::kThreads;
     const int s0 = min(p.n_seqs, (int)threadIdx.x * per), s1 = min(p.n_seqs, s0 + per);
     int local = 0, n, ctx, kt, groups;
-    bool wide = false;
     for (int s = s0; s < s1; ++s) {
       if (!tree_seq(p, s, n, ctx, kt, groups) && blockIdx.x == 0)
         sckv_report(p.g.status, SCKV_ERR_BOUNDS, s, KID_TREE_ATTN);
       local += kt * groups * p.g.H;
-      wide |= n * p.G > kRows;
     }
     // inclusive scan within each warp, then over the warps
     int x = local;
@@ -312,21 +384,23 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
     if (lane == 31) partial[warp] = x;
     if (threadIdx.x == 0) {
       for (int i = 0; i < C::kNumBars; ++i) {
-        uint64_t* bar = &bars[i];
+        const uint32_t bar = bar0 + 8 * i;
         uint32_t count = 1;
-        if (C::kB8 && ((bar >= k_full && bar < k_empty) || (bar >= v_full && bar < v_empty))) count = 8;
-        if ((bar >= p_full && bar < p_full + 2) || (bar >= q_full && bar < mma_done)) count = 4;
+        if (C::kB8 && ((bar >= k_full && bar < k_full + 8 * kStages) || (bar >= v_full && bar < v_full + 8 * kStages))) count = 8;
+        if (bar >= p_full && bar < p_full + 16) count = 8;
         if (bar == mma_done) count = 2;
-        if (C::kB8 && bar >= st_full && bar < st_full + C::kStaging) count = 2;
-        if (C::kB8 && bar >= st_empty && bar < st_empty + C::kStaging) count = 8;
-        mbar_init(bar, count);
+        if (bar == q_full || bar == o_full || bar == x_done) count = 8;
+        if (bar == x_full || bar == x_full + 8) count = 4;
+        if (C::kB8 && bar >= st_full && bar < st_full + 8 * C::kStaging) count = 2;
+        if (C::kB8 && bar >= st_empty && bar < st_empty + 8 * C::kStaging) count = 8;
+        bar_init(bar, count);
       }
       for (int i = 0; i < 2 * kMaskWordsMax; ++i) s_bad[i] = 0;
       *abort_flag = 0;
       fence_mbar_init();
     }
     if (warp == kWarpMma) tmem_alloc(tmem_slot, kTmemCols);
-    has_two = __syncthreads_or(wide) && !C::kB8;
+    __syncthreads();
     int before = 0;
     for (int i = 0; i < warp; ++i) before += partial[i];
     int run = before + x - local;
@@ -335,7 +409,7 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
       tree_seq(p, s, n, ctx, kt, groups);
       run += kt * groups * p.g.H;
     }
-    if (threadIdx.x == kThreadsTree - 1) cum[p.n_seqs] = before + x;
+    if (threadIdx.x == C::kThreads - 1) cum[p.n_seqs] = before + x;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -373,152 +447,137 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
   }
 
   const int64_t layer_base = (int64_t)p.layer * p.g.P;
-  const int n_st = C::kB8 || has_two ? 2 : 3;
-  uint8_t* const k_ring = base + (has_two ? 2 * kQTile : 0);
-  uint8_t* const v_ring = k_ring + n_st * kSlot;
-  // ring slot of tile g and the parity of its use
-  auto slot_of = [&](int g) { return n_st == 2 ? g & 1 : g % 3; };
-  auto turn_of = [&](int g) -> uint32_t { return (n_st == 2 ? g >> 1 : g / 3) & 1; };
-  // Registers: 128 a thread at launch; the softmax warpgroups take 176 for a row's 64 scores and their P, the two
-  // others give theirs up (256 x 80 + 256 x 176 = 512 x 128). Each role does it in its own branch, so that the
-  // compiler knows the count of every region.
+  // Registers: 128 a thread at launch (one-byte pools: 96); the softmax warpgroups take 176 (128) for a row's 64 scores
+  // and their P, the others give theirs up: 256 x 80 + 256 x 176 = 512 x 128 (384 x 72 + 256 x 128 = 60,416 <= 640 x
+  // 96). Each role does it in its own branch, so that the compiler knows the count of every region.
   if (warp == kWarpProdA || warp == kWarpProdB) {
     // ------------------------------------------------------------ producers
-    reg_give();
-    const int part = warp == kWarpProdB ? 1 : 0;  // 16-bit: V; one-byte: pages 2, 3 of a half tile
+    reg_give<C::kGiveRegs>();
+    // A lane owns a page of the tile: its id is loaded one tile ahead (and not looked at in the turn that loads it,
+    // which would wait for it), and the copies of all pages go out as one instruction (one lane after the other
+    // issued them in ~180 cycles each, which paced the kernel).
+    const int part = warp == kWarpProdB ? 1 : 0;  // 16-bit: K, V; one-byte: codes, scales
     if (lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap)) : "memory");
     TreeSeg s;
     int g = 0;
     bool aborted = false;
+    auto valid_page = [&](int page) -> int {
+      if (page >= 0 && page < p.g.P) return page;
+      sckv_report(p.g.status, SCKV_ERR_BOUNDS, page, KID_TREE_ATTN);
+      return 0;
+    };
     if constexpr (!C::kB8) {
-      if (lane == 0) {
-        uint64_t* fulls = part ? v_full : k_full;
-        uint64_t* empties = part ? v_empty : k_empty;
-        uint8_t* ring = part ? v_ring : k_ring;
-        while (!aborted && tree_next(p, cum, walk, s)) {
-          const int32_t* bt_row = p.bt + (int64_t)s.seq * p.bt_stride;
-          int ids[kTilePages], nxt[kTilePages];  // page ids, fetched one tile ahead
-          auto fetch = [&](int j, int (&v)[kTilePages]) {
-#pragma unroll
-            for (int i = 0; i < kTilePages; ++i) {
-              const int blk = j * kTilePages + i;
-              v[i] = blk < s.pages ? __ldg(bt_row + blk) : 0;
-            }
-          };
-          fetch(s.ka, nxt);
-          for (int j = s.ka; j < s.ka + s.nk; ++j, ++g) {
-#pragma unroll
-            for (int i = 0; i < kTilePages; ++i) ids[i] = nxt[i];
-            if (j + 1 < s.ka + s.nk) fetch(j + 1, nxt);
-            const int st = slot_of(g);
-            if (g >= n_st && (*abort_flag || !mbar_wait_polled(&empties[st], turn_of(g) ^ 1, SCKV_WAIT_LIMIT_NS))) {
-              aborted = true;
-              break;
-            }
-            const int np = min(kTilePages, s.pages - j * kTilePages);
-            mbar_arrive_expect_tx(&fulls[st], (uint32_t)np * kPageTile);
-            const uint32_t dst = smem_u32(ring + st * kSlot);
-#pragma unroll
-            for (int i = 0; i < kTilePages; ++i) {
-              if (i >= np) break;
-              int page = ids[i];
-              if (page < 0 || page >= p.g.P) {
-                sckv_report(p.g.status, SCKV_ERR_BOUNDS, page, KID_TREE_ATTN);
-                page = 0;
-              }
-              const int slab = (int)(((layer_base + page) * 2 + part) * p.g.H + s.h);
-              tma_load_5d(dst + i * kPageTile, &tmap, 0, 0, 0, 0, slab, &fulls[st]);
-            }
-          }
-        }
-        // nothing of ours may still be landing when the CTA retires
-        for (int t = g > n_st ? g - n_st : 0; t < g; ++t)
-          mbar_wait_polled(&fulls[slot_of(t)], turn_of(t), SCKV_WAIT_LIMIT_NS);
-      }
-    } else {
-      // int8 scales of a half tile: four tokens' fp16 per lane (K, V; 4 pages; 4 x 4 tokens)
-      const int skv = lane >> 4, spg = (lane >> 2) & 3;
-      const bool has_scale = C::kINT8 && part == 0;
+      const uint32_t fulls = part ? v_full : k_full, empties = part ? v_empty : k_empty;
+      const uint32_t ring = smem_u32(base + (part ? C::kOffV : C::kOffK)) + lane * kPageTile;
       while (!aborted && tree_next(p, cum, walk, s)) {
         const int32_t* bt_row = p.bt + (int64_t)s.seq * p.bt_stride;
-        const int je = 2 * (s.ka + s.nk);
-        // (as loaded: looking at an id in the turn that loads it would wait for it)
-        auto fetch = [&](int blk) -> int { return blk < s.pages ? __ldg(bt_row + blk) : 0; };
-        auto load_scale = [&](int page) -> uint2 {
-          if (page < 0 || page >= p.g.P) page = 0;
-          return __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const __half*>(p.g.scales) +
-                                                      (((layer_base + page) * 2 + skv) * p.g.H + s.h) * 16) + (lane & 3));
-        };
-        uint2 sc = make_uint2(0u, 0u);
-        int sid = 0;
-        if (has_scale) {
-          sc = load_scale(fetch(2 * s.ka * kHalfPages + spg));
-          sid = fetch((2 * s.ka + 1) * kHalfPages + spg);
-        }
-        int nid[2] = {0, 0};
-        auto fetch_ids = [&](int j) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int blk = j * kHalfPages + 2 * part + i;
-            nid[i] = blk < s.pages ? __ldg(bt_row + blk) : 0;
-          }
-        };
-        if (lane == 0) fetch_ids(2 * s.ka);
-        for (int j = 2 * s.ka; j < je; ++j, ++g) {
-          const int st = g % C::kStaging;
-          const int ab = __shfl_sync(0xffffffffu, *abort_flag, 0);
-          if (g >= C::kStaging && (ab || !warp_wait_polled(&st_empty[st], ((g / C::kStaging) - 1) & 1))) {
+        auto there = [&](int j) { return lane < kTilePages && j * kTilePages + lane < s.pages; };
+        const int je = s.ka + s.nk;
+        int nxt = there(s.ka) ? __ldg(bt_row + s.ka * kTilePages + lane) : 0;
+        for (int j = s.ka; j < je; ++j, ++g) {
+          const int id = nxt;
+          if (j + 1 < je && there(j + 1)) nxt = __ldg(bt_row + (j + 1) * kTilePages + lane);
+          const int st = g % kStages;
+          if (*abort_flag || (g >= kStages && !warp_wait_bar(empties + 8 * st, ((g / kStages) - 1) & 1))) {
             aborted = true;
             break;
           }
-          if (has_scale) {
-            reinterpret_cast<uint2*>(base + C::kOffScale + (g % kScaleSlots) * 256)[lane] = sc;
-            if (j + 1 < je) {
-              sc = load_scale(sid);
-              if (j + 2 < je) sid = fetch((j + 2) * kHalfPages + spg);
-            }
-          }
+          if (lane == 0) bar_expect(fulls + 8 * st, (uint32_t)min(kTilePages, s.pages - j * kTilePages) * kPageTile);
           __syncwarp();
-          if (lane == 0) {
-            const int ids[2] = {nid[0], nid[1]};
-            if (j + 1 < je) fetch_ids(j + 1);
-            const int np = max(0, min(2, s.pages - j * kHalfPages - 2 * part));
-            mbar_arrive_expect_tx(&st_full[st], (uint32_t)np * 4096u);
-            const uint32_t dst = smem_u32(base + kOffStage + st * kHalfSlot + 2 * part * 4096);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              if (i >= np) break;
-              int page = ids[i];
-              if (page < 0 || page >= p.g.P) {
-                sckv_report(p.g.status, SCKV_ERR_BOUNDS, page, KID_TREE_ATTN);
-                page = 0;
-              }
-              tma_load_5d(dst + i * 4096, &tmap, 0, 0, s.h, 0, (int)(layer_base + page), &st_full[st]);
-            }
+          if (there(j)) {
+            const int slab = (int)(((layer_base + valid_page(id)) * 2 + part) * p.g.H + s.h);
+            tma_load(ring + st * kSlot, &tmap, 0, 0, 0, 0, slab, fulls + 8 * st);
           }
           __syncwarp();
         }
       }
-      if (lane == 0)
-        for (int t = g > C::kStaging ? g - C::kStaging : 0; t < g; ++t)
-          mbar_wait_polled(&st_full[t % C::kStaging], (t / C::kStaging) & 1, SCKV_WAIT_LIMIT_NS);
+      // nothing of ours may still be landing when the CTA retires
+      for (int t = g > kStages ? g - kStages : 0; t < g; ++t) warp_wait_bar(fulls + 8 * (t % kStages), (t / kStages) & 1);
+    } else if (part == 0) {
+      const uint32_t ring = smem_u32(base + C::kOffStage) + lane * 4096;
+      while (!aborted && tree_next(p, cum, walk, s)) {
+        const int32_t* bt_row = p.bt + (int64_t)s.seq * p.bt_stride;
+        auto there = [&](int j) { return lane < kHalfPages && j * kHalfPages + lane < s.pages; };
+        const int je = 2 * (s.ka + s.nk);
+        int nxt = there(2 * s.ka) ? __ldg(bt_row + 2 * s.ka * kHalfPages + lane) : 0;
+        for (int j = 2 * s.ka; j < je; ++j, ++g) {
+          const int id = nxt;
+          if (j + 1 < je && there(j + 1)) nxt = __ldg(bt_row + (j + 1) * kHalfPages + lane);
+          const int st = g % C::kStaging;
+          if (*abort_flag || (g >= C::kStaging && !warp_wait_bar(st_empty + 8 * st, ((g / C::kStaging) - 1) & 1))) {
+            aborted = true;
+            break;
+          }
+          if (lane == 0)
+            bar_expect(st_full + 8 * st, (uint32_t)max(0, min(kHalfPages, s.pages - j * kHalfPages)) * 4096u);
+          __syncwarp();
+          if (there(j))
+            tma_load(ring + st * kHalfSlot, &tmap, 0, 0, s.h, 0, (int)(layer_base + valid_page(id)), st_full + 8 * st);
+          __syncwarp();
+        }
+      }
+      for (int t = g > C::kStaging ? g - C::kStaging : 0; t < g; ++t)
+        warp_wait_bar(st_full + 8 * (t % C::kStaging), (t / C::kStaging) & 1);
+    } else {
+      // scales of a half tile: int8 four tokens' fp16 per lane (K, V; 4 pages; 4 x 4 tokens); FP8 lanes 0-3 the K,
+      // 4-7 the V scales of its pages, a page past the last node scales by 1 (K, masked anyway) and 0 (V). Loaded one
+      // half tile ahead, the page ids two.
+      const int skv = C::kINT8 ? lane >> 4 : (lane >> 2) & 1, spg = C::kINT8 ? (lane >> 2) & 3 : lane & 3;
+      const bool mine = C::kINT8 || lane < 8;
+      while (!aborted && tree_next(p, cum, walk, s)) {
+        const int32_t* bt_row = p.bt + (int64_t)s.seq * p.bt_stride;
+        const int je = 2 * (s.ka + s.nk);
+        auto there = [&](int j) { return mine && j < je && j * kHalfPages + spg < s.pages; };
+        auto fetch = [&](int j) -> int { return there(j) ? __ldg(bt_row + j * kHalfPages + spg) : 0; };
+        auto load_scale = [&](int page, int j) -> uint2 {
+          uint2 r = make_uint2(C::kFP8 && skv == 0 ? 0x3f800000u : 0u, 0u);
+          if (page < 0 || page >= p.g.P) page = 0;
+          const int64_t at = ((layer_base + page) * 2 + skv) * p.g.H + s.h;
+          if (there(j)) {
+            if (C::kINT8)
+              r = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const __half*>(p.g.scales) + at * 16) + (lane & 3));
+            else
+              r.x = __ldg(reinterpret_cast<const uint32_t*>(p.g.scales) + at);
+          }
+          return r;
+        };
+        uint2 sc = load_scale(fetch(2 * s.ka), 2 * s.ka);
+        int sid = fetch(2 * s.ka + 1);
+        for (int j = 2 * s.ka; j < je; ++j, ++g) {
+          const int st = g % C::kStaging;
+          const uint2 now = sc;
+          sc = load_scale(sid, j + 1);
+          sid = fetch(j + 2);
+          if (*abort_flag || (g >= C::kStaging && !warp_wait_bar(st_empty + 8 * st, ((g / C::kStaging) - 1) & 1))) {
+            aborted = true;
+            break;
+          }
+          uint8_t* slot = base + C::kOffScale + (g % kScaleSlots) * 256;
+          if (C::kINT8)
+            reinterpret_cast<uint2*>(slot)[lane] = now;
+          else if (lane < 8)  // (a K scale of 0 would turn masked scores, -inf, into NaN; NaN stays)
+            reinterpret_cast<float*>(slot)[lane] = skv == 0 && __uint_as_float(now.x) < 1e-30f ? 1e-30f : __uint_as_float(now.x);
+          __syncwarp();
+          if (lane == 0) bar_arrive(st_full + 8 * st);
+        }
+      }
     }
     if (aborted && lane == 0) {
       if (!*abort_flag) sckv_report(p.g.status, SCKV_ERR_TIMEOUT, blockIdx.x, KID_TREE_ATTN);
       *abort_flag = 1;
     }
-  } else if (C::kB8 && (warp == 3 || warp >= 8) && warp != kWarpMma2) {
+  } else if (C::kB8 && (warp == 3 || warp >= 13)) {
     // ------------------------------------------------------------ decoding of one-byte pages
     // Warp `role` decodes page role & 3 of K (role < 4) or V of each half tile. Lane
     // (quarter, rowbit, c): rows r and r ^ 5 of a quarter's eight lanes keep both the
     // swizzled 16-byte reads and the two 16-byte writes free of bank conflicts.
-    reg_give();
+    reg_give<C::kGiveRegs>();
     if constexpr (C::kB8) {
-      const int role = warp == 3 ? 0 : warp >= 13 ? warp - 12 : warp - 4;  // 0, 1-3 (K); 4-7 (V)
+      const int role = warp == 3 ? 0 : warp - 12;
       const int kv = role >> 2, pg = role & 3;
-      uint64_t* fulls = kv ? v_full : k_full;
-      uint64_t* empties = kv ? v_empty : k_empty;
-      uint8_t* ring = kv ? v_ring : k_ring;
+      const uint32_t fulls = kv ? v_full : k_full;
+      const uint32_t empties = kv ? v_empty : k_empty;
+      uint8_t* ring = base + (kv ? C::kOffV : C::kOffK);
       const int qt = lane >> 3;
       const int r8 = (lane & 4) ? qt ^ 5 : qt;  // row of the 8-row group
       TreeSeg s;
@@ -527,15 +586,15 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
       while (!aborted && tree_next(p, cum, walk, s)) {
         for (int j = 2 * s.ka; j < 2 * (s.ka + s.nk); ++j, ++g) {
           const int ss = g % C::kStaging, gt = g >> 1, st = gt & 1;
-          if (((g & 1) == 0 && gt >= 2 && (*abort_flag || !warp_wait_polled(&empties[st], ((gt >> 1) - 1) & 1))) ||
-              !warp_wait_polled(&st_full[ss], (g / C::kStaging) & 1)) {
+          if (((g & 1) == 0 && gt >= 2 && (*abort_flag || !warp_wait_bar(empties + 8 * st, ((gt >> 1) - 1) & 1))) ||
+              !warp_wait_bar(st_full + 8 * ss, (g / C::kStaging) & 1)) {
             aborted = true;
             break;
           }
           if (j * kHalfPages + pg < s.pages) {
             const __half* tok = reinterpret_cast<const __half*>(base + C::kOffScale + (g % kScaleSlots) * 256) + kv * 64 +
                                 pg * SCKV_PAGE_TOKENS;
-            const uint8_t* src = base + kOffStage + ss * kHalfSlot + pg * 4096 + kv * 2048;
+            const uint8_t* src = base + C::kOffStage + ss * kHalfSlot + pg * 4096 + kv * 2048;
             uint8_t* dst = ring + st * kSlot + (g & 1) * kHalfSlot + pg * kPageTile;
             uint4 w[4];
 #pragma unroll
@@ -568,8 +627,8 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
           }
           __syncwarp();
           if (lane == 0) {
-            mbar_arrive(&fulls[st]);
-            mbar_arrive(&st_empty[ss]);
+            bar_arrive(fulls + 8 * st);
+            bar_arrive(st_empty + 8 * ss);
           }
         }
       }
@@ -581,54 +640,45 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
   } else if (warp == kWarpMma || warp == kWarpMma2) {
     // ------------------------------------------------------------ MMA issuers
     // A whole warp walks and waits, one elected lane issues (a role on one lane alone measured 1.3 x slower).
-    reg_give();
+    reg_give<C::kGiveRegs>();
     const int mw = warp == kWarpMma2 ? 1 : 0;
     const uint32_t el = elect_one();
     constexpr uint32_t kIdescS = instr_desc_f16(kBF16, kKeys, false);
     constexpr uint32_t kIdescPV = instr_desc_f16(kBF16, kHD, true);
     const uint64_t q_desc0 = smem_desc_sw128(smem_u32(base), 16, 1024);
-    const uint64_t k_desc0 = smem_desc_sw128(smem_u32(k_ring), 16, 2048);
-    const uint64_t v_desc0 = smem_desc_sw128(smem_u32(v_ring), 1024, 2048);
-    // S[x] = Q . K of slot st; Q from tensor memory, or (w >= 0) query tile w in shared memory
+    const uint64_t k_desc0 = smem_desc_sw128(smem_u32(base + C::kOffK), 16, 2048);
+    const uint64_t v_desc0 = smem_desc_sw128(smem_u32(base + C::kOffV), 1024, 2048);
+    // S[x] = Q tile w . K of slot st
     auto issue_s = [&](int x, int w, int st) {
       const uint64_t qd = desc_advance(q_desc0, (uint32_t)(w * kQTile));
       const uint64_t kd = desc_advance(k_desc0, (uint32_t)(st * kSlot));
-      const uint32_t d = tmem + kColS + (uint32_t)(x * kKeys);
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) {
         const int half = ks >> 2, kk = ks & 3;
-        const uint64_t bdesc = desc_advance(kd, (uint32_t)(half * 1024 + kk * 32));
-        if (w < 0)
-          umma_ts(d, tmem + kColQ + (uint32_t)(ks * 8), bdesc, kIdescS, ks > 0);
-        else
-          umma_ss(d, desc_advance(qd, (uint32_t)(half * kQHalf + kk * 32)), bdesc, kIdescS, ks > 0);
+        umma_ss(tmem + kColS + (uint32_t)(x * kKeys), desc_advance(qd, (uint32_t)(half * kQHalf + kk * 32)),
+                desc_advance(kd, (uint32_t)(half * 1024 + kk * 32)), kIdescS, ks > 0);
       }
-      umma_commit(&s_full[x]);
+      bar_commit(s_full + 8 * x);
     };
-    // O[w] (+)= P[x] . V of slot st; `both`: the second half holds keys
-    auto issue_pv = [&](int x, int w, int st, bool first, bool both) {
-      const uint64_t vd = desc_advance(v_desc0, (uint32_t)(st * kSlot));
-      const uint32_t pa = tmem + kColS + (uint32_t)(x * kKeys), o = tmem + kColO + (uint32_t)(w * kHD);
+    // O[w] (+)= P[x], half h . V of slot st, half h
+    auto issue_pv = [&](int x, int h, int w, int st, bool first) {
+      const uint64_t vd = desc_advance(v_desc0, (uint32_t)(st * kSlot + h * kHalfSlot));
+      const uint32_t pa = tmem + kColS + (uint32_t)(x * kKeys + h * kHalf), o = tmem + kColO + (uint32_t)(w * kHD);
 #pragma unroll
-      for (int pg = 0; pg < kTilePages; ++pg) {
-        if (pg == kHalfPages && !both) break;
+      for (int pg = 0; pg < kHalfPages; ++pg) {
         // B = V rows of page pg: 128 dims in two 64-dim halves (LBO), 16 keys in two 8-row groups (SBO)
         const uint64_t bdesc = desc_advance(vd, (uint32_t)(pg * kPageTile));
-        const uint32_t a = pa + (uint32_t)((pg >> 2) * kHalf + (pg & 3) * 8);
-        umma_ts(o, a, bdesc, kIdescPV, (!first || pg > 0) ? 1u : 0u);
-        if (kBF16) umma_ts(o, a + 32u, bdesc, kIdescPV, 1u);
+        umma_ts(o, pa + (uint32_t)(pg * 8), bdesc, kIdescPV, (!first || pg > 0) ? 1u : 0u);
+        if (kBF16) umma_ts(o, pa + (uint32_t)(pg * 8 + 32), bdesc, kIdescPV, 1u);
       }
-      umma_commit(&pv_done[x]);
     };
     TreeSeg s;
     bool ok = true;
     int gt = 0;              // tiles of earlier items
     int cnt[2] = {0, 0};     // uses of each set in earlier items
-    int n_two = 0;           // earlier items with two query tiles
     for (int k = 0; ok && tree_next(p, cum, walk, s); ++k) {
-      const bool two = s.nq == 2;
-      if (mw == 0 && (*abort_flag || !warp_wait_polled(&q_full[0], k & 1) ||
-                      (two && !warp_wait_polled(&q_full[1], n_two & 1)))) {
+      const bool two = C::kQTiles == 2 && s.nq == 2;
+      if (mw == 0 && (*abort_flag || !warp_wait_bar(q_full, k & 1))) {
         ok = false;
         break;
       }
@@ -636,59 +686,66 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
       if (!two && mw == 0) {
         // ---- S of every tile
         for (int i = 0; i < s.nk; ++i) {
-          const int g = gt + i, st = slot_of(g), x = i & 1, use = cnt[x] + (i >> 1);
+          const int g = gt + i, st = g % kStages, x = i & 1, use = cnt[x] + (i >> 1);
           // (S replaces the P that the set's last PV read)
-          if (*abort_flag || !warp_wait_polled(&k_full[st], turn_of(g)) ||
-              (use > 0 && !warp_wait_polled(&pv_done[x], (use - 1) & 1))) {
+          if (*abort_flag || !warp_wait_bar(k_full + 8 * st, (g / kStages) & 1) ||
+              (use > 0 && !warp_wait_bar(pv_done + 8 * x, (use - 1) & 1))) {
             ok = false;
             break;
           }
           tc_fence_after();
           if (el) {
-            issue_s(x, -1, st);
-            umma_commit(&k_empty[st]);
+            issue_s(x, 0, st);
+            bar_commit(k_empty + 8 * st);
           }
           __syncwarp();
         }
       } else if (!two) {
         // ---- P V of every tile
         for (int i = 0; i < s.nk; ++i) {
-          const int g = gt + i, st = slot_of(g), x = i & 1, use = cnt[x] + (i >> 1);
-          if (*abort_flag || !warp_wait_polled(&v_full[st], turn_of(g)) || !warp_wait_polled(&p_full[x], use & 1)) {
+          const int g = gt + i, st = g % kStages, x = i & 1, use = cnt[x] + (i >> 1);
+          if (*abort_flag || !warp_wait_bar(v_full + 8 * st, (g / kStages) & 1) ||
+              !warp_wait_bar(p_full + 8 * x, use & 1)) {
             ok = false;
             break;
           }
           tc_fence_after();
           if (el) {
-            issue_pv(x, 0, st, i == 0, (s.ka + i) * kKeys + kHalf < s.L);
-            umma_commit(&v_empty[st]);
+            issue_pv(x, 0, 0, st, i == 0);
+            if ((s.ka + i) * kKeys + kHalf < s.L) issue_pv(x, 1, 1, st, i == 0);  // the second half holds keys
+            bar_commit(pv_done + 8 * x);
+            bar_commit(v_empty + 8 * st);
           }
           __syncwarp();
         }
-      } else if (mw == 0) {
+      } else if (two && mw == 0) {
         // ---- two query tiles: S(i) of each follows its PV(i - 1) into the columns that held its P
         for (int i = 0; ok && i <= s.nk; ++i) {
-          const int g = gt + i, st = slot_of(g), su = slot_of(g + n_st - 1);
-          if (i < s.nk && (*abort_flag || !warp_wait_polled(&k_full[st], turn_of(g)))) ok = false;
-          if (ok && i > 0 && !warp_wait_polled(&v_full[su], turn_of(g - 1))) ok = false;
+          const int g = gt + i, st = g % kStages, su = (g + kStages - 1) % kStages;
+          if (i < s.nk && (*abort_flag || !warp_wait_bar(k_full + 8 * st, (g / kStages) & 1))) ok = false;
+          if (ok && i > 0 && !warp_wait_bar(v_full + 8 * su, ((g - 1) / kStages) & 1)) ok = false;
           for (int w = 0; ok && w < 2; ++w) {
             const int use = cnt[w] + i;
-            // (the first S of the item: the set's last PV may be the other warp's)
-            if (i > 0 ? !warp_wait_polled(&p_full[w], (use - 1) & 1)
-                      : use > 0 && !warp_wait_polled(&pv_done[w], (use - 1) & 1)) {
+            // (the first S of the item: the set's last PV may be another warp's)
+            if (i > 0 ? !warp_wait_bar(p_full + 8 * w, (use - 1) & 1)
+                      : use > 0 && !warp_wait_bar(pv_done + 8 * w, (use - 1) & 1)) {
               ok = false;
               break;
             }
             tc_fence_after();
             if (el) {
-              if (i > 0) issue_pv(w, w, su, i == 1, (s.ka + i - 1) * kKeys + kHalf < s.L);
+              if (i > 0) {
+                issue_pv(w, 0, w, su, i == 1);
+                if ((s.ka + i - 1) * kKeys + kHalf < s.L) issue_pv(w, 1, w, su, false);
+                bar_commit(pv_done + 8 * w);
+              }
               if (i < s.nk) issue_s(w, w, st);
             }
             __syncwarp();
           }
           if (ok && el) {
-            if (i < s.nk) umma_commit(&k_empty[st]);
-            if (i > 0) umma_commit(&v_empty[su]);
+            if (i < s.nk) bar_commit(k_empty + 8 * st);
+            if (i > 0) bar_commit(v_empty + 8 * su);
           }
           __syncwarp();
         }
@@ -697,89 +754,71 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
       gt += s.nk;
       cnt[0] += two ? s.nk : (s.nk + 1) >> 1;
       cnt[1] += two ? s.nk : s.nk >> 1;
-      n_two += two;
     }
     if (!ok && lane == 0) {
       if (!*abort_flag) sckv_report(p.g.status, SCKV_ERR_TIMEOUT, blockIdx.x, KID_TREE_ATTN);
       *abort_flag = 1;
     }
-    if (el) umma_commit(mma_done);  // every MMA of both warps has finished before the tensor memory is released
+    if (el) bar_commit(mma_done);  // every MMA of both warps has finished before the tensor memory is released
     __syncwarp();
-    warp_wait_polled(mma_done, 0);
-  } else if (warp >= 4 && warp < (C::kB8 ? 8 : 12)) {
+    warp_wait_bar(mma_done, 0);
+  } else if (warp >= 4 && warp < 12) {
     // ------------------------------------------------------------ softmax, Q, results
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
-    const int w = (warp - 4) >> 2;     // warpgroup = query tile
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftRegs));
+    const int w = (warp - 4) >> 2;     // warpgroup
     const int quad = warp & 3;         // tensor memory lanes 32 quad ..
     const int row = quad * 32 + lane;  // query row of the tile = tensor memory lane
+    const int tid = threadIdx.x - 128; // 0 .. 255
     const uint32_t t_row = tmem + ((uint32_t)(quad * 32) << 16);
     const uint32_t col_o = kColO + (uint32_t)(w * kHD);
+    // Q rows of an item into shared memory (128-byte swizzled, K-major): with one
+    // query tile all 256 threads load it, with two each warpgroup its own.
+    // Rows past the last keep what they have: no other row sees it.
+    auto load_q = [&](const TreeSeg& s) {
+      const bool two = C::kQTiles == 2 && s.nq == 2;
+      const int n_it = two ? 16 : 8, step = two ? 128 : 256;
+      const int t = two ? tid & 127 : tid;
+      const int tile_row0 = two ? w * kRows : 0;
+      uint8_t* q_tile = base + (two ? w * kQTile : 0);
+      const int64_t q0 = (int64_t)s.q_base * p.hq + (int64_t)s.h * p.G;
+#pragma unroll 1
+      for (int b8 = 0; b8 < n_it; b8 += 8) {
+        uint4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int c = t + (b8 + i) * step;
+          const int r = tile_row0 + (c >> 4);
+          if (r < s.rows) {
+            const int rr = s.row0 + r, node = rr / p.G;
+            v[i] = load_q8<kBF16>(p.q, (q0 + (int64_t)node * p.hq + (rr - node * p.G)) * kHD + (c & 15) * 8, p.q_dtype);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int c = t + (b8 + i) * step;
+          const int r = c >> 4, half = (c >> 3) & 1, ch = c & 7;
+          if (tile_row0 + r < s.rows)
+            for (int e = 0; e < kRows; e += kRows / s.copies)
+              *reinterpret_cast<uint4*>(q_tile + half * kQHalf + (r + e) * 128 + ((ch ^ (r & 7)) << 4)) = v[i];
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) bar_arrive(q_full);
+    };
     bool ok = true;
     int gt = 0;           // tiles of earlier items
     int cnt[2] = {0, 0};  // uses of each set in earlier items
-    int n_two = 0;        // earlier items with two query tiles
-    int xchg = 0;         // uses of the exchange buffer
-    TreeSeg s{};
-    // Q of the item: one query tile: this thread's row (the copies have the same ones) into its lane of tensor
-    // memory; two: the warpgroup's tile into shared memory, 128-byte swizzled, K-major. Rows past the last are 0.
-    auto load_q = [&]() -> bool {
-      const bool two = s.nq == 2;
-      const int64_t q0 = (int64_t)s.q_base * p.hq + (int64_t)s.h * p.G;
-      auto at = [&](int r) -> int64_t {
-        const int rr = s.row0 + r, node = rr / p.G;
-        return (q0 + (int64_t)node * p.hq + (rr - node * p.G)) * kHD;
-      };
-      if (!two) {
-        // (O[1] of an item with two query tiles shares these columns)
-        if (n_two > 0 && !warp_wait_polled(o1_free, (n_two - 1) & 1)) return false;
-        tc_fence_after();
-        const int r = row & (kRows / s.copies - 1);
-        const int64_t src = r < s.rows ? at(r) : 0;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t v[32];
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            const uint4 x = r < s.rows ? load_q8<kBF16>(p.q, src + half * 64 + c * 8, p.q_dtype) : make_uint4(0u, 0u, 0u, 0u);
-            v[4 * c] = x.x;
-            v[4 * c + 1] = x.y;
-            v[4 * c + 2] = x.z;
-            v[4 * c + 3] = x.w;
-          }
-          tmem_st32(t_row + kColQ + 32 * half, v);
-        }
-        tc_wait_st();
-        tc_fence_before();
-      } else {
-        uint8_t* q_tile = base + w * kQTile;
-        const int t = threadIdx.x & 127;
-#pragma unroll 1
-        for (int b8 = 0; b8 < 16; b8 += 8) {
-          uint4 v[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int c = t + (b8 + i) * 128, r = w * kRows + (c >> 4);
-            v[i] = r < s.rows ? load_q8<kBF16>(p.q, at(r) + (c & 15) * 8, p.q_dtype) : make_uint4(0u, 0u, 0u, 0u);
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int c = t + (b8 + i) * 128, r = c >> 4;
-            *reinterpret_cast<uint4*>(q_tile + ((c >> 3) & 1) * kQHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[i];
-          }
-        }
-        fence_proxy_async_smem();
-        tc_fence_before();
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full[w]);
-      return true;
-    };
-    // One item (or part of one); false if a wait ran out. kCopies: copies of the rows (1 with two query tiles).
-    auto run_item = [&](auto copies_c, const int k) -> bool {
+    TreeSeg s;
+    bool more = tree_next(p, cum, walk, s);
+    if (more) load_q(s);
+    int xchg = 0;  // uses of the exchange buffer
+    // One item (or part of one); false if a wait ran out. kTwo: two query tiles; kCopies: copies of the rows.
+    auto run_item = [&](auto two_c, auto copies_c, const int k) -> bool {
+      constexpr bool two = decltype(two_c)::value;
       constexpr int R = decltype(copies_c)::value;
-      constexpr int kCols = R == 4 ? 32 : kHalf;  // keys that this thread weighs at a time (R = 1: both halves)
+      constexpr int kCols = kHalf / R;       // keys of a half that this thread weighs
       constexpr int kPg = kCols / SCKV_PAGE_TOKENS;
-      const bool two = R == 1 && s.nq == 2;
       const int copy = row / (kRows / R);
       const int r_in = (two ? w * kRows : 0) + (row & (kRows / R - 1));  // row of the group
       const bool valid = r_in < s.rows;
@@ -790,44 +829,32 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
       unsigned long long* bad = s_bad + (k & 1) * kMaskWordsMax;
       float m = -INFINITY, l = 0.f;
       float vref = 0.f;  // FP8: the V scale that this warp's O counts in
-      // FP8: lanes 0-7 the K, 8-15 the V scales of a tile's pages, loaded one tile ahead, their page ids two (as
-      // loaded: looking at a value in the turn that loads it would wait for it). A page past the last node scales by 1
-      // (K, masked anyway) and 0 (V).
       const int32_t* bt_row = p.bt + (int64_t)s.seq * p.bt_stride;
-      auto scale_there = [&](int i) { return lane < 16 && i < s.nk && (s.ka + i) * kTilePages + (lane & 7) < s.pages; };
-      auto scale_id = [&](int i) -> int {
-        return scale_there(i) ? __ldg(bt_row + (s.ka + i) * kTilePages + (lane & 7)) : 0;
-      };
-      auto scale_raw = [&](int page, int i) -> float {
-        if (page < 0 || page >= p.g.P) page = 0;
-        return scale_there(i) ? __ldg(reinterpret_cast<const float*>(p.g.scales) +
-                                      ((layer_base + page) * 2 + ((lane >> 3) & 1)) * p.g.H + s.h)
-                              : (lane & 8) ? 0.f : 1.f;
-      };
-      float sc_next = 0.f;
-      int sc_id = 0;
-      if (C::kFP8) {
-        sc_next = scale_raw(scale_id(0), 0);
-        sc_id = scale_id(1);
-      }
 #pragma unroll 1
       for (int i = 0; i < s.nk; ++i) {
         const int x = two ? w : i & 1;
         const int use = cnt[x] + (two ? i : i >> 1);
         const int key0 = (s.ka + i) * kKeys;
-        const int nh = R == 1 && key0 + kHalf < s.L ? 2 : 1;
-        // (what does not need the scores comes before the wait for them)
-        float sc_now = 0.f, alpha = 1.f, inv_vref = 0.f;
+        const bool both = key0 + kHalf < s.L;
+        // this warpgroup's halves: one query tile: half w; two: both
+        const int h0 = two ? 0 : w, nh = two ? (both ? 2 : 1) : (w == 0 || both ? 1 : 0);
+        if (*abort_flag || !warp_wait_bar(s_full + 8 * x, use & 1)) return false;
+        tc_fence_after();
+        float ks[kPg], vs[kPg];
+        float alpha = 1.f, inv_vref = 0.f;
         bool rescale = false;
+#pragma unroll
+        for (int q = 0; q < kPg; ++q) ks[q] = p.scale_log2;
         if (C::kFP8) {
-          // (a K scale of 0 would turn masked scores, -inf, into NaN)
-          sc_now = (lane & 8) || sc_next != sc_next ? sc_next : fmaxf(sc_next, 1e-30f);
-          sc_next = scale_raw(sc_id, i + 1);
-          sc_id = scale_id(i + 2);
+          // the tile's page scales (written before the codes were decoded, and so before S was made)
+          const float* sc = reinterpret_cast<const float*>(base + C::kOffScale + ((2 * (gt + i) + w) % kScaleSlots) * 256) + copy * kPg;
           float vm = 0.f;
 #pragma unroll
-          for (int q = 0; q < kTilePages / R; ++q)
-            vm = fmaxf(vm, __shfl_sync(0xffffffffu, sc_now, 8 + copy * (kTilePages / R) + q));
+          for (int q = 0; q < kPg; ++q) {
+            ks[q] *= sc[q];
+            vs[q] = sc[4 + q];
+            vm = fmaxf(vm, vs[q]);
+          }
           if (vm > vref) {  // (the same for the whole warp) twice the largest: growth below 2 needs no rescale
             if (vref > 0.f) {
               alpha = vref / (2.f * vm);
@@ -837,29 +864,34 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
           }
           inv_vref = vref > 0.f ? __frcp_rn(vref) : 0.f;
         }
-        if (*abort_flag || !warp_wait_polled(&s_full[x], use & 1)) return false;
-        tc_fence_after();
         const uint32_t col_s = t_row + kColS + (uint32_t)(x * kKeys);
-        if (live) {
-          float sv[kCols], ks[kPg];
-          // scores of piece h (R = 1: a half; else this copy's keys) and their scales
-          auto load_piece = [&](int h) {
-            const int c0 = R == 1 ? h * kHalf : copy * kCols;
-            uint32_t r0[32], r1[32];
-            tmem_ld32(col_s + c0, r0);
-            if (kCols == 64) tmem_ld32(col_s + c0 + 32, r1);
-            tc_wait_ld();
+        if (live && nh > 0) {
+          float sv[kCols];
+          auto load_half = [&](int h) {
+            if constexpr (kCols == 64) {
+              uint32_t r0[32], r1[32];
+              tmem_ld32(col_s + h * kHalf, r0);
+              tmem_ld32(col_s + h * kHalf + 32, r1);
+              tc_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              sv[c] = __uint_as_float(r0[c]);
-              if (kCols == 64) sv[32 + c] = __uint_as_float(r1[c]);
-            }
+              for (int c = 0; c < 32; ++c) {
+                sv[c] = __uint_as_float(r0[c]);
+                sv[32 + c] = __uint_as_float(r1[c]);
+              }
+            } else if constexpr (kCols == 32) {
+              uint32_t r0[32];
+              tmem_ld32(col_s + h * kHalf + copy * 32, r0);
+              tc_wait_ld();
 #pragma unroll
-            for (int q = 0; q < kPg; ++q) {
-              ks[q] = p.scale_log2;
-              if (C::kFP8) ks[q] *= __shfl_sync(0xffffffffu, sc_now, c0 / SCKV_PAGE_TOKENS + q);
+              for (int c = 0; c < 32; ++c) sv[c] = __uint_as_float(r0[c]);
+            } else {
+              uint32_t r0[16];
+              tmem_ld16(col_s + h * kHalf + copy * 16, r0);
+              tc_wait_ld();
+#pragma unroll
+              for (int c = 0; c < 16; ++c) sv[c] = __uint_as_float(r0[c]);
             }
-            const int off = key0 + c0 - s.ctx;
+            const int off = key0 + h * kHalf + copy * kCols - s.ctx;
             if (off + kCols > 0) {
               const unsigned long long win = valid ? tree_window(mask, p.mask_words, s.n, off) : 0ull;
               const uint32_t lo = (uint32_t)win, hi = (uint32_t)(win >> 32);
@@ -870,8 +902,8 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
           // the row's largest score; the scale is positive
           float pm = -INFINITY;
 #pragma unroll 1
-          for (int h = 0; h < nh; ++h) {
-            load_piece(h);
+          for (int hh = 0; hh < nh; ++hh) {
+            load_half(h0 + hh);
             float t = -INFINITY;
 #pragma unroll
             for (int q = 0; q < kPg; ++q) {  // (a short chain per page)
@@ -897,7 +929,7 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
             // O holds PV of this item's earlier tiles: wait for the last, then scale this warp's rows
             const int xp = two ? w : (i - 1) & 1;
             const int usep = cnt[xp] + (two ? i - 1 : (i - 1) >> 1);
-            if (!warp_wait_polled(&pv_done[xp], usep & 1)) return false;
+            if (!warp_wait_bar(pv_done + 8 * xp, usep & 1)) return false;
             tc_fence_after();
 #pragma unroll 1
             for (int cc = 0; cc < 4; ++cc) {
@@ -909,27 +941,23 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
               tmem_st32(t_row + col_o + cc * 32, r);
             }
             tc_wait_st();
-            load_piece(nh - 1);  // (the scores' registers were given up for this)
+            // (the scores' registers were given up for this)
+            load_half(h0 + nh - 1);
           }
           // 2^6 times the weight; a row that sees no key yet (m = -inf) has every score -inf: 2^-inf = 0
           const float mm = (m == -INFINITY) ? 0.f : m - 6.f;
           const uint64_t negm2 = f32x2(-mm, -mm), minus1 = f32x2(-1.f, -1.f);
           uint64_t ls2 = f32x2(0.f, 0.f);
 #pragma unroll 1
-          for (int h = nh - 1; h >= 0; --h) {
-            if (R == 1 && h < nh - 1) load_piece(h);
-            const int pg0 = R == 1 ? h * kHalfPages : copy * kPg;  // first page of the piece
-            // P of page pg: 8 columns at 64 (pg / 4) + 8 (pg % 4), its bf16 lo part 32 further on
-            const uint32_t pc = col_s + (pg0 >> 2) * kHalf + (pg0 & 3) * 8;
+          for (int hh = nh - 1; hh >= 0; --hh) {
+            if (two && hh < nh - 1) load_half(h0 + hh);
+            const uint32_t pc = col_s + (h0 + hh) * kHalf;
 #pragma unroll
-            for (int q = 0; q < kPg; ++q) {
+            for (int q = 0; q < kPg; ++q) {  // a page (16 keys) at a time
               uint32_t ph[8], plo[8];
               const uint64_t scale2 = f32x2(ks[q], ks[q]);
               uint64_t v2 = 0;
-              if (C::kFP8) {
-                const float vs = __shfl_sync(0xffffffffu, sc_now, 8 + pg0 + q) * inv_vref;
-                v2 = f32x2(vs, vs);
-              }
+              if (C::kFP8) v2 = f32x2(vs[q] * inv_vref, vs[q] * inv_vref);
 #pragma unroll
               for (int d = 0; d < 8; ++d) {
                 float x0, x1;
@@ -945,18 +973,17 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
                   plo[d] = pack2<true>(l0, l1);
                 }
               }
-              tmem_st8(pc + 8 * q, ph);
-              if (kBF16) tmem_st8(pc + 32 + 8 * q, plo);
+              tmem_st8(pc + 8 * (copy * kPg + q), ph);
+              if (kBF16) tmem_st8(pc + 32 + 8 * (copy * kPg + q), plo);
             }
-          }
-          if constexpr (R > 1) {  // the keys of the other copies
-            const uint32_t z[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+            if constexpr (R > 1) {  // the keys of the other copies
+              const uint32_t z[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
 #pragma unroll
-            for (int q = 0; q < kTilePages - kPg; ++q) {
-              const int pg = q < copy * kPg ? q : q + kPg;
-              const uint32_t pc = col_s + (pg >> 2) * kHalf + (pg & 3) * 8;
-              tmem_st8(pc, z);
-              if (kBF16) tmem_st8(pc + 32, z);
+              for (int q = 0; q < kHalfPages - kPg; ++q) {
+                const int pg = q < copy * kPg ? q : q + kPg;
+                tmem_st8(pc + 8 * pg, z);
+                if (kBF16) tmem_st8(pc + 32 + 8 * pg, z);
+              }
             }
           }
           float ls0, ls1;
@@ -964,15 +991,14 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
           l += ls0 + ls1;
           tc_wait_st();
         }
-        if (key0 + kKeys > s.ctx && w == 0) {
+        if (key0 + kKeys > s.ctx && (!two || w == 0)) {
           // V rows past the last node become 0, and so does what is not finite in a node's row (noted). The V tile of
-          // S(i) cannot be replaced before P(i) is written, and those before it in this slot were complete before S(i)
-          // (their PV finished, or went out from the same warp, earlier): the wait is for this tile's phase. (With two
-          // query tiles the first one's PV is first.)
-          const int st = slot_of(gt + i);
-          if (!warp_wait_polled(&v_full[st], turn_of(gt + i))) return false;
-          uint8_t* vt = v_ring + st * kSlot;
-          const int r0 = max(0, s.ctx - key0), r1 = key0 + kHalf < s.L ? kKeys : kHalf;
+          // S(i) cannot be replaced before P(i) is written, and the one before it in this slot was complete before S(i)
+          // (its PV went out earlier): the wait is for this tile's phase.
+          const int st = (gt + i) % kStages;
+          if (!warp_wait_bar(v_full + 8 * st, ((gt + i) / kStages) & 1)) return false;
+          uint8_t* vt = base + C::kOffV + st * kSlot;
+          const int r0 = max(h0 * kHalf, s.ctx - key0), r1 = (h0 + nh) * kHalf;
 #pragma unroll 1
           for (int c = row; c < (r1 - r0) * 16; c += 128) {
             const int r = r0 + (c >> 4), ch = c & 15;
@@ -1001,44 +1027,54 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[x]);
+        if (lane == 0) bar_arrive_n(p_full + 8 * x, two ? 2 : 1);  // 8 arrivals either way
       }
       // ---- the item's result, once its last PV finished
-      if constexpr (R > 1) {
-        s_ml[row] = make_float2(m, l);
-      }
       {
         const int i = s.nk - 1, x = two ? w : i & 1;
         const int use = cnt[x] + (two ? i : i >> 1);
-        if (!warp_wait_polled(&pv_done[x], use & 1)) return false;
+        if (!warp_wait_bar(pv_done + 8 * x, use & 1)) return false;
       }
+      s_ml[w * kRows + row] = make_float2(m, l);
+      if (lane == 0) s_vref[w * 4 + quad] = C::kFP8 ? vref : 1.f;
+      // both warpgroups' O are complete and every S product has finished (a bounded wait, not a named barrier: a
+      // warp that gave up must not leave the others waiting)
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(o_full);
+      if (!warp_wait_bar(o_full, k & 1)) return false;
       tc_fence_after();
-      float f0 = C::kFP8 ? vref : 1.f, M = m, Lsum = l;
-      float* xb = reinterpret_cast<float*>(base + C::kOffXchg);
-      // every warp of the warpgroup wrote its piece / read the pieces (bounded waits, not named barriers: a warp
-      // that gave up must not leave the others waiting)
-      auto meet = [&](uint64_t* bar) -> bool {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar);
-        return warp_wait_polled(bar, xchg & 1);
-      };
-      if constexpr (R > 1) {
-        if (!meet(x_full) || !meet(x_done)) return false;
-        ++xchg;
+      // one query tile: O[0] and O[1] (and the copies) join, warpgroup w writes dims 64 w ..; two: its own rows
+      const bool join = !two && s.ka * kKeys + kHalf < s.L;  // a second half held keys
+      float f0 = 1.f, f1 = 0.f, M = m, Lsum = l;
+      if constexpr (!two) {
         M = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < R; ++e) M = fmaxf(M, s_ml[(row & (kRows / R - 1)) + e * (kRows / R)].x);
+        for (int e = 0; e < R; ++e) {
+          const int o = (row & (kRows / R - 1)) + e * (kRows / R);
+          M = fmaxf(M, s_ml[o].x);
+          if (join) M = fmaxf(M, s_ml[kRows + o].x);
+        }
         auto weight = [&](float mx) { return mx == -INFINITY ? 1.f : ex2_approx(mx - M); };
         Lsum = 0.f;
 #pragma unroll
         for (int e = 0; e < R; ++e) {
-          const float2 a = s_ml[(row & (kRows / R - 1)) + e * (kRows / R)];
-          Lsum = fmaf(a.y, weight(a.x), Lsum);
+          const int o = (row & (kRows / R - 1)) + e * (kRows / R);
+          Lsum = fmaf(s_ml[o].y, weight(s_ml[o].x), Lsum);
+          if (join) Lsum = fmaf(s_ml[kRows + o].y, weight(s_ml[kRows + o].x), Lsum);
         }
-        f0 *= weight(m);
+        f0 = weight(s_ml[row].x);
+        if (join) f1 = weight(s_ml[kRows + row].x);
       }
+      f0 *= s_vref[two ? w * 4 + quad : quad];
+      f1 *= s_vref[4 + quad];
       const bool full = s.nk == s.kt;
-      if (full) f0 *= Lsum == 0.f ? 0.f : 1.f / Lsum;  // no key seen: zeros; NaN stays NaN
+      if (full) {
+        const float inv = Lsum == 0.f ? 0.f : 1.f / Lsum;  // no key seen: zeros; NaN stays NaN
+        f0 *= inv;
+        f1 *= inv;
+      }
+      const int d0 = two ? 0 : 64 * w, nd = two ? kHD : 64;
       const int64_t obase = ((int64_t)(s.q_base + node) * p.hq + head) * kHD;
       float* part = p.parts + (int64_t)(2 * blockIdx.x + (k > 0 ? 1 : 0)) * slot_floats(p.part_rows);
       auto put4 = [&](int d, float a, float b, float c, float e) {
@@ -1047,7 +1083,7 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
         else
           reinterpret_cast<float4*>(part)[(int64_t)(d >> 2) * p.part_rows + r_in] = make_float4(a, b, c, e);
       };
-      // f(page, slot) of the nodes that this row sees and whose V is not finite somewhere
+      // f(word, pos): the nodes that this row sees and whose V is not finite somewhere, by their position
       auto each_bad = [&](auto f) {
 #pragma unroll 1
         for (int wd = 0; wd < p.mask_words; ++wd) {
@@ -1062,111 +1098,122 @@ __global__ void __launch_bounds__(kThreadsTree, 1)
           }
         }
       };
-      if (live || R > 1) {
-#pragma unroll 1
-        for (int cc = 0; cc < kHD; cc += 32) {
-          float y[32];
-          {
-            uint32_t r[32];
-            tmem_ld32(t_row + col_o + cc, r);
-            tc_wait_ld();
+      // this thread's merged O, 32 dims from d0 + cc
+      auto merged = [&](int cc, float (&y)[32]) {
+        uint32_t r[32];
+        tmem_ld32(t_row + kColO + (two ? w * kHD : 0) + d0 + cc, r);
+        tc_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 32; ++c) y[c] = __uint_as_float(r[c]) * f0;
-          }
-          if constexpr (R == 1) {
+        for (int c = 0; c < 32; ++c) y[c] = __uint_as_float(r[c]) * f0;
+        if (join) {
+          tmem_ld32(t_row + kColO + kHD + d0 + cc, r);
+          tc_wait_ld();
+#pragma unroll
+          for (int c = 0; c < 32; ++c) y[c] = fmaf(__uint_as_float(r[c]), f1, y[c]);
+        }
+      };
+      if constexpr (R == 1) {
+        if (live) {
+#pragma unroll 1
+          for (int cc = 0; cc < nd; cc += 32) {
+            float y[32];
+            merged(cc, y);
             if (valid) {
 #pragma unroll
-              for (int c = 0; c < 32; c += 4) put4(cc + c, y[c], y[c + 1], y[c + 2], y[c + 3]);
+              for (int c = 0; c < 32; c += 4) put4(d0 + cc + c, y[c], y[c + 1], y[c + 2], y[c + 3]);
             }
             __syncwarp();
-          } else {
-            // the copies' rows are added up through the exchange buffer, 32 dims at a time: [row] of 128 bytes,
-            // 16-byte chunks swizzled by the row
+          }
+          if (valid) {
+            each_bad([&](int page, int slot) {
+#pragma unroll 1
+              for (int d = d0; d < d0 + nd; ++d) {
+                const float v = tree_v(p.g, p.layer, page, s.h, slot, d);
+                if (isfinite(v)) continue;
+                if (full)
+                  sckv_store_from_float(p.out, obase + d, p.out_dtype,
+                                        sckv_load_as_float(p.out, obase + d, p.out_dtype) + v);
+                else
+                  part[((int64_t)(d >> 2) * p.part_rows + r_in) * 4 + (d & 3)] += v;
+              }
+            });
+          }
+        }
+      } else {
+        // the copies' rows are added up through the (now idle) Q tile, 32 dims of each warpgroup at a time:
+        // [w][row] of 128 bytes, 16-byte chunks swizzled by the row
+        float* xb = reinterpret_cast<float*>(base) + w * kRows * 32;
+#pragma unroll 1
+        for (int cc = 0; cc < nd; cc += 32) {
+          {
+            float y[32];
+            merged(cc, y);
             float4* mine = reinterpret_cast<float4*>(xb + row * 32);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
               mine[j ^ (row & 7)] = valid ? make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3])
                                           : make_float4(0.f, 0.f, 0.f, 0.f);
-            if (valid && copy == 0) {
-              each_bad([&](int page, int slot) {
-#pragma unroll 1
-                for (int d = 0; d < 32; ++d) {
-                  const float v = tree_v(p.g, p.layer, page, s.h, slot, cc + d);
-                  if (!isfinite(v)) xb[row * 32 + (((d >> 2) ^ (row & 7)) << 2) + (d & 3)] += v;
-                }
-              });
-            }
-            if (!meet(x_full)) return false;
-            if (valid) {
-              const int sub = row & (kRows / R - 1);
-#pragma unroll
-              for (int jj = 0; jj < 8 / R; ++jj) {
-                const int j = copy * (8 / R) + jj;
-                float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                for (int e = 0; e < R; ++e) {
-                  const float4 b4 = reinterpret_cast<const float4*>(xb + (sub + e * (kRows / R)) * 32)[j ^ (sub & 7)];
-                  a.x += b4.x;
-                  a.y += b4.y;
-                  a.z += b4.z;
-                  a.w += b4.w;
-                }
-                put4(cc + 4 * j, a.x, a.y, a.z, a.w);
-              }
-            }
-            if (!meet(x_done)) return false;
-            ++xchg;
           }
-        }
-      }
-      if constexpr (R == 1) {
-        if (valid) {
-          each_bad([&](int page, int slot) {
+          if (valid && copy == 0) {
+            each_bad([&](int page, int slot) {
 #pragma unroll 1
-            for (int d = 0; d < kHD; ++d) {
-              const float v = tree_v(p.g, p.layer, page, s.h, slot, d);
-              if (isfinite(v)) continue;
-              if (full)
-                sckv_store_from_float(p.out, obase + d, p.out_dtype, sckv_load_as_float(p.out, obase + d, p.out_dtype) + v);
-              else
-                part[((int64_t)(d >> 2) * p.part_rows + r_in) * 4 + (d & 3)] += v;
+              for (int d = 0; d < 32; ++d) {
+                const float v = tree_v(p.g, p.layer, page, s.h, slot, d0 + cc + d);
+                if (!isfinite(v)) xb[row * 32 + (((d >> 2) ^ (row & 7)) << 2) + (d & 3)] += v;
+              }
+            });
+          }
+          __syncwarp();
+          if (lane == 0) bar_arrive(x_full + 8 * w);
+          if (!warp_wait_bar(x_full + 8 * w, xchg & 1)) return false;
+          if (valid) {
+            const int sub = row & (kRows / R - 1);
+#pragma unroll
+            for (int jj = 0; jj < 8 / R; ++jj) {
+              const int j = copy * (8 / R) + jj;
+              float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+              for (int e = 0; e < R; ++e) {
+                const float4 b4 = reinterpret_cast<const float4*>(xb + (sub + e * (kRows / R)) * 32)[j ^ (sub & 7)];
+                a.x += b4.x;
+                a.y += b4.y;
+                a.z += b4.z;
+                a.w += b4.w;
+              }
+              put4(d0 + cc + 4 * j, a.x, a.y, a.z, a.w);
             }
-          });
+          }
+          __syncwarp();
+          if (lane == 0) bar_arrive(x_done);
+          if (!warp_wait_bar(x_done, xchg & 1)) return false;
+          ++xchg;
         }
       }
-      if (!full && valid && copy == 0)
+      if (!full && valid && copy == 0 && (two || w == 0))
         reinterpret_cast<float2*>(part + (int64_t)p.part_rows * kHD)[r_in] = make_float2(M, Lsum);
-      // the other flags were last read (by both warpgroups) in the item before and are next set in the one after
-      if (w == 0 && row < kMaskWordsMax) s_bad[((k + 1) & 1) * kMaskWordsMax + row] = 0;
+      // the other flags were last read in the item before and are next set in the one after
+      if (tid < kMaskWordsMax) s_bad[((k + 1) & 1) * kMaskWordsMax + tid] = 0;
       tc_fence_before();
-      __syncwarp();
-      return true;
-    };
-    bool more = tree_next(p, cum, walk, s);
-    for (int k = 0; ok && more; ++k) {
-      if (w == 0 || s.nq == 2) {
-        ok = load_q();
-        if (ok) {
-          if (s.copies == 1) ok = run_item(std::integral_constant<int, 1>{}, k);
-          else if (s.copies == 2) ok = run_item(std::integral_constant<int, 2>{}, k);
-          else ok = run_item(std::integral_constant<int, 4>{}, k);
-        }
-        if (!ok) break;
-      }
-      const bool two = s.nq == 2;
-      if (two && w == 1 && lane == 0) mbar_arrive(o1_free);
       gt += s.nk;
       cnt[0] += two ? s.nk : (s.nk + 1) >> 1;
       cnt[1] += two ? s.nk : s.nk >> 1;
-      n_two += two;
+      return true;
+    };
+    for (int k = 0; ok && more; ++k) {
+      if (C::kQTiles == 2 && s.nq == 2) ok = run_item(std::integral_constant<bool, C::kQTiles == 2>{}, std::integral_constant<int, 1>{}, k);
+      else if (s.copies == 1) ok = run_item(std::false_type{}, std::integral_constant<int, 1>{}, k);
+      else if (s.copies == 2) ok = run_item(std::false_type{}, std::integral_constant<int, 2>{}, k);
+      else ok = run_item(std::false_type{}, std::integral_constant<int, 4>{}, k);
+      if (!ok) break;
       more = tree_next(p, cum, walk, s);
+      if (more) load_q(s);
     }
     if (!ok) {
       if (lane == 0 && !*abort_flag) sckv_report(p.g.status, SCKV_ERR_TIMEOUT, blockIdx.x, KID_TREE_ATTN);
       if (lane == 0) *abort_flag = 1;
     }
   } else {
-    reg_give();
+    reg_give<C::kGiveRegs>();
   }
   if (warp < 4 || warp >= 12) __syncwarp();
   tc_fence_before();
@@ -1257,7 +1304,7 @@ int launch_tree(sckv_pool* p, const TreeParams& t, cudaStream_t stream) {
   const int smem = C::kFixedSmem + 4 * t.n_seqs;
   static_assert(C::kFixedSmem + 4 * kMaxSeqs <= 227 * 1024, "shared memory of the largest batch");
   SCKV_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  kern<<<p->num_sms, kThreadsTree, smem, stream>>>(t, *map);
+  kern<<<p->num_sms, C::kThreads, smem, stream>>>(t, *map);
   SCKV_LAUNCH_CHECK();
   SCKV_CUDA_CHECK(sckv_launch_pdl(tree_join_kernel, dim3(p->num_sms, t.part_rows / 32), dim3(256), 0, stream, t));
   SCKV_LAUNCH_CHECK();

@@ -47,6 +47,23 @@ __device__ __forceinline__ int64_t int8_scale_idx(const Geo& g, int64_t layer, i
   return (((layer * g.P + page) * 2 + kv) * g.H + h) * SCKV_PAGE_TOKENS + slot;
 }
 
+// 8 values of 16 bits as float.
+__device__ __forceinline__ void unpack8(const uint4& raw, int dtype, float v[8]) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (dtype == SCKV_DTYPE_F16) {
+      __half2 h2 = *reinterpret_cast<const __half2*>(&w[i]);
+      float2 f = __half22float2(h2);
+      v[2 * i] = f.x; v[2 * i + 1] = f.y;
+    } else {
+      __nv_bfloat162 b2 = *reinterpret_cast<const __nv_bfloat162*>(&w[i]);
+      float2 f = __bfloat1622float2(b2);
+      v[2 * i] = f.x; v[2 * i + 1] = f.y;
+    }
+  }
+}
+
 // Load 8 consecutive source values as float.
 __device__ __forceinline__ void load8(const void* src, int64_t idx, int dtype, float v[8]) {
   if (dtype == SCKV_DTYPE_F32) {
@@ -54,20 +71,7 @@ __device__ __forceinline__ void load8(const void* src, int64_t idx, int dtype, f
     float4 a = p[0], b = p[1];
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   } else {
-    uint4 raw = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(src) + idx);
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (dtype == SCKV_DTYPE_F16) {
-        __half2 h2 = *reinterpret_cast<const __half2*>(&w[i]);
-        float2 f = __half22float2(h2);
-        v[2 * i] = f.x; v[2 * i + 1] = f.y;
-      } else {
-        __nv_bfloat162 b2 = *reinterpret_cast<const __nv_bfloat162*>(&w[i]);
-        float2 f = __bfloat1622float2(b2);
-        v[2 * i] = f.x; v[2 * i + 1] = f.y;
-      }
-    }
+    unpack8(*reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(src) + idx), dtype, v);
   }
 }
 

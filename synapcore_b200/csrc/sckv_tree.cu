@@ -5,8 +5,13 @@
 #include <math.h>
 
 #include "sckv_geo.cuh"
+#include "sckv_tcgen05.cuh"
 
 using namespace sckv_geo;
+using sckv_tc::f32x2;
+using sckv_tc::f32x2_split;
+using sckv_tc::fma_f32x2;
+using sckv_tc::mul_f32x2;
 
 namespace {
 
@@ -21,17 +26,23 @@ namespace {
 // drafted tree sit in consecutive slots but rotate by depth, and image tokens
 // rotate by (time, height, width).
 //
-// Bound by HBM: (Hq + 2 Hkv) rows read and written once. Eight lanes own a
-// head row, each 8 dims of the first half and their 8 partners of the second
-// (two 16-byte loads and stores per 16-bit row, rotation without exchange, a
-// norm of three shuffles); a CTA takes `tpb` tokens so their angles are
-// computed once for all heads. The angle is formed and reduced to [-pi, pi] in
-// 64 bits (a far position times a frequency near 1 has no useful fp32 bits
-// left after the reduction); sin and cos then run in fp32.
+// Bound by HBM: (Hq + 2 Hkv) rows read and written once. A CTA takes `tpb`
+// tokens, whose angles are computed once for all heads; eight lanes own a head
+// row, each 8 dims of the first half and their 8 partners of the second (two
+// 16-byte loads and stores per 16-bit row, rotation without exchange, a norm
+// of three shuffles). With q, k and v of one 16-bit type a thread has its next
+// row on the way while it works on one, the first before the angles are
+// computed and the pages looked up, and what a row needs by address is kept
+// per token. The arithmetic runs on packed pairs: issue slots are the second
+// bound. 8,192 tokens of 32 + 2 x 8 bf16 heads: 41 us, 4.9 TB/s (74 % of a
+// copy's rate); two rows on the way and CTAs of 256 threads were slower (51, 43
+// us). The angle is formed and reduced to [-pi, pi] in 64 bits (a
+// far position times a frequency near 1 has no useful fp32 bits left after the
+// reduction); sin and cos then run in fp32.
 // ---------------------------------------------------------------------------
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 128;
 constexpr int kRopeD = 128;
-constexpr int kRopeTokens = 4;  // most tokens of one CTA
+constexpr int kRopeTokens = 4;   // most tokens of a CTA
 
 struct RopeAxes {
   Geo g;
@@ -112,12 +123,41 @@ __device__ __forceinline__ void store_row8_int8(const Geo& g, int layer, int64_t
     reinterpret_cast<__half*>(g.scales)[int8_scale_idx(g, layer, page, kv, h, slot)] = __float2half_rn(s);
 }
 
+// kDT: the 16-bit type of q, k and v, or -1: any types, not fetched ahead.
+template <int kDT>
 __global__ void __launch_bounds__(kRopeThreads) rope_axes_kernel(const RopeAxes p) {
-  __shared__ float s_cos[kRopeTokens * (kRopeD / 2)], s_sin[kRopeTokens * (kRopeD / 2)];
+  constexpr bool kAhead = kDT >= 0;
+  __shared__ __align__(16) float s_cos[kRopeTokens * (kRopeD / 2)], s_sin[kRopeTokens * (kRopeD / 2)];
+  __shared__ __align__(16) float s_w[2][kRopeD];
+  __shared__ const uint8_t* s_src[kRopeTokens][4];  // head 0 of q, k, v
+  __shared__ uint8_t* s_dst[kRopeTokens][4];        // head 0's row of a 16-bit kDT output, or null
   __shared__ int64_t s_page[kRopeTokens];
   __shared__ int s_slot[kRopeTokens];  // -1: not a token of any sequence
-  const int t0 = blockIdx.x * p.tpb;
-  const int nt = min(p.tpb, p.n_tokens - t0);
+  const int t0 = blockIdx.x * p.tpb, nt = min(p.tpb, p.n_tokens - t0);
+  const int l8 = threadIdx.x & 7;
+  const unsigned m = 0xffu << (threadIdx.x & 24);
+  const int H = p.g.H, rows = p.hq + 2 * H;
+  constexpr int kStep = kRopeThreads / 8;  // rows of the CTA at once
+  auto kind_of = [&](int hr) { return hr < p.hq ? 0 : hr < p.hq + H ? 1 : 2; };  // q, k, v
+  auto head_of = [&](int hr, int kind) { return hr - (kind == 0 ? 0 : kind == 1 ? p.hq : p.hq + H); };
+  auto src_of = [&](int kind) { return kind == 0 ? p.q : kind == 1 ? p.k : p.v; };
+  auto ld_of = [&](int kind) { return kind == 0 ? p.q_stride : kind == 1 ? p.k_stride : p.v_stride; };
+  auto wrap = [&](int& tt, int& hr) {
+    while (hr >= rows) {
+      hr -= rows;
+      ++tt;
+    }
+  };
+  int tt = 0, hr = threadIdx.x >> 3;  // the thread's next row: token, row of q | k | v
+  wrap(tt, hr);
+  uint4 ra = make_uint4(0u, 0u, 0u, 0u), rb = ra;
+  if (kAhead && tt < nt) {
+    const int kind = kind_of(hr);
+    const uint4* x = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(src_of(kind)) +
+                                                    (t0 + tt) * ld_of(kind) + head_of(hr, kind) * kRopeD) + l8;
+    ra = __ldg(x);
+    rb = __ldg(x + kRopeD / 2 / 8);
+  }
   for (int i = threadIdx.x; i < nt * (kRopeD / 2); i += kRopeThreads) {
     const int t = t0 + i / (kRopeD / 2), f = i % (kRopeD / 2);
     int axis = __ldg(p.axis_map + f);
@@ -129,8 +169,11 @@ __global__ void __launch_bounds__(kRopeThreads) rope_axes_kernel(const RopeAxes 
     const double r = a - 6.283185307179586 * rint(a * 0.15915494309189535);
     sincosf((float)r, &s_sin[i], &s_cos[i]);
   }
-  if (threadIdx.x < nt) {
-    const int t = t0 + threadIdx.x;
+  static_assert(kRopeThreads == kRopeD, "a thread brings its dim's weights");
+  if (p.q_w != nullptr) s_w[0][threadIdx.x] = __half2float(p.q_w[threadIdx.x]);
+  if (p.k_w != nullptr) s_w[1][threadIdx.x] = __half2float(p.k_w[threadIdx.x]);
+  if (kRopeThreads - 1 - (int)threadIdx.x < nt) {
+    const int tl = kRopeThreads - 1 - threadIdx.x, t = t0 + tl;
     int slot = -1;
     int64_t page = -1;
     if (t >= __ldg(p.cu) && t < __ldg(p.cu + p.n_seqs)) {
@@ -139,55 +182,87 @@ __global__ void __launch_bounds__(kRopeThreads) rope_axes_kernel(const RopeAxes 
       page = resolve_page(p.g, p.bt, p.bt_stride, p.max_blocks, b, pos, KID_ROPE_AXES);
       slot = page >= 0 ? pos % SCKV_PAGE_TOKENS : 0;
     }
-    s_page[threadIdx.x] = page;
-    s_slot[threadIdx.x] = slot;
-  }
-  __syncthreads();
-  const int l8 = threadIdx.x & 7;
-  const unsigned m = 0xffu << (threadIdx.x & 24);
-  const int H = p.g.H, rows = p.hq + 2 * H;
-  for (int r = threadIdx.x >> 3; r < nt * rows; r += kRopeThreads / 8) {
-    const int tt = r / rows, hr = r - tt * rows;
-    const int64_t page = s_page[tt];
-    const int slot = s_slot[tt];
-    if (slot < 0) continue;
-    const int t = t0 + tt;
-    const int kind = hr < p.hq ? 0 : hr < p.hq + H ? 1 : 2;  // q, k, v
-    const int h = kind == 0 ? hr : kind == 1 ? hr - p.hq : hr - p.hq - H;
-    if (kind != 0 && page < 0) continue;
-    const void* src = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
-    const int64_t stride = kind == 0 ? p.q_stride : kind == 1 ? p.k_stride : p.v_stride;
-    const int dt = kind == 0 ? p.q_dtype : p.src_dtype;
-    const int64_t base = t * stride + (int64_t)h * kRopeD + 8 * l8;
-    float a[8], b[8];
-    load8(src, base, dt, a);
-    load8(src, base + kRopeD / 2, dt, b);
-    if (kind < 2) {
-      const __half* w = kind == 0 ? p.q_w : p.k_w;
-      if (w != nullptr) {
-        float ss = 0.f;
+    s_page[tl] = page;
+    s_slot[tl] = slot;
+    if (kAhead) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
-        const float inv = 1.f / sqrtf(row_sum(ss, m) * (1.f / kRopeD) + p.eps);
-        float wa[8], wb[8];
-        load8(w, 8 * l8, SCKV_DTYPE_F16, wa);
-        load8(w, kRopeD / 2 + 8 * l8, SCKV_DTYPE_F16, wb);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          a[i] = a[i] * inv * wa[i];
-          b[i] = b[i] * inv * wb[i];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int f = tt * (kRopeD / 2) + 8 * l8 + i;
-        const float c = s_cos[f], s = s_sin[f];
-        const float x = a[i], y = b[i];
-        a[i] = x * c - y * s;
-        b[i] = y * c + x * s;
+      for (int kind = 0; kind < 3; ++kind) {
+        s_src[tl][kind] = reinterpret_cast<const uint8_t*>(src_of(kind)) + t * ld_of(kind) * 2;
+        uint8_t* dst = nullptr;
+        if (kind == 0 && p.q_out_dtype == kDT) dst = reinterpret_cast<uint8_t*>(p.q_out) + (int64_t)t * p.hq * kRopeD * 2;
+        if (kind > 0 && p.g.dtype == kDT && page >= 0)
+          dst = reinterpret_cast<uint8_t*>(p.g.data) + row_off(p.g, p.layer, page, kind - 1, 0, slot) * 2;
+        s_dst[tl][kind] = dst;
       }
     }
-    if (kind == 0) {
+  }
+  __syncthreads();
+  while (tt < nt) {
+    const int tl = tt, kind = kind_of(hr), h = head_of(hr, kind), t = t0 + tl;
+    const int dt = kAhead ? kDT : kind == 0 ? p.q_dtype : p.src_dtype;
+    float a[8], b[8];
+    if (kAhead) {
+      unpack8(ra, dt, a);
+      unpack8(rb, dt, b);
+    }
+    hr += kStep;
+    wrap(tt, hr);
+    if (kAhead && tt < nt) {
+      const int k2 = kind_of(hr);
+      const uint4* x = reinterpret_cast<const uint4*>(s_src[tt][k2] + head_of(hr, k2) * (kRopeD * 2)) + l8;
+      ra = __ldg(x);
+      rb = __ldg(x + kRopeD / 2 / 8);
+    }
+    const int64_t page = s_page[tl];
+    const int slot = s_slot[tl];
+    if (slot < 0 || (kind != 0 && page < 0)) continue;
+    if (!kAhead) {
+      const int64_t at = t * ld_of(kind) + (int64_t)h * kRopeD + 8 * l8;
+      load8(src_of(kind), at, dt, a);
+      load8(src_of(kind), at + kRopeD / 2, dt, b);
+    }
+    if (kind < 2) {
+      uint64_t x[4], y[4];  // pairs of the first and the second half
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = f32x2(a[2 * e], a[2 * e + 1]);
+        y[e] = f32x2(b[2 * e], b[2 * e + 1]);
+      }
+      if ((kind == 0 ? p.q_w : p.k_w) != nullptr) {
+        uint64_t ss2 = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ss2 = fma_f32x2(x[e], x[e], fma_f32x2(y[e], y[e], ss2));
+        float s0, s1;
+        f32x2_split(ss2, s0, s1);
+        const float inv = rsqrtf(row_sum(s0 + s1, m) * (1.f / kRopeD) + p.eps);
+        const uint64_t inv2 = f32x2(inv, inv);
+        const ulonglong2* wa = reinterpret_cast<const ulonglong2*>(&s_w[kind][8 * l8]);
+        const ulonglong2* wb = reinterpret_cast<const ulonglong2*>(&s_w[kind][kRopeD / 2 + 8 * l8]);
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          const ulonglong2 u = wa[e / 2], v = wb[e / 2];
+          x[e] = mul_f32x2(mul_f32x2(x[e], inv2), u.x);
+          x[e + 1] = mul_f32x2(mul_f32x2(x[e + 1], inv2), u.y);
+          y[e] = mul_f32x2(mul_f32x2(y[e], inv2), v.x);
+          y[e + 1] = mul_f32x2(mul_f32x2(y[e + 1], inv2), v.y);
+        }
+      }
+      const ulonglong2* pc = reinterpret_cast<const ulonglong2*>(s_cos + tl * (kRopeD / 2) + 8 * l8);
+      const ulonglong2* ps = reinterpret_cast<const ulonglong2*>(s_sin + tl * (kRopeD / 2) + 8 * l8);
+      const uint64_t neg = f32x2(-1.f, -1.f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint64_t c = e & 1 ? pc[e / 2].y : pc[e / 2].x, sn = e & 1 ? ps[e / 2].y : ps[e / 2].x;
+        f32x2_split(fma_f32x2(x[e], c, mul_f32x2(mul_f32x2(y[e], sn), neg)), a[2 * e], a[2 * e + 1]);
+        f32x2_split(fma_f32x2(y[e], c, mul_f32x2(x[e], sn)), b[2 * e], b[2 * e + 1]);
+      }
+    }
+    uint8_t* d16 = kAhead ? s_dst[tl][kind] : nullptr;
+    if (d16 != nullptr) {
+      uint16_t* o = reinterpret_cast<uint16_t*>(d16) + h * (kind == 0 ? kRopeD : SCKV_PAGE_TOKENS * kRopeD) + 8 * l8;
+      store8_16(o, 0, dt, a);
+      store8_16(o, kRopeD / 2, dt, b);
+    } else if (kind == 0) {
       const int64_t o = ((int64_t)t * p.hq + h) * kRopeD + 8 * l8;
       store8(p.q_out, o, p.q_out_dtype, a);
       store8(p.q_out, o + kRopeD / 2, p.q_out_dtype, b);
@@ -236,18 +311,23 @@ __global__ void rope_axes_fp8_kernel(const RopeAxes p) {
 // path[j] >= j: rows only move down, and a row is read before anything lands
 // on it when destinations are taken in order.
 //
-// Bound by HBM (each moved row read and written once). One warp owns
-// (sequence, layer, K|V, head) and takes one destination page at a time: all
-// of its loads are issued, then its stores, 16 bytes a lane. Rows that stay
-// where they are are not touched.
+// Bound by HBM (each moved row read and written once, as single rows of 128 or
+// 256 bytes). A CTA takes slices (layer, K|V, head) of one sequence: it checks
+// the path and looks the moved rows' pages up once, kMoves at a time, and each
+// warp moves these rows of its slices: the 16-byte pieces of kMoveBatch loads
+// a lane at a time, all loads before the stores. Pieces are taken by slice,
+// then by path, so whatever lands on a row was preceded by all of its reads.
 //
 // FP8: a page-head has one scale for its 16 rows. Rows that come from other
 // pages are values code * s_src; the destination's scale grows to
 // max(s, max|value| / 448) as an append's does, and the rows it already held
 // are re-encoded when it grew. A destination page is only a source for rows
-// of itself and of earlier pages, so scales are read before they change.
+// of itself and of earlier pages, so scales are read before they change. One
+// warp owns a slice and takes a destination page at a time.
 // ---------------------------------------------------------------------------
-constexpr int kCompactWarps = 8;
+constexpr int kCompactWarps = 4;
+constexpr int kMoves = 256;    // moved rows whose pages are known at a time
+constexpr int kMoveBatch = 4;  // 16-byte pieces that a lane holds
 
 struct Compact {
   Geo g;
@@ -258,10 +338,97 @@ struct Compact {
   const int32_t* bt;
   int64_t bt_stride;
   int max_blocks;
+  int per_warp;  // slices of a warp (not FP8)
 };
 
-template <bool kFP8>
+// i / d for i < 2^16, 0 < d < 2^16, mul = 2^32 / d + 1
+__device__ __forceinline__ uint32_t div_by(uint32_t i, uint32_t mul, uint32_t d) { return d == 1 ? i : __umulhi(i, mul); }
+
 __global__ void __launch_bounds__(kCompactWarps * 32) compact_kernel(const Compact p) {
+  const Geo& g = p.g;
+  const int n_slices = p.n_layers * 2 * g.H;
+  const int groups = (n_slices + kCompactWarps * p.per_warp - 1) / (kCompactWarps * p.per_warp);
+  const int b = blockIdx.x / groups, grp = blockIdx.x - b * groups;
+  const bool reporter = grp == 0;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ int64_t s_src[kMoves], s_dst[kMoves];  // page * 16 + slot; -1: not moved
+  const int keep = __ldg(p.n_keep + b), ctx = __ldg(p.ctx + b);
+  const int32_t* path = p.path + (int64_t)b * p.max_path;
+  const int cap = p.max_blocks * SCKV_PAGE_TOKENS;
+  if (keep < 0 || keep > p.max_path || ctx < 0 || ctx > cap) {
+    if (reporter && threadIdx.x == 0) sckv_report(g.status, SCKV_ERR_BOUNDS, b, KID_COMPACT);
+    return;
+  }
+  // the path increases and stays inside the table; rows 0 .. j0 - 1 do not move
+  bool bad = false;
+  for (int j = threadIdx.x; j < keep; j += kCompactWarps * 32) {
+    const int pj = __ldg(path + j), before = j > 0 ? __ldg(path + j - 1) : -1;
+    bad |= pj <= before || pj >= cap - ctx;
+  }
+  if (__syncthreads_or(bad)) {
+    if (reporter && threadIdx.x == 0) sckv_report(g.status, SCKV_ERR_BOUNDS, b, KID_COMPACT);
+    return;
+  }
+  int j0 = 0;  // (an increasing path that left the diagonal stays off it)
+  for (int jb = 0; jb < keep; jb += kCompactWarps * 32) {
+    const int j = jb + threadIdx.x;
+    j0 += __syncthreads_count(j < keep && __ldg(path + j) == j);
+  }
+  const int32_t* bt = p.bt + (int64_t)b * p.bt_stride;
+  const int eb = g.dtype == SCKV_DTYPE_F16 || g.dtype == SCKV_DTYPE_BF16 ? 2 : 1;
+  const uint32_t cpr = (uint32_t)(g.D * eb / 16), cpr_mul = (uint32_t)(0x100000000ull / cpr) + 1u;  // pieces of a row
+  uint8_t* data = reinterpret_cast<uint8_t*>(g.data);
+  __half* hscale = reinterpret_cast<__half*>(g.scales);
+  const int sl0 = (grp * kCompactWarps + warp) * p.per_warp, n_mine = max(0, min(p.per_warp, n_slices - sl0));
+  for (int jb = j0; jb < keep; jb += kMoves) {
+    const int nm = min(kMoves, keep - jb);
+    for (int i = threadIdx.x; i < nm; i += kCompactWarps * 32) {
+      const int from = ctx + __ldg(path + jb + i), to = ctx + jb + i;
+      const int ps = __ldg(bt + from / SCKV_PAGE_TOKENS), pd = __ldg(bt + to / SCKV_PAGE_TOKENS);
+      const bool ok = ps >= 0 && ps < g.P && pd >= 0 && pd < g.P;
+      if (!ok && reporter) sckv_report(g.status, SCKV_ERR_BOUNDS, pd >= 0 && pd < g.P ? ps : pd, KID_COMPACT);
+      s_src[i] = ok ? (int64_t)ps * SCKV_PAGE_TOKENS + from % SCKV_PAGE_TOKENS : -1;
+      s_dst[i] = ok ? (int64_t)pd * SCKV_PAGE_TOKENS + to % SCKV_PAGE_TOKENS : -1;
+    }
+    __syncthreads();
+    const uint32_t per = (uint32_t)nm * cpr, nm_mul = (uint32_t)(0x100000000ull / nm) + 1u, n = (uint32_t)n_mine * per;
+    for (uint32_t i0 = 0; i0 < n; i0 += 32 * kMoveBatch) {
+      uint4 r[kMoveBatch];
+      __half sc[kMoveBatch];
+      int64_t dst[kMoveBatch];
+#pragma unroll
+      for (int k = 0; k < kMoveBatch; ++k) {
+        const uint32_t i = i0 + 32 * k + lane;
+        dst[k] = -1;
+        if (i >= n) continue;
+        const uint32_t row = div_by(i, cpr_mul, cpr), ch = i - row * cpr;
+        const uint32_t sl = div_by(row, nm_mul, nm), j = row - sl * nm;
+        const int64_t ps = s_src[j], pd = s_dst[j];
+        if (ps < 0) continue;
+        const int s_abs = sl0 + (int)sl, h = s_abs % g.H, lk = s_abs / g.H;
+        const int layer = p.layer0 + (lk >> 1), kv = lk & 1;
+        const int64_t so = row_off(g, layer, ps / SCKV_PAGE_TOKENS, kv, h, (int)(ps % SCKV_PAGE_TOKENS));
+        const int64_t po = row_off(g, layer, pd / SCKV_PAGE_TOKENS, kv, h, (int)(pd % SCKV_PAGE_TOKENS));
+        r[k] = *reinterpret_cast<const uint4*>(data + so * eb + ch * 16);
+        dst[k] = po * eb + ch * 16;
+        if (g.dtype == SCKV_DTYPE_INT8 && ch == 0)
+          sc[k] = hscale[int8_scale_idx(g, layer, ps / SCKV_PAGE_TOKENS, kv, h, (int)(ps % SCKV_PAGE_TOKENS))];
+      }
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < kMoveBatch; ++k) {
+        if (dst[k] < 0) continue;
+        *reinterpret_cast<uint4*>(data + dst[k]) = r[k];
+        // (int8: a row has D bytes, its scale one entry)
+        if (g.dtype == SCKV_DTYPE_INT8 && dst[k] % g.D == 0) hscale[dst[k] / g.D] = sc[k];
+      }
+      __syncwarp();
+    }
+    __syncthreads();
+  }
+}
+
+__global__ void __launch_bounds__(kCompactWarps * 32) compact_fp8_kernel(const Compact p) {
   const Geo& g = p.g;
   const int lane = threadIdx.x & 31;
   const int64_t units = (int64_t)p.n_seqs * p.n_layers * 2 * g.H;
@@ -296,11 +463,9 @@ __global__ void __launch_bounds__(kCompactWarps * 32) compact_kernel(const Compa
   j0 = __reduce_min_sync(0xffffffffu, j0);
   if (j0 >= keep) return;
   const int32_t* bt = p.bt + (int64_t)b * p.bt_stride;
-  const int eb = g.dtype == SCKV_DTYPE_F16 || g.dtype == SCKV_DTYPE_BF16 ? 2 : 1;
-  const int cpr = g.D * eb / 16;  // 16-byte chunks of a row
+  const int cpr = g.D / 16;  // 16-byte chunks of a row
   uint8_t* data = reinterpret_cast<uint8_t*>(g.data);
   float* fscale = reinterpret_cast<float*>(g.scales);
-  __half* hscale = reinterpret_cast<__half*>(g.scales);
   for (int blk = (ctx + j0) / SCKV_PAGE_TOKENS; blk <= (ctx + keep - 1) / SCKV_PAGE_TOKENS; ++blk) {
     const int32_t dpage = __ldg(bt + blk);
     if (dpage < 0 || dpage >= g.P) {
@@ -319,87 +484,53 @@ __global__ void __launch_bounds__(kCompactWarps * 32) compact_kernel(const Compa
         return -1;
       }
       *from = page;
-      return row_off(g, layer, page, kv, h, pos % SCKV_PAGE_TOKENS) * eb;
+      return row_off(g, layer, page, kv, h, pos % SCKV_PAGE_TOKENS);
     };
-    const int64_t dst0 = row_off(g, layer, dpage, kv, h, 0) * eb;
-    constexpr int kBatch = 8;
-    if constexpr (!kFP8) {
-      for (int i0 = 0; i0 < SCKV_PAGE_TOKENS * cpr; i0 += 32 * kBatch) {
-        uint4 r[kBatch];
-        bool mv[kBatch];
+    const int64_t dst0 = row_off(g, layer, dpage, kv, h, 0);
+    const float s_dst = fscale[fp8_scale_idx(g, layer, dpage, kv, h)];
+    // pass 1: the largest value that comes from another page
+    float top = 0.f;
+    for (int i = lane; i < SCKV_PAGE_TOKENS * cpr; i += 32) {
+      int32_t from = dpage;
+      const int64_t off = source(i / cpr, &from);
+      if (off < 0 || from == dpage) continue;
+      const float sc = fscale[fp8_scale_idx(g, layer, from, kv, h)];
+      const uint4 w = *reinterpret_cast<const uint4*>(data + off + (i % cpr) * 16);
+      const uint8_t* c = reinterpret_cast<const uint8_t*>(&w);
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-          const int i = i0 + 32 * k + lane;
-          int32_t from;
-          const int64_t off = i < SCKV_PAGE_TOKENS * cpr ? source(i / cpr, &from) : -1;
-          mv[k] = off >= 0;
-          if (mv[k]) r[k] = *reinterpret_cast<const uint4*>(data + off + (i % cpr) * 16);
-        }
-        __syncwarp();
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(sckv_fp8_to_float(c[e]) * sc));
+    }
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k)
-          if (mv[k]) *reinterpret_cast<uint4*>(data + dst0 + (int64_t)(i0 + 32 * k + lane) * 16) = r[k];
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float s_new = fmaxf(s_dst, top / 448.0f);
+    // pass 2: rows in order, 32 / cpr of them at a time (loads before stores)
+    for (int i0 = 0; i0 < SCKV_PAGE_TOKENS * cpr; i0 += 32) {
+      const int i = i0 + lane;
+      int32_t from = dpage;
+      int64_t off = i < SCKV_PAGE_TOKENS * cpr ? source(i / cpr, &from) : -1;
+      bool store = off >= 0;
+      off += (i % cpr) * 16;
+      if (!store && i < SCKV_PAGE_TOKENS * cpr && first + i / cpr < j0 && s_new > s_dst) {
+        off = dst0 + (int64_t)i * 16;  // a row that stays: re-encoded under the grown scale
+        from = dpage;
+        store = true;
       }
-      if (g.dtype == SCKV_DTYPE_INT8) {
-        const int s = lane & 15, j = first + s;
-        const bool mine = lane < SCKV_PAGE_TOKENS && j >= j0 && j < keep;
-        __half sc = __float2half_rn(0.f);
-        bool have = false;
-        if (mine) {
-          const int pos = ctx + __ldg(path + j);
-          const int32_t page = __ldg(bt + pos / SCKV_PAGE_TOKENS);
-          have = page >= 0 && page < g.P;
-          if (have) sc = hscale[int8_scale_idx(g, layer, page, kv, h, pos % SCKV_PAGE_TOKENS)];
-        }
-        __syncwarp();
-        if (have) hscale[int8_scale_idx(g, layer, dpage, kv, h, s)] = sc;
-      }
-    } else {
-      const float s_dst = fscale[fp8_scale_idx(g, layer, dpage, kv, h)];
-      // pass 1: the largest value that comes from another page
-      float top = 0.f;
-      for (int i = lane; i < SCKV_PAGE_TOKENS * cpr; i += 32) {
-        int32_t from = dpage;
-        const int64_t off = source(i / cpr, &from);
-        if (off < 0 || from == dpage) continue;
-        const float sc = fscale[fp8_scale_idx(g, layer, from, kv, h)];
-        const uint4 w = *reinterpret_cast<const uint4*>(data + off + (i % cpr) * 16);
-        const uint8_t* c = reinterpret_cast<const uint8_t*>(&w);
+      uint4 w = make_uint4(0u, 0u, 0u, 0u);
+      if (store) {
+        w = *reinterpret_cast<const uint4*>(data + off);
+        const float sc = from == dpage ? s_dst : fscale[fp8_scale_idx(g, layer, from, kv, h)];
+        if (sc != s_new) {
+          uint8_t* c = reinterpret_cast<uint8_t*>(&w);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(sckv_fp8_to_float(c[e]) * sc));
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float s_new = fmaxf(s_dst, top / 448.0f);
-      // pass 2: rows in order, 32 / cpr of them at a time (loads before stores)
-      for (int i0 = 0; i0 < SCKV_PAGE_TOKENS * cpr; i0 += 32) {
-        const int i = i0 + lane;
-        int32_t from = dpage;
-        int64_t off = i < SCKV_PAGE_TOKENS * cpr ? source(i / cpr, &from) : -1;
-        bool store = off >= 0;
-        off += (i % cpr) * 16;
-        if (!store && i < SCKV_PAGE_TOKENS * cpr && first + i / cpr < j0 && s_new > s_dst) {
-          off = dst0 + (int64_t)i * 16;  // a row that stays: re-encoded under the grown scale
-          from = dpage;
-          store = true;
+          for (int e = 0; e < 16; ++e)
+            c[e] = s_new > 0.f ? sckv_float_to_fp8(sckv_fp8_to_float(c[e]) * sc / s_new) : (uint8_t)0;
         }
-        uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        if (store) {
-          w = *reinterpret_cast<const uint4*>(data + off);
-          const float sc = from == dpage ? s_dst : fscale[fp8_scale_idx(g, layer, from, kv, h)];
-          if (sc != s_new) {
-            uint8_t* c = reinterpret_cast<uint8_t*>(&w);
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              c[e] = s_new > 0.f ? sckv_float_to_fp8(sckv_fp8_to_float(c[e]) * sc / s_new) : (uint8_t)0;
-          }
-        }
-        __syncwarp();
-        if (store) *reinterpret_cast<uint4*>(data + dst0 + (int64_t)i * 16) = w;
       }
       __syncwarp();
-      if (lane == 0 && s_new > s_dst) fscale[fp8_scale_idx(g, layer, dpage, kv, h)] = s_new;
+      if (store) *reinterpret_cast<uint4*>(data + dst0 + (int64_t)i * 16) = w;
     }
+    __syncwarp();
+    if (lane == 0 && s_new > s_dst) fscale[fp8_scale_idx(g, layer, dpage, kv, h)] = s_new;
     __syncwarp();
   }
 }
@@ -409,9 +540,13 @@ __global__ void __launch_bounds__(kCompactWarps * 32) compact_kernel(const Compa
 // index of equal values; NaN counts as the largest, as torch.argmax has it),
 // then from node 0 on the child whose token is t of its parent, the first of
 // equals, until there is none. Bound by HBM (the logits, read once): rows are
-// cut into `chunks` so that few rows still fill the GPU, every CTA leaves its
-// chunk's best as one 64-bit word (ordered value, then the complement of the
-// index), and one warp per sequence joins them and walks.
+// cut into `chunks` of 16-byte pieces (a row's first and last elements that
+// fill none go to its first and last chunk) so that few rows still fill the
+// GPU. A thread keeps the largest value of its pieces and the first piece that
+// holds it, eight 16-bit values by four packed maxima and one comparison, and
+// looks its index up at the end. Every CTA leaves its chunk's best as one
+// 64-bit word (ordered value, then the complement of the index), and one warp
+// per sequence joins them and walks.
 // ---------------------------------------------------------------------------
 constexpr int kVerifyThreads = 256;
 constexpr int kVerifyMaxNodes = 1024;
@@ -431,29 +566,92 @@ __device__ __forceinline__ float logit_at(const void* base, int64_t i) {
   return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(base)[i]);
 }
 
+__device__ __forceinline__ uint4 ld_once(const uint4* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+
+// Largest value of a piece, NaN if there is one.
+template <int DT>
+__device__ __forceinline__ float piece_max(const uint4& w) {
+  if constexpr (DT == SCKV_DTYPE_F32) {
+    float m, a = __uint_as_float(w.x), b = __uint_as_float(w.y), c = __uint_as_float(w.z), d = __uint_as_float(w.w);
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(a), "f"(b));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(c), "f"(d));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(c));
+    return m;
+  } else if constexpr (DT == SCKV_DTYPE_F16) {
+    const __half2* x = reinterpret_cast<const __half2*>(&w);
+    const __half2 m = __hmax2_nan(__hmax2_nan(x[0], x[1]), __hmax2_nan(x[2], x[3]));
+    return __half2float(__hmax_nan(__low2half(m), __high2half(m)));
+  } else {
+    const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&w);
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(x[0], x[1]), __hmax2_nan(x[2], x[3]));
+    return __bfloat162float(__hmax_nan(__low2bfloat16(m), __high2bfloat16(m)));
+  }
+}
+
 template <int DT>
 __global__ void __launch_bounds__(kVerifyThreads) verify_argmax_kernel(const void* logits, int64_t ld, int vocab,
                                                                        int chunks, unsigned long long* best) {
+  constexpr int kEl = DT == SCKV_DTYPE_F32 ? 4 : 2, kPer = 16 / kEl;
   const int row = blockIdx.x / chunks, c = blockIdx.x - row * chunks;
-  const int64_t per = ((int64_t)vocab + chunks - 1) / chunks;
-  const int lo = (int)min((int64_t)vocab, c * per), hi = (int)min((int64_t)vocab, (c + 1) * per);
   const int64_t base = row * ld;
+  const uint8_t* at = reinterpret_cast<const uint8_t*>(logits) + base * kEl;
+  const int head = min(vocab, (int)((16 - (reinterpret_cast<uintptr_t>(at) & 15)) & 15) / kEl);
+  const int pieces = (vocab - head) / kPer, tail0 = head + pieces * kPer;
+  const uint4* x = reinterpret_cast<const uint4*>(at + head * kEl);
+  const int per = (pieces + chunks - 1) / chunks;
+  const int lo = min(pieces, c * per), hi = min(pieces, lo + per);
   unsigned long long w = 0;
-  for (int i = lo + threadIdx.x; i < hi; i += kVerifyThreads) {
-    const unsigned long long x = rank_word(logit_at<DT>(logits, base + i), (uint32_t)i);
-    w = x > w ? x : w;
+  auto single = [&](int i) {
+    const unsigned long long y = rank_word(logit_at<DT>(logits, base + i), (uint32_t)i);
+    w = y > w ? y : w;
+  };
+  if (c == 0 && (int)threadIdx.x < head) single(threadIdx.x);
+  if (c == chunks - 1 && tail0 + (int)threadIdx.x < vocab) single(tail0 + threadIdx.x);
+  int i = lo + threadIdx.x;
+  if (i < hi) {
+    float top = piece_max<DT>(ld_once(x + i));
+    int where = i;
+    auto take = [&](float m, int idx) {  // (nothing passes a NaN)
+      if (!(m <= top) && top == top) {
+        top = m;
+        where = idx;
+      }
+    };
+    for (i += kVerifyThreads; i + 3 * kVerifyThreads < hi; i += 4 * kVerifyThreads) {
+      uint4 v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = ld_once(x + i + e * kVerifyThreads);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) take(piece_max<DT>(v[e]), i + e * kVerifyThreads);
+    }
+    for (; i < hi; i += kVerifyThreads) take(piece_max<DT>(ld_once(x + i)), i);
+    for (int e = 0; e < kPer; ++e) {
+      const int idx = head + where * kPer + e;
+      const float y = logit_at<DT>(logits, base + idx);
+      if (y == top || (top != top && y != y)) {
+        const unsigned long long z = rank_word(y, (uint32_t)idx);
+        w = z > w ? z : w;
+        break;
+      }
+    }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long x = __shfl_xor_sync(0xffffffffu, w, o);
-    w = x > w ? x : w;
+    const unsigned long long y = __shfl_xor_sync(0xffffffffu, w, o);
+    w = y > w ? y : w;
   }
   __shared__ unsigned long long s[kVerifyThreads / 32];
   if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = w;
   __syncthreads();
   if (threadIdx.x == 0) {
 #pragma unroll
-    for (int i = 1; i < kVerifyThreads / 32; ++i) w = s[i] > w ? s[i] : w;
+    for (int e = 1; e < kVerifyThreads / 32; ++e) w = s[e] > w ? s[e] : w;
     best[blockIdx.x] = w;
   }
 }
@@ -511,6 +709,14 @@ int verify_chunks(int num_sms, int n_tokens, int vocab) {
   int c = (8 * num_sms + n_tokens - 1) / n_tokens;
   if (c > most) c = most;
   return c < 1 ? 1 : c;
+}
+
+// Tokens of a CTA: one until every SM has 16 CTAs (8 are resident), then more,
+// whose angles and page lookups are one latency (8,192 tokens of 48 heads: 41 us
+// with 3, 44 with 1).
+int rope_tokens(int num_sms, int n_tokens) {
+  const int n = n_tokens / (16 * num_sms);
+  return n < 1 ? 1 : n > kRopeTokens ? kRopeTokens : n;
 }
 
 }  // namespace
@@ -575,7 +781,6 @@ extern "C" int sckv_append_rope_axes(sckv_pool* p, int layer, const void* q, int
   a.hq = num_q_heads;
   a.n_seqs = n_seqs;
   a.n_tokens = n_tokens;
-  a.tpb = 1;
   a.cu = cu_tokens;
   a.start_pos = start_pos;
   a.bt = block_table;
@@ -583,7 +788,14 @@ extern "C" int sckv_append_rope_axes(sckv_pool* p, int layer, const void* q, int
   a.max_blocks = max_blocks;
   SCKV_DEVICE_GUARD(p->device);
   cudaStream_t s = as_stream(stream);
-  rope_axes_kernel<<<(n_tokens + a.tpb - 1) / a.tpb, kRopeThreads, 0, s>>>(a);
+  a.tpb = rope_tokens(p->num_sms, n_tokens);
+  const int blocks = (n_tokens + a.tpb - 1) / a.tpb;
+  if (q_dtype != src_dtype || src_dtype == SCKV_DTYPE_F32)
+    rope_axes_kernel<-1><<<blocks, kRopeThreads, 0, s>>>(a);
+  else if (src_dtype == SCKV_DTYPE_F16)
+    rope_axes_kernel<SCKV_DTYPE_F16><<<blocks, kRopeThreads, 0, s>>>(a);
+  else
+    rope_axes_kernel<SCKV_DTYPE_BF16><<<blocks, kRopeThreads, 0, s>>>(a);
   SCKV_LAUNCH_CHECK();
   if (p->kv_dtype == SCKV_DTYPE_FP8_E4M3) {
     const int64_t units = (int64_t)n_seqs * 2 * p->num_kv_heads;
@@ -601,14 +813,21 @@ extern "C" int sckv_compact_tree(sckv_pool* p, int layer0, int n_layers, int n_s
   if (n_seqs == 0 || max_path == 0) return SCKV_OK;
   if (!path || !n_keep || !ctx_lens || !block_table || bt_stride < max_blocks || max_blocks <= 0)
     return SCKV_ERR_INVALID_ARG;
-  Compact c{geo_of(p), layer0, n_layers, n_seqs, max_path, path, n_keep, ctx_lens, block_table, bt_stride, max_blocks};
-  const int64_t blocks = ((int64_t)n_seqs * n_layers * 2 * p->num_kv_heads + kCompactWarps - 1) / kCompactWarps;
+  // slices of a warp: as many as leave every SM 32 warps, at most 8 (its pieces are counted in 16 bits)
+  const int64_t n_slices = (int64_t)n_layers * 2 * p->num_kv_heads;
+  const bool fp8 = p->kv_dtype == SCKV_DTYPE_FP8_E4M3;
+  const int64_t share = n_seqs * n_slices / (32 * p->num_sms);
+  const int per_warp = fp8 || share < 1 ? 1 : share > 8 ? 8 : (int)share;
+  Compact c{geo_of(p), layer0, n_layers, n_seqs, max_path, path, n_keep, ctx_lens, block_table, bt_stride, max_blocks,
+            per_warp};
+  const int64_t blocks = fp8 ? (n_seqs * n_slices + kCompactWarps - 1) / kCompactWarps
+                             : n_seqs * ((n_slices + kCompactWarps * per_warp - 1) / (kCompactWarps * per_warp));
   if (blocks > INT32_MAX) return SCKV_ERR_INVALID_ARG;
   SCKV_DEVICE_GUARD(p->device);
-  if (p->kv_dtype == SCKV_DTYPE_FP8_E4M3)
-    compact_kernel<true><<<(unsigned)blocks, kCompactWarps * 32, 0, as_stream(stream)>>>(c);
+  if (fp8)
+    compact_fp8_kernel<<<(unsigned)blocks, kCompactWarps * 32, 0, as_stream(stream)>>>(c);
   else
-    compact_kernel<false><<<(unsigned)blocks, kCompactWarps * 32, 0, as_stream(stream)>>>(c);
+    compact_kernel<<<(unsigned)blocks, kCompactWarps * 32, 0, as_stream(stream)>>>(c);
   SCKV_LAUNCH_CHECK();
   return SCKV_OK;
 }

@@ -115,6 +115,9 @@ def _dev_i32(x, device) -> torch.Tensor:
     return to_device(x, torch.int32, device)
 
 
+_NOTHING = nullcontext()  # (on a stream argument, the call's temporaries belong to that stream)
+
+
 class KVPool:
     """One page pool on one GPU."""
 
@@ -591,19 +594,16 @@ class KVPool:
         return out
 
     # ------------------------------------------------- speculative decoding
-    def _stream_scope(self, stream: Optional[torch.cuda.Stream]):
-        """Temporaries of a call on `stream` belong to that stream."""
-        return nullcontext() if stream is None else torch.cuda.stream(stream)
-
     def _here(self, stream: Optional[torch.cuda.Stream]) -> int:
-        return (stream if stream is not None else torch.cuda.current_stream(self.device)).cuda_stream
+        return torch.cuda.current_stream(self.device.index).cuda_stream if stream is None else stream.cuda_stream
 
     def _table(self, block_table: torch.Tensor, n_seqs: int, max_blocks: Optional[int]) -> Tuple[torch.Tensor, int]:
         bt = block_table if block_table.dim() == 2 else block_table.view(1, -1)
-        mb = bt.shape[1] if max_blocks is None else int(max_blocks)
+        rows, cols = bt.shape
+        ld, unit = bt.stride()
+        mb = cols if max_blocks is None else int(max_blocks)
         _need(bt, "block_table", self.device, torch.int32, contiguous=False)
-        if bt.shape[0] < n_seqs or mb > bt.shape[1] or (mb > 1 and bt.stride(1) != 1) or \
-                (n_seqs > 1 and bt.stride(0) < mb):
+        if rows < n_seqs or mb > cols or (mb > 1 and unit != 1) or (n_seqs > 1 and ld < mb):
             raise ValueError("block_table must be [>= n_seqs, >= max_blocks] rows with unit column stride")
         return bt, mb
 
@@ -636,11 +636,11 @@ class KVPool:
         scale = float(d) ** -0.5 if scale is None else float(scale)
         if not 0.0 < scale < float("inf"):
             raise ValueError("scale must be positive")
-        with self._stream_scope(stream):
+        with _NOTHING if stream is None else torch.cuda.stream(stream):
             q = q.contiguous()
             _need(q, "q", self.device)
             if out is None:
-                out = torch.empty((n_tok, hq, d), dtype=out_dtype or q.dtype, device=self.device)
+                out = torch.empty(n_tok, hq, d, dtype=out_dtype or q.dtype, device=self.device)
             else:
                 _need(out, "out", self.device)
                 if tuple(out.shape) != (n_tok, hq, d):
@@ -662,15 +662,17 @@ class KVPool:
         return int(self.lib.sckv_tree_attn_workspace_bytes(self.handle, n_tokens, num_q_heads))
 
     @staticmethod
-    def _head_rows(t: torch.Tensor) -> torch.Tensor:
-        """[T, H, D] with packed heads and 16-byte aligned tokens: t itself (a
-        slice of a wider projection, say), or a contiguous copy."""
-        T, H, D = t.shape
-        packed = t.stride(2) == 1 and (H == 1 or t.stride(1) == D)
-        el = t.element_size()
-        if packed and (T <= 1 or (t.stride(0) >= H * D and t.stride(0) * el % 16 == 0)) and t.data_ptr() % 16 == 0:
-            return t
-        return t.contiguous()
+    def _head_rows(t: torch.Tensor, T: int, H: int, D: int) -> Tuple[torch.Tensor, int]:
+        """[T, H, D] with packed heads and 16-byte aligned tokens, t itself (a
+        slice of a wider projection, say) or a contiguous copy, and the
+        elements between its tokens."""
+        st, sh, sd = t.stride()
+        if sd == 1 and (H == 1 or sh == D) and t.data_ptr() % 16 == 0:
+            if T <= 1:
+                return t, H * D
+            if st >= H * D and st * t.element_size() % 16 == 0:
+                return t, st
+        return t.contiguous(), H * D
 
     def append_rope_axes(self, layer: int, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
                          positions: torch.Tensor, axis_map: torch.Tensor, cu_tokens: torch.Tensor,
@@ -687,55 +689,63 @@ class KVPool:
         k_new / v_new [n_tokens, Hkv, D] may be slices of one projection
         (heads packed); per-head norms (fp16 weights of D elements) only.
         Returns the rotated q. Every pool type."""
-        if q.dim() != 3 or k_new.dim() != 3 or v_new.dim() != 3:
+        dev, kv_shape = self.device, k_new.shape
+        if q.dim() != 3 or len(kv_shape) != 3 or v_new.dim() != 3:
             raise ValueError("q, k_new and v_new must be [n_tokens, heads, D]")
         nt, hq, d = q.shape
+        hkv = self.num_kv_heads
         n_seqs = cu_tokens.numel() - 1
-        if d != self.head_dim or tuple(k_new.shape) != (nt, self.num_kv_heads, d) or k_new.shape != v_new.shape:
+        if d != self.head_dim or kv_shape != (nt, hkv, d) or kv_shape != v_new.shape:
             raise ValueError("q must be [n_tokens, Hq, D] and k_new / v_new [n_tokens, Hkv, D]")
         if k_new.dtype != v_new.dtype:
             raise TypeError("k_new and v_new must have the same dtype")
         if not 0 <= layer < self.num_layers:
             raise ValueError("layer out of range")
         pos = positions if positions.dim() == 2 else positions.view(1, -1)
-        _need(pos, "positions", self.device, torch.int32, contiguous=False)
-        if pos.shape[1] != nt or pos.shape[0] < 1:
+        _need(pos, "positions", dev, torch.int32, contiguous=False)
+        axes, n_pos = pos.shape
+        if n_pos != nt or axes < 1:
             raise ValueError("positions must be [axes, n_tokens]")
-        _need(axis_map, "axis_map", self.device, torch.int32)
+        _need(axis_map, "axis_map", dev, torch.int32)
         if axis_map.numel() != d // 2:
             raise ValueError("axis_map must have D / 2 entries")
-        _need(inv_freq, "inv_freq", self.device, torch.float32, d // 2)
-        _need(cu_tokens, "cu_tokens", self.device, torch.int32, 1)
-        _need(start_pos, "start_pos", self.device, torch.int32, n_seqs)
+        _need(inv_freq, "inv_freq", dev, torch.float32, d // 2)
+        _need(cu_tokens, "cu_tokens", dev, torch.int32, 1)
+        _need(start_pos, "start_pos", dev, torch.int32, n_seqs)
         bt, mb = self._table(block_table, n_seqs, max_blocks)
         for name, w in (("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w)):
             if w is not None:
-                _need(w, name, self.device, torch.float16)
+                _need(w, name, dev, torch.float16)
                 if w.numel() != d:
                     raise ValueError(f"{name} must have D elements (a norm of each head)")
-        for name, t in (("q", q), ("k_new", k_new), ("v_new", v_new)):
-            _need(t, name, self.device, contiguous=False)
-        with self._stream_scope(stream):
-            q, k_new, v_new = self._head_rows(q), self._head_rows(k_new), self._head_rows(v_new)
-            if pos.stride(1) != 1 and nt > 1:
+        _need(q, "q", dev, contiguous=False)
+        _need(k_new, "k_new", dev, contiguous=False)
+        _need(v_new, "v_new", dev, contiguous=False)
+        with _NOTHING if stream is None else torch.cuda.stream(stream):
+            q, q_ld = self._head_rows(q, nt, hq, d)
+            k_new, k_ld = self._head_rows(k_new, nt, hkv, d)
+            v_new, v_ld = self._head_rows(v_new, nt, hkv, d)
+            pos_ld, pos_unit = pos.stride()
+            if pos_unit != 1 and nt > 1:
                 pos = pos.contiguous()
+                pos_ld = nt
             if q_out is None:
-                q_out = torch.empty((nt, hq, d), dtype=q_out_dtype or q.dtype, device=self.device)
+                q_out = torch.empty(nt, hq, d, dtype=q_out_dtype or q.dtype, device=dev)
             else:
-                _need(q_out, "q_out", self.device)
-                if tuple(q_out.shape) != (nt, hq, d):
+                _need(q_out, "q_out", dev)
+                if q_out.shape != (nt, hq, d):
                     raise ValueError("q_out must have q's shape")
-            need = int(self.lib.sckv_append_rope_axes_workspace_bytes(self.handle, nt))
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-            stride = lambda t: max(t.stride(0), t.shape[1] * d) if nt > 1 else t.shape[1] * d  # noqa: E731
+            need, ws = 0, None
+            if self.kv_dtype == "fp8_e4m3":
+                need = int(self.lib.sckv_append_rope_axes_workspace_bytes(self.handle, nt))
+                ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
             N.check(self.lib.sckv_append_rope_axes(
-                self.handle, layer, q.data_ptr(), stride(q), q_out.data_ptr(), hq, torch_dtype_code(q.dtype),
-                torch_dtype_code(q_out.dtype), k_new.data_ptr(), stride(k_new), v_new.data_ptr(), stride(v_new),
+                self.handle, layer, q.data_ptr(), q_ld, q_out.data_ptr(), hq, torch_dtype_code(q.dtype),
+                torch_dtype_code(q_out.dtype), k_new.data_ptr(), k_ld, v_new.data_ptr(), v_ld,
                 torch_dtype_code(k_new.dtype), _ptr(q_norm_w), _ptr(k_norm_w), float(eps), inv_freq.data_ptr(),
-                float(rope_scaling), pos.data_ptr(), pos.stride(0) if pos.shape[0] > 1 else nt, pos.shape[0],
-                axis_map.data_ptr(), n_seqs, nt, cu_tokens.data_ptr(), start_pos.data_ptr(), bt.data_ptr(),
-                bt.stride(0), mb, _ptr(ws), need, self._here(stream)),
-                "sckv_append_rope_axes")
+                float(rope_scaling), pos.data_ptr(), pos_ld if axes > 1 else nt, axes, axis_map.data_ptr(), n_seqs, nt,
+                cu_tokens.data_ptr(), start_pos.data_ptr(), bt.data_ptr(), bt.stride(0), mb, _ptr(ws), need,
+                self._here(stream)), "sckv_append_rope_axes")
         return q_out
 
     def compact_tree(self, block_table: torch.Tensor, ctx_lens: torch.Tensor, path: torch.Tensor,
@@ -781,12 +791,12 @@ class KVPool:
         _need(tokens, "tokens", self.device, torch.int32, nt)
         _need(parents, "parents", self.device, torch.int32, nt)
         _need(cu_tokens, "cu_tokens", self.device, torch.int32, 1)
-        with self._stream_scope(stream):
+        with _NOTHING if stream is None else torch.cuda.stream(stream):
             if (vocab > 1 and logits.stride(1) != 1) or (nt > 1 and logits.stride(0) < vocab):
                 logits = logits.contiguous()
-            out = torch.empty(n_seqs * (mp + 2), dtype=torch.int32, device=self.device)
-            path, keep, nxt = out[:n_seqs * mp].view(n_seqs, mp), out[n_seqs * mp:n_seqs * (mp + 1)], \
-                out[n_seqs * (mp + 1):]
+            path = torch.empty(n_seqs, mp, dtype=torch.int32, device=self.device)
+            keep = torch.empty(n_seqs, dtype=torch.int32, device=self.device)
+            nxt = torch.empty(n_seqs, dtype=torch.int32, device=self.device)
             need = int(self.lib.sckv_verify_tree_workspace_bytes(self.handle, nt, vocab))
             ws = torch.empty(max(need, 8), dtype=torch.uint8, device=self.device)
             N.check(self.lib.sckv_verify_tree(self.handle, logits.data_ptr(), torch_dtype_code(logits.dtype),

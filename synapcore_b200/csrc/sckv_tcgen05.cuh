@@ -124,6 +124,23 @@ namespace sckv_tc {
 
 using sckv_mma::pack2;
 
+// 8 values of the other 16-bit type as the MMA's, rounded once (they are exact in fp32).
+template <bool kBF16>
+__device__ __forceinline__ uint4 cvt_q8(const uint4& raw) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (kBF16) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      o[i] = pack2<true>(f.x, f.y);
+    } else {
+      o[i] = pack2<false>(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+    }
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
 // 8 query values (dims d..d+7 of one row) as packed f16 / bf16 pairs.
 template <bool kBF16>
 __device__ __forceinline__ uint4 load_q8(const void* q, int64_t idx, int dtype) {

@@ -136,7 +136,8 @@ struct TreeParams {
   const unsigned long long* mask;
   int mask_words;
   int max_blocks, n_seqs, n_tokens, hq, G;
-  int group_rows;  // rows of a row group: 256, one-byte pools 128
+  uint32_t g_mul;   // 2^32 / G + 1 (0: G is 1)
+  int group_shift;  // log2 of a row group's rows: 8, one-byte pools 7
   int q_dtype, out_dtype;
   float scale_log2;
   // workspace: JoinHead [grid], then per CTA two slots of float4 [32][part_rows] (O by 4 dims and row)
@@ -157,9 +158,13 @@ __device__ __forceinline__ bool tree_seq(const TreeParams& p, int s, int& n, int
   const bool ok = t0 >= 0 && t1 >= t0 && t1 <= p.n_tokens && n <= 64 * p.mask_words && ctx >= 0 && ctx <= cap - n;
   if (!ok) n = ctx = 0;
   kt = n > 0 ? (ctx + n + kKeys - 1) / kKeys : 0;
-  groups = (n * p.G + p.group_rows - 1) / p.group_rows;
+  groups = (n * p.G + (1 << p.group_shift) - 1) >> p.group_shift;
   return ok;
 }
+
+// Node of row rr of a sequence's group: rr / G. Exact while rr G < 2^32; rr < 256 G.
+__device__ __forceinline__ int tree_node(const TreeParams& p, int rr) { return p.g_mul ? (int)__umulhi((uint32_t)rr, p.g_mul) : rr; }
+constexpr int kMaxGroup = 4095;
 
 // A CTA's walk over its share of the line of key tiles, one item (or part of one) at a time.
 struct TreeWalk {
@@ -184,8 +189,8 @@ __device__ __forceinline__ bool tree_next(const TreeParams& p, const int* cum, T
   s.ka = rem - item * s.kt;
   s.nk = min(s.kt - s.ka, w.t1 - w.t);
   s.h = item / groups;
-  s.row0 = (item - s.h * groups) * p.group_rows;
-  s.rows = min(p.group_rows, s.n * p.G - s.row0);
+  s.row0 = (item - s.h * groups) << p.group_shift;
+  s.rows = min(1 << p.group_shift, s.n * p.G - s.row0);
   s.nq = s.rows > kRows ? 2 : 1;
   s.copies = s.rows <= kRows / 4 ? 4 : s.rows <= kRows / 2 ? 2 : 1;
   s.L = s.ctx + s.n;
@@ -199,7 +204,10 @@ __device__ __forceinline__ bool tree_next(const TreeParams& p, const int* cum, T
 __device__ __forceinline__ int tree_owner(int t, int total, int n) {
   return (int)((((int64_t)t + 1) * n - 1) / total);
 }
-__device__ __forceinline__ int tree_begin(int c, int total, int n) { return (int)((int64_t)total * c / n); }
+__device__ __forceinline__ int tree_begin(int c, int total, int n) {
+  const int q = total / n, r = total - q * n;  // (32-bit divisions; c, r <= n, the number of SMs)
+  return c * q + c * r / n;
+}
 
 // 64 bits from bit `off` of a row's view of keys ctx + i: ones for committed tokens (i < 0), the mask for nodes
 // i < n, zeros after.
@@ -364,6 +372,7 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
   const int lane = threadIdx.x & 31;
 
   pdl_trigger();
+  if (warp == kWarpMma) tmem_alloc(tmem_slot, kTmemCols);
   // ---- key tiles per sequence, prefix-summed by the whole CTA
   {
     const int per = (p.n_seqs + C::kThreads - 1) / C::kThreads;
@@ -382,32 +391,31 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
       if (lane >= o) x += y;
     }
     if (lane == 31) partial[warp] = x;
-    if (threadIdx.x == 0) {
-      for (int i = 0; i < C::kNumBars; ++i) {
-        const uint32_t bar = bar0 + 8 * i;
-        uint32_t count = 1;
-        if (C::kB8 && ((bar >= k_full && bar < k_full + 8 * kStages) || (bar >= v_full && bar < v_full + 8 * kStages))) count = 8;
-        if (bar >= p_full && bar < p_full + 16) count = 8;
-        if (bar == mma_done) count = 2;
-        if (bar == q_full || bar == o_full || bar == x_done) count = 8;
-        if (bar == x_full || bar == x_full + 8) count = 4;
-        if (C::kB8 && bar >= st_full && bar < st_full + 8 * C::kStaging) count = 2;
-        if (C::kB8 && bar >= st_empty && bar < st_empty + 8 * C::kStaging) count = 8;
-        bar_init(bar, count);
-      }
-      for (int i = 0; i < 2 * kMaskWordsMax; ++i) s_bad[i] = 0;
-      *abort_flag = 0;
+    if ((int)threadIdx.x < C::kNumBars) {
+      const uint32_t bar = bar0 + 8 * threadIdx.x;
+      uint32_t count = 1;
+      if (C::kB8 && ((bar >= k_full && bar < k_full + 8 * kStages) || (bar >= v_full && bar < v_full + 8 * kStages))) count = 8;
+      if (bar >= p_full && bar < p_full + 16) count = 8;
+      if (bar == mma_done) count = 2;
+      if (bar == q_full || bar == o_full || bar == x_done) count = 8;
+      if (bar == x_full || bar == x_full + 8) count = 4;
+      if (C::kB8 && bar >= st_full && bar < st_full + 8 * C::kStaging) count = 2;
+      if (C::kB8 && bar >= st_empty && bar < st_empty + 8 * C::kStaging) count = 8;
+      bar_init(bar, count);
       fence_mbar_init();
     }
-    if (warp == kWarpMma) tmem_alloc(tmem_slot, kTmemCols);
+    if (threadIdx.x < 2 * kMaskWordsMax) s_bad[threadIdx.x] = 0;
+    if (threadIdx.x == 0) *abort_flag = 0;
     __syncthreads();
     int before = 0;
     for (int i = 0; i < warp; ++i) before += partial[i];
     int run = before + x - local;
     for (int s = s0; s < s1; ++s) {
       cum[s] = run;
-      tree_seq(p, s, n, ctx, kt, groups);
-      run += kt * groups * p.g.H;
+      if (s + 1 < s1) {
+        tree_seq(p, s, n, ctx, kt, groups);
+        run += kt * groups * p.g.H;
+      }
     }
     if (threadIdx.x == C::kThreads - 1) cum[p.n_seqs] = before + x;
     tc_fence_before();
@@ -429,23 +437,6 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
     }
     walk.seq = lo;
   }
-  if (threadIdx.x == 0) {
-    JoinHead hd{};
-    TreeWalk w = walk;
-    TreeSeg s;
-    if (tree_next(p, cum, w, s) && s.ka > 0 && s.ka + s.nk == s.kt) {
-      const int first = walk.t - s.ka;  // the item's first tile
-      hd.c0 = tree_owner(first, total, n_cta);
-      hd.slot0 = tree_begin(hd.c0, total, n_cta) == first ? 0 : 1;
-      hd.n_parts = (int)blockIdx.x - hd.c0 + 1;
-      hd.rows = s.rows;
-      hd.row0 = s.row0;
-      hd.q_base = s.q_base;
-      hd.h = s.h;
-    }
-    p.heads[blockIdx.x] = hd;
-  }
-
   const int64_t layer_base = (int64_t)p.layer * p.g.P;
   // Registers: 128 a thread at launch (one-byte pools: 96); the softmax warpgroups take 176 (128) for a row's 64 scores
   // and their P, the others give theirs up: 256 x 80 + 256 x 176 = 512 x 128 (384 x 72 + 256 x 128 = 60,416 <= 640 x
@@ -642,6 +633,23 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
     // A whole warp walks and waits, one elected lane issues (a role on one lane alone measured 1.3 x slower).
     reg_give<C::kGiveRegs>();
     const int mw = warp == kWarpMma2 ? 1 : 0;
+    if (mw == 1 && lane == 0) {  // what the joining kernel needs; by a warp that waits long for its first P
+      JoinHead hd{};
+      TreeWalk w = walk;
+      TreeSeg s;
+      if (tree_next(p, cum, w, s) && s.ka > 0 && s.ka + s.nk == s.kt) {
+        const int first = walk.t - s.ka;  // the item's first tile
+        hd.c0 = tree_owner(first, total, n_cta);
+        hd.slot0 = tree_begin(hd.c0, total, n_cta) == first ? 0 : 1;
+        hd.n_parts = (int)blockIdx.x - hd.c0 + 1;
+        hd.rows = s.rows;
+        hd.row0 = s.row0;
+        hd.q_base = s.q_base;
+        hd.h = s.h;
+      }
+      p.heads[blockIdx.x] = hd;
+    }
+    __syncwarp();
     const uint32_t el = elect_one();
     constexpr uint32_t kIdescS = instr_desc_f16(kBF16, kKeys, false);
     constexpr uint32_t kIdescPV = instr_desc_f16(kBF16, kHD, true);
@@ -773,26 +781,44 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
     const uint32_t col_o = kColO + (uint32_t)(w * kHD);
     // Q rows of an item into shared memory (128-byte swizzled, K-major): with one
     // query tile all 256 threads load it, with two each warpgroup its own.
-    // Rows past the last keep what they have: no other row sees it.
-    auto load_q = [&](const TreeSeg& s) {
+    // Rows past the last keep what they have: no other row sees it. (The 16-bit
+    // types share one load, which nothing waits for before the last is out.)
+    int xchg = 0;  // uses of the exchange buffer
+    auto load_q = [&](const TreeSeg& s) -> bool {
       const bool two = C::kQTiles == 2 && s.nq == 2;
       const int n_it = two ? 16 : 8, step = two ? 128 : 256;
       const int t = two ? tid & 127 : tid;
       const int tile_row0 = two ? w * kRows : 0;
       uint8_t* q_tile = base + (two ? w * kQTile : 0);
-      const int64_t q0 = (int64_t)s.q_base * p.hq + (int64_t)s.h * p.G;
+      const int64_t q0 = ((int64_t)s.q_base * p.hq + (int64_t)s.h * p.G) * kHD + (t & 15) * 8;
+      bool ready = true;
 #pragma unroll 1
       for (int b8 = 0; b8 < n_it; b8 += 8) {
         uint4 v[8];
+        auto at = [&](int i) -> int64_t {  // element of piece i of this thread, -1: past the last row
+          const int r = tile_row0 + ((t + (b8 + i) * step) >> 4), rr = s.row0 + r, node = tree_node(p, rr);
+          return r < s.rows ? q0 + (int64_t)(node * (p.hq - p.G) + rr) * kHD : -1;
+        };
+        if (p.q_dtype == SCKV_DTYPE_F32) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int c = t + (b8 + i) * step;
-          const int r = tile_row0 + (c >> 4);
-          if (r < s.rows) {
-            const int rr = s.row0 + r, node = rr / p.G;
-            v[i] = load_q8<kBF16>(p.q, (q0 + (int64_t)node * p.hq + (rr - node * p.G)) * kHD + (c & 15) * 8, p.q_dtype);
+          for (int i = 0; i < 8; ++i) {
+            const int64_t o = at(i);
+            if (o >= 0) v[i] = load_q8<kBF16>(p.q, o, SCKV_DTYPE_F32);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int64_t o = at(i);
+            v[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (o >= 0) v[i] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.q) + o));
+          }
+          if (p.q_dtype != (kBF16 ? SCKV_DTYPE_BF16 : SCKV_DTYPE_F16)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = cvt_q8<kBF16>(v[i]);
           }
         }
+        // the exchange of the item before lay in the Q tile
+        if (b8 == 0 && xchg > 0) ready = warp_wait_bar(x_done, (xchg - 1) & 1);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int c = t + (b8 + i) * step;
@@ -805,14 +831,14 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) bar_arrive(q_full);
+      return ready;
     };
     bool ok = true;
     int gt = 0;           // tiles of earlier items
     int cnt[2] = {0, 0};  // uses of each set in earlier items
     TreeSeg s;
     bool more = tree_next(p, cum, walk, s);
-    if (more) load_q(s);
-    int xchg = 0;  // uses of the exchange buffer
+    if (more) ok = load_q(s);
     // One item (or part of one); false if a wait ran out. kTwo: two query tiles; kCopies: copies of the rows.
     auto run_item = [&](auto two_c, auto copies_c, const int k) -> bool {
       constexpr bool two = decltype(two_c)::value;
@@ -822,7 +848,7 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
       const int copy = row / (kRows / R);
       const int r_in = (two ? w * kRows : 0) + (row & (kRows / R - 1));  // row of the group
       const bool valid = r_in < s.rows;
-      const int node = (s.row0 + r_in) / p.G;
+      const int node = tree_node(p, s.row0 + r_in);
       const int head = s.h * p.G + (s.row0 + r_in) - node * p.G;
       const unsigned long long* mask = p.mask + (int64_t)(s.q_base + (valid ? node : 0)) * p.mask_words;
       const bool live = __any_sync(0xffffffffu, valid);
@@ -1140,28 +1166,33 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
           }
         }
       } else {
-        // the copies' rows are added up through the (now idle) Q tile, 32 dims of each warpgroup at a time:
+        // the copies' rows are added up through the (now idle) Q tiles, 32 dims of each warpgroup at a time and tile:
         // [w][row] of 128 bytes, 16-byte chunks swizzled by the row
         float* xb = reinterpret_cast<float*>(base) + w * kRows * 32;
 #pragma unroll 1
-        for (int cc = 0; cc < nd; cc += 32) {
-          {
+        for (int c0 = 0; c0 < nd; c0 += 32 * C::kQTiles) {
+          // (a second pass writes what the first has read)
+          if (c0 > 0 && !warp_wait_bar(x_done, (xchg - 1) & 1)) return false;
+#pragma unroll 1
+          for (int b = 0; b < C::kQTiles; ++b) {
+            const int cc = c0 + 32 * b;
+            float* xt = xb + b * (kQTile / 4);
             float y[32];
             merged(cc, y);
-            float4* mine = reinterpret_cast<float4*>(xb + row * 32);
+            float4* mine = reinterpret_cast<float4*>(xt + row * 32);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
               mine[j ^ (row & 7)] = valid ? make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3])
                                           : make_float4(0.f, 0.f, 0.f, 0.f);
-          }
-          if (valid && copy == 0) {
-            each_bad([&](int page, int slot) {
+            if (valid && copy == 0) {
+              each_bad([&](int page, int slot) {
 #pragma unroll 1
-              for (int d = 0; d < 32; ++d) {
-                const float v = tree_v(p.g, p.layer, page, s.h, slot, d0 + cc + d);
-                if (!isfinite(v)) xb[row * 32 + (((d >> 2) ^ (row & 7)) << 2) + (d & 3)] += v;
-              }
-            });
+                for (int d = 0; d < 32; ++d) {
+                  const float v = tree_v(p.g, p.layer, page, s.h, slot, d0 + cc + d);
+                  if (!isfinite(v)) xt[row * 32 + (((d >> 2) ^ (row & 7)) << 2) + (d & 3)] += v;
+                }
+              });
+            }
           }
           __syncwarp();
           if (lane == 0) bar_arrive(x_full + 8 * w);
@@ -1169,23 +1200,26 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
           if (valid) {
             const int sub = row & (kRows / R - 1);
 #pragma unroll
-            for (int jj = 0; jj < 8 / R; ++jj) {
-              const int j = copy * (8 / R) + jj;
-              float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int b = 0; b < C::kQTiles; ++b) {
 #pragma unroll
-              for (int e = 0; e < R; ++e) {
-                const float4 b4 = reinterpret_cast<const float4*>(xb + (sub + e * (kRows / R)) * 32)[j ^ (sub & 7)];
-                a.x += b4.x;
-                a.y += b4.y;
-                a.z += b4.z;
-                a.w += b4.w;
+              for (int jj = 0; jj < 8 / R; ++jj) {
+                const int j = copy * (8 / R) + jj;
+                float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int e = 0; e < R; ++e) {
+                  const float4 b4 = reinterpret_cast<const float4*>(xb + b * (kQTile / 4) +
+                                                                    (sub + e * (kRows / R)) * 32)[j ^ (sub & 7)];
+                  a.x += b4.x;
+                  a.y += b4.y;
+                  a.z += b4.z;
+                  a.w += b4.w;
+                }
+                put4(d0 + c0 + 32 * b + 4 * j, a.x, a.y, a.z, a.w);
               }
-              put4(d0 + cc + 4 * j, a.x, a.y, a.z, a.w);
             }
           }
           __syncwarp();
-          if (lane == 0) bar_arrive(x_done);
-          if (!warp_wait_bar(x_done, xchg & 1)) return false;
+          if (lane == 0) bar_arrive(x_done);  // (waited for before the tiles are written again)
           ++xchg;
         }
       }
@@ -1206,7 +1240,7 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
       else ok = run_item(std::false_type{}, std::integral_constant<int, 4>{}, k);
       if (!ok) break;
       more = tree_next(p, cum, walk, s);
-      if (more) load_q(s);
+      if (more) ok = load_q(s);
     }
     if (!ok) {
       if (lane == 0 && !*abort_flag) sckv_report(p.g.status, SCKV_ERR_TIMEOUT, blockIdx.x, KID_TREE_ATTN);
@@ -1224,40 +1258,53 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
   }
 }
 
-// Joins the partials of items that CTA borders cut: block (c, 32 rows) takes
-// the item that ends in CTA c's first segment, thread (row, 16 dims).
-__global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
+// Joins the partials of the items that end in CTA blockIdx.x and began earlier: 16 rows a CTA, 4 dims of a row a
+// thread. Eight parts' values are on the way while the parts' references and sums are weighed (one item may have as
+// many parts as there are SMs).
+constexpr int kJoinRows = 16, kJoinThreads = kJoinRows * kHD / 4, kJoinBatch = 8;
+
+__global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const TreeParams p) {
+  extern __shared__ float2 s_part[];  // [n_parts][kJoinRows]: m, l
   pdl_wait();
   const JoinHead hd = p.heads[blockIdx.x];
-  const int r = blockIdx.y * 32 + (threadIdx.x & 31), dg = threadIdx.x >> 5;
-  if (r >= hd.rows || hd.n_parts == 0) return;
-  auto slot = [&](int i) { return p.parts + (int64_t)(2 * (hd.c0 + i) + (i == 0 ? hd.slot0 : 0)) * slot_floats(p.part_rows); };
-  auto ml = [&](int i) { return reinterpret_cast<const float2*>(slot(i) + (int64_t)p.part_rows * kHD)[r]; };
+  const int rl = threadIdx.x % kJoinRows, dg = threadIdx.x / kJoinRows, r = blockIdx.y * kJoinRows + rl;
+  if ((int)blockIdx.y * kJoinRows >= hd.rows || hd.n_parts == 0) return;
+  auto slot = [&](int i) { return p.parts + (2 * (hd.c0 + i) + (i == 0 ? hd.slot0 : 0)) * slot_floats(p.part_rows); };
+  float4 v[kJoinBatch];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int e = 0; e < kJoinBatch; ++e)
+      if (i0 + e < hd.n_parts && r < hd.rows)
+        v[e] = reinterpret_cast<const float4*>(slot(i0 + e))[(int64_t)dg * p.part_rows + r];
+  };
+  load(0);
+  for (int i = dg; i < hd.n_parts; i += kHD / 4)
+    s_part[i * kJoinRows + rl] = r < hd.rows ? reinterpret_cast<const float2*>(slot(i) + (int64_t)p.part_rows * kHD)[r]
+                                             : make_float2(-INFINITY, 0.f);
+  __syncthreads();
+  if (r >= hd.rows) return;
   float M = -INFINITY;
-  for (int i = 0; i < hd.n_parts; ++i) M = fmaxf(M, ml(i).x);
-  float L = 0.f, x[16];
+#pragma unroll 4
+  for (int i = 0; i < hd.n_parts; ++i) M = fmaxf(M, s_part[i * kJoinRows + rl].x);
+  float L = 0.f, x0 = 0.f, x1 = 0.f, x2 = 0.f, x3 = 0.f;
+  for (int i0 = 0; i0 < hd.n_parts; i0 += kJoinBatch) {
+    if (i0 > 0) load(i0);
 #pragma unroll
-  for (int e = 0; e < 16; ++e) x[e] = 0.f;
-  for (int i = 0; i < hd.n_parts; ++i) {
-    const float2 a = ml(i);
-    const float f = a.x == -INFINITY ? 1.f : ex2_approx(a.x - M);
-    L = fmaf(a.y, f, L);
-    const float4* o = reinterpret_cast<const float4*>(slot(i));
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const float4 v = o[(int64_t)(4 * dg + c) * p.part_rows + r];
-      x[4 * c] = fmaf(v.x, f, x[4 * c]);
-      x[4 * c + 1] = fmaf(v.y, f, x[4 * c + 1]);
-      x[4 * c + 2] = fmaf(v.z, f, x[4 * c + 2]);
-      x[4 * c + 3] = fmaf(v.w, f, x[4 * c + 3]);
+    for (int e = 0; e < kJoinBatch; ++e) {
+      if (i0 + e >= hd.n_parts) break;
+      const float2 a = s_part[(i0 + e) * kJoinRows + rl];
+      const float f = a.x == -INFINITY ? 1.f : ex2_approx(a.x - M);
+      L = fmaf(a.y, f, L);
+      x0 = fmaf(v[e].x, f, x0);
+      x1 = fmaf(v[e].y, f, x1);
+      x2 = fmaf(v[e].z, f, x2);
+      x3 = fmaf(v[e].w, f, x3);
     }
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  const int rr = hd.row0 + r, node = rr / p.G;
-  const int64_t o = ((int64_t)(hd.q_base + node) * p.hq + hd.h * p.G + (rr - node * p.G)) * kHD + 16 * dg;
-#pragma unroll
-  for (int c = 0; c < 16; c += 4)
-    tree_store4(p.out, o + c, p.out_dtype, x[c] * inv, x[c + 1] * inv, x[c + 2] * inv, x[c + 3] * inv);
+  const float inv = L == 0.f ? 0.f : 1.f / L;  // no key seen: zeros; NaN stays NaN
+  const int rr = hd.row0 + r, node = tree_node(p, rr);
+  const int64_t o = ((int64_t)(hd.q_base + node) * p.hq + hd.h * p.G + (rr - node * p.G)) * kHD + 4 * dg;
+  tree_store4(p.out, o, p.out_dtype, x0 * inv, x1 * inv, x2 * inv, x3 * inv);
 }
 
 // Rank-5 view of a 16-bit pool whose boxes are whole page-heads in 8-row
@@ -1306,7 +1353,8 @@ int launch_tree(sckv_pool* p, const TreeParams& t, cudaStream_t stream) {
   SCKV_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   kern<<<p->num_sms, C::kThreads, smem, stream>>>(t, *map);
   SCKV_LAUNCH_CHECK();
-  SCKV_CUDA_CHECK(sckv_launch_pdl(tree_join_kernel, dim3(p->num_sms, t.part_rows / 32), dim3(256), 0, stream, t));
+  SCKV_CUDA_CHECK(sckv_launch_pdl(tree_join_kernel, dim3(p->num_sms, t.part_rows / kJoinRows), dim3(kJoinThreads),
+                                  p->num_sms * kJoinRows * sizeof(float2), stream, t));
   SCKV_LAUNCH_CHECK();
   return SCKV_OK;
 }
@@ -1341,7 +1389,7 @@ extern "C" int sckv_tree_attn(sckv_pool* p, int layer, const void* q, int q_dtyp
   const int G = num_q_heads / p->num_kv_heads;
   // tile and box numbers are 32-bit
   const int64_t groups = ((int64_t)(n_tokens < 64 * mask_words ? n_tokens : 64 * mask_words) * G + kRows - 1) / kRows;
-  if (n_seqs > kMaxSeqs || max_blocks > INT32_MAX / SCKV_PAGE_TOKENS ||
+  if (n_seqs > kMaxSeqs || G > kMaxGroup || max_blocks > INT32_MAX / SCKV_PAGE_TOKENS ||
       (int64_t)n_seqs * (max_blocks / kTilePages + 1) * groups * p->num_kv_heads > INT32_MAX ||
       (int64_t)p->num_layers * p->max_pages * 2 * p->num_kv_heads > INT32_MAX)
     return SCKV_ERR_UNSUPPORTED;
@@ -1361,12 +1409,14 @@ extern "C" int sckv_tree_attn(sckv_pool* p, int layer, const void* q, int q_dtyp
   t.n_tokens = n_tokens;
   t.hq = num_q_heads;
   t.G = G;
+  t.g_mul = G == 1 ? 0u : 0xFFFFFFFFu / (uint32_t)G + 1u;
   t.q_dtype = q_dtype;
   t.out_dtype = out_dtype;
   t.scale_log2 = scale * 1.4426950408889634f;
   t.heads = reinterpret_cast<JoinHead*>(workspace);
   t.parts = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + tree_head_bytes(p));
-  t.group_rows = tree_group_rows(p);
+  t.group_shift = tree_group_rows(p) == 2 * kRows ? 8 : 7;
+  static_assert(kRows == 1 << 7, "rows of a query tile");
   t.part_rows = tree_part_rows(p, n_tokens, mask_words, G);
   SCKV_DEVICE_GUARD(p->device);
   cudaStream_t s = as_stream(stream);

@@ -116,7 +116,7 @@ struct TreeCfg {
   static constexpr int kOffPartial = kOffTmem + 16;                         // int [warps]
   static constexpr int kOffCum = kOffPartial + kMaxWarps * 4;               // int [n_seqs + 1]
   static constexpr int kFixedSmem = 1024 + kOffCum + 4;                     // + 4 n_seqs
-  static_assert(2 * kStages + kStaging < kScaleSlots, "scale slots outlive their half tiles");
+  static_assert(2 * (2 + kStages) + 1 + kStaging < kScaleSlots, "scale slots outlive their half tiles");
 };
 
 // What the joining kernel needs of a CTA whose first item began in an earlier one and ends in it.
@@ -317,6 +317,12 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
+}
+
+// Waits for the load of x.
+__device__ __forceinline__ void after_load(uint32_t x) {
+  [[maybe_unused]] uint32_t r;
+  asm volatile("and.b32 %0, %1, 0;" : "=r"(r) : "r"(x) : "memory");
 }
 
 __device__ __forceinline__ void bar_arrive_n(uint32_t bar, uint32_t n) {
@@ -577,25 +583,39 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
       while (!aborted && tree_next(p, cum, walk, s)) {
         for (int j = 2 * s.ka; j < 2 * (s.ka + s.nk); ++j, ++g) {
           const int ss = g % C::kStaging, gt = g >> 1, st = gt & 1;
-          if (((g & 1) == 0 && gt >= 2 && (*abort_flag || !warp_wait_bar(empties + 8 * st, ((gt >> 1) - 1) & 1))) ||
-              !warp_wait_bar(st_full + 8 * ss, (g / C::kStaging) & 1)) {
+          if (*abort_flag || !warp_wait_bar(st_full + 8 * ss, (g / C::kStaging) & 1)) {
             aborted = true;
             break;
           }
-          if (j * kHalfPages + pg < s.pages) {
-            const __half* tok = reinterpret_cast<const __half*>(base + C::kOffScale + (g % kScaleSlots) * 256) + kv * 64 +
-                                pg * SCKV_PAGE_TOKENS;
+          // the codes (and int8 scales) into registers; the slot is free once every lane has them
+          uint4 w[4];
+          __half sc[2] = {__half(1.f), __half(1.f)};
+          {
             const uint8_t* src = base + C::kOffStage + ss * kHalfSlot + pg * 4096 + kv * 2048;
-            uint8_t* dst = ring + st * kSlot + (g & 1) * kHalfSlot + pg * kPageTile;
-            uint4 w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)  // row 8 (e / 2) + r8, codes of dims 64 (e % 2) + 16 (lane % 4) ..
               w[e] = *reinterpret_cast<const uint4*>(src + ((e >> 1) * 8 + r8) * 128 +
                                                      ((((e & 1) * 4 + (lane & 3)) ^ r8) << 4));
+            if (C::kINT8) {
+              const __half* tok = reinterpret_cast<const __half*>(base + C::kOffScale + (g % kScaleSlots) * 256) + kv * 64 +
+                                  pg * SCKV_PAGE_TOKENS;
+              sc[0] = tok[r8];
+              sc[1] = tok[8 + r8];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) after_load(w[e].x);
+            __syncwarp();
+            if (lane == 0) bar_arrive(st_empty + 8 * ss);
+          }
+          if ((g & 1) == 0 && gt >= 2 && (*abort_flag || !warp_wait_bar(empties + 8 * st, ((gt >> 1) - 1) & 1))) {
+            aborted = true;
+            break;
+          }
+          if (j * kHalfPages + pg < s.pages) {
+            uint8_t* dst = ring + st * kSlot + (g & 1) * kHalfSlot + pg * kPageTile;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              __half2 s2 = __half2half2(__half(1.f));
-              if (C::kINT8) s2 = __half2half2(tok[(e >> 1) * 8 + r8]);
+              const __half2 s2 = __half2half2(sc[e >> 1]);
               const uint32_t ws[4] = {w[e].x, w[e].y, w[e].z, w[e].w};
               uint32_t o[8];
 #pragma unroll
@@ -617,10 +637,7 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
             fence_proxy_async_smem();  // read by the tensor cores
           }
           __syncwarp();
-          if (lane == 0) {
-            bar_arrive(fulls + 8 * st);
-            bar_arrive(st_empty + 8 * ss);
-          }
+          if (lane == 0) bar_arrive(fulls + 8 * st);
         }
       }
       if (aborted && lane == 0) {

@@ -99,7 +99,7 @@ struct TreeCfg {
   static constexpr bool kB8 = kFP8 || kINT8;
   static constexpr bool kBF16 = KVDT == SCKV_DTYPE_BF16;
   static constexpr int kThreads = kB8 ? 640 : 512;
-  static constexpr int kSoftRegs = kB8 ? 128 : 176, kGiveRegs = kB8 ? 72 : 80;  // registers after the roles split
+  static constexpr int kSoftRegs = kB8 ? 144 : 176, kGiveRegs = kB8 ? 64 : 80;  // registers after the roles split
   static constexpr int kQTiles = kB8 ? 1 : 2;
   static constexpr int kStaging = kB8 ? 3 : 0;        // staged half tiles of codes (K and V)
   static constexpr int kOffK = kQTiles * kQTile;
@@ -444,8 +444,8 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
     walk.seq = lo;
   }
   const int64_t layer_base = (int64_t)p.layer * p.g.P;
-  // Registers: 128 a thread at launch (one-byte pools: 96); the softmax warpgroups take 176 (128) for a row's 64 scores
-  // and their P, the others give theirs up: 256 x 80 + 256 x 176 = 512 x 128 (384 x 72 + 256 x 128 = 60,416 <= 640 x
+  // Registers: 128 a thread at launch (one-byte pools: 96); the softmax warpgroups take 176 (144) for a row's 64 scores
+  // and their P, the others give theirs up: 256 x 80 + 256 x 176 = 512 x 128 (384 x 64 + 256 x 144 = 640 x
   // 96). Each role does it in its own branch, so that the compiler knows the count of every region.
   if (warp == kWarpProdA || warp == kWarpProdB) {
     // ------------------------------------------------------------ producers
@@ -871,7 +871,7 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
       const bool live = __any_sync(0xffffffffu, valid);
       unsigned long long* bad = s_bad + (k & 1) * kMaskWordsMax;
       float m = -INFINITY, l = 0.f;
-      float vref = 0.f;  // FP8: the V scale that this warp's O counts in
+      float vref = 0.f, inv_vref = 0.f;  // FP8: the V scale that this warp's O counts in
       const int32_t* bt_row = p.bt + (int64_t)s.seq * p.bt_stride;
 #pragma unroll 1
       for (int i = 0; i < s.nk; ++i) {
@@ -884,7 +884,7 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
         if (*abort_flag || !warp_wait_bar(s_full + 8 * x, use & 1)) return false;
         tc_fence_after();
         float ks[kPg], vs[kPg];
-        float alpha = 1.f, inv_vref = 0.f;
+        float alpha = 1.f;
         bool rescale = false;
 #pragma unroll
         for (int q = 0; q < kPg; ++q) ks[q] = p.scale_log2;
@@ -904,8 +904,8 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
               rescale = true;
             }
             vref = 2.f * vm;
+            inv_vref = __frcp_rn(vref);
           }
-          inv_vref = vref > 0.f ? __frcp_rn(vref) : 0.f;
         }
         const uint32_t col_s = t_row + kColS + (uint32_t)(x * kKeys);
         if (live && nh > 0) {

@@ -888,3 +888,174 @@ def test_scheduler_drafter_refusals(cuda_device):
     s.step_batch()
     with pytest.raises(ValueError):
         s.step_batch()
+
+
+# ----------------------------------------------------------- wider ranges
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hq,nodes", [(1, 1), (8, 5), (8, 64)])
+def test_tree_attn_one_item_over_all_sms(cuda_device, kind, hq, nodes):
+    """One K/V head of one sequence: a part of the sum in nearly every SM."""
+    check_attn(cuda_device, kind, hq, 1, [16000], [nodes], seed=hq + nodes)
+
+
+def test_tree_attn_limits(cuda_device):
+    dev = cuda_device
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    pool = KVPool(1, 1, D, 4, "fp16", device=dev)
+    fill_pool(pool, gen(1, dev))
+    for seqs, ok in ((2048, True), (2049, False)):
+        bt = i32([[0]] * seqs)
+        q = torch.randn(seqs, 2, D, generator=gen(2, dev), device=dev).half()
+        mask = torch.ones(seqs, 1, dtype=torch.int64, device=dev)
+        args = (0, q, i32(range(seqs + 1)), i32([i % 15 for i in range(seqs)]), bt, mask)
+        if ok:
+            out = pool.tree_attn(*args)
+            ref, absum, big = reference(values(pool), 0, q[:40], list(range(41)), [i % 15 for i in range(40)], bt,
+                                        mask[:40], D ** -0.5)
+            tol = tolerance("fp16", q.dtype, q.dtype, ref, absum, big)
+            assert ((out[:40].double() - ref).abs() <= tol).all()
+        else:
+            with pytest.raises(SCKVError):
+                pool.tree_attn(*args)
+    wide = torch.zeros(1, 4096, D, dtype=torch.float16, device=dev)
+    one = torch.ones(1, 1, dtype=torch.int64, device=dev)
+    with pytest.raises(SCKVError):
+        pool.tree_attn(0, wide, i32([0, 1]), i32([3]), i32([[0]]), one)
+    check_attn(dev, "fp16", 4095, 1, [20], [1], seed=3)
+    pool.raise_on_status()
+
+
+@pytest.mark.parametrize("src", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lens", [[2500], [4000, 1200], [7100, 1], [9000, 17, 1203]])
+def test_append_rope_axes_of_long_prompts(cuda_device, src, lens):
+    """Token counts that give a CTA one to four tokens; no sequence owns the last three."""
+    dev, g = cuda_device, gen(len(lens), cuda_device)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    hq, hkv, T = 3, 2, sum(lens) + 3
+    start = [5 + b for b in range(len(lens))]
+    bt, pages = tables([a + n for a, n in zip(start, lens)], dev, 2)
+    cu = [sum(lens[:b]) for b in range(len(lens) + 1)]
+    kind = "bf16" if src == torch.bfloat16 else "fp16"
+    pool = KVPool(1, hkv, D, pages, kind, device=dev)
+    x = torch.randn(T, hq + 2 * hkv, D, generator=g, device=dev).to(src)
+    q, k, v = x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:]
+    w = [(1 + 0.2 * torch.randn(D, generator=g, device=dev)).half() for _ in range(2)]
+    pos = torch.randint(0, 10 ** 6, (2, T), generator=g, device=dev, dtype=torch.int32)
+    axis, freq = rope_axis_map([40, 24], device=dev), rope_inv_freq(1e6, D, dev)
+    q_out = torch.full((T, hq, D), 7.0, dtype=src, device=dev)
+    pool.append_rope_axes(0, q, k, v, pos, axis, i32(cu), i32(start), bt, freq, q_norm_w=w[0], k_norm_w=w[1], eps=1e-5,
+                          q_out=q_out)
+    pool.raise_on_status()
+    n = T - 3
+    assert (q_out[n:] == 7).all()
+    t = torch.arange(n, device=dev)
+    b = torch.searchsorted(i32(cu), t.int(), right=True) - 1
+    at = i32(start).long()[b] + t - i32(cu).long()[b]
+    rows = pool.pool_view()[0][bt.long()[b, at // 16], :, :, at % 16]  # [n, 2, hkv, D]
+    # (the same roundings as in test_append_rope_axes)
+    for y, wx, got, out in ((q, w[0], q_out[:n], src), (k, w[1], rows[:, 0], TORCH[kind])):
+        ref, size = rope_reference(y[:n], wx, 1e-5, pos[:, :n], axis, freq, 1.0)
+        tol = size * 80 * 2.0 ** -24
+        assert ((got.double() - ref).abs() <= tol + HALF[out] * (ref.abs() + tol) + 1e-7).all()
+    assert torch.equal(rows[:, 1], v[:n].to(TORCH[kind]))
+
+
+@pytest.mark.parametrize("kind", ["fp16", "int8"])
+def test_compact_tree_long_paths(cuda_device, kind):
+    """More moved rows than one batch of looked-up pages, over and past pages that they came from."""
+    dev, g = cuda_device, gen(5, cuda_device)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    ctx = [5, 48]
+    paths = [list(range(10)) + list(range(11, 611)), list(range(0, 900, 2))]
+    bt, pages = tables([c + p[-1] + 1 for c, p in zip(ctx, paths)], dev, 2)
+    pool = KVPool(2, 3, D, pages, kind, device=dev)
+    fill_pool(pool, g)
+    views = [pool.pool_view()] + ([pool.scale_view()] if kind == "int8" else [])
+    want = [v.clone() for v in views]
+    for b, path in enumerate(paths):
+        src, dst = torch.tensor(path, device=dev) + ctx[b], torch.arange(len(path), device=dev) + ctx[b]
+        ids = bt[b].long()
+        for v, x in zip(views, want):
+            x[:, ids[dst // 16], :, :, dst % 16] = v[:, ids[src // 16], :, :, src % 16]
+    P = max(len(p) for p in paths)
+    pool.compact_tree(bt, i32(ctx), i32([p + [-1] * (P - len(p)) for p in paths]), i32([len(p) for p in paths]))
+    pool.raise_on_status()
+    assert all(torch.equal(v, x) for v, x in zip(views, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_verify_tree_rows_of_any_alignment(cuda_device, dtype):
+    """Rows that begin and end anywhere in 16 bytes, their largest value (the first of equals, 0 and -0 among them) or
+    NaN anywhere."""
+    dev, g = cuda_device, gen(9, cuda_device)
+    T = 64
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    pool = KVPool(1, 1, D, 1, "fp16", device=dev)
+    zero, cu = torch.zeros(T, dtype=torch.int32, device=dev), i32(range(T + 1))
+    for vocab in (1, 2, 5, 8, 13, 24, 31, 77, 2049, 4100):
+        for off in range(0, 9, 1 if vocab < 40 else 3):
+            full = torch.randint(-3, 4, (T, vocab + off + vocab % 5), generator=g, device=dev).to(dtype)
+            full[full == 3] = -0.0
+            x = full[:, off:off + vocab]
+            full[:, :off] = 100
+            full[:, off + vocab:] = 100
+            x[:16].clamp_(max=0)
+            where = torch.randint(0, vocab, (16,), generator=g, device=dev)
+            x[torch.arange(16, 32, device=dev), where] = math.nan
+            x[32:40] = -math.inf
+            path, keep, nxt = pool.verify_tree(x, zero, zero - 1, cu, max_path=1)
+            assert nxt.tolist() == walk(x, [0] * T, [-1] * T, list(range(T + 1)), 1)[2], (vocab, off)
+    pool.raise_on_status()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_captured_tree_step_equals_the_calls(cuda_device, kind):
+    """append, attend, verify and move as one captured graph, replayed on new inputs and lengths."""
+    dev = cuda_device
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    trees = [[-1, 0, 0, 1, 1, 2, 2], [-1], [-1, 0, 1, 2, 0]]
+    n = [len(t) for t in trees]
+    cu = i32([0, n[0], n[0] + n[1], sum(n)])
+    mask, depth = tree_mask(trees, dev)
+    parents = i32([p for t in trees for p in t])
+    T, hq, hkv = sum(n), 4, 2
+    src = torch.bfloat16 if kind == "bf16" else torch.float16
+    bt, pages = tables([200] * 3, dev, 4)
+    pools = [KVPool(1, hkv, D, pages, kind, device=dev) for _ in range(2)]
+    for p in pools:
+        fill_pool(p, gen(6, dev))
+    axis, freq = rope_axis_map([64], device=dev), rope_inv_freq(1e4, D, dev)
+
+    def inputs(i):
+        g = gen(20 + i, dev)
+        x = torch.randn(T, hq + 2 * hkv, D, generator=g, device=dev).to(src)
+        ctx = i32([17 + 31 * i, 1 + i, 100 - 7 * i])
+        pos = (torch.repeat_interleave(ctx, i32(n).long()) + depth).to(torch.int32)
+        logits = torch.randint(0, 2, (T, 50), generator=g, device=dev).float()
+        tokens = torch.randint(0, 3, (T,), generator=g, device=dev, dtype=torch.int32)
+        return [x, ctx, pos, logits, tokens]
+
+    def step(pool, x, ctx, pos, logits, tokens):
+        q = pool.append_rope_axes(0, x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:], pos, axis, cu, ctx, bt, freq)
+        out = pool.tree_attn(0, q, cu, ctx, bt, mask)
+        path, keep, nxt = pool.verify_tree(logits, tokens, parents, cu, max_path=8)
+        pool.compact_tree(bt, ctx, path, keep)
+        return q, out, path, keep, nxt
+
+    held = inputs(0)
+    step(pools[0], *held), step(pools[1], *held)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(pools[0], *held)
+    for i in (1, 2):
+        new = inputs(i)
+        for a, b in zip(held, new):
+            a.copy_(b)
+        graph.replay()
+        want = step(pools[1], *new)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert torch.equal(pools[0].pool_view(), pools[1].pool_view())
+    for p in pools:
+        p.raise_on_status()

@@ -1367,7 +1367,10 @@ int launch_tree(sckv_pool* p, const TreeParams& t, cudaStream_t stream) {
   auto kern = tree_attn_kernel<KVDT>;
   const int smem = C::kFixedSmem + 4 * t.n_seqs;
   static_assert(C::kFixedSmem + 4 * kMaxSeqs <= 227 * 1024, "shared memory of the largest batch");
-  SCKV_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (!p->tree_smem_ready) {  // the largest batch's, once per pool (a pool has one kernel)
+    SCKV_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kFixedSmem + 4 * kMaxSeqs));
+    p->tree_smem_ready = 1;
+  }
   kern<<<p->num_sms, C::kThreads, smem, stream>>>(t, *map);
   SCKV_LAUNCH_CHECK();
   SCKV_CUDA_CHECK(sckv_launch_pdl(tree_join_kernel, dim3(p->num_sms, t.part_rows / kJoinRows), dim3(kJoinThreads),

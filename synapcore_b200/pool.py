@@ -86,7 +86,7 @@ def _need(t: torch.Tensor, name: str, device: torch.device, dtype: Optional[torc
     """Reject tensors the kernels would read out of bounds or misinterpret."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if t.device != device:
+    if t.get_device() != device.index and t.device != device:
         raise ValueError(f"{name} is on {t.device}, the pool is on {device}")
     if dtype is not None and t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
@@ -115,6 +115,9 @@ def _dev_i32(x, device) -> torch.Tensor:
     return to_device(x, torch.int32, device)
 
 
+# The current stream's handle of a device (the Stream object around it costs 2 us a call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
 _NOTHING = nullcontext()  # (on a stream argument, the call's temporaries belong to that stream)
 
 
@@ -595,7 +598,9 @@ class KVPool:
 
     # ------------------------------------------------- speculative decoding
     def _here(self, stream: Optional[torch.cuda.Stream]) -> int:
-        return torch.cuda.current_stream(self.device.index).cuda_stream if stream is None else stream.cuda_stream
+        if stream is not None:
+            return stream.cuda_stream
+        return _raw_stream(self.device.index)
 
     def _table(self, block_table: torch.Tensor, n_seqs: int, max_blocks: Optional[int]) -> Tuple[torch.Tensor, int]:
         bt = block_table if block_table.dim() == 2 else block_table.view(1, -1)

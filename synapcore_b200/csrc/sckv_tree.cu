@@ -327,6 +327,7 @@ __global__ void rope_axes_fp8_kernel(const RopeAxes p) {
 // ---------------------------------------------------------------------------
 constexpr int kCompactWarps = 4;
 constexpr int kMoves = 256;    // moved rows whose pages are known at a time
+constexpr int kMaxSlices = 8;  // slices of a warp
 constexpr int kMoveBatch = 4;  // 16-byte pieces that a lane holds
 
 struct Compact {
@@ -351,7 +352,8 @@ __global__ void __launch_bounds__(kCompactWarps * 32) compact_kernel(const Compa
   const int b = blockIdx.x / groups, grp = blockIdx.x - b * groups;
   const bool reporter = grp == 0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  __shared__ int64_t s_src[kMoves], s_dst[kMoves];  // page * 16 + slot; -1: not moved
+  // rows of the pool: of a moved token in slice (layer 0, K, head 0), -1: not moved; and what a slice adds to them
+  __shared__ int64_t s_src[kMoves], s_dst[kMoves], s_slice[kCompactWarps][kMaxSlices];
   const int keep = __ldg(p.n_keep + b), ctx = __ldg(p.ctx + b);
   const int32_t* path = p.path + (int64_t)b * p.max_path;
   const int cap = p.max_blocks * SCKV_PAGE_TOKENS;
@@ -380,6 +382,12 @@ __global__ void __launch_bounds__(kCompactWarps * 32) compact_kernel(const Compa
   uint8_t* data = reinterpret_cast<uint8_t*>(g.data);
   __half* hscale = reinterpret_cast<__half*>(g.scales);
   const int sl0 = (grp * kCompactWarps + warp) * p.per_warp, n_mine = max(0, min(p.per_warp, n_slices - sl0));
+  if (lane < n_mine) {
+    const int sl = sl0 + lane, h = sl % g.H, lk = sl / g.H;
+    s_slice[warp][lane] = row_off(g, p.layer0 + (lk >> 1), 0, lk & 1, h, 0) / g.D;
+  }
+  const int64_t page_rows = (int64_t)2 * g.H * SCKV_PAGE_TOKENS;
+  const uint32_t row_bytes = (uint32_t)(g.D * eb);
   for (int jb = j0; jb < keep; jb += kMoves) {
     const int nm = min(kMoves, keep - jb);
     for (int i = threadIdx.x; i < nm; i += kCompactWarps * 32) {
@@ -387,8 +395,8 @@ __global__ void __launch_bounds__(kCompactWarps * 32) compact_kernel(const Compa
       const int ps = __ldg(bt + from / SCKV_PAGE_TOKENS), pd = __ldg(bt + to / SCKV_PAGE_TOKENS);
       const bool ok = ps >= 0 && ps < g.P && pd >= 0 && pd < g.P;
       if (!ok && reporter) sckv_report(g.status, SCKV_ERR_BOUNDS, pd >= 0 && pd < g.P ? ps : pd, KID_COMPACT);
-      s_src[i] = ok ? (int64_t)ps * SCKV_PAGE_TOKENS + from % SCKV_PAGE_TOKENS : -1;
-      s_dst[i] = ok ? (int64_t)pd * SCKV_PAGE_TOKENS + to % SCKV_PAGE_TOKENS : -1;
+      s_src[i] = ok ? ps * page_rows + from % SCKV_PAGE_TOKENS : -1;
+      s_dst[i] = ok ? pd * page_rows + to % SCKV_PAGE_TOKENS : -1;
     }
     __syncthreads();
     const uint32_t per = (uint32_t)nm * cpr, nm_mul = (uint32_t)(0x100000000ull / nm) + 1u, n = (uint32_t)n_mine * per;
@@ -396,31 +404,27 @@ __global__ void __launch_bounds__(kCompactWarps * 32) compact_kernel(const Compa
       uint4 r[kMoveBatch];
       __half sc[kMoveBatch];
       int64_t dst[kMoveBatch];
+      uint32_t piece[kMoveBatch];
 #pragma unroll
       for (int k = 0; k < kMoveBatch; ++k) {
         const uint32_t i = i0 + 32 * k + lane;
         dst[k] = -1;
         if (i >= n) continue;
-        const uint32_t row = div_by(i, cpr_mul, cpr), ch = i - row * cpr;
+        const uint32_t row = div_by(i, cpr_mul, cpr);
         const uint32_t sl = div_by(row, nm_mul, nm), j = row - sl * nm;
-        const int64_t ps = s_src[j], pd = s_dst[j];
-        if (ps < 0) continue;
-        const int s_abs = sl0 + (int)sl, h = s_abs % g.H, lk = s_abs / g.H;
-        const int layer = p.layer0 + (lk >> 1), kv = lk & 1;
-        const int64_t so = row_off(g, layer, ps / SCKV_PAGE_TOKENS, kv, h, (int)(ps % SCKV_PAGE_TOKENS));
-        const int64_t po = row_off(g, layer, pd / SCKV_PAGE_TOKENS, kv, h, (int)(pd % SCKV_PAGE_TOKENS));
-        r[k] = *reinterpret_cast<const uint4*>(data + so * eb + ch * 16);
-        dst[k] = po * eb + ch * 16;
-        if (g.dtype == SCKV_DTYPE_INT8 && ch == 0)
-          sc[k] = hscale[int8_scale_idx(g, layer, ps / SCKV_PAGE_TOKENS, kv, h, (int)(ps % SCKV_PAGE_TOKENS))];
+        const int64_t from = s_src[j], add = s_slice[warp][sl];
+        if (from < 0) continue;
+        piece[k] = i - row * cpr;
+        dst[k] = s_dst[j] + add;
+        r[k] = *reinterpret_cast<const uint4*>(data + (from + add) * row_bytes + piece[k] * 16);
+        if (g.dtype == SCKV_DTYPE_INT8 && piece[k] == 0) sc[k] = hscale[from + add];  // (one a row)
       }
       __syncwarp();
 #pragma unroll
       for (int k = 0; k < kMoveBatch; ++k) {
         if (dst[k] < 0) continue;
-        *reinterpret_cast<uint4*>(data + dst[k]) = r[k];
-        // (int8: a row has D bytes, its scale one entry)
-        if (g.dtype == SCKV_DTYPE_INT8 && dst[k] % g.D == 0) hscale[dst[k] / g.D] = sc[k];
+        *reinterpret_cast<uint4*>(data + dst[k] * row_bytes + piece[k] * 16) = r[k];
+        if (g.dtype == SCKV_DTYPE_INT8 && piece[k] == 0) hscale[dst[k]] = sc[k];
       }
       __syncwarp();
     }
@@ -817,7 +821,7 @@ extern "C" int sckv_compact_tree(sckv_pool* p, int layer0, int n_layers, int n_s
   const int64_t n_slices = (int64_t)n_layers * 2 * p->num_kv_heads;
   const bool fp8 = p->kv_dtype == SCKV_DTYPE_FP8_E4M3;
   const int64_t share = n_seqs * n_slices / (32 * p->num_sms);
-  const int per_warp = fp8 || share < 1 ? 1 : share > 8 ? 8 : (int)share;
+  const int per_warp = fp8 || share < 1 ? 1 : share > kMaxSlices ? kMaxSlices : (int)share;
   Compact c{geo_of(p), layer0, n_layers, n_seqs, max_path, path, n_keep, ctx_lens, block_table, bt_stride, max_blocks,
             per_warp};
   const int64_t blocks = fp8 ? (n_seqs * n_slices + kCompactWarps - 1) / kCompactWarps

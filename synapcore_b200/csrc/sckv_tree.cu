@@ -3,6 +3,7 @@
 // rows next to the committed ones, and the choice of the accepted path from
 // the logits.
 #include <math.h>
+#include <type_traits>
 
 #include "sckv_geo.cuh"
 #include "sckv_tcgen05.cuh"
@@ -553,8 +554,8 @@ __global__ void __launch_bounds__(kCompactWarps * 32) compact_fp8_kernel(const C
 // GPU. A thread keeps the largest value of its pieces and the first piece that
 // holds it, eight 16-bit values by four packed maxima and one comparison, and
 // looks its index up at the end. Every CTA leaves its chunk's best as one
-// 64-bit word (ordered value, then the complement of the index), and one warp
-// per sequence joins them and walks. 1,152 rows of 151,936 bf16 logits: 54.6
+// 64-bit word (ordered value, then the complement of the index), and one CTA
+// per sequence joins them and walks. 1,152 rows of 151,936 bf16 logits: 54.5
 // us with the walk, 6.4 TB/s (98 % of a copy's rate); twice the chunks 62 us,
 // CTAs of 512 threads 72; single elements instead of pieces 127.
 // ---------------------------------------------------------------------------
@@ -607,9 +608,9 @@ __device__ __forceinline__ float piece_max(const uint4& w) {
 template <int DT>
 __global__ void __launch_bounds__(kVerifyThreads) verify_argmax_kernel(const void* logits, int64_t ld, int vocab,
                                                                        int chunks, unsigned long long* best) {
-  constexpr int kEl = DT == SCKV_DTYPE_F32 ? 4 : 2, kPer = 16 / kEl;
   const int row = blockIdx.x / chunks, c = blockIdx.x - row * chunks;
   const int64_t base = row * ld;
+  constexpr int kEl = DT == SCKV_DTYPE_F32 ? 4 : 2, kPer = 16 / kEl;
   const uint8_t* at = reinterpret_cast<const uint8_t*>(logits) + base * kEl;
   const int head = min(vocab, (int)((16 - (reinterpret_cast<uintptr_t>(at) & 15)) & 15) / kEl);
   const int pieces = (vocab - head) / kPer, tail0 = head + pieces * kPer;
@@ -666,36 +667,48 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_argmax_kernel(const voi
   }
 }
 
-__global__ void verify_walk_kernel(const unsigned long long* best, int chunks, const int32_t* tokens,
-                                   const int32_t* parents, const int32_t* cu, int n_tokens, int max_path,
-                                   int32_t* path, int32_t* n_keep, int32_t* next, int32_t* status) {
-  __shared__ int32_t s_best[kVerifyMaxNodes];
-  const int b = blockIdx.x, lane = threadIdx.x;
-  const int t0 = __ldg(cu + b), n = __ldg(cu + b + 1) - t0;
-  int32_t* out = path + (int64_t)b * max_path;
-  const bool ok = t0 >= 0 && n >= 0 && n <= kVerifyMaxNodes && t0 + n <= n_tokens;
-  if (!ok && lane == 0) sckv_report(status, SCKV_ERR_BOUNDS, b, KID_VERIFY);
+struct Verify {
+  int chunks, n_tokens, max_path;
+  unsigned long long* best;  // [n_tokens][chunks], written by the launch before
+  const int32_t* tokens;
+  const int32_t* parents;
+  const int32_t* cu;
+  int32_t* path;
+  int32_t* n_keep;
+  int32_t* next;
+  int32_t* status;
+};
+
+// One CTA per sequence joins the chunks' words of its rows, its first warp walks.
+__global__ void __launch_bounds__(kVerifyThreads) verify_walk_kernel(const Verify p) {
+  __shared__ unsigned long long s_best[kVerifyMaxNodes];
+  const int b = blockIdx.x, t0 = __ldg(p.cu + b);
+  int n = __ldg(p.cu + b + 1) - t0;
+  const bool ok = t0 >= 0 && n >= 0 && n <= kVerifyMaxNodes && t0 + n <= p.n_tokens;
+  if (!ok) n = 0;
+  for (int i = threadIdx.x; i < n; i += kVerifyThreads) s_best[i] = 0;
+  __syncthreads();
+  const unsigned long long* words = p.best + (int64_t)t0 * p.chunks;
+#pragma unroll 4
+  for (int u = threadIdx.x; u < n * p.chunks; u += kVerifyThreads) atomicMax(s_best + u / p.chunks, __ldg(words + u));
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+  const int lane = threadIdx.x;
+  if (!ok && lane == 0) sckv_report(p.status, SCKV_ERR_BOUNDS, b, KID_VERIFY);
+  auto best_of = [&](int i) { return (int32_t)~(uint32_t)s_best[i]; };
+  int32_t* out = p.path + (int64_t)b * p.max_path;
   int keep = 0, token = -1;
-  if (ok && n > 0) {
-    for (int i = lane; i < n; i += 32) {
-      unsigned long long w = 0;
-      for (int c = 0; c < chunks; ++c) {
-        const unsigned long long x = best[(int64_t)(t0 + i) * chunks + c];
-        w = x > w ? x : w;
-      }
-      s_best[i] = (int32_t)~(uint32_t)w;
-    }
-    __syncwarp();
+  if (n > 0) {
     int cur = 0;
     if (lane == 0) out[0] = 0;
     keep = 1;
-    token = s_best[0];
-    while (keep < max_path) {
+    token = best_of(0);
+    while (keep < p.max_path) {
       // the first later node that hangs on `cur` and carries its token
       int child = -1;
       for (int j0 = cur + 1; j0 < n && child < 0; j0 += 32) {
         const int j = j0 + lane;
-        const bool hit = j < n && __ldg(parents + t0 + j) == cur && __ldg(tokens + t0 + j) == token;
+        const bool hit = j < n && __ldg(p.parents + t0 + j) == cur && __ldg(p.tokens + t0 + j) == token;
         const unsigned m = __ballot_sync(0xffffffffu, hit);
         if (m) child = j0 + __ffs(m) - 1;
       }
@@ -703,13 +716,13 @@ __global__ void verify_walk_kernel(const unsigned long long* best, int chunks, c
       if (lane == 0) out[keep] = child;
       ++keep;
       cur = child;
-      token = s_best[cur];
+      token = best_of(cur);
     }
   }
-  for (int j = keep + lane; j < max_path; j += 32) out[j] = -1;
+  for (int j = keep + lane; j < p.max_path; j += 32) out[j] = -1;
   if (lane == 0) {
-    n_keep[b] = keep;
-    next[b] = token;
+    p.n_keep[b] = keep;
+    p.next[b] = token;
   }
 }
 
@@ -864,26 +877,25 @@ extern "C" int sckv_verify_tree(sckv_pool* p, const void* logits, int logits_dty
   if (reinterpret_cast<uintptr_t>(logits) & (el - 1)) return SCKV_ERR_ALIGNMENT;
   SCKV_DEVICE_GUARD(p->device);
   cudaStream_t s = as_stream(stream);
-  unsigned long long* best = reinterpret_cast<unsigned long long*>(workspace);
-  int chunks = 1;
+  Verify a{1, n_tokens, max_path, reinterpret_cast<unsigned long long*>(workspace), tokens, parents,
+           cu_tokens, path, n_keep, next_token, p->status};
   if (n_tokens > 0) {
-    chunks = verify_chunks(p->num_sms, n_tokens, vocab);
-    const int64_t blocks = (int64_t)n_tokens * chunks;
+    a.chunks = verify_chunks(p->num_sms, n_tokens, vocab);
+    const int64_t blocks = (int64_t)n_tokens * a.chunks;
     if (blocks > INT32_MAX) return SCKV_ERR_INVALID_ARG;
-    switch (logits_dtype) {
-      case SCKV_DTYPE_F32:
-        verify_argmax_kernel<SCKV_DTYPE_F32><<<(unsigned)blocks, kVerifyThreads, 0, s>>>(logits, ld, vocab, chunks, best);
-        break;
-      case SCKV_DTYPE_F16:
-        verify_argmax_kernel<SCKV_DTYPE_F16><<<(unsigned)blocks, kVerifyThreads, 0, s>>>(logits, ld, vocab, chunks, best);
-        break;
-      default:
-        verify_argmax_kernel<SCKV_DTYPE_BF16><<<(unsigned)blocks, kVerifyThreads, 0, s>>>(logits, ld, vocab, chunks, best);
-    }
+    auto launch = [&](auto dt) {
+      verify_argmax_kernel<decltype(dt)::value>
+          <<<(unsigned)blocks, kVerifyThreads, 0, s>>>(logits, ld, vocab, a.chunks, a.best);
+    };
+    if (logits_dtype == SCKV_DTYPE_F32)
+      launch(std::integral_constant<int, SCKV_DTYPE_F32>{});
+    else if (logits_dtype == SCKV_DTYPE_F16)
+      launch(std::integral_constant<int, SCKV_DTYPE_F16>{});
+    else
+      launch(std::integral_constant<int, SCKV_DTYPE_BF16>{});
     SCKV_LAUNCH_CHECK();
   }
-  verify_walk_kernel<<<n_seqs, 32, 0, s>>>(best, chunks, tokens, parents, cu_tokens, n_tokens, max_path, path, n_keep,
-                                           next_token, p->status);
+  verify_walk_kernel<<<n_seqs, kVerifyThreads, 0, s>>>(a);
   SCKV_LAUNCH_CHECK();
   return SCKV_OK;
 }

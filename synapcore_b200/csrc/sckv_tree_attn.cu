@@ -36,8 +36,9 @@
 //                page-head, which a rank-5 view of the pool lays out as 8-row
 //                groups [rows 0-7 | 8-15][dims 0-63 | 64-127], so that groups
 //                of consecutive pages have one stride. One-byte pools: K and
-//                V of a page in one 4 KiB box into a staging ring, half a tile
-//                at a time; the scales.
+//                V of a page in one 4 KiB box into a staging ring, and the
+//                scales; the two take half tiles in turn (one alone: FP8 557
+//                us for the copies, against 412).
 //   warps 3, 13-19  one-byte pools (20 warps): decode a staged page-head each
 //                into the f16 rings. int8 codes times their token's fp16 scale
 //                (the rounding that the cache's values have); e4m3 codes
@@ -54,10 +55,10 @@
 //
 // Measured (floor: bytes at a copy's rate): 32 x 4,096 tokens, 16 fp16 heads
 // without groups, 24 nodes: 168 us (137), 5.3 TB/s: the rings' loads, and ~4,500
-// cycles per item to write it. 64 x 16,384 tokens, 32 / 8 heads, FP8: 619 us
-// (292): 557 with all work taken out, so the staging ring's turns (48 KiB on
-// the way), then the chain S - softmax - P V. 4 x 65,536 tokens, 32 / 8 heads,
-// 64 nodes, bf16: 370 us (164, and 246 of tensor time with P in two parts): the
+// cycles per item to write it. 64 x 16,384 tokens, 32 / 8 heads, FP8: 616 us
+// (292): 412 for the copies alone, then the chain decoding - S - softmax - P V,
+// whose parts cost 11 - 14 % each. 4 x 65,536 tokens, 32 / 8 heads,
+// 64 nodes, bf16: 360 us (164, and 246 of tensor time with P in two parts): the
 // exponentials, 2,048 cycles of a pair of tiles, behind the waits for S.
 //
 // P is held as 2^6 times the weight, so that f16's smallest step is 2^-31 of

@@ -166,7 +166,8 @@ __global__ void __launch_bounds__(kRopeThreads) rope_axes_kernel(const RopeAxes 
       if (blockIdx.x == 0) sckv_report(p.g.status, SCKV_ERR_BOUNDS, axis, KID_ROPE_AXES);
       axis = 0;
     }
-    const double a = (double)__ldg(p.positions + axis * p.pos_stride + t) * p.inv_scaling * (double)__ldg(p.inv_freq + f);
+    const double pos = (double)__ldg(p.positions + axis * p.pos_stride + t) * p.inv_scaling;
+    const double a = pos * (double)__ldg(p.inv_freq + f);
     const double r = a - 6.283185307179586 * rint(a * 0.15915494309189535);
     sincosf((float)r, &s_sin[i], &s_cos[i]);
   }
@@ -190,7 +191,8 @@ __global__ void __launch_bounds__(kRopeThreads) rope_axes_kernel(const RopeAxes 
       for (int kind = 0; kind < 3; ++kind) {
         s_src[tl][kind] = reinterpret_cast<const uint8_t*>(src_of(kind)) + t * ld_of(kind) * 2;
         uint8_t* dst = nullptr;
-        if (kind == 0 && p.q_out_dtype == kDT) dst = reinterpret_cast<uint8_t*>(p.q_out) + (int64_t)t * p.hq * kRopeD * 2;
+        if (kind == 0 && p.q_out_dtype == kDT)
+          dst = reinterpret_cast<uint8_t*>(p.q_out) + (int64_t)t * p.hq * kRopeD * 2;
         if (kind > 0 && p.g.dtype == kDT && page >= 0)
           dst = reinterpret_cast<uint8_t*>(p.g.data) + row_off(p.g, p.layer, page, kind - 1, 0, slot) * 2;
         s_dst[tl][kind] = dst;
@@ -348,7 +350,9 @@ struct Compact {
 };
 
 // i / d for i < 2^16, 0 < d < 2^16, mul = 2^32 / d + 1
-__device__ __forceinline__ uint32_t div_by(uint32_t i, uint32_t mul, uint32_t d) { return d == 1 ? i : __umulhi(i, mul); }
+__device__ __forceinline__ uint32_t div_by(uint32_t i, uint32_t mul, uint32_t d) {
+  return d == 1 ? i : __umulhi(i, mul);
+}
 
 __global__ void __launch_bounds__(kCompactWarps * 32) compact_kernel(const Compact p) {
   const Geo& g = p.g;

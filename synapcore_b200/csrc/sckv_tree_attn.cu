@@ -176,7 +176,9 @@ __device__ __forceinline__ bool tree_seq(const TreeParams& p, int s, int& n, int
 }
 
 // Node of row rr of a sequence's group: rr / G. Exact while rr G < 2^32; rr < 256 G.
-__device__ __forceinline__ int tree_node(const TreeParams& p, int rr) { return p.g_mul ? (int)__umulhi((uint32_t)rr, p.g_mul) : rr; }
+__device__ __forceinline__ int tree_node(const TreeParams& p, int rr) {
+  return p.g_mul ? (int)__umulhi((uint32_t)rr, p.g_mul) : rr;
+}
 constexpr int kMaxGroup = 4095;
 
 // A CTA's walk over its share of the line of key tiles, one item (or part of one) at a time.
@@ -371,13 +373,16 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
   const uint32_t s_full = v_empty + 8 * kStages;      // [x] S in tensor memory (commit)
   const uint32_t p_full = s_full + 8 * 2;             // [x] P in tensor memory, V tile fixed (8 arrivals)
   const uint32_t pv_done = p_full + 8 * 2;            // [x] PV finished (commit)
-  // the item's Q is in shared memory and the O of the item before was read (one arrival per softmax warp)
+  // the item's Q is in shared memory and the O of the item before was read (one arrival per softmax warp), and the PV
+  // warp is at the item too
   const uint32_t q_full = pv_done + 8 * 2;
   const uint32_t mma_done = q_full + 8 * 1;           // every issued MMA finished
-  const uint32_t o_full = mma_done + 8 * 1;           // the item's sums are written and its O is complete (one arrival per softmax warp)
-  const uint32_t x_full = o_full + 8 * 1;             // [w] a piece of O is in the exchange buffer (one arrival per warp of w)
+  // the item's sums are written and its O is complete (one arrival per softmax warp)
+  const uint32_t o_full = mma_done + 8 * 1;
+  // [w] a piece of O is in the exchange buffer (one arrival per warp of w)
+  const uint32_t x_full = o_full + 8 * 1;
   const uint32_t x_done = x_full + 8 * 2;             // the exchange buffer was read (one arrival per softmax warp)
-  const uint32_t st_full = x_done + 8 * 1;            // one-byte pools: [SS] staged half tile landed, its scales are written
+  const uint32_t st_full = x_done + 8 * 1;            // one-byte pools: [SS] staged half tile, scales are there
   const uint32_t st_empty = st_full + 8 * C::kStaging;  // [SS] decoded (one arrival per decoding warp)
   float2* s_ml = reinterpret_cast<float2*>(base + C::kOffMl);
   float* s_vref = reinterpret_cast<float*>(base + C::kOffVref);
@@ -413,10 +418,12 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
     if ((int)threadIdx.x < C::kNumBars) {
       const uint32_t bar = bar0 + 8 * threadIdx.x;
       uint32_t count = 1;
-      if (C::kB8 && ((bar >= k_full && bar < k_full + 8 * kStages) || (bar >= v_full && bar < v_full + 8 * kStages))) count = 8;
+      const bool full = (bar >= k_full && bar < k_full + 8 * kStages) || (bar >= v_full && bar < v_full + 8 * kStages);
+      if (C::kB8 && full) count = 8;  // half tiles of the decoding warps
       if (bar >= p_full && bar < p_full + 16) count = 8;
       if (bar == mma_done) count = 2;
-      if (bar == q_full || bar == o_full || bar == x_done) count = 8;
+      if (bar == o_full || bar == x_done) count = 8;
+      if (bar == q_full) count = 9;
       if (bar == x_full || bar == x_full + 8) count = 4;
       if (C::kB8 && bar >= st_empty && bar < st_empty + 8 * C::kStaging) count = 8;
       bar_init(bar, count);
@@ -502,12 +509,13 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
         }
       }
       // nothing of ours may still be landing when the CTA retires
-      for (int t = g > kStages ? g - kStages : 0; t < g; ++t) warp_wait_bar(fulls + 8 * (t % kStages), (t / kStages) & 1);
+      for (int t = g > kStages ? g - kStages : 0; t < g; ++t)
+        warp_wait_bar(fulls + 8 * (t % kStages), (t / kStages) & 1);
     } else {
       // One-byte pools: the two warps take half tiles in turn (a slot is filled again ~1,000 cycles after it is free;
       // its copies' issue is most of them). Lanes 0-3 copy a page's K and V each. Scales of a half tile: int8 four
       // tokens' fp16 per lane (K, V; 4 pages; 4 x 4 tokens); FP8 lanes 0-3 the K, 4-7 the V scales of its pages, a page
-      // past the last node scales by 1 (K, masked anyway) and 0 (V). Loaded one turn (two half tiles) ahead, page ids two.
+      // past the last node scales by 1 (K, masked anyway) and 0 (V). Loaded one turn (two half tiles) ahead, ids two.
       const uint32_t ring = smem_u32(base + C::kOffStage) + lane * 4096;
       const int skv = C::kINT8 ? lane >> 4 : (lane >> 2) & 1, spg = C::kINT8 ? (lane >> 2) & 3 : lane & 3;
       const bool mine = C::kINT8 || lane < 8;
@@ -523,7 +531,7 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
           const int64_t at = ((layer_base + page) * 2 + skv) * p.g.H + s.h;
           if (mine && there(j, spg)) {
             if (C::kINT8)
-              r = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const __half*>(p.g.scales) + at * 16) + (lane & 3));
+              r = __ldg(reinterpret_cast<const uint2*>(p.g.scales) + at * 4 + (lane & 3));
             else
               r.x = __ldg(reinterpret_cast<const uint32_t*>(p.g.scales) + at);
           }
@@ -602,8 +610,8 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
               w[e] = *reinterpret_cast<const uint4*>(src + ((e >> 1) * 8 + r8) * 128 +
                                                      ((((e & 1) * 4 + (lane & 3)) ^ r8) << 4));
             if (C::kINT8) {
-              const __half* tok = reinterpret_cast<const __half*>(base + C::kOffScale + (g % kScaleSlots) * 256) + kv * 64 +
-                                  pg * SCKV_PAGE_TOKENS;
+              const __half* tok = reinterpret_cast<const __half*>(base + C::kOffScale + (g % kScaleSlots) * 256) +
+                                  kv * 64 + pg * SCKV_PAGE_TOKENS;
               sc[0] = tok[r8];
               sc[1] = tok[8 + r8];
             }
@@ -708,7 +716,10 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
     int cnt[2] = {0, 0};     // uses of each set in earlier items
     for (int k = 0; ok && tree_next(p, cum, walk, s); ++k) {
       const bool two = C::kQTiles == 2 && s.nq == 2;
-      if (mw == 0 && (*abort_flag || !warp_wait_bar(q_full, k & 1))) {
+      // Both warps begin an item together: the PV warp, which has nothing to do for an item of two query tiles, would
+      // otherwise wait for phases of P and V several uses ahead, which their parity cannot tell from earlier ones.
+      if (mw == 1 && lane == 0) bar_arrive(q_full);
+      if (*abort_flag || !warp_wait_bar(q_full, k & 1)) {
         ok = false;
         break;
       }
@@ -895,7 +906,8 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
         for (int q = 0; q < kPg; ++q) ks[q] = p.scale_log2;
         if (C::kFP8) {
           // the tile's page scales (written before the codes were decoded, and so before S was made)
-          const float* sc = reinterpret_cast<const float*>(base + C::kOffScale + ((2 * (gt + i) + w) % kScaleSlots) * 256) + copy * kPg;
+          const int slot = (2 * (gt + i) + w) % kScaleSlots;
+          const float* sc = reinterpret_cast<const float*>(base + C::kOffScale + slot * 256) + copy * kPg;
           float vm = 0.f;
 #pragma unroll
           for (int q = 0; q < kPg; ++q) {
@@ -1051,8 +1063,8 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
           for (int c = row; c < (r1 - r0) * 16; c += 128) {
             const int r = r0 + (c >> 4), ch = c & 15;
             const int key = key0 + r;
-            uint4* cell = reinterpret_cast<uint4*>(vt + (r >> 4) * kPageTile + ((r >> 3) & 1) * 2048 + (ch >> 3) * 1024 +
-                                                   (r & 7) * 128 + (((ch & 7) ^ (r & 7)) << 4));
+            const int at = (r >> 4) * kPageTile + ((r >> 3) & 1) * 2048 + (ch >> 3) * 1024 + (r & 7) * 128;
+            uint4* cell = reinterpret_cast<uint4*>(vt + at + (((ch & 7) ^ (r & 7)) << 4));
             if (key >= s.L) {
               *cell = make_uint4(0u, 0u, 0u, 0u);
             } else {
@@ -1256,10 +1268,15 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
       return true;
     };
     for (int k = 0; ok && more; ++k) {
-      if (C::kQTiles == 2 && s.nq == 2) ok = run_item(std::integral_constant<bool, C::kQTiles == 2>{}, std::integral_constant<int, 1>{}, k);
-      else if (s.copies == 1) ok = run_item(std::false_type{}, std::integral_constant<int, 1>{}, k);
-      else if (s.copies == 2) ok = run_item(std::false_type{}, std::integral_constant<int, 2>{}, k);
-      else ok = run_item(std::false_type{}, std::integral_constant<int, 4>{}, k);
+      constexpr bool kPair = C::kQTiles == 2;
+      if (kPair && s.nq == 2)
+        ok = run_item(std::integral_constant<bool, kPair>{}, std::integral_constant<int, 1>{}, k);
+      else if (s.copies == 1)
+        ok = run_item(std::false_type{}, std::integral_constant<int, 1>{}, k);
+      else if (s.copies == 2)
+        ok = run_item(std::false_type{}, std::integral_constant<int, 2>{}, k);
+      else
+        ok = run_item(std::false_type{}, std::integral_constant<int, 4>{}, k);
       if (!ok) break;
       more = tree_next(p, cum, walk, s);
       if (more) ok = load_q(s);
@@ -1341,8 +1358,8 @@ int ensure_tree_tmap(sckv_pool* p) {
   const cuuint64_t strides[4] = {256, 128, 2048, 4096};
   const cuuint32_t box[5] = {64, 8, 2, 2, 1};
   const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-  const CUresult r = encode(reinterpret_cast<CUtensorMap*>(p->tmap_tree), CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, p->data, dims,
-                            strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  const CUresult r = encode(reinterpret_cast<CUtensorMap*>(p->tmap_tree), CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, p->data,
+                            dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     char what[64];
@@ -1373,7 +1390,8 @@ int launch_tree(sckv_pool* p, const TreeParams& t, cudaStream_t stream) {
   const int smem = C::kFixedSmem + 4 * t.n_seqs;
   static_assert(C::kFixedSmem + 4 * kMaxSeqs <= 227 * 1024, "shared memory of the largest batch");
   if (!p->tree_smem_ready) {  // the largest batch's, once per pool (a pool has one kernel)
-    SCKV_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kFixedSmem + 4 * kMaxSeqs));
+    SCKV_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         C::kFixedSmem + 4 * kMaxSeqs));
     p->tree_smem_ready = 1;
   }
   kern<<<p->num_sms, C::kThreads, smem, stream>>>(t, *map);

@@ -898,6 +898,16 @@ def test_tree_attn_one_item_over_all_sms(cuda_device, kind, hq, nodes):
     check_attn(cuda_device, kind, hq, 1, [16000], [nodes], seed=hq + nodes)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("seqs,ctx,hq,hkv", [(60, 700, 16, 2), (15, 1251, 64, 8), (40, 300, 48, 3)])
+def test_tree_attn_row_groups_of_all_sizes_in_turn(cuda_device, kind, seqs, ctx, hq, hkv):
+    """An SM takes items of two query tiles and of one, with one, two and four copies of its rows, in any order."""
+    r = torch.Generator().manual_seed(seqs)
+    nodes = torch.randint(1, 41, (seqs,), generator=r).tolist()
+    nodes[0::4] = [35] * len(nodes[0::4])
+    check_attn(cuda_device, kind, hq, hkv, [ctx - 3 * b for b in range(seqs)], nodes, seed=seqs)
+
+
 def test_tree_attn_limits(cuda_device):
     dev = cuda_device
     i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731

@@ -36,9 +36,8 @@
 //                page-head, which a rank-5 view of the pool lays out as 8-row
 //                groups [rows 0-7 | 8-15][dims 0-63 | 64-127], so that groups
 //                of consecutive pages have one stride. One-byte pools: K and
-//                V of a page in one 4 KiB box into a staging ring, and the
-//                scales; the two take half tiles in turn (one alone: FP8 557
-//                us for the copies, against 412).
+//                V of a page in one 4 KiB box into a staging ring, half a tile
+//                at a time; the scales.
 //   warps 3, 13-19  one-byte pools (20 warps): decode a staged page-head each
 //                into the f16 rings. int8 codes times their token's fp16 scale
 //                (the rounding that the cache's values have); e4m3 codes
@@ -55,9 +54,9 @@
 //
 // Measured (floor: bytes at a copy's rate): 32 x 4,096 tokens, 16 fp16 heads
 // without groups, 24 nodes: 168 us (137), 5.3 TB/s: the rings' loads, and ~4,500
-// cycles per item to write it. 64 x 16,384 tokens, 32 / 8 heads, FP8: 616 us
-// (292): 412 for the copies alone, then the chain decoding - S - softmax - P V,
-// whose parts cost 11 - 14 % each. 4 x 65,536 tokens, 32 / 8 heads,
+// cycles per item to write it. 64 x 16,384 tokens, 32 / 8 heads, FP8: 655 us
+// (292): 557 for the copies alone, the staging ring's turns (48 KiB on the way),
+// then the chain decoding - S - softmax - P V. 4 x 65,536 tokens, 32 / 8 heads,
 // 64 nodes, bf16: 360 us (164, and 246 of tensor time with P in two parts): the
 // exponentials, 2,048 cycles of a pair of tiles, behind the waits for S.
 //
@@ -129,7 +128,7 @@ struct TreeCfg {
   static constexpr int kOffPartial = kOffTmem + 16;                         // int [warps]
   static constexpr int kOffCum = kOffPartial + kMaxWarps * 4;               // int [n_seqs + 1]
   static constexpr int kFixedSmem = 1024 + kOffCum + 4;                     // + 4 n_seqs
-  static_assert(2 * (2 + kStages) + 1 + kStaging < kScaleSlots, "scale slots outlive their half tiles");
+  static_assert(2 * kStages + kStaging < kScaleSlots, "scale slots outlive their half tiles");
 };
 
 // What the joining kernel needs of a CTA whose first item began in an earlier one and ends in it.
@@ -176,9 +175,7 @@ __device__ __forceinline__ bool tree_seq(const TreeParams& p, int s, int& n, int
 }
 
 // Node of row rr of a sequence's group: rr / G. Exact while rr G < 2^32; rr < 256 G.
-__device__ __forceinline__ int tree_node(const TreeParams& p, int rr) {
-  return p.g_mul ? (int)__umulhi((uint32_t)rr, p.g_mul) : rr;
-}
+__device__ __forceinline__ int tree_node(const TreeParams& p, int rr) { return p.g_mul ? (int)__umulhi((uint32_t)rr, p.g_mul) : rr; }
 constexpr int kMaxGroup = 4095;
 
 // A CTA's walk over its share of the line of key tiles, one item (or part of one) at a time.
@@ -334,12 +331,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr));
 }
 
-// Waits for the load of x.
-__device__ __forceinline__ void after_load(uint32_t x) {
-  [[maybe_unused]] uint32_t r;
-  asm volatile("and.b32 %0, %1, 0;" : "=r"(r) : "r"(x) : "memory");
-}
-
 __device__ __forceinline__ void bar_arrive_n(uint32_t bar, uint32_t n) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n) : "memory");
 }
@@ -377,12 +368,10 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
   // warp is at the item too
   const uint32_t q_full = pv_done + 8 * 2;
   const uint32_t mma_done = q_full + 8 * 1;           // every issued MMA finished
-  // the item's sums are written and its O is complete (one arrival per softmax warp)
-  const uint32_t o_full = mma_done + 8 * 1;
-  // [w] a piece of O is in the exchange buffer (one arrival per warp of w)
-  const uint32_t x_full = o_full + 8 * 1;
+  const uint32_t o_full = mma_done + 8 * 1;           // the item's sums are written and its O is complete (one arrival per softmax warp)
+  const uint32_t x_full = o_full + 8 * 1;             // [w] a piece of O is in the exchange buffer (one arrival per warp of w)
   const uint32_t x_done = x_full + 8 * 2;             // the exchange buffer was read (one arrival per softmax warp)
-  const uint32_t st_full = x_done + 8 * 1;            // one-byte pools: [SS] staged half tile, scales are there
+  const uint32_t st_full = x_done + 8 * 1;            // one-byte pools: [SS] staged half tile landed, its scales are written
   const uint32_t st_empty = st_full + 8 * C::kStaging;  // [SS] decoded (one arrival per decoding warp)
   float2* s_ml = reinterpret_cast<float2*>(base + C::kOffMl);
   float* s_vref = reinterpret_cast<float*>(base + C::kOffVref);
@@ -418,13 +407,13 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
     if ((int)threadIdx.x < C::kNumBars) {
       const uint32_t bar = bar0 + 8 * threadIdx.x;
       uint32_t count = 1;
-      const bool full = (bar >= k_full && bar < k_full + 8 * kStages) || (bar >= v_full && bar < v_full + 8 * kStages);
-      if (C::kB8 && full) count = 8;  // half tiles of the decoding warps
+      if (C::kB8 && ((bar >= k_full && bar < k_full + 8 * kStages) || (bar >= v_full && bar < v_full + 8 * kStages))) count = 8;
       if (bar >= p_full && bar < p_full + 16) count = 8;
       if (bar == mma_done) count = 2;
       if (bar == o_full || bar == x_done) count = 8;
       if (bar == q_full) count = 9;
       if (bar == x_full || bar == x_full + 8) count = 4;
+      if (C::kB8 && bar >= st_full && bar < st_full + 8 * C::kStaging) count = 2;
       if (C::kB8 && bar >= st_empty && bar < st_empty + 8 * C::kStaging) count = 8;
       bar_init(bar, count);
       fence_mbar_init();
@@ -472,11 +461,10 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
     // A lane owns a page of the tile: its id is loaded one tile ahead (and not looked at in the turn that loads it,
     // which would wait for it), and the copies of all pages go out as one instruction (one lane after the other
     // issued them in ~180 cycles each, which paced the kernel).
-    const int part = warp == kWarpProdB ? 1 : 0;  // 16-bit: K, V; one-byte: even, odd half tiles
+    const int part = warp == kWarpProdB ? 1 : 0;  // 16-bit: K, V; one-byte: codes, scales
     if (lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap)) : "memory");
     TreeSeg s;
     int g = 0;
-    [[maybe_unused]] int issued = 0;
     bool aborted = false;
     auto valid_page = [&](int page) -> int {
       if (page >= 0 && page < p.g.P) return page;
@@ -509,44 +497,62 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
         }
       }
       // nothing of ours may still be landing when the CTA retires
-      for (int t = g > kStages ? g - kStages : 0; t < g; ++t)
-        warp_wait_bar(fulls + 8 * (t % kStages), (t / kStages) & 1);
-    } else {
-      // One-byte pools: the two warps take half tiles in turn (a slot is filled again ~1,000 cycles after it is free;
-      // its copies' issue is most of them). Lanes 0-3 copy a page's K and V each. Scales of a half tile: int8 four
-      // tokens' fp16 per lane (K, V; 4 pages; 4 x 4 tokens); FP8 lanes 0-3 the K, 4-7 the V scales of its pages, a page
-      // past the last node scales by 1 (K, masked anyway) and 0 (V). Loaded one turn (two half tiles) ahead, ids two.
+      for (int t = g > kStages ? g - kStages : 0; t < g; ++t) warp_wait_bar(fulls + 8 * (t % kStages), (t / kStages) & 1);
+    } else if (part == 0) {
       const uint32_t ring = smem_u32(base + C::kOffStage) + lane * 4096;
-      const int skv = C::kINT8 ? lane >> 4 : (lane >> 2) & 1, spg = C::kINT8 ? (lane >> 2) & 3 : lane & 3;
-      const bool mine = C::kINT8 || lane < 8;
-      int g0 = 0;  // half tiles of earlier items (even)
       while (!aborted && tree_next(p, cum, walk, s)) {
         const int32_t* bt_row = p.bt + (int64_t)s.seq * p.bt_stride;
-        const int js = 2 * s.ka, je = 2 * (s.ka + s.nk);
-        auto there = [&](int j, int pg) { return j < je && j * kHalfPages + pg < s.pages; };
-        auto fetch = [&](int j) -> int { return there(j, spg) ? __ldg(bt_row + j * kHalfPages + spg) : 0; };
+        auto there = [&](int j) { return lane < kHalfPages && j * kHalfPages + lane < s.pages; };
+        const int je = 2 * (s.ka + s.nk);
+        int nxt = there(2 * s.ka) ? __ldg(bt_row + 2 * s.ka * kHalfPages + lane) : 0;
+        for (int j = 2 * s.ka; j < je; ++j, ++g) {
+          const int id = nxt;
+          if (j + 1 < je && there(j + 1)) nxt = __ldg(bt_row + (j + 1) * kHalfPages + lane);
+          const int st = g % C::kStaging;
+          if (*abort_flag || (g >= C::kStaging && !warp_wait_bar(st_empty + 8 * st, ((g / C::kStaging) - 1) & 1))) {
+            aborted = true;
+            break;
+          }
+          if (lane == 0)
+            bar_expect(st_full + 8 * st, (uint32_t)max(0, min(kHalfPages, s.pages - j * kHalfPages)) * 4096u);
+          __syncwarp();
+          if (there(j))
+            tma_load(ring + st * kHalfSlot, &tmap, 0, 0, s.h, 0, (int)(layer_base + valid_page(id)), st_full + 8 * st);
+          __syncwarp();
+        }
+      }
+      for (int t = g > C::kStaging ? g - C::kStaging : 0; t < g; ++t)
+        warp_wait_bar(st_full + 8 * (t % C::kStaging), (t / C::kStaging) & 1);
+    } else {
+      // scales of a half tile: int8 four tokens' fp16 per lane (K, V; 4 pages; 4 x 4 tokens); FP8 lanes 0-3 the K,
+      // 4-7 the V scales of its pages, a page past the last node scales by 1 (K, masked anyway) and 0 (V). Loaded one
+      // half tile ahead, the page ids two.
+      const int skv = C::kINT8 ? lane >> 4 : (lane >> 2) & 1, spg = C::kINT8 ? (lane >> 2) & 3 : lane & 3;
+      const bool mine = C::kINT8 || lane < 8;
+      while (!aborted && tree_next(p, cum, walk, s)) {
+        const int32_t* bt_row = p.bt + (int64_t)s.seq * p.bt_stride;
+        const int je = 2 * (s.ka + s.nk);
+        auto there = [&](int j) { return mine && j < je && j * kHalfPages + spg < s.pages; };
+        auto fetch = [&](int j) -> int { return there(j) ? __ldg(bt_row + j * kHalfPages + spg) : 0; };
         auto load_scale = [&](int page, int j) -> uint2 {
           uint2 r = make_uint2(C::kFP8 && skv == 0 ? 0x3f800000u : 0u, 0u);
           if (page < 0 || page >= p.g.P) page = 0;
           const int64_t at = ((layer_base + page) * 2 + skv) * p.g.H + s.h;
-          if (mine && there(j, spg)) {
+          if (there(j)) {
             if (C::kINT8)
-              r = __ldg(reinterpret_cast<const uint2*>(p.g.scales) + at * 4 + (lane & 3));
+              r = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const __half*>(p.g.scales) + at * 16) + (lane & 3));
             else
               r.x = __ldg(reinterpret_cast<const uint32_t*>(p.g.scales) + at);
           }
           return r;
         };
-        int sid = fetch(js + part), sid1 = fetch(js + part + 2);
-        uint2 sc = load_scale(sid, js + part);
-        for (int j = js + part; j < je; j += 2) {
-          const int g = g0 + j - js, st = g % C::kStaging;
-          // (lane L < 4 holds the id of page L in FP8, of its lane's page in int8)
-          const int id = __shfl_sync(0xffffffffu, sid, C::kINT8 ? 4 * (lane & 3) : lane & 3);
+        uint2 sc = load_scale(fetch(2 * s.ka), 2 * s.ka);
+        int sid = fetch(2 * s.ka + 1);
+        for (int j = 2 * s.ka; j < je; ++j, ++g) {
+          const int st = g % C::kStaging;
           const uint2 now = sc;
-          sc = load_scale(sid1, j + 2);
-          sid = sid1;
-          sid1 = fetch(j + 4);
+          sc = load_scale(sid, j + 1);
+          sid = fetch(j + 2);
           if (*abort_flag || (g >= C::kStaging && !warp_wait_bar(st_empty + 8 * st, ((g / C::kStaging) - 1) & 1))) {
             aborted = true;
             break;
@@ -555,22 +561,11 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
           if (C::kINT8)
             reinterpret_cast<uint2*>(slot)[lane] = now;
           else if (lane < 8)  // (a K scale of 0 would turn masked scores, -inf, into NaN; NaN stays)
-            reinterpret_cast<float*>(slot)[lane] =
-                skv == 0 && __uint_as_float(now.x) < 1e-30f ? 1e-30f : __uint_as_float(now.x);
+            reinterpret_cast<float*>(slot)[lane] = skv == 0 && __uint_as_float(now.x) < 1e-30f ? 1e-30f : __uint_as_float(now.x);
           __syncwarp();
-          if (lane == 0)
-            bar_expect(st_full + 8 * st, (uint32_t)max(0, min(kHalfPages, s.pages - j * kHalfPages)) * 4096u);
-          __syncwarp();
-          if (lane < kHalfPages && there(j, lane))
-            tma_load(ring + st * kHalfSlot, &tmap, 0, 0, s.h, 0, (int)(layer_base + valid_page(id)), st_full + 8 * st);
-          __syncwarp();
-          issued = g + 1;
+          if (lane == 0) bar_arrive(st_full + 8 * st);
         }
-        if (!aborted) g0 += je - js;
       }
-      // nothing of ours may still be landing when the CTA retires (slots that the other warp filled since have landed)
-      for (int t = aborted ? issued - 1 : max(0, g0 - C::kStaging); t < (aborted ? issued : g0); ++t)
-        if (t >= 0 && (t & 1) == part) warp_wait_bar(st_full + 8 * (t % C::kStaging), (t / C::kStaging) & 1);
     }
     if (aborted && lane == 0) {
       if (!*abort_flag) sckv_report(p.g.status, SCKV_ERR_TIMEOUT, blockIdx.x, KID_TREE_ATTN);
@@ -596,39 +591,25 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
       while (!aborted && tree_next(p, cum, walk, s)) {
         for (int j = 2 * s.ka; j < 2 * (s.ka + s.nk); ++j, ++g) {
           const int ss = g % C::kStaging, gt = g >> 1, st = gt & 1;
-          if (*abort_flag || !warp_wait_bar(st_full + 8 * ss, (g / C::kStaging) & 1)) {
-            aborted = true;
-            break;
-          }
-          // the codes (and int8 scales) into registers; the slot is free once every lane has them
-          uint4 w[4];
-          __half sc[2] = {__half(1.f), __half(1.f)};
-          {
-            const uint8_t* src = base + C::kOffStage + ss * kHalfSlot + pg * 4096 + kv * 2048;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)  // row 8 (e / 2) + r8, codes of dims 64 (e % 2) + 16 (lane % 4) ..
-              w[e] = *reinterpret_cast<const uint4*>(src + ((e >> 1) * 8 + r8) * 128 +
-                                                     ((((e & 1) * 4 + (lane & 3)) ^ r8) << 4));
-            if (C::kINT8) {
-              const __half* tok = reinterpret_cast<const __half*>(base + C::kOffScale + (g % kScaleSlots) * 256) +
-                                  kv * 64 + pg * SCKV_PAGE_TOKENS;
-              sc[0] = tok[r8];
-              sc[1] = tok[8 + r8];
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) after_load(w[e].x);
-            __syncwarp();
-            if (lane == 0) bar_arrive(st_empty + 8 * ss);
-          }
-          if ((g & 1) == 0 && gt >= 2 && (*abort_flag || !warp_wait_bar(empties + 8 * st, ((gt >> 1) - 1) & 1))) {
+          if (((g & 1) == 0 && gt >= 2 && (*abort_flag || !warp_wait_bar(empties + 8 * st, ((gt >> 1) - 1) & 1))) ||
+              !warp_wait_bar(st_full + 8 * ss, (g / C::kStaging) & 1)) {
             aborted = true;
             break;
           }
           if (j * kHalfPages + pg < s.pages) {
+            const __half* tok = reinterpret_cast<const __half*>(base + C::kOffScale + (g % kScaleSlots) * 256) + kv * 64 +
+                                pg * SCKV_PAGE_TOKENS;
+            const uint8_t* src = base + C::kOffStage + ss * kHalfSlot + pg * 4096 + kv * 2048;
             uint8_t* dst = ring + st * kSlot + (g & 1) * kHalfSlot + pg * kPageTile;
+            uint4 w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)  // row 8 (e / 2) + r8, codes of dims 64 (e % 2) + 16 (lane % 4) ..
+              w[e] = *reinterpret_cast<const uint4*>(src + ((e >> 1) * 8 + r8) * 128 +
+                                                     ((((e & 1) * 4 + (lane & 3)) ^ r8) << 4));
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const __half2 s2 = __half2half2(sc[e >> 1]);
+              __half2 s2 = __half2half2(__half(1.f));
+              if (C::kINT8) s2 = __half2half2(tok[(e >> 1) * 8 + r8]);
               const uint32_t ws[4] = {w[e].x, w[e].y, w[e].z, w[e].w};
               uint32_t o[8];
 #pragma unroll
@@ -650,7 +631,10 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
             fence_proxy_async_smem();  // read by the tensor cores
           }
           __syncwarp();
-          if (lane == 0) bar_arrive(fulls + 8 * st);
+          if (lane == 0) {
+            bar_arrive(fulls + 8 * st);
+            bar_arrive(st_empty + 8 * ss);
+          }
         }
       }
       if (aborted && lane == 0) {
@@ -906,8 +890,7 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
         for (int q = 0; q < kPg; ++q) ks[q] = p.scale_log2;
         if (C::kFP8) {
           // the tile's page scales (written before the codes were decoded, and so before S was made)
-          const int slot = (2 * (gt + i) + w) % kScaleSlots;
-          const float* sc = reinterpret_cast<const float*>(base + C::kOffScale + slot * 256) + copy * kPg;
+          const float* sc = reinterpret_cast<const float*>(base + C::kOffScale + ((2 * (gt + i) + w) % kScaleSlots) * 256) + copy * kPg;
           float vm = 0.f;
 #pragma unroll
           for (int q = 0; q < kPg; ++q) {
@@ -1063,8 +1046,8 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
           for (int c = row; c < (r1 - r0) * 16; c += 128) {
             const int r = r0 + (c >> 4), ch = c & 15;
             const int key = key0 + r;
-            const int at = (r >> 4) * kPageTile + ((r >> 3) & 1) * 2048 + (ch >> 3) * 1024 + (r & 7) * 128;
-            uint4* cell = reinterpret_cast<uint4*>(vt + at + (((ch & 7) ^ (r & 7)) << 4));
+            uint4* cell = reinterpret_cast<uint4*>(vt + (r >> 4) * kPageTile + ((r >> 3) & 1) * 2048 + (ch >> 3) * 1024 +
+                                                   (r & 7) * 128 + (((ch & 7) ^ (r & 7)) << 4));
             if (key >= s.L) {
               *cell = make_uint4(0u, 0u, 0u, 0u);
             } else {
@@ -1268,15 +1251,10 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
       return true;
     };
     for (int k = 0; ok && more; ++k) {
-      constexpr bool kPair = C::kQTiles == 2;
-      if (kPair && s.nq == 2)
-        ok = run_item(std::integral_constant<bool, kPair>{}, std::integral_constant<int, 1>{}, k);
-      else if (s.copies == 1)
-        ok = run_item(std::false_type{}, std::integral_constant<int, 1>{}, k);
-      else if (s.copies == 2)
-        ok = run_item(std::false_type{}, std::integral_constant<int, 2>{}, k);
-      else
-        ok = run_item(std::false_type{}, std::integral_constant<int, 4>{}, k);
+      if (C::kQTiles == 2 && s.nq == 2) ok = run_item(std::integral_constant<bool, C::kQTiles == 2>{}, std::integral_constant<int, 1>{}, k);
+      else if (s.copies == 1) ok = run_item(std::false_type{}, std::integral_constant<int, 1>{}, k);
+      else if (s.copies == 2) ok = run_item(std::false_type{}, std::integral_constant<int, 2>{}, k);
+      else ok = run_item(std::false_type{}, std::integral_constant<int, 4>{}, k);
       if (!ok) break;
       more = tree_next(p, cum, walk, s);
       if (more) ok = load_q(s);
@@ -1358,8 +1336,8 @@ int ensure_tree_tmap(sckv_pool* p) {
   const cuuint64_t strides[4] = {256, 128, 2048, 4096};
   const cuuint32_t box[5] = {64, 8, 2, 2, 1};
   const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-  const CUresult r = encode(reinterpret_cast<CUtensorMap*>(p->tmap_tree), CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, p->data,
-                            dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  const CUresult r = encode(reinterpret_cast<CUtensorMap*>(p->tmap_tree), CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, p->data, dims,
+                            strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     char what[64];

@@ -54,10 +54,10 @@
 //
 // Measured (floor: bytes at a copy's rate): 32 x 4,096 tokens, 16 fp16 heads
 // without groups, 24 nodes: 168 us (137), 5.3 TB/s: the rings' loads, and ~4,500
-// cycles per item to write it. 64 x 16,384 tokens, 32 / 8 heads, FP8: 655 us
+// cycles per item to write it. 64 x 16,384 tokens, 32 / 8 heads, FP8: 657 us
 // (292): 557 for the copies alone, the staging ring's turns (48 KiB on the way),
 // then the chain decoding - S - softmax - P V. 4 x 65,536 tokens, 32 / 8 heads,
-// 64 nodes, bf16: 360 us (164, and 246 of tensor time with P in two parts): the
+// 64 nodes, bf16: 370 us (164, and 246 of tensor time with P in two parts): the
 // exponentials, 2,048 cycles of a pair of tiles, behind the waits for S.
 //
 // P is held as 2^6 times the weight, so that f16's smallest step is 2^-31 of
@@ -175,7 +175,9 @@ __device__ __forceinline__ bool tree_seq(const TreeParams& p, int s, int& n, int
 }
 
 // Node of row rr of a sequence's group: rr / G. Exact while rr G < 2^32; rr < 256 G.
-__device__ __forceinline__ int tree_node(const TreeParams& p, int rr) { return p.g_mul ? (int)__umulhi((uint32_t)rr, p.g_mul) : rr; }
+__device__ __forceinline__ int tree_node(const TreeParams& p, int rr) {
+  return p.g_mul ? (int)__umulhi((uint32_t)rr, p.g_mul) : rr;
+}
 constexpr int kMaxGroup = 4095;
 
 // A CTA's walk over its share of the line of key tiles, one item (or part of one) at a time.
@@ -368,10 +370,12 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
   // warp is at the item too
   const uint32_t q_full = pv_done + 8 * 2;
   const uint32_t mma_done = q_full + 8 * 1;           // every issued MMA finished
-  const uint32_t o_full = mma_done + 8 * 1;           // the item's sums are written and its O is complete (one arrival per softmax warp)
-  const uint32_t x_full = o_full + 8 * 1;             // [w] a piece of O is in the exchange buffer (one arrival per warp of w)
+  // the item's sums are written and its O is complete (one arrival per softmax warp)
+  const uint32_t o_full = mma_done + 8 * 1;
+  // [w] a piece of O is in the exchange buffer (one arrival per warp of w)
+  const uint32_t x_full = o_full + 8 * 1;
   const uint32_t x_done = x_full + 8 * 2;             // the exchange buffer was read (one arrival per softmax warp)
-  const uint32_t st_full = x_done + 8 * 1;            // one-byte pools: [SS] staged half tile landed, its scales are written
+  const uint32_t st_full = x_done + 8 * 1;            // one-byte pools: [SS] staged half tile, scales are there
   const uint32_t st_empty = st_full + 8 * C::kStaging;  // [SS] decoded (one arrival per decoding warp)
   float2* s_ml = reinterpret_cast<float2*>(base + C::kOffMl);
   float* s_vref = reinterpret_cast<float*>(base + C::kOffVref);
@@ -497,7 +501,8 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
         }
       }
       // nothing of ours may still be landing when the CTA retires
-      for (int t = g > kStages ? g - kStages : 0; t < g; ++t) warp_wait_bar(fulls + 8 * (t % kStages), (t / kStages) & 1);
+      for (int t = g > kStages ? g - kStages : 0; t < g; ++t)
+        warp_wait_bar(fulls + 8 * (t % kStages), (t / kStages) & 1);
     } else if (part == 0) {
       const uint32_t ring = smem_u32(base + C::kOffStage) + lane * 4096;
       while (!aborted && tree_next(p, cum, walk, s)) {
@@ -540,7 +545,7 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
           const int64_t at = ((layer_base + page) * 2 + skv) * p.g.H + s.h;
           if (there(j)) {
             if (C::kINT8)
-              r = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const __half*>(p.g.scales) + at * 16) + (lane & 3));
+              r = __ldg(reinterpret_cast<const uint2*>(p.g.scales) + at * 4 + (lane & 3));
             else
               r.x = __ldg(reinterpret_cast<const uint32_t*>(p.g.scales) + at);
           }
@@ -561,7 +566,8 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
           if (C::kINT8)
             reinterpret_cast<uint2*>(slot)[lane] = now;
           else if (lane < 8)  // (a K scale of 0 would turn masked scores, -inf, into NaN; NaN stays)
-            reinterpret_cast<float*>(slot)[lane] = skv == 0 && __uint_as_float(now.x) < 1e-30f ? 1e-30f : __uint_as_float(now.x);
+            reinterpret_cast<float*>(slot)[lane] =
+                skv == 0 && __uint_as_float(now.x) < 1e-30f ? 1e-30f : __uint_as_float(now.x);
           __syncwarp();
           if (lane == 0) bar_arrive(st_full + 8 * st);
         }
@@ -597,8 +603,8 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
             break;
           }
           if (j * kHalfPages + pg < s.pages) {
-            const __half* tok = reinterpret_cast<const __half*>(base + C::kOffScale + (g % kScaleSlots) * 256) + kv * 64 +
-                                pg * SCKV_PAGE_TOKENS;
+            const __half* tok = reinterpret_cast<const __half*>(base + C::kOffScale + (g % kScaleSlots) * 256) +
+                                kv * 64 + pg * SCKV_PAGE_TOKENS;
             const uint8_t* src = base + C::kOffStage + ss * kHalfSlot + pg * 4096 + kv * 2048;
             uint8_t* dst = ring + st * kSlot + (g & 1) * kHalfSlot + pg * kPageTile;
             uint4 w[4];
@@ -890,7 +896,8 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
         for (int q = 0; q < kPg; ++q) ks[q] = p.scale_log2;
         if (C::kFP8) {
           // the tile's page scales (written before the codes were decoded, and so before S was made)
-          const float* sc = reinterpret_cast<const float*>(base + C::kOffScale + ((2 * (gt + i) + w) % kScaleSlots) * 256) + copy * kPg;
+          const int slot = (2 * (gt + i) + w) % kScaleSlots;
+          const float* sc = reinterpret_cast<const float*>(base + C::kOffScale + slot * 256) + copy * kPg;
           float vm = 0.f;
 #pragma unroll
           for (int q = 0; q < kPg; ++q) {
@@ -1251,10 +1258,15 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
       return true;
     };
     for (int k = 0; ok && more; ++k) {
-      if (C::kQTiles == 2 && s.nq == 2) ok = run_item(std::integral_constant<bool, C::kQTiles == 2>{}, std::integral_constant<int, 1>{}, k);
-      else if (s.copies == 1) ok = run_item(std::false_type{}, std::integral_constant<int, 1>{}, k);
-      else if (s.copies == 2) ok = run_item(std::false_type{}, std::integral_constant<int, 2>{}, k);
-      else ok = run_item(std::false_type{}, std::integral_constant<int, 4>{}, k);
+      constexpr bool kPair = C::kQTiles == 2;
+      if (kPair && s.nq == 2)
+        ok = run_item(std::integral_constant<bool, kPair>{}, std::integral_constant<int, 1>{}, k);
+      else if (s.copies == 1)
+        ok = run_item(std::false_type{}, std::integral_constant<int, 1>{}, k);
+      else if (s.copies == 2)
+        ok = run_item(std::false_type{}, std::integral_constant<int, 2>{}, k);
+      else
+        ok = run_item(std::false_type{}, std::integral_constant<int, 4>{}, k);
       if (!ok) break;
       more = tree_next(p, cum, walk, s);
       if (more) ok = load_q(s);

@@ -25,6 +25,7 @@ SCKV_ERR_POOL_EXHAUSTED = -6
 SCKV_ERR_TIMEOUT = -7
 SCKV_ERR_UNSUPPORTED = -8
 SCKV_ERR_SCRATCH_LIMIT = -9
+KERNEL_ALLOC = 7  # sckv_alloc_pages, as the status word names it
 
 # Size of the fixed per-GPU scratch behind sckv_decode_attn_noalloc
 # (SCKV_NOALLOC_SCRATCH_BYTES in include/sckv.h).

@@ -192,9 +192,11 @@ class PagedKVCache:
                              "(sequences added one after another do)")
         return r0
 
-    def _grow_rows(self, r0: int, n_new: Sequence[int]) -> None:
+    def _grow_rows(self, r0: int, n_new: Sequence[int], checked: bool = False) -> None:
         """Pinned pages for rows r0.. so each can hold n_new[i] more tokens:
-        one allocation launch and one block-table scatter for all rows."""
+        one allocation launch and one block-table scatter for all rows.
+        checked: the allocation's outcome is read back (it gives all pages or
+        none), and SCKVPoolExhausted raised with nothing changed."""
         self._no_tree()
         rows, cols = [], []
         for i, t in enumerate(n_new):
@@ -207,6 +209,11 @@ class PagedKVCache:
             cols.extend(range(have, need))
         if rows:
             ids, _ = self.pool.alloc_pages(len(rows), pin=True)
+            if checked and int(ids[0]) < 0:
+                code, _, kernel, count = self.pool.status()
+                if (code, kernel, count) == (N.SCKV_ERR_POOL_EXHAUSTED, N.KERNEL_ALLOC, 1):
+                    self.pool.clear_status()  # this call's report alone, which the exception carries
+                raise N.SCKVPoolExhausted(N.SCKV_ERR_POOL_EXHAUSTED, f"{len(rows)} more pages")
             idx = to_device([rows, cols], torch.int64, self.device)
             self.block_table[idx[0], idx[1]] = ids
 
@@ -399,13 +406,15 @@ class PagedKVCache:
         of rows 0..len(n_nodes)-1: pages for all of them are reserved, the
         lengths stay. Returns the device int32 cu_tokens [n + 1] and the
         committed lengths [n] that the step's calls take. Closed by
-        commit_tree; until then the rows cannot change otherwise."""
+        commit_tree; until then the rows cannot change otherwise. Raises
+        SCKVPoolExhausted, with everything as it was, when the pool has too few
+        pages (it reads the allocation's outcome when pages are needed)."""
         nodes = [int(n) for n in n_nodes]
         if not 0 < len(nodes) <= self.n_live or min(nodes) < 0:
             raise ValueError("begin_tree needs one node count >= 0 for each of rows 0..n-1")
         if max(nodes) > MAX_TREE_NODES:
             raise ValueError(f"a tree has more than {MAX_TREE_NODES} nodes")
-        self._grow_rows(0, nodes)
+        self._grow_rows(0, nodes, checked=True)
         self._tree = nodes
         cu = [0]
         for n in nodes:

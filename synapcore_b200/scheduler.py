@@ -32,6 +32,7 @@ from typing import Deque, Dict, List, Optional, Protocol, Sequence, Set, TypedDi
 
 import torch
 
+from . import _native as N
 from .paged_cache import PAGE_TOKENS, PagedKVCache
 from .pool import to_device
 from .tree import MAX_TREE_NODES, TreeDrafter, tree_mask
@@ -273,7 +274,9 @@ class ContinuousBatchScheduler:
     tokens and the one after it are emitted, and the other nodes' rows are
     dropped. The tokens are those of one-by-one greedy decoding, up to the
     rounding of a differently batched pass; a step's accepted_tokens lists
-    them (emitted_tokens has the last). Not together with capture_decode."""
+    them (emitted_tokens has the last). Where the pool has too few pages for
+    all drafts, a step takes those that need no more than its last tokens do.
+    Not together with capture_decode."""
 
     def __init__(self, model, cache=None, max_batch_size: int = 8,
                  prefix_index: Optional[PrefixPageIndex] = None, eos_token_id: Optional[int] = None,
@@ -516,20 +519,26 @@ class ContinuousBatchScheduler:
         trees = [self._draft(req) for req in reqs]
         for r, req in enumerate(reqs):
             cache.move_to_row(req.request_id, r)
+        try:
+            cu, ctx = cache.begin_tree([len(t) for t, _ in trees])
+        except N.SCKVPoolExhausted:
+            # drafts are optional: those that fit the pages a plain step takes
+            fit = [PAGE_TOKENS - cache.lengths[r] % PAGE_TOKENS for r in range(B)]
+            trees = [(t[:m], p[:m]) for (t, p), m in zip(trees, fit)]
+            cu, ctx = cache.begin_tree([len(t) for t, _ in trees])
         n = [len(t) for t, _ in trees]
-        mask, depth = tree_mask([p for _, p in trees])
-        first = [req.pos_offset for req, k in zip(reqs, n) for _ in range(k)]
-        meta = to_device([[t for ts, _ in trees for t in ts], [p for _, ps in trees for p in ps],
-                          [a + d for a, d in zip(first, depth.tolist())]], torch.int64, self.device)
-        small = meta[:2].to(torch.int32)
-        mask = to_device(mask, torch.int64, self.device)
-        cu, ctx = cache.begin_tree(n)
 
         def attend(l, q, k, v):
             cache.append_tree(l, k, v, cu, ctx)
             return cache.tree_attention(l, q, cu, ctx, mask, scale=self.attn_scale, out_dtype=torch.float32)
 
         try:
+            mask, depth = tree_mask([p for _, p in trees])
+            first = [req.pos_offset for req, k in zip(reqs, n) for _ in range(k)]
+            meta = to_device([[t for ts, _ in trees for t in ts], [p for _, ps in trees for p in ps],
+                              [a + d for a, d in zip(first, depth.tolist())]], torch.int64, self.device)
+            small = meta[:2].to(torch.int32)
+            mask = to_device(mask, torch.int64, self.device)
             logits = self.model.logits(self._layers(self.model.embed(meta[0]), meta[2], attend, n_layers))
             path, keep, nxt = cache.pool.verify_tree(logits, small[0], small[1], cu, max_path=max(n))
             host = torch.cat([path, keep[:, None], nxt[:, None]], dim=1).tolist()

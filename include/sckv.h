@@ -386,7 +386,7 @@ SCKV_API size_t sckv_tree_attn_workspace_bytes(const sckv_pool* pool, int n_toke
  * positions : int32 [n_axes] rows of pos_stride elements; axis_map int32 [64],
  *           entries 0 .. n_axes - 1 (others are reported and read as 0).
  * All pool types. int8 rows are quantised as sckv_append_rope does; FP8 pools
- * stage the rotated k in fp16 (workspace) and fold K and V into the pages in a
+ * stage the rotated k in fp32 (workspace) and fold K and V into the pages in a
  * second launch. Tokens outside cu_tokens[0] .. cu_tokens[n_seqs] - 1 are
  * skipped. head_dim 128. */
 SCKV_API int sckv_append_rope_axes(sckv_pool* pool, int layer, const void* q,

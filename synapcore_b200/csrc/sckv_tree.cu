@@ -55,7 +55,7 @@ struct RopeAxes {
   int q_dtype, src_dtype;
   void* q_out;
   int q_out_dtype;
-  __half* k_stage;  // FP8 pools: rotated k [n_tokens][H][D], appended by the next launch
+  float* k_stage;  // FP8 pools: rotated k [n_tokens][H][D], appended (and rounded) by the next launch
   const __half* q_w;
   const __half* k_w;
   float eps;
@@ -274,8 +274,8 @@ __global__ void __launch_bounds__(kRopeThreads) rope_axes_kernel(const RopeAxes 
     } else if (p.g.dtype == SCKV_DTYPE_FP8_E4M3) {
       if (kind == 1) {
         const int64_t o = ((int64_t)t * H + h) * kRopeD + 8 * l8;
-        store8_16(p.k_stage, o, SCKV_DTYPE_F16, a);
-        store8_16(p.k_stage, o + kRopeD / 2, SCKV_DTYPE_F16, b);
+        store8(p.k_stage, o, SCKV_DTYPE_F32, a);
+        store8(p.k_stage, o + kRopeD / 2, SCKV_DTYPE_F32, b);
       }
     } else {
       const int64_t o = row_off(p.g, p.layer, page, kind - 1, h, slot) + 8 * l8;
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_axes_kernel(const RopeAxes 
 
 // FP8 pools, second launch: one warp per (sequence, K|V, head) folds the new
 // rows into its pages (page scales span 16 tokens, so a row cannot be stored
-// by itself). K comes from the rotated fp16 rows, V from its source.
+// by itself). K comes from the rotated fp32 rows, V from its source.
 __global__ void rope_axes_fp8_kernel(const RopeAxes p) {
   const int units = p.n_seqs * 2 * p.g.H;
   const int u = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
@@ -303,7 +303,7 @@ __global__ void rope_axes_fp8_kernel(const RopeAxes p) {
     const int64_t page = resolve_page(p.g, p.bt, p.bt_stride, p.max_blocks, b, pos, KID_ROPE_AXES);
     if (page >= 0)
       fp8_page_head_update(p.g, p.layer, page, kv, h, slot0, n_new, kv ? p.v : (const void*)p.k_stage,
-                           (int64_t)t * stride + (int64_t)h * kRopeD, stride, kv ? p.src_dtype : SCKV_DTYPE_F16);
+                           (int64_t)t * stride + (int64_t)h * kRopeD, stride, kv ? p.src_dtype : SCKV_DTYPE_F32);
     t += n_new;
   }
 }
@@ -750,7 +750,7 @@ int rope_tokens(int num_sms, int n_tokens) {
 
 extern "C" size_t sckv_append_rope_axes_workspace_bytes(const sckv_pool* p, int n_tokens) {
   if (p == nullptr || n_tokens <= 0 || p->kv_dtype != SCKV_DTYPE_FP8_E4M3) return 0;
-  return (size_t)n_tokens * p->num_kv_heads * p->head_dim * 2;
+  return (size_t)n_tokens * p->num_kv_heads * p->head_dim * sizeof(float);
 }
 
 extern "C" int sckv_append_rope_axes(sckv_pool* p, int layer, const void* q, int64_t q_stride, void* q_out,
@@ -795,7 +795,7 @@ extern "C" int sckv_append_rope_axes(sckv_pool* p, int layer, const void* q, int
   a.src_dtype = src_dtype;
   a.q_out = q_out;
   a.q_out_dtype = q_out_dtype;
-  a.k_stage = reinterpret_cast<__half*>(workspace);
+  a.k_stage = reinterpret_cast<float*>(workspace);
   a.q_w = reinterpret_cast<const __half*>(q_norm_w);
   a.k_w = reinterpret_cast<const __half*>(k_norm_w);
   a.eps = eps;

@@ -7,8 +7,9 @@ import pytest
 import torch
 
 from stub_model import CFG, TorchStubModel, make_weights, prompts
-from synapcore_b200 import ContinuousBatchScheduler, PagedKVCache
+from synapcore_b200 import ContinuousBatchScheduler, KVPool, PagedKVCache, rope_inv_freq
 from synapcore_b200 import _native as N
+from test_gpu_tree import gen, rope_reference, tables, values
 
 pytestmark = pytest.mark.gpu
 
@@ -70,3 +71,31 @@ def test_scheduler_drafts_less_when_pages_are_few(cuda_device):
     got, s = run(Flat(), 5)
     assert got == plain and s.drafted_tokens > 0
     assert run(Flat(), 64)[1].drafted_tokens > s.drafted_tokens
+
+
+# ---------------------------------------------------------- e4m3 page scales
+@pytest.mark.parametrize("src", [torch.bfloat16, torch.float32])
+def test_append_rope_axes_fp8_keeps_keys_past_f16(cuda_device, src):
+    """A key beyond f16's range (1e6 here) enters an FP8 pool with its value, rounded once."""
+    dev, g = cuda_device, gen(3, cuda_device)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    T, hq, hkv = 21, 4, 2
+    bt, pages = tables([T], dev, 2)
+    pool = KVPool(1, hkv, D, pages, "fp8_e4m3", device=dev)
+    x = (1e6 * torch.randn(T, hq + 2 * hkv, D, generator=g, device=dev)).to(src)
+    freq, axis = rope_inv_freq(1e4, D, dev), torch.zeros(64, dtype=torch.int32, device=dev)
+    pos = torch.arange(T, dtype=torch.int32, device=dev)
+    pool.append_rope_axes(0, x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:], pos, axis, i32([0, T]), i32([0]), bt, freq)
+    pool.raise_on_status()
+    k, size = rope_reference(x[:, hq:hq + hkv], None, 0.0, pos[None], axis, freq, 1.0)
+    ref = [(k, size), (x[:, hq + hkv:].double(), torch.zeros_like(size))]
+    now = values(pool)[0]
+    for t in range(T):
+        pg, sl = int(bt[0, t // 16]), t % 16
+        for kv, (want, size) in enumerate(ref):
+            # e4m3: half a step of the value (2^-4) or of the smallest code (2^-10 of a scale unit), 2^-23 of the
+            # division; the rotation: a few fp32 steps of the row's size
+            s = pool.scale_view()[0, pg, kv].double()[:, None]
+            assert torch.isfinite(s).all()
+            err, tol = (now[pg, kv, :, sl] - want[t]).abs(), 80 * 2.0 ** -24 * size[t]
+            assert (err <= 1.001 * tol + (2.0 ** -4 + 2.0 ** -20) * want[t].abs() + s * 2.0 ** -10).all()

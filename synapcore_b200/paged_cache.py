@@ -17,7 +17,7 @@ reads on the decode path).
 """
 from __future__ import annotations
 
-from typing import Dict, Hashable, List, Optional, Sequence, Tuple
+from typing import Dict, Hashable, List, Optional, Sequence, Set, Tuple
 
 import torch
 
@@ -57,6 +57,11 @@ class PagedKVCache:
         self.seq_at: List[Hashable] = []       # row -> sequence id
         self._arange = torch.arange(self.max_seqs + 1, dtype=torch.int32, device=self.device)
         self._tree: Optional[List[int]] = None  # nodes per row of a tree step between begin_tree and commit_tree
+        # e4m3 pools, while a step is open: the last, partly filled pages (ids, codes, scales) before it, the nodes'
+        # K and V rows float32 [2, L, total, Hkv, D], and the layers that have theirs
+        self._tree_pages: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None
+        self._tree_kv: Optional[torch.Tensor] = None
+        self._tree_layers: Set[int] = set()
 
     # ------------------------------------------------------------------ rows
     @property
@@ -408,7 +413,12 @@ class PagedKVCache:
         committed lengths [n] that the step's calls take. Closed by
         commit_tree; until then the rows cannot change otherwise. Raises
         SCKVPoolExhausted, with everything as it was, when the pool has too few
-        pages (it reads the allocation's outcome when pages are needed)."""
+        pages (it reads the allocation's outcome when pages are needed).
+
+        On FP8 pools the nodes share their page's scale, with each other and
+        with the committed tokens of a partly filled page, while the step is
+        open; commit_tree undoes that. For it, those pages are copied here and
+        append_tree and append_tree_rope keep the nodes' rows (float32)."""
         nodes = [int(n) for n in n_nodes]
         if not 0 < len(nodes) <= self.n_live or min(nodes) < 0:
             raise ValueError("begin_tree needs one node count >= 0 for each of rows 0..n-1")
@@ -420,7 +430,25 @@ class PagedKVCache:
         for n in nodes:
             cu.append(cu[-1] + n)
         meta = to_device(cu + self.lengths[:len(nodes)], torch.int32, self.device)
+        if self.pool.kv_dtype == "fp8_e4m3":
+            part = [r for r, n in enumerate(nodes) if n and self.lengths[r] % PAGE_TOKENS]
+            ids = torch.zeros(0, dtype=torch.int64, device=self.device)
+            if part:
+                at = to_device([part, [self.lengths[r] // PAGE_TOKENS for r in part]], torch.int64, self.device)
+                ids = self.block_table[at[0], at[1]].long()
+            self._tree_pages = ids, self._words()[:, ids], self.pool.scale_view()[:, ids]
+            self._tree_kv = torch.empty(2, self.num_layers, cu[-1], self.num_kv_heads, self.head_dim,
+                                        dtype=torch.float32, device=self.device)
         return meta[:len(cu)], meta[len(cu):]
+
+    def _words(self) -> torch.Tensor:
+        """The pool's codes, eight to an element: int64 [L, P, 2, H, 16, D / 8]."""
+        return self.pool.pool_view().view(torch.int64)
+
+    def _keeps_rows(self) -> bool:
+        """Whether the appends of a step keep their rows (a captured one does
+        not: its replays would write to rows of a closed step)."""
+        return self._tree_kv is not None and not torch.cuda.is_current_stream_capturing()
 
     def _open_tree(self) -> int:
         if self._tree is None:
@@ -433,6 +461,13 @@ class PagedKVCache:
         cached (rotated already), at slots length + node."""
         n = self._open_tree()
         self.pool.append(k, v, cu_tokens, ctx_lens, self.block_table[:n], layer0=layer, max_blocks=self.max_blocks)
+        if self._keeps_rows():
+            total = self._tree_kv.shape[2]
+            k, v = (x if x.dim() == 4 else x[None] for x in (k, v))
+            layers = range(layer, layer + k.shape[0])
+            for rows, x in zip(self._tree_kv, (k, v)):
+                rows[layers.start:layers.stop].copy_(x[:, :total])
+            self._tree_layers.update(layers)
 
     def append_tree_rope(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                          positions: torch.Tensor, axis_map: torch.Tensor, cu_tokens: torch.Tensor,
@@ -441,8 +476,23 @@ class PagedKVCache:
         nodes first (KVPool.append_rope_axes, whose keywords it takes);
         returns the rotated q."""
         n = self._open_tree()
-        return self.pool.append_rope_axes(layer, q, k, v, positions, axis_map, cu_tokens, ctx_lens,
-                                          self.block_table[:n], inv_freq, max_blocks=self.max_blocks, **kw)
+        ws = None
+        if self._keeps_rows():  # the call leaves the rotated k in its workspace
+            total, nt = self._tree_kv.shape[2], k.shape[0]
+            mine = self._tree_kv[0, layer] if 0 <= layer < self.num_layers and nt == total else None
+            ws = (mine if mine is not None and nt > 0 else
+                  torch.empty(max(nt, 1), self.num_kv_heads, self.head_dim, dtype=torch.float32, device=self.device))
+            kw["workspace"] = ws.view(torch.uint8).view(-1)
+        out = self.pool.append_rope_axes(layer, q, k, v, positions, axis_map, cu_tokens, ctx_lens,
+                                         self.block_table[:n], inv_freq, max_blocks=self.max_blocks, **kw)
+        if ws is not None:
+            stream = kw.get("stream")
+            with torch.cuda.stream(stream):  # (None: the current one)
+                if mine is None:
+                    self._tree_kv[0, layer].copy_(ws[:total])
+                self._tree_kv[1, layer].copy_(v[:total])
+            self._tree_layers.add(layer)
+        return out
 
     def tree_attention(self, layer: int, q: torch.Tensor, cu_tokens: torch.Tensor, ctx_lens: torch.Tensor,
                        tree_mask: torch.Tensor, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
@@ -458,7 +508,10 @@ class PagedKVCache:
         [n, P] and n_keep [n], int32 on the device, as verify_tree gives them)
         move next to its committed ones, the lengths advance by keep[r] (the
         same counts on the host; 0 drops the whole tree) and the pages past
-        them are released."""
+        them are released. The committed tokens' rows and those kept are then
+        what an append of the kept tokens alone leaves (FP8 pools: in layers
+        appended through this cache, outside a capture; elsewhere a page's
+        scale, and the rounding of its rows, stay those of all its nodes)."""
         n = self._open_tree()
         kept = [int(c) for c in keep]
         if len(kept) != n or path.dim() != 2 or path.shape[0] != n or n_keep.numel() != n:
@@ -466,19 +519,57 @@ class PagedKVCache:
         if any(not 0 <= c <= min(m, path.shape[1]) for c, m in zip(kept, self._tree)):
             raise ValueError("a row cannot keep more tokens than its tree or its path has")
         old = to_device(self.lengths[:n], torch.int32, self.device)
-        self.pool.compact_tree(self.block_table[:n], old, path, n_keep, max_blocks=self.max_blocks)
+        self._settle(path, n_keep, kept, old)
         rows, cols = [], []
         for r, (c, m) in enumerate(zip(kept, self._tree)):
             first, end = _ceil_div(self.lengths[r] + c, PAGE_TOKENS), _ceil_div(self.lengths[r] + m, PAGE_TOKENS)
             rows.extend([r] * (end - first))
             cols.extend(range(first, end))
             self.lengths[r] += c
-        self._tree = None
+        self._tree = self._tree_pages = self._tree_kv = None
+        self._tree_layers = set()
         if rows:
             at = to_device([rows, cols], torch.int64, self.device)
             self.pool.release_pages(self.block_table[at[0], at[1]])
             self.block_table[at[0], at[1]] = -1
         self.ctx_lens[:n].copy_(to_device(self.lengths[:n], torch.int32, self.device))
+
+    def _settle(self, path: torch.Tensor, n_keep: torch.Tensor, kept: Sequence[int], old: torch.Tensor) -> None:
+        """The accepted rows to their places, in every layer: moved, or, in
+        layers of an FP8 pool whose rows were kept, appended once more to the
+        pages as they were before the step (what an append of the accepted
+        tokens alone gives, bit for bit)."""
+        n, bt = len(kept), self.block_table[:len(kept)]
+        runs: List[List[int]] = []  # [first layer, end, rows were kept] of consecutive layers alike
+        for l in range(self.num_layers):
+            if runs and runs[-1][2] == (l in self._tree_layers):
+                runs[-1][1] = l + 1
+            else:
+                runs.append([l, l + 1, l in self._tree_layers])
+        if not self._tree_layers:
+            self.pool.compact_tree(bt, old, path, n_keep, max_blocks=self.max_blocks)
+            return
+        # (a path that is none is reported by the move; one layer's does where no other needs it)
+        moved = [(a, b) for a, b, again in runs if not again] or [(runs[0][0], runs[0][0] + 1)]
+        for a, b in moved:
+            self.pool.compact_tree(bt, old, path, n_keep, layer0=a, n_layers=b - a, max_blocks=self.max_blocks)
+        ids, words, scales = self._tree_pages
+        src = cu = None
+        if any(kept):
+            at = to_device([[r for r, c in enumerate(kept) for _ in range(c)], [j for c in kept for j in range(c)],
+                            [sum(self._tree[:r]) for r, c in enumerate(kept) for _ in range(c)],
+                            [self._tree[r] - 1 for r, c in enumerate(kept) for _ in range(c)]], torch.int64,
+                           self.device)
+            src = at[2] + torch.minimum(path[at[0], at[1]].long().clamp_min(0), at[3])
+            cu = to_device([sum(kept[:r]) for r in range(n + 1)], torch.int32, self.device)
+        for a, b, again in runs:
+            if not again:
+                continue
+            self._words()[a:b, ids] = words[a:b]
+            self.pool.scale_view()[a:b, ids] = scales[a:b]
+            if src is not None:
+                k, v = (x[a:b, src] for x in self._tree_kv)
+                self.pool.append(k, v, cu, old, bt, layer0=a, max_blocks=self.max_blocks)
 
     # ------------------------------------------------------ sharing / fork
     def share_prefix(self, seq_id: Hashable, page_ids: Sequence[int]) -> None:

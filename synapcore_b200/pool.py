@@ -687,7 +687,8 @@ class KVPool:
                          rope_scaling: float = 1.0, q_norm_w: Optional[torch.Tensor] = None,
                          k_norm_w: Optional[torch.Tensor] = None, eps: float = 1e-6,
                          q_out: Optional[torch.Tensor] = None, q_out_dtype: Optional[torch.dtype] = None,
-                         max_blocks: Optional[int] = None, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+                         max_blocks: Optional[int] = None, stream: Optional[torch.cuda.Stream] = None,
+                         workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
         """append_rope with positions of their own: rotary frequency i of token
         t turns by positions[axis_map[i], t] (int32 [A, n_tokens]; axis_map
         int32 [D / 2], see rope_axis_map), while its K/V row goes to slot
@@ -695,7 +696,10 @@ class KVPool:
         for tree nodes, whose position is their depth. q [n_tokens, Hq, D],
         k_new / v_new [n_tokens, Hkv, D] may be slices of one projection
         (heads packed); per-head norms (fp16 weights of D elements) only.
-        Returns the rotated q. Every pool type."""
+        Returns the rotated q. Every pool type. workspace (uint8, FP8 pools
+        only): append_rope_axes_workspace_bytes bytes, which hold the rotated
+        k, float32 [n_tokens, Hkv, D], afterwards; not shared by calls that
+        overlap on the GPU."""
         dev, kv_shape = self.device, k_new.shape
         if q.dim() != 3 or len(kv_shape) != 3 or v_new.dim() != 3:
             raise ValueError("q, k_new and v_new must be [n_tokens, heads, D]")
@@ -744,8 +748,12 @@ class KVPool:
                     raise ValueError("q_out must have q's shape")
             need, ws = 0, None
             if self.kv_dtype == "fp8_e4m3":
-                need = int(self.lib.sckv_append_rope_axes_workspace_bytes(self.handle, nt))
-                ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+                need = self.append_rope_axes_workspace_bytes(nt)
+                if workspace is not None:
+                    _need(workspace, "workspace", dev, torch.uint8, min_numel=need)
+                    ws = workspace
+                else:
+                    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
             N.check(self.lib.sckv_append_rope_axes(
                 self.handle, layer, q.data_ptr(), q_ld, q_out.data_ptr(), hq, torch_dtype_code(q.dtype),
                 torch_dtype_code(q_out.dtype), k_new.data_ptr(), k_ld, v_new.data_ptr(), v_ld,
@@ -754,6 +762,9 @@ class KVPool:
                 cu_tokens.data_ptr(), start_pos.data_ptr(), bt.data_ptr(), bt.stride(0), mb, _ptr(ws), need,
                 self._here(stream)), "sckv_append_rope_axes")
         return q_out
+
+    def append_rope_axes_workspace_bytes(self, n_tokens: int) -> int:
+        return int(self.lib.sckv_append_rope_axes_workspace_bytes(self.handle, n_tokens))
 
     def compact_tree(self, block_table: torch.Tensor, ctx_lens: torch.Tensor, path: torch.Tensor,
                      n_keep: torch.Tensor, layer0: int = 0, n_layers: Optional[int] = None,

@@ -273,8 +273,10 @@ class ContinuousBatchScheduler:
     the model together (attn_in sees their positions), the accepted path's
     tokens and the one after it are emitted, and the other nodes' rows are
     dropped. The tokens are those of one-by-one greedy decoding, up to the
-    rounding of a differently batched pass; a step's accepted_tokens lists
-    them (emitted_tokens has the last). Where the pool has too few pages for
+    rounding of a differently batched pass (on FP8 pools the nodes of a page
+    share its scale while they are checked; what is kept is then stored as if
+    it had come alone); a step's accepted_tokens lists them (emitted_tokens has
+    the last). Where the pool has too few pages for
     all drafts, a step takes those that need no more than its last tokens do.
     Not together with capture_decode."""
 

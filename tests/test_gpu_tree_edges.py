@@ -3,6 +3,8 @@ rejected nodes, values past f16, infinite values, fp32 outputs, repeated calls.
 
 Tolerances count roundings, half a step each, as in test_gpu_tree.
 """
+import math
+
 import pytest
 import torch
 
@@ -99,3 +101,180 @@ def test_append_rope_axes_fp8_keeps_keys_past_f16(cuda_device, src):
             assert torch.isfinite(s).all()
             err, tol = (now[pg, kv, :, sl] - want[t]).abs(), 80 * 2.0 ** -24 * size[t]
             assert (err <= 1.001 * tol + (2.0 ** -4 + 2.0 ** -20) * want[t].abs() + s * 2.0 ** -10).all()
+
+
+def _fp8_cache(dev, ctx, L=2, H=2, pages=64):
+    g = gen(13, dev)
+    c = PagedKVCache(L, H, D, pages, len(ctx) + 1, 12, "fp8_e4m3", device=dev)
+    for i, n in enumerate(ctx):
+        c.add_sequence(i)
+        if n:
+            c.append_prefill(i, *(torch.randn(L, n, H, D, generator=g, device=dev).half() for _ in range(2)))
+    return c
+
+
+def _page_bytes(c):
+    """Codes and scales of every row's pages, in order of the table."""
+    out = []
+    for s in range(c.n_live):
+        ids = torch.tensor(c.page_ids(s), dtype=torch.int64, device=c.device)
+        out.append((c.pool.pool_view()[:, ids].clone(), c.pool.scale_view()[:, ids].clone()))
+    return out
+
+
+@pytest.mark.parametrize("size", [40.0, 1e5, math.inf, math.nan])
+@pytest.mark.parametrize("rope", [False, True])
+def test_fp8_rows_survive_rejected_nodes_bit_for_bit(cuda_device, size, rope):
+    """Nodes of any size in a row's last page, none accepted: codes and scales of the committed pages are as before."""
+    dev, g = cuda_device, gen(14, cuda_device)
+    ctx, n = [14, 33, 16, 0, 47], [9, 20, 3, 5, 1]
+    c = _fp8_cache(dev, ctx)
+    before, free = _page_bytes(c), c.pool.alloc_state()["free"]
+    freq, axis = rope_inv_freq(1e4, D, dev), torch.zeros(64, dtype=torch.int32, device=dev)
+    cu, ctx_d = c.begin_tree(n)
+    T = sum(n)
+    for l in range(2):
+        x = torch.randn(T, 8, D, generator=g, device=dev)
+        x[::2] *= size
+        x = x.bfloat16()
+        if rope:
+            c.append_tree_rope(l, x[:, :4], x[:, 4:6], x[:, 6:], torch.zeros(T, dtype=torch.int32, device=dev), axis, cu,
+                               ctx_d, freq)
+        else:
+            c.append_tree(l, x[:, 4:6].contiguous(), x[:, 6:].contiguous(), cu, ctx_d)
+    none = torch.zeros(len(n), dtype=torch.int32, device=dev)
+    c.commit_tree(none[:, None], none, [0] * len(n))
+    c.check()
+    assert c.lengths == ctx and c.pool.alloc_state()["free"] == free
+    for (codes, scales), (b_codes, b_scales), m in zip(_page_bytes(c), before, ctx):
+        assert torch.equal(scales, b_scales)
+        assert torch.equal(codes.permute(0, 2, 3, 1, 4, 5).reshape(2, 2, 2, -1, D)[:, :, :, :m],
+                           b_codes.permute(0, 2, 3, 1, 4, 5).reshape(2, 2, 2, -1, D)[:, :, :, :m])
+
+
+@pytest.mark.parametrize("src", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rope", [False, True])
+def test_fp8_commit_equals_an_append_of_the_accepted_rows(cuda_device, src, rope):
+    """Codes and scales after a step are those of appending the accepted tokens alone, whatever the others held."""
+    dev, g = cuda_device, gen(15, cuda_device)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    ctx, n = [14, 33, 16, 0, 47, 5], [30, 20, 3, 40, 1, 2]
+    paths = [[0, 3, 4, 17, 29], [0], [0, 2], list(range(0, 40, 2)), [], [0, 1]]
+    a, b = _fp8_cache(dev, ctx), _fp8_cache(dev, ctx)
+    cu, ctx_d = a.begin_tree(n)
+    T = sum(n)
+    first = [sum(n[:r]) for r in range(len(n))]
+    rows = torch.tensor([first[r] + j for r, p in enumerate(paths) for j in p], dtype=torch.int64, device=dev)
+    keep = [len(p) for p in paths]
+    kcu = i32([sum(keep[:r]) for r in range(len(n) + 1)])
+    freq, axis = rope_inv_freq(1e4, D, dev), torch.zeros(64, dtype=torch.int32, device=dev)
+    pos = torch.randint(0, 500, (T,), generator=g, device=dev, dtype=torch.int32)
+    kept = torch.zeros(T, dtype=torch.bool, device=dev)
+    kept[rows] = True
+    b._grow_rows(0, keep)
+    for l in range(2):
+        x = torch.randn(T, 8, D, generator=g, device=dev)
+        x[~kept] *= 300.0
+        x = x.to(src)
+        k, v = x[:, 4:6], x[:, 6:]
+        if rope:
+            a.append_tree_rope(l, x[:, :4], k, v, pos, axis, cu, ctx_d, freq)
+            b.pool.append_rope_axes(l, x[rows, :4], k[rows], v[rows], pos[rows], axis, kcu, ctx_d, b.block_table[:len(n)],
+                                    freq)
+        else:
+            a.append_tree(l, k.contiguous(), v.contiguous(), cu, ctx_d)
+            b.pool.append(k[rows], v[rows], kcu, ctx_d, b.block_table[:len(n)], layer0=l)
+        x.fill_(7.0)  # the caller's buffers are its own again
+    P = max(keep)
+    a.commit_tree(i32([p + [-1] * (P - len(p)) for p in paths]), i32(keep), keep)
+    a.check()
+    b.check()
+    for r in range(len(n)):
+        b.lengths[r] += keep[r]
+    assert a.lengths == b.lengths
+    for (ca, sa), (cb, sb), m in zip(_page_bytes(a), _page_bytes(b), a.lengths):
+        assert torch.equal(sa, sb)
+        rows = [x.permute(0, 2, 3, 1, 4, 5).reshape(2, 2, 2, -1, D)[:, :, :, :m] for x in (ca, cb)]
+        assert torch.equal(*rows)
+
+
+def test_fp8_commit_reports_a_bad_path(cuda_device):
+    """A path out of range is reported and reads nothing out of bounds."""
+    dev = cuda_device
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    for path in ([[0, 900]], [[0, -5]], [[3, 2]], [[0, 2 ** 31 - 1]]):
+        c = _fp8_cache(dev, [20])
+        cu, ctx = c.begin_tree([4])
+        k = torch.randn(4, 2, D, device=dev).half()
+        for l in range(2):
+            c.append_tree(l, k, k, cu, ctx)
+        c.commit_tree(i32(path), i32([2]), [2])
+        assert c.pool.status()[0] == N.SCKV_ERR_BOUNDS and c.lengths == [22]
+        c.pool.clear_status()
+
+
+def test_fp8_commit_of_some_layers(cuda_device):
+    """A step over the first layers only leaves the others' pages alone."""
+    dev, g = cuda_device, gen(16, cuda_device)
+    c = _fp8_cache(dev, [20, 7], L=3)
+    before = _page_bytes(c)
+    cu, ctx = c.begin_tree([4, 6])
+    k, v = (torch.randn(10, 2, D, generator=g, device=dev).half() for _ in range(2))
+    for l in range(2):
+        c.append_tree(l, k, v, cu, ctx)
+    path = torch.tensor([[0, 3], [0, 2]], dtype=torch.int32, device=dev)
+    c.commit_tree(path, torch.tensor([2, 1], dtype=torch.int32, device=dev), [2, 1])
+    c.check()
+    assert c.lengths == [22, 8]
+    for (codes, scales), (b_codes, b_scales), m in zip(_page_bytes(c), before, (20, 7)):
+        rows = [x[2].permute(1, 2, 0, 3, 4).reshape(2, 2, -1, D)[:, :, :m] for x in (codes, b_codes)]
+        assert torch.equal(*rows) and torch.equal(scales[2], b_scales[2])
+    got = c.gather(0, torch.float32)[0]
+    for at, node in ((20, 0), (21, 3)):
+        for l in range(2):
+            # one rounding of e4m3 (2^-4, or half the smallest code's 2^-9 of the page's scale unit)
+            want = k[node].float()
+            assert ((got[l, :, at] - want).abs() <= 2.0 ** -4 * want.abs() + 5.0 / 448 * 2.0 ** -10).all()
+
+
+@pytest.mark.parametrize("rope", [False, True])
+def test_fp8_step_of_a_padded_batch_and_of_a_capture(cuda_device, rope):
+    """Rows behind the last node are nobody's; a captured append leaves its rows to the move."""
+    dev, g = cuda_device, gen(17, cuda_device)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    freq, axis = rope_inv_freq(1e4, D, dev), torch.zeros(64, dtype=torch.int32, device=dev)
+    x = torch.randn(9, 8, D, generator=g, device=dev).half()
+    pos, path = torch.zeros(9, dtype=torch.int32, device=dev), i32([[0, 2], [1, -1]])
+
+    def step(c, captured):
+        cu, ctx = c.begin_tree([4, 2])
+
+        def append():
+            for l in range(2):
+                if rope:
+                    c.append_tree_rope(l, x[:, :4], x[:, 4:6], x[:, 6:], pos, axis, cu, ctx, freq)
+                else:
+                    c.append_tree(l, x[:, 4:6].contiguous(), x[:, 6:].contiguous(), cu, ctx)
+
+        if captured:
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                append()
+            graph.replay()
+            assert not c._tree_layers
+        else:
+            append()
+        c.commit_tree(path, i32([2, 1]), [2, 1])
+        c.check()
+        torch.cuda.synchronize()
+        return [c.gather(s, torch.float32) for s in range(2)]
+
+    a, b = (step(_fp8_cache(dev, [20, 5]), captured) for captured in (False, True))
+    for s, rows in ((0, [0, 2]), (1, [5])):  # (positions of 0: the rotation changes nothing)
+        for kv, col in ((0, slice(4, 6)), (1, slice(6, 8))):
+            want = x[rows][:, col].float().permute(1, 0, 2)
+            for got, n in ((a, 1), (b, 3)):
+                # e4m3: half a step (2^-4), or of the smallest code, for the append and, moved, two growths
+                new = got[s][kv][:, :, -len(rows):]
+                assert ((new - want).abs() <= n * (2.0 ** -4 * want.abs() + 6.0 / 448 * 2.0 ** -10)).all()

@@ -542,7 +542,12 @@ class ContinuousBatchScheduler:
             small = meta[:2].to(torch.int32)
             mask = to_device(mask, torch.int64, self.device)
             logits = self.model.logits(self._layers(self.model.embed(meta[0]), meta[2], attend, n_layers))
-            path, keep, nxt = cache.pool.verify_tree(logits, small[0], small[1], cu, max_path=max(n))
+            marks = logits
+            if logits.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+                # (types that verify_tree does not take: only where each row's largest value is)
+                marks = torch.zeros(logits.shape, dtype=torch.float16, device=self.device)
+                marks.scatter_(1, torch.argmax(logits, dim=-1, keepdim=True), 1.0)
+            path, keep, nxt = cache.pool.verify_tree(marks, small[0], small[1], cu, max_path=max(n))
             host = torch.cat([path, keep[:, None], nxt[:, None]], dim=1).tolist()
         except BaseException:
             none = torch.zeros(B, dtype=torch.int32, device=self.device)

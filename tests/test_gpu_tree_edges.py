@@ -5,11 +5,12 @@ Tolerances count roundings, half a step each, as in test_gpu_tree.
 """
 import math
 
+import numpy as np
 import pytest
 import torch
 
 from stub_model import CFG, TorchStubModel, make_weights, prompts
-from synapcore_b200 import ContinuousBatchScheduler, KVPool, PagedKVCache, rope_inv_freq
+from synapcore_b200 import ContinuousBatchScheduler, KVPool, PagedKVCache, PromptLookupDrafter, rope_inv_freq
 from synapcore_b200 import _native as N
 from test_gpu_tree import gen, rope_reference, tables, values
 
@@ -278,3 +279,73 @@ def test_fp8_step_of_a_padded_batch_and_of_a_capture(cuda_device, rope):
                 # e4m3: half a step (2^-4), or of the smallest code, for the append and, moved, two growths
                 new = got[s][kv][:, :, -len(rows):]
                 assert ((new - want).abs() <= n * (2.0 ** -4 * want.abs() + 6.0 / 448 * 2.0 ** -10)).all()
+
+
+# ----------------------------------------------------------------- scheduler
+@pytest.mark.parametrize("drafter", ["flat", "lookup"])
+def test_engine_scheduler_with_a_drafter_says_the_same(cuda_device, drafter):
+    """A reference-style engine: its tokens with a drafter are those without."""
+    from stub_model import StubEngine
+
+    def run(d):
+        s = ContinuousBatchScheduler(StubEngine(make_weights(), "11" * 32), 4, device=cuda_device, drafter=d)
+        for i, p in enumerate(prompts()):
+            s.submit_request(f"r{i}", p, max_new_tokens=9, stop_token_ids=set())
+        steps = s.run_until_complete()
+        s.cache.check()
+        return s, steps
+
+    plain, _ = run(None)
+    s, steps = run(Flat() if drafter == "flat" else PromptLookupDrafter())
+    assert {r: q.generated_ids for r, q in s.completed_requests.items()} == \
+        {r: q.generated_ids for r, q in plain.completed_requests.items()}
+    for rid, q in s.completed_requests.items():
+        assert isinstance(q.last_logits, np.ndarray) and q.last_logits.ndim == 1
+        assert int(q.last_logits.argmax()) == q.generated_ids[-1]
+        assert [t for st in steps for t in st["accepted_tokens"].get(rid, [])] == q.generated_ids
+
+
+def test_scheduler_picks_as_the_plain_step_where_fp32_ties(cuda_device):
+    """64-bit logits that differ below fp32: the largest wins, not the first of what fp32 holds as equal."""
+    dev = cuda_device
+
+    class Close(TorchStubModel):
+        def logits(self, h):
+            x = super().logits(h).double()
+            top = x.max(-1, keepdim=True)
+            x[:, 3:4] = top.values * (1 - 1e-12 * top.values.sign())  # a hair below the largest, at a low index
+            return x
+
+    def run(d):
+        m = Close(make_weights(), dev)
+        c = PagedKVCache(CFG["num_layers"], CFG["hkv"], CFG["head_dim"], 64, 4, 16, "fp16", device=dev)
+        s = ContinuousBatchScheduler(m, c, max_batch_size=2, drafter=d)
+        s.submit_request("r", prompts()[0], max_new_tokens=6, stop_token_ids=set())
+        s.run_until_complete()
+        return s.completed_requests["r"].generated_ids
+
+    plain = run(None)
+    assert 3 not in plain and run(Flat()) == plain
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8", "fp8_e4m3"])
+def test_scheduler_with_a_drafter_on_every_pool(cuda_device, kind):
+    """Runs of every pool type end with clean pages; each emitted token is the argmax of the logits given with it."""
+    dev = cuda_device
+
+    class Typed(TorchStubModel):
+        def attn_in(self, layer, h, positions):
+            q, k, v = super().attn_in(layer, h, positions)
+            return (q.bfloat16(), k.bfloat16(), v.bfloat16()) if kind == "bf16" else (q, k, v)
+
+    model = Typed(make_weights(), dev)
+    c = PagedKVCache(CFG["num_layers"], CFG["hkv"], CFG["head_dim"], 64, 8, 16, kind, device=dev)
+    s = ContinuousBatchScheduler(model, c, max_batch_size=4, drafter=PromptLookupDrafter(ngram=1, length=4))
+    for i, p in enumerate(prompts()):
+        s.submit_request(f"r{i}", p, max_new_tokens=9, stop_token_ids=set())
+    steps = s.run_until_complete()
+    c.check()
+    assert c.n_live == 0 and c.pool.alloc_state()["allocated"] == 0
+    for rid, q in s.completed_requests.items():
+        assert len(q.generated_ids) == 9 and int(q.last_logits.argmax()) == q.generated_ids[-1]
+        assert [t for st in steps for t in st["accepted_tokens"].get(rid, [])] == q.generated_ids

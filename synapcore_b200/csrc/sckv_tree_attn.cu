@@ -69,7 +69,8 @@
 // Rows of K/V tiles past the sequence's last node hold anything: their scores
 // are masked and their V rows zeroed. A node's V that is not finite must not
 // reach rows that do not see it (0 x NaN): such elements are zeroed in the
-// tile and added to the rows that see them at the end.
+// tile and added to the rows that see them at the end. Every row sees the
+// committed tokens; there a NaN result is looked into (its sum is none).
 #include <cuda.h>
 #include <math.h>
 #include <type_traits>
@@ -1127,7 +1128,10 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
       const int d0 = two ? 0 : 64 * w, nd = two ? kHD : 64;
       const int64_t obase = ((int64_t)(s.q_base + node) * p.hq + head) * kHD;
       float* part = p.parts + (int64_t)(2 * blockIdx.x + (k > 0 ? 1 : 0)) * slot_floats(p.part_rows);
+      bool odd = false;  // this thread wrote a NaN, or infinities of both signs
       auto put4 = [&](int d, float a, float b, float c, float e) {
+        const float sum = (a + b) + (c + e);
+        odd |= sum != sum;
         if (full)
           tree_store4(p.out, obase + d, p.out_dtype, a, b, c, e);
         else
@@ -1247,6 +1251,37 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
           ++xchg;
         }
       }
+      // An infinite V of a committed token, which every row sees: 0 x Inf, of a lane that does not weigh its key (a copy's,
+      // the lo part of an exact weight, a half whose sum is nothing beside the other's), left NaN where the row's value
+      // is that infinity. Each lane looks through 4 dims of this part's committed V.
+      if (!C::kFP8 && __any_sync(0xffffffffu, valid && odd && Lsum == Lsum)) {
+        auto kind_of = [](float v) -> uint32_t { return v != v ? 4u : v == INFINITY ? 1u : v == -INFINITY ? 2u : 0u; };
+        uint32_t kinds = 0;
+        const int k1 = min((s.ka + s.nk) * kKeys, s.ctx);
+#pragma unroll 4
+        for (int key = s.ka * kKeys; key < k1; ++key) {
+          int page = __ldg(bt_row + key / SCKV_PAGE_TOKENS);
+          if (page < 0 || page >= p.g.P) page = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            kinds |= kind_of(tree_v(p.g, p.layer, page, s.h, key % SCKV_PAGE_TOKENS, 4 * lane + e)) << (4 * e);
+        }
+#pragma unroll 1
+        for (int d = d0; d < d0 + nd; ++d) {
+          uint32_t seen = (__shfl_sync(0xffffffffu, kinds, d >> 2) >> (4 * (d & 3))) & 7u;
+          if (!valid || seen == 0 || Lsum != Lsum || (R > 1 && ((d & 31) >> 2) / (8 / R) != copy)) continue;
+          float* at = part + ((int64_t)(d >> 2) * p.part_rows + r_in) * 4 + (d & 3);
+          const float x = full ? sckv_load_as_float(p.out, obase + d, p.out_dtype) : *at;
+          if (x == x) continue;
+          each_bad([&](int page, int slot) { seen |= kind_of(tree_v(p.g, p.layer, page, s.h, slot, d)); });
+          if (seen != 1u && seen != 2u) continue;
+          const float v = seen == 1u ? INFINITY : -INFINITY;
+          if (full)
+            sckv_store_from_float(p.out, obase + d, p.out_dtype, v);
+          else
+            *at = v;
+        }
+      }
       if (!full && valid && copy == 0 && (two || w == 0))
         reinterpret_cast<float2*>(part + (int64_t)p.part_rows * kHD)[r_in] = make_float2(M, Lsum);
       // the other flags were last read in the item before and are next set in the one after
@@ -1322,7 +1357,8 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const TreeParam
     for (int e = 0; e < kJoinBatch; ++e) {
       if (i0 + e >= hd.n_parts) break;
       const float2 a = s_part[(i0 + e) * kJoinRows + rl];
-      const float f = a.x == -INFINITY ? 1.f : ex2_approx(a.x - M);
+      // (at least the smallest float: an infinite sum of a part that weighs nothing stays infinite)
+      const float f = a.x == -INFINITY ? 1.f : fmaxf(ex2_approx(a.x - M), 1.17549435e-38f);
       L = fmaf(a.y, f, L);
       x0 = fmaf(v[e].x, f, x0);
       x1 = fmaf(v[e].y, f, x1);

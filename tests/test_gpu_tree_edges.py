@@ -10,9 +10,10 @@ import pytest
 import torch
 
 from stub_model import CFG, TorchStubModel, make_weights, prompts
-from synapcore_b200 import ContinuousBatchScheduler, KVPool, PagedKVCache, PromptLookupDrafter, rope_inv_freq
+from synapcore_b200 import (ContinuousBatchScheduler, KVPool, PagedKVCache, PromptLookupDrafter, rope_inv_freq,
+                            tree_mask)
 from synapcore_b200 import _native as N
-from test_gpu_tree import gen, rope_reference, tables, values
+from test_gpu_tree import fill_pool, gen, reference, rope_reference, tables, tolerance, values
 
 pytestmark = pytest.mark.gpu
 
@@ -349,3 +350,54 @@ def test_scheduler_with_a_drafter_on_every_pool(cuda_device, kind):
     for rid, q in s.completed_requests.items():
         assert len(q.generated_ids) == 9 and int(q.last_logits.argmax()) == q.generated_ids[-1]
         assert [t for st in steps for t in st["accepted_tokens"].get(rid, [])] == q.generated_ids
+
+
+# ----------------------------------------------------------------- attention
+@pytest.mark.parametrize("kind", ["fp16", "bf16", "int8"])
+@pytest.mark.parametrize("hq,hkv,ctx,nodes", [
+    (4, 2, [300], [4]),              # 8 rows: four copies in the query tile
+    (8, 2, [140, 77], [13, 9]),      # 52, 36: two
+    (8, 2, [500], [31]),             # 124: one
+    (16, 2, [400, 30], [40, 25]),    # 320, 200: two query tiles, and 64 more rows
+    (8, 1, [9000], [6]),             # one item over many SMs
+])
+def test_tree_attn_infinite_values_of_committed_tokens(cuda_device, kind, hq, hkv, ctx, nodes):
+    """A committed V of +inf, -inf, both or NaN gives every row that, in its dim alone."""
+    dev = cuda_device
+    bt, pages = tables([c + n for c, n in zip(ctx, nodes)], dev, 1)
+    pool = KVPool(1, hkv, D, pages, kind, device=dev)
+    fill_pool(pool, gen(1, dev))
+
+    def put(b, pos, d, x):
+        page, slot = int(bt[b, pos // 16]), pos % 16
+        if kind == "int8":  # code * scale past f16's range; the row's other codes are 0
+            pool.pool_view()[0, page, 1, :, slot] = 0
+            pool.scale_view()[0, page, 1, :, slot] = 60000.0
+            pool.pool_view()[0, page, 1, :, slot, d] = 100 if x > 0 else -100
+        else:
+            pool.pool_view()[0, page, 1, :, slot, d] = x
+
+    inf = math.inf
+    for b, c in enumerate(ctx):
+        put(b, c // 2, 5, inf)
+        put(b, c - 1, 70, -inf)
+        put(b, 0, 71, inf)
+        put(b, 1, 71 if c > 30 else 72, -inf)
+        if kind != "int8":
+            put(b, 2, 100, math.nan)
+            put(b, c + 1, 5, -inf)     # a node's: rows that see it have both signs
+            put(b, c + 1, 120, inf)
+    cu = [sum(nodes[:i]) for i in range(len(nodes) + 1)]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    mask = tree_mask([[-1] + [i // 2 for i in range(n - 1)] for n in nodes], dev)[0]
+    qt = torch.bfloat16 if kind == "bf16" else torch.float16
+    q = torch.randn(cu[-1], hq, D, generator=gen(2, dev), device=dev).to(qt)
+    ref, absum, big = reference(values(pool), 0, q, cu, ctx, bt, mask, D ** -0.5)
+    assert ref.isinf().any() and ref.isnan().any()
+    for out_dtype in (qt, torch.float32):
+        out = pool.tree_attn(0, q, i32(cu), i32(ctx), bt, mask, out_dtype=out_dtype).double()
+        pool.raise_on_status()
+        assert torch.equal(out.isnan(), ref.isnan())
+        assert torch.equal(out.isinf(), ref.isinf()) and torch.equal(out[ref.isinf()], ref[ref.isinf()])
+        ok = torch.isfinite(ref)
+        assert ((out - ref).abs()[ok] <= tolerance(kind, qt, out_dtype, ref, absum, big)[ok]).all()

@@ -362,8 +362,11 @@ SCKV_API size_t sckv_o_proj_workspace_bytes(const sckv_pool* pool,
  * (reported in the status word, kernel id 18). All pool types, any group size
  * num_q_heads / num_kv_heads up to 4,095; head_dim 128, at most 2,048
  * sequences and 2^31 - 1 tiles of 128 keys over all heads and groups of rows,
- * else SCKV_ERR_UNSUPPORTED. fp32 accumulation. workspace: sckv_tree_attn_workspace_bytes(...) bytes of device
- * memory, 16-byte aligned, not shared by calls that overlap on the GPU. */
+ * else SCKV_ERR_UNSUPPORTED. fp32 accumulation; the weights enter their product
+ * with V rounded by at most 2^-16 (bf16 pools), 2^-22 (fp32 outputs) or 2^-11
+ * (16-bit outputs of other pools). int8 codes stand for fp16(code * scale).
+ * workspace: sckv_tree_attn_workspace_bytes(...) bytes of device memory, 16-byte
+ * aligned, not shared by calls that overlap on the GPU. */
 SCKV_API int sckv_tree_attn(sckv_pool* pool, int layer, const void* q, int q_dtype,
                    int num_q_heads, int n_seqs, int n_tokens,
                    const int32_t* cu_q, const int32_t* ctx_lens,

@@ -101,7 +101,7 @@ struct sckv_pool {
   int tmap2_ready;
   // A fourth map with whole 16-bit page-heads in 8-row groups (tree attention).
   alignas(64) unsigned char tmap_tree[128];
-  int tree_smem_ready;
+  int tree_smem_ready;  // bit per tree attention kernel whose shared memory was set
   int tmap_tree_ready;
 };
 

@@ -62,9 +62,16 @@
 //
 // P is held as 2^6 times the weight, so that f16's smallest step is 2^-31 of
 // a weight of 1 (m is stale by at most 2^8: P <= 2^14); e4m3 pages multiply it
-// by their V scale over a reference that has seen the largest one. bf16 pools
-// split P into bf16 hi + lo parts (rounding 2^-16); f16 P rounds by 2^-11 at
-// most, as the 16-bit output does. Sums, references and O are fp32.
+// by their V scale over a reference that has seen the largest one. P is split
+// into hi + lo parts on bf16 pools (rounding 2^-16) and for fp32 outputs (f16:
+// 2^-22), which costs a second P V product. For 16-bit outputs the other pools
+// have one f16 part, 2^-11 at most: an eighth of a bf16 output's own step.
+// Beside an f16 output's it shows (32 x 4,096 tokens against 64 bits: 2.8e-4,
+// the output's rounding alone 2.1e-4); two parts cost 187 us instead of 172
+// there, 786 instead of 661 (FP8) and 75 instead of 66 (int8). Sums, references
+// and O are fp32. int8 codes stand for fp16(code x scale), as the arena's
+// dequantisation, gather and the prefill kernel have them (one-token decode
+// multiplies in fp32: a difference of 2^-11 of a value at most).
 //
 // Rows of K/V tiles past the sequence's last node hold anything: their scores
 // are masked and their V rows zeroed. A node's V that is not finite must not
@@ -350,11 +357,13 @@ __device__ __forceinline__ void reg_give() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-template <int KVDT>
+// kSplit: the weights P in two parts (hi + lo) in tensor memory.
+template <int KVDT, bool kSplit>
 __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
     tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap tmap) {
   using C = TreeCfg<KVDT>;
   constexpr bool kBF16 = C::kBF16;
+  static_assert(kSplit || !kBF16, "one bf16 part would round a weight by 2^-9");
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   // barriers, as shared-memory addresses (8 bytes each)
@@ -698,7 +707,7 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
         // B = V rows of page pg: 128 dims in two 64-dim halves (LBO), 16 keys in two 8-row groups (SBO)
         const uint64_t bdesc = desc_advance(vd, (uint32_t)(pg * kPageTile));
         umma_ts(o, pa + (uint32_t)(pg * 8), bdesc, kIdescPV, (!first || pg > 0) ? 1u : 0u);
-        if (kBF16) umma_ts(o, pa + (uint32_t)(pg * 8 + 32), bdesc, kIdescPV, 1u);
+        if (kSplit) umma_ts(o, pa + (uint32_t)(pg * 8 + 32), bdesc, kIdescPV, 1u);
       }
     };
     TreeSeg s;
@@ -1015,17 +1024,29 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
                 f32x2_split(fma_f32x2(f32x2(sv[16 * q + 2 * d], sv[16 * q + 2 * d + 1]), scale2, negm2), x0, x1);
                 const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
                 ls2 = add_f32x2(ls2, f32x2(p0, p1));
-                ph[d] = C::kFP8 ? mul_pack2<false>(p0, p1, v2) : pack2<kBF16>(p0, p1);
-                if (kBF16) {
-                  // lo = p - bf16(p), exact
-                  const uint64_t hi2 = f32x2(__uint_as_float(ph[d] << 16), __uint_as_float(ph[d] & 0xFFFF0000u));
+                uint64_t w2 = f32x2(p0, p1);
+                if (C::kFP8) w2 = mul_f32x2(w2, v2);
+                float w0, w1;
+                f32x2_split(w2, w0, w1);
+                ph[d] = pack2<kBF16>(w0, w1);
+                if (kSplit) {
+                  // lo = w - hi, exact
+                  float h0, h1;
+                  if (kBF16) {
+                    h0 = __uint_as_float(ph[d] << 16);
+                    h1 = __uint_as_float(ph[d] & 0xFFFF0000u);
+                  } else {
+                    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&ph[d]));
+                    h0 = h.x;
+                    h1 = h.y;
+                  }
                   float l0, l1;
-                  f32x2_split(fma_f32x2(hi2, minus1, f32x2(p0, p1)), l0, l1);
-                  plo[d] = pack2<true>(l0, l1);
+                  f32x2_split(fma_f32x2(f32x2(h0, h1), minus1, w2), l0, l1);
+                  plo[d] = pack2<kBF16>(l0, l1);
                 }
               }
               tmem_st8(pc + 8 * (copy * kPg + q), ph);
-              if (kBF16) tmem_st8(pc + 32 + 8 * (copy * kPg + q), plo);
+              if (kSplit) tmem_st8(pc + 32 + 8 * (copy * kPg + q), plo);
             }
             if constexpr (R > 1) {  // the keys of the other copies
               const uint32_t z[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
@@ -1033,7 +1054,7 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
               for (int q = 0; q < kHalfPages - kPg; ++q) {
                 const int pg = q < copy * kPg ? q : q + kPg;
                 tmem_st8(pc + 8 * pg, z);
-                if (kBF16) tmem_st8(pc + 32 + 8 * pg, z);
+                if (kSplit) tmem_st8(pc + 32 + 8 * pg, z);
               }
             }
           }
@@ -1406,19 +1427,19 @@ int tree_part_rows(const sckv_pool* p, int n_tokens, int mask_words, int G) {
 
 size_t tree_head_bytes(const sckv_pool* p) { return ((size_t)p->num_sms * sizeof(JoinHead) + 255) / 256 * 256; }
 
-template <int KVDT>
+template <int KVDT, bool kSplit>
 int launch_tree(sckv_pool* p, const TreeParams& t, cudaStream_t stream) {
   using C = TreeCfg<KVDT>;
   const int rc = C::kB8 ? ensure_tmap(p, 1, p->tmap_kv1, &p->tmap1_ready) : ensure_tree_tmap(p);
   if (rc != SCKV_OK) return rc;
   const CUtensorMap* map = reinterpret_cast<const CUtensorMap*>(C::kB8 ? p->tmap_kv1 : p->tmap_tree);
-  auto kern = tree_attn_kernel<KVDT>;
+  auto kern = tree_attn_kernel<KVDT, kSplit>;
   const int smem = C::kFixedSmem + 4 * t.n_seqs;
   static_assert(C::kFixedSmem + 4 * kMaxSeqs <= 227 * 1024, "shared memory of the largest batch");
-  if (!p->tree_smem_ready) {  // the largest batch's, once per pool (a pool has one kernel)
+  if (!(p->tree_smem_ready & (1 << kSplit))) {  // the largest batch's, once per pool and kernel
     SCKV_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          C::kFixedSmem + 4 * kMaxSeqs));
-    p->tree_smem_ready = 1;
+    p->tree_smem_ready |= 1 << kSplit;
   }
   kern<<<p->num_sms, C::kThreads, smem, stream>>>(t, *map);
   SCKV_LAUNCH_CHECK();
@@ -1489,11 +1510,15 @@ extern "C" int sckv_tree_attn(sckv_pool* p, int layer, const void* q, int q_dtyp
   t.part_rows = tree_part_rows(p, n_tokens, mask_words, G);
   SCKV_DEVICE_GUARD(p->device);
   cudaStream_t s = as_stream(stream);
+  const bool split = out_dtype == SCKV_DTYPE_F32;  // one f16 part would be all of an fp32 output's error
   switch (p->kv_dtype) {
-    case SCKV_DTYPE_F16: return launch_tree<SCKV_DTYPE_F16>(p, t, s);
-    case SCKV_DTYPE_BF16: return launch_tree<SCKV_DTYPE_BF16>(p, t, s);
-    case SCKV_DTYPE_INT8: return launch_tree<SCKV_DTYPE_INT8>(p, t, s);
-    case SCKV_DTYPE_FP8_E4M3: return launch_tree<SCKV_DTYPE_FP8_E4M3>(p, t, s);
+    case SCKV_DTYPE_F16:
+      return split ? launch_tree<SCKV_DTYPE_F16, true>(p, t, s) : launch_tree<SCKV_DTYPE_F16, false>(p, t, s);
+    case SCKV_DTYPE_BF16: return launch_tree<SCKV_DTYPE_BF16, true>(p, t, s);
+    case SCKV_DTYPE_INT8:
+      return split ? launch_tree<SCKV_DTYPE_INT8, true>(p, t, s) : launch_tree<SCKV_DTYPE_INT8, false>(p, t, s);
+    case SCKV_DTYPE_FP8_E4M3:
+      return split ? launch_tree<SCKV_DTYPE_FP8_E4M3, true>(p, t, s) : launch_tree<SCKV_DTYPE_FP8_E4M3, false>(p, t, s);
     default: return SCKV_ERR_UNSUPPORTED;
   }
 }

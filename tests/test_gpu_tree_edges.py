@@ -13,7 +13,7 @@ from stub_model import CFG, TorchStubModel, make_weights, prompts
 from synapcore_b200 import (ContinuousBatchScheduler, KVPool, PagedKVCache, PromptLookupDrafter, rope_inv_freq,
                             tree_mask)
 from synapcore_b200 import _native as N
-from test_gpu_tree import fill_pool, gen, reference, rope_reference, tables, tolerance, values
+from test_gpu_tree import KINDS, fill_pool, gen, reference, rope_reference, tables, tolerance, values
 
 pytestmark = pytest.mark.gpu
 
@@ -401,3 +401,44 @@ def test_tree_attn_infinite_values_of_committed_tokens(cuda_device, kind, hq, hk
         assert torch.equal(out.isinf(), ref.isinf()) and torch.equal(out[ref.isinf()], ref[ref.isinf()])
         ok = torch.isfinite(ref)
         assert ((out - ref).abs()[ok] <= tolerance(kind, qt, out_dtype, ref, absum, big)[ok]).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hq,hkv,ctx,nodes", [
+    (4, 4, [0, 1, 15, 16, 17, 63, 64, 65, 130, 200], [1, 2, 1, 5, 16, 17, 0, 33, 64, 3]),
+    (8, 2, [3, 77], [20, 9]),
+    (7, 1, [1, 2, 5], [13, 1, 2]),
+    (16, 2, [2, 33, 5], [40, 35, 7]),
+    (8, 1, [6000], [16]),
+])
+def test_tree_attn_fp32_outputs_have_fp32_weights(cuda_device, kind, hq, hkv, ctx, nodes):
+    """An fp32 output is not held to f16 weights (2^-11): on every pool its error is that of two-part weights."""
+    dev = cuda_device
+    bt, pages = tables([c + n for c, n in zip(ctx, nodes)], dev, 3)
+    pool = KVPool(1, hkv, D, pages, kind, device=dev)
+    fill_pool(pool, gen(4, dev))
+    cu = [sum(nodes[:i]) for i in range(len(nodes) + 1)]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    mask = tree_mask([[-1] + [i // 2 for i in range(n - 1)] if n else [] for n in nodes], dev)[0]
+    qt = torch.bfloat16 if kind == "bf16" else torch.float16
+    q = torch.randn(cu[-1], hq, D, generator=gen(5, dev), device=dev).to(qt)
+    scale = D ** -0.5 / 16  # small scores: the dot products' own rounding is below the weights'
+    vals = values(pool)
+    ref, absum, big = reference(vals, 0, q, cu, ctx, bt, mask, scale)
+    out = pool.tree_attn(0, q, i32(cu), i32(ctx), bt, mask, scale=scale, out_dtype=torch.float32)
+    pool.raise_on_status()
+    # a weight: its two parts 2^-16 (bf16; f16 2^-22), 128-term fp32 dot products, the exponential and the sums 2^-16
+    w = 2.0 ** -16 + big * 128 * 2.0 ** -24 + 2.0 ** -16
+    # and half a step of the smallest f16, 2^-25 of 2^6 times the weight, of every |v| (FP8: in units of at most
+    # four times the largest page scale)
+    floor = torch.zeros_like(ref)
+    for b, (t0, t1) in enumerate(zip(cu, cu[1:])):
+        ids = bt[b, :-(-(ctx[b] + t1 - t0) // 16)].long()
+        for h in range(hq):
+            size = vals[0, ids, 1, h // (hq // hkv)].abs().sum((0, 1))
+            if kind == "fp8_e4m3":
+                s = pool.scale_view()[0, ids, 1, h // (hq // hkv)]
+                size = size * 4 * float(s.max() / s.min()) if len(ids) else size
+            floor[t0:t1, h] = size * 2.0 ** -31
+    err, tol = (out.double() - ref).abs(), 2.0 ** -24 * ref.abs() + 2 * w * absum + floor + 1e-7
+    assert (err <= tol).all(), float((err / tol).max())

@@ -442,3 +442,36 @@ def test_tree_attn_fp32_outputs_have_fp32_weights(cuda_device, kind, hq, hkv, ct
             floor[t0:t1, h] = size * 2.0 ** -31
     err, tol = (out.double() - ref).abs(), 2.0 ** -24 * ref.abs() + 2 * w * absum + floor + 1e-7
     assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("seqs,ctx,hq,hkv", [(40, 300, 4, 2), (15, 1251, 64, 8), (3, 5000, 8, 2)])
+def test_tree_attn_repeats_itself(cuda_device, kind, seqs, ctx, hq, hkv):
+    """Shares and orders are fixed: a thousand calls give the same bits, with another stream's calls beside them."""
+    dev = cuda_device
+    r = torch.Generator().manual_seed(seqs)
+    nodes = torch.randint(1, 30, (seqs,), generator=r).tolist()
+    lens = [ctx - 3 * b for b in range(seqs)]
+    bt, pages = tables([c + n for c, n in zip(lens, nodes)], dev, 3)
+    pools = [KVPool(1, hkv, D, pages, kind, device=dev) for _ in range(2)]
+    cu = [sum(nodes[:i]) for i in range(seqs + 1)]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    mask = torch.randint(-2 ** 62, 2 ** 62, (cu[-1], 1), generator=gen(6, dev), device=dev)
+    qt = torch.bfloat16 if kind == "bf16" else torch.float16
+    args = []
+    for i, p in enumerate(pools):
+        fill_pool(p, gen(7 + i, dev))
+        q = torch.randn(cu[-1], hq, D, generator=gen(9 + i, dev), device=dev).to(qt)
+        args.append((0, q, i32(cu), i32(lens), bt, mask))
+    first = [p.tree_attn(*a) for p, a in zip(pools, args)]
+    wrong = [torch.zeros((), dtype=torch.int64, device=dev) for _ in range(2)]
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(1000):
+        for p, a, f, w, s in zip(pools, args, first, wrong, streams):
+            with torch.cuda.stream(s):
+                w += (p.tree_attn(*a, stream=s).view(torch.int16) != f.view(torch.int16)).any()
+    torch.cuda.synchronize()
+    assert [int(w) for w in wrong] == [0, 0]
+    for p in pools:
+        p.raise_on_status()

@@ -19,6 +19,7 @@ from __future__ import annotations
 
 from typing import Dict, Hashable, List, Optional, Sequence, Set, Tuple
 
+import numpy as np
 import torch
 
 from . import _native as N
@@ -58,9 +59,10 @@ class PagedKVCache:
         self._arange = torch.arange(self.max_seqs + 1, dtype=torch.int32, device=self.device)
         self._tree: Optional[List[int]] = None  # nodes per row of a tree step between begin_tree and commit_tree
         # e4m3 pools, while a step is open: the last, partly filled pages (ids, codes, scales) before it, the nodes'
-        # K and V rows float32 [2, L, total, Hkv, D], and the layers that have theirs
+        # K and V rows, float32 [2, total, Hkv, D] of each layer in one buffer, and the layers that have theirs
         self._tree_pages: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None
         self._tree_kv: Optional[torch.Tensor] = None
+        self._tree_rows: Tuple[torch.Tensor, ...] = ()
         self._tree_layers: Set[int] = set()
 
     # ------------------------------------------------------------------ rows
@@ -436,9 +438,10 @@ class PagedKVCache:
             if part:
                 at = to_device([part, [self.lengths[r] // PAGE_TOKENS for r in part]], torch.int64, self.device)
                 ids = self.block_table[at[0], at[1]].long()
-            self._tree_pages = ids, self._words()[:, ids], self.pool.scale_view()[:, ids]
-            self._tree_kv = torch.empty(2, self.num_layers, cu[-1], self.num_kv_heads, self.head_dim,
+            self._tree_pages = (ids, self._words().index_select(1, ids), self.pool.scale_view().index_select(1, ids))
+            self._tree_kv = torch.empty(self.num_layers, 2, cu[-1], self.num_kv_heads, self.head_dim,
                                         dtype=torch.float32, device=self.device)
+            self._tree_rows = self._tree_kv.unbind(0)
         return meta[:len(cu)], meta[len(cu):]
 
     def _words(self) -> torch.Tensor:
@@ -463,11 +466,11 @@ class PagedKVCache:
         self.pool.append(k, v, cu_tokens, ctx_lens, self.block_table[:n], layer0=layer, max_blocks=self.max_blocks)
         if self._keeps_rows():
             total = self._tree_kv.shape[2]
-            k, v = (x if x.dim() == 4 else x[None] for x in (k, v))
-            layers = range(layer, layer + k.shape[0])
-            for rows, x in zip(self._tree_kv, (k, v)):
-                rows[layers.start:layers.stop].copy_(x[:, :total])
-            self._tree_layers.update(layers)
+            for l, (kl, vl) in enumerate(zip(k, v) if k.dim() == 4 else ((k, v),), layer):
+                if kl.shape[0] != total:
+                    kl, vl = kl[:total], vl[:total]
+                torch.stack((kl, vl), out=self._tree_rows[l])
+                self._tree_layers.add(l)
 
     def append_tree_rope(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                          positions: torch.Tensor, axis_map: torch.Tensor, cu_tokens: torch.Tensor,
@@ -479,7 +482,7 @@ class PagedKVCache:
         ws = None
         if self._keeps_rows():  # the call leaves the rotated k in its workspace
             total, nt = self._tree_kv.shape[2], k.shape[0]
-            mine = self._tree_kv[0, layer] if 0 <= layer < self.num_layers and nt == total else None
+            mine = self._tree_rows[layer][0] if 0 <= layer < self.num_layers and nt == total else None
             ws = (mine if mine is not None and nt > 0 else
                   torch.empty(max(nt, 1), self.num_kv_heads, self.head_dim, dtype=torch.float32, device=self.device))
             kw["workspace"] = ws.view(torch.uint8).view(-1)
@@ -489,8 +492,8 @@ class PagedKVCache:
             stream = kw.get("stream")
             with torch.cuda.stream(stream):  # (None: the current one)
                 if mine is None:
-                    self._tree_kv[0, layer].copy_(ws[:total])
-                self._tree_kv[1, layer].copy_(v[:total])
+                    self._tree_rows[layer][0].copy_(ws[:total])
+                self._tree_rows[layer][1].copy_(v[:total])
             self._tree_layers.add(layer)
         return out
 
@@ -527,7 +530,7 @@ class PagedKVCache:
             cols.extend(range(first, end))
             self.lengths[r] += c
         self._tree = self._tree_pages = self._tree_kv = None
-        self._tree_layers = set()
+        self._tree_rows, self._tree_layers = (), set()
         if rows:
             at = to_device([rows, cols], torch.int64, self.device)
             self.pool.release_pages(self.block_table[at[0], at[1]])
@@ -556,19 +559,20 @@ class PagedKVCache:
         ids, words, scales = self._tree_pages
         src = cu = None
         if any(kept):
-            at = to_device([[r for r, c in enumerate(kept) for _ in range(c)], [j for c in kept for j in range(c)],
-                            [sum(self._tree[:r]) for r, c in enumerate(kept) for _ in range(c)],
-                            [self._tree[r] - 1 for r, c in enumerate(kept) for _ in range(c)]], torch.int64,
-                           self.device)
+            m, c = np.array(self._tree), np.array(kept)
+            end = c.cumsum()
+            r = np.repeat(np.arange(n), c)
+            at = to_device(torch.from_numpy(np.stack([r, np.arange(end[-1]) - (end - c)[r], (m.cumsum() - m)[r],
+                                                      m[r] - 1])), torch.int64, self.device)
             src = at[2] + torch.minimum(path[at[0], at[1]].long().clamp_min(0), at[3])
-            cu = to_device([sum(kept[:r]) for r in range(n + 1)], torch.int32, self.device)
+            cu = to_device([0, *end.tolist()], torch.int32, self.device)
         for a, b, again in runs:
             if not again:
                 continue
-            self._words()[a:b, ids] = words[a:b]
-            self.pool.scale_view()[a:b, ids] = scales[a:b]
+            self._words()[a:b].index_copy_(1, ids, words[a:b])
+            self.pool.scale_view()[a:b].index_copy_(1, ids, scales[a:b])
             if src is not None:
-                k, v = (x[a:b, src] for x in self._tree_kv)
+                k, v = (self._tree_kv[a:b, i].index_select(1, src) for i in range(2))
                 self.pool.append(k, v, cu, old, bt, layer0=a, max_blocks=self.max_blocks)
 
     # ------------------------------------------------------ sharing / fork

@@ -420,38 +420,45 @@ class PagedKVCache:
         On FP8 pools the nodes share their page's scale, with each other and
         with the committed tokens of a partly filled page, while the step is
         open; commit_tree undoes that. For it, those pages are copied here and
-        append_tree and append_tree_rope keep the nodes' rows (float32)."""
+        append_tree and append_tree_rope keep the nodes' rows (float32: 8 Hkv D
+        bytes a node and layer until then)."""
         nodes = [int(n) for n in n_nodes]
         if not 0 < len(nodes) <= self.n_live or min(nodes) < 0:
             raise ValueError("begin_tree needs one node count >= 0 for each of rows 0..n-1")
         if max(nodes) > MAX_TREE_NODES:
             raise ValueError(f"a tree has more than {MAX_TREE_NODES} nodes")
-        self._grow_rows(0, nodes, checked=True)
-        self._tree = nodes
         cu = [0]
         for n in nodes:
             cu.append(cu[-1] + n)
         meta = to_device(cu + self.lengths[:len(nodes)], torch.int32, self.device)
+        pages = kv = None
         if self.pool.kv_dtype == "fp8_e4m3":
             part = [r for r, n in enumerate(nodes) if n and self.lengths[r] % PAGE_TOKENS]
             ids = torch.zeros(0, dtype=torch.int64, device=self.device)
             if part:
                 at = to_device([part, [self.lengths[r] // PAGE_TOKENS for r in part]], torch.int64, self.device)
                 ids = self.block_table[at[0], at[1]].long()
-            self._tree_pages = (ids, self._words().index_select(1, ids), self.pool.scale_view().index_select(1, ids))
-            self._tree_kv = torch.empty(self.num_layers, 2, cu[-1], self.num_kv_heads, self.head_dim,
-                                        dtype=torch.float32, device=self.device)
-            self._tree_rows = self._tree_kv.unbind(0)
+            pages = ids, self._words().index_select(1, ids), self.pool.scale_view().index_select(1, ids)
+            kv = torch.empty(self.num_layers, 2, cu[-1], self.num_kv_heads, self.head_dim, dtype=torch.float32,
+                             device=self.device)
+        self._grow_rows(0, nodes, checked=True)  # (last: nothing is open when anything of it fails)
+        self._tree, self._tree_pages, self._tree_kv = nodes, pages, kv
+        self._tree_rows = kv.unbind(0) if kv is not None else ()
         return meta[:len(cu)], meta[len(cu):]
 
     def _words(self) -> torch.Tensor:
         """The pool's codes, eight to an element: int64 [L, P, 2, H, 16, D / 8]."""
         return self.pool.pool_view().view(torch.int64)
 
-    def _keeps_rows(self) -> bool:
-        """Whether the appends of a step keep their rows (a captured one does
-        not: its replays would write to rows of a closed step)."""
-        return self._tree_kv is not None and not torch.cuda.is_current_stream_capturing()
+    def _keeps_rows(self, k: torch.Tensor) -> bool:
+        """Whether an append of a step keeps its rows k [.., total, Hkv, D] (a
+        captured one does not: its replays would write to rows of a closed
+        step)."""
+        if self._tree_kv is None:
+            return False
+        if k.dim() >= 3 and k.shape[-3] < self._tree_kv.shape[2]:
+            raise ValueError("k, v must have a row for every node of the step")
+        return not torch.cuda.is_current_stream_capturing()
 
     def _open_tree(self) -> int:
         if self._tree is None:
@@ -463,8 +470,9 @@ class PagedKVCache:
         """One layer's K/V rows of the nodes, k, v [total, Hkv, D] as they are
         cached (rotated already), at slots length + node."""
         n = self._open_tree()
+        kept = self._keeps_rows(k)
         self.pool.append(k, v, cu_tokens, ctx_lens, self.block_table[:n], layer0=layer, max_blocks=self.max_blocks)
-        if self._keeps_rows():
+        if kept:
             total = self._tree_kv.shape[2]
             for l, (kl, vl) in enumerate(zip(k, v) if k.dim() == 4 else ((k, v),), layer):
                 if kl.shape[0] != total:
@@ -480,7 +488,7 @@ class PagedKVCache:
         returns the rotated q."""
         n = self._open_tree()
         ws = None
-        if self._keeps_rows():  # the call leaves the rotated k in its workspace
+        if self._keeps_rows(k):  # the call leaves the rotated k in its workspace
             total, nt = self._tree_kv.shape[2], k.shape[0]
             mine = self._tree_rows[layer][0] if 0 <= layer < self.num_layers and nt == total else None
             ws = (mine if mine is not None and nt > 0 else

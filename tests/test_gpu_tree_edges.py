@@ -215,6 +215,24 @@ def test_fp8_commit_reports_a_bad_path(cuda_device):
         c.pool.clear_status()
 
 
+def test_fp8_step_refuses_fewer_rows_than_nodes(cuda_device):
+    dev = cuda_device
+    c = _fp8_cache(dev, [20, 7])
+    before = _page_bytes(c)
+    cu, ctx = c.begin_tree([4, 6])
+    x = torch.randn(9, 8, D, device=dev).half()
+    axis = torch.zeros(64, dtype=torch.int32, device=dev)
+    with pytest.raises(ValueError):
+        c.append_tree(0, x[:, 4:6].contiguous(), x[:, 6:].contiguous(), cu, ctx)
+    with pytest.raises(ValueError):
+        c.append_tree_rope(0, x[:, :4], x[:, 4:6], x[:, 6:], torch.zeros(9, dtype=torch.int32, device=dev), axis, cu, ctx,
+                           rope_inv_freq(1e4, D, dev))
+    none = torch.zeros(2, dtype=torch.int32, device=dev)
+    c.commit_tree(none[:, None], none, [0, 0])
+    c.check()
+    assert all(torch.equal(a, b) for x, y in zip(_page_bytes(c), before) for a, b in zip(x, y))
+
+
 def test_fp8_commit_of_some_layers(cuda_device):
     """A step over the first layers only leaves the others' pages alone."""
     dev, g = cuda_device, gen(16, cuda_device)

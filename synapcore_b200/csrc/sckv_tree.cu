@@ -34,10 +34,11 @@ namespace {
 // of three shuffles). With q, k and v of one 16-bit type a thread has its next
 // row on the way while it works on one, the first before the angles are
 // computed and the pages looked up, and what a row needs by address is kept
-// per token. The arithmetic runs on packed pairs: issue slots are the second
-// bound. 8,192 tokens of 32 + 2 x 8 bf16 heads: 41 us, 4.9 TB/s (74 % of a
-// copy's rate); two rows on the way and CTAs of 256 threads were slower (51, 43
-// us). The angle is formed and reduced to [-pi, pi] in 64 bits (a
+// per token. The arithmetic runs on packed pairs; the most frequent stall is the
+// read of cos, sin and weights from shared memory. 8,192 tokens of 32 + 2 x 8 bf16
+// heads: 43.5 us with several states in turn, 4.6 TB/s (71 % of a copy's rate);
+// one state over and over 42, two rows on the way and CTAs of 256 threads slower
+// (51, 43 us). The angle is formed and reduced to [-pi, pi] in 64 bits (a
 // far position times a frequency near 1 has no useful fp32 bits left after the
 // reduction); sin and cos then run in fp32.
 // ---------------------------------------------------------------------------
@@ -320,10 +321,13 @@ __global__ void rope_axes_fp8_kernel(const RopeAxes p) {
 // warp moves these rows of its slices: the 16-byte pieces of kMoveBatch loads
 // a lane at a time, all loads before the stores. Pieces are taken by slice,
 // then by path, so whatever lands on a row was preceded by all of its reads.
-// 64 sequences, 5 of 6 rows moved, 36 layers of 8 bf16 heads: 15.4 us, 4.9 TB/s
-// (75 % of a copy's rate) with 4 loads a lane, 4 warps a CTA and 8 slices a
-// warp; 8 loads or 8 warps 17 us, 4 slices 16.9. The rows' offsets are looked
-// up and not computed per piece: index arithmetic took 21.6.
+// 64 sequences, 3 to 5 moved rows of each (257), 36 layers of 8 bf16 heads, 76
+// MB read and written: 21.8 us with several states in turn, 3.5 TB/s (53 % of a
+// copy's rate; before the first row come n_keep, the path and the table, one
+// after the other). One state over and over, out of L2: 15.9 us with 4 loads a
+// lane, 4 warps a CTA and 8 slices a warp; 8 loads or 8 warps 17 us, 4 slices
+// 16.9. The rows' offsets are looked up and not computed per piece: index
+// arithmetic took 21.6 there.
 //
 // FP8: a page-head has one scale for its 16 rows. Rows that come from other
 // pages are values code * s_src; the destination's scale grows to
@@ -559,9 +563,10 @@ __global__ void __launch_bounds__(kCompactWarps * 32) compact_fp8_kernel(const C
 // holds it, eight 16-bit values by four packed maxima and one comparison, and
 // looks its index up at the end. Every CTA leaves its chunk's best as one
 // 64-bit word (ordered value, then the complement of the index), and one CTA
-// per sequence joins them and walks. 1,152 rows of 151,936 bf16 logits: 54.5
-// us with the walk, 6.4 TB/s (98 % of a copy's rate); twice the chunks 62 us,
-// CTAs of 512 threads 72; single elements instead of pieces 127.
+// per sequence joins them and walks. 1,152 rows of 151,936 bf16 logits: 66.2
+// us with the walk and several states in turn, 5.3 TB/s (81 % of a copy's
+// rate). One state over and over, a third of it in L2: 54.9 us; twice the chunks
+// 62 us, CTAs of 512 threads 72; single elements instead of pieces 127.
 // ---------------------------------------------------------------------------
 constexpr int kVerifyThreads = 256;
 constexpr int kVerifyMaxNodes = 1024;
@@ -739,8 +744,8 @@ int verify_chunks(int num_sms, int n_tokens, int vocab) {
 }
 
 // Tokens of a CTA: one until every SM has 16 CTAs (8 are resident), then more,
-// whose angles and page lookups are one latency (8,192 tokens of 48 heads: 41 us
-// with 3, 44 with 1).
+// whose angles and page lookups are one latency (8,192 tokens of 48 heads, one
+// state over and over: 41 us with 3, 44 with 1).
 int rope_tokens(int num_sms, int n_tokens) {
   const int n = n_tokens / (16 * num_sms);
   return n < 1 ? 1 : n > kRopeTokens ? kRopeTokens : n;

@@ -52,13 +52,15 @@
 //   warps 4-11   softmax, one thread per query row; they also load Q and
 //                write the results.
 //
-// Measured (floor: bytes at a copy's rate): 32 x 4,096 tokens, 16 fp16 heads
-// without groups, 24 nodes: 168 us (137), 5.3 TB/s: the rings' loads, and ~4,500
-// cycles per item to write it. 64 x 16,384 tokens, 32 / 8 heads, FP8: 657 us
-// (292): 557 for the copies alone, the staging ring's turns (48 KiB on the way),
-// then the chain decoding - S - softmax - P V. 4 x 65,536 tokens, 32 / 8 heads,
-// 64 nodes, bf16: 370 us (164, and 246 of tensor time with P in two parts): the
-// exponentials, 2,048 cycles of a pair of tiles, behind the waits for S.
+// Measured with several states in turn, so that nothing is left in L2 (floor:
+// bytes at a copy's rate): 32 x 4,096 tokens, 16 fp16 heads without groups, 24
+// nodes: 184 us (137), 4.9 TB/s: the rings' loads, and ~4,500 cycles per item to
+// write it. 64 x 16,384 tokens, 32 / 8 heads, FP8: 714 us (292; 660 in a short run
+// at full clocks, 557 of them the copies alone): the staging ring's turns (48 KiB
+// on the way), then the chain decoding - S - softmax - P V. 4 x 65,536 tokens, 32 /
+// 8 heads, 64 nodes, bf16: 419 us (164, and 246 of tensor time with P in two parts;
+// 379 in a short run): the exponentials, 2,048 cycles of a pair of tiles, behind
+// the waits for S.
 //
 // P is held as 2^6 times the weight, so that f16's smallest step is 2^-31 of
 // a weight of 1 (m is stale by at most 2^8: P <= 2^14); e4m3 pages multiply it
@@ -67,8 +69,8 @@
 // 2^-22), which costs a second P V product. For 16-bit outputs the other pools
 // have one f16 part, 2^-11 at most: an eighth of a bf16 output's own step.
 // Beside an f16 output's it shows (32 x 4,096 tokens against 64 bits: 2.8e-4,
-// the output's rounding alone 2.1e-4); two parts cost 187 us instead of 172
-// there, 786 instead of 661 (FP8) and 75 instead of 66 (int8). Sums, references
+// the output's rounding alone 2.1e-4); two parts cost 203 us instead of 184
+// there, 817 instead of 714 (FP8) and 71 instead of 63 (int8). Sums, references
 // and O are fp32. int8 codes stand for fp16(code x scale), as the arena's
 // dequantisation, gather and the prefill kernel have them (one-token decode
 // multiplies in fp32: a difference of 2^-11 of a value at most).
@@ -646,6 +648,8 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
             }
             fence_proxy_async_smem();  // read by the tensor cores
           }
+          // The staged slot is free too: what was stored needed the loads from it to be complete, and the proxy fence
+          // stands between them and the next copy (TMA, the async proxy) into it. A release before the stores has neither.
           __syncwarp();
           if (lane == 0) {
             bar_arrive(fulls + 8 * st);

@@ -450,15 +450,19 @@ class PagedKVCache:
         """The pool's codes, eight to an element: int64 [L, P, 2, H, 16, D / 8]."""
         return self.pool.pool_view().view(torch.int64)
 
-    def _keeps_rows(self, k: torch.Tensor) -> bool:
+    def _keeps_rows(self, layer: int, k: torch.Tensor) -> bool:
         """Whether an append of a step keeps its rows k [.., total, Hkv, D] (a
         captured one does not: its replays would write to rows of a closed
-        step)."""
+        step; what an earlier call of the layer kept is no longer what its
+        pages hold)."""
         if self._tree_kv is None:
             return False
         if k.dim() >= 3 and k.shape[-3] < self._tree_kv.shape[2]:
             raise ValueError("k, v must have a row for every node of the step")
-        return not torch.cuda.is_current_stream_capturing()
+        if torch.cuda.is_current_stream_capturing():
+            self._tree_layers.difference_update(range(layer, layer + (k.shape[0] if k.dim() == 4 else 1)))
+            return False
+        return True
 
     def _open_tree(self) -> int:
         if self._tree is None:
@@ -470,7 +474,7 @@ class PagedKVCache:
         """One layer's K/V rows of the nodes, k, v [total, Hkv, D] as they are
         cached (rotated already), at slots length + node."""
         n = self._open_tree()
-        kept = self._keeps_rows(k)
+        kept = self._keeps_rows(layer, k)
         self.pool.append(k, v, cu_tokens, ctx_lens, self.block_table[:n], layer0=layer, max_blocks=self.max_blocks)
         if kept:
             total = self._tree_kv.shape[2]
@@ -488,7 +492,7 @@ class PagedKVCache:
         returns the rotated q."""
         n = self._open_tree()
         ws = None
-        if self._keeps_rows(k):  # the call leaves the rotated k in its workspace
+        if self._keeps_rows(layer, k):  # the call leaves the rotated k in its workspace
             total, nt = self._tree_kv.shape[2], k.shape[0]
             mine = self._tree_rows[layer][0] if 0 <= layer < self.num_layers and nt == total else None
             ws = (mine if mine is not None and nt > 0 else

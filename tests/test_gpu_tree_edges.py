@@ -215,6 +215,31 @@ def test_fp8_commit_reports_a_bad_path(cuda_device):
         c.pool.clear_status()
 
 
+def test_fp8_step_captured_after_an_eager_call(cuda_device):
+    """What a replay writes counts, not what an eager call of the same layer wrote before it."""
+    dev = cuda_device
+    c = _fp8_cache(dev, [20])
+    cu, ctx = c.begin_tree([3])
+    x = torch.randn(3, 2, D, generator=gen(18, dev), device=dev).half()
+    half, buf = (x * 0.5).half(), (x * 0.5).half()
+    for l in range(2):
+        c.append_tree(l, half, half, cu, ctx)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for l in range(2):
+            c.append_tree(l, buf, buf, cu, ctx)
+    buf.copy_(x)
+    graph.replay()
+    c.commit_tree(torch.tensor([[0, 2]], dtype=torch.int32, device=dev), torch.tensor([2], dtype=torch.int32, device=dev), [2])
+    c.check()
+    torch.cuda.synchronize()
+    for got in c.gather(0, torch.float32):
+        want = x[[0, 2]].float().permute(1, 0, 2)
+        # e4m3: half a step (2^-4) or of the smallest code, for the append and, moved, two growths
+        assert ((got[:, :, -2:] - want).abs() <= 3 * (2.0 ** -4 * want.abs() + 6.0 / 448 * 2.0 ** -10)).all()
+
+
 def test_fp8_step_refuses_fewer_rows_than_nodes(cuda_device):
     dev = cuda_device
     c = _fp8_cache(dev, [20, 7])

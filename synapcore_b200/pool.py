@@ -623,8 +623,9 @@ class KVPool:
         mask, tree_mask int64 [n_tokens, W] (bit j % 64 of word j / 64; W <= 4,
         at most 64 W nodes per sequence; synapcore_b200.tree_mask builds it
         from parent indices). Returns out [n_tokens, Hq, D]; rows that see
-        nothing are 0, rows of no sequence stay as they are in `out`. At most
-        2,048 sequences. workspace: as decode_attn's, of
+        nothing are 0, rows of no sequence stay as they are in `out`. q enters
+        the products rounded to the pool's 16-bit type (f16 for one-byte pools;
+        what lies beyond its range is infinite there). At most 2,048 sequences. workspace: as decode_attn's, of
         tree_attn_workspace_bytes bytes; calls that overlap on the GPU, those
         of captured graphs among them, need one each."""
         if q.dim() != 3 or q.shape[2] != self.head_dim or q.shape[1] % self.num_kv_heads != 0 or q.shape[1] == 0:

@@ -649,7 +649,8 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
             fence_proxy_async_smem();  // read by the tensor cores
           }
           // The staged slot is free too: what was stored needed the loads from it to be complete, and the proxy fence
-          // stands between them and the next copy (TMA, the async proxy) into it. A release before the stores has neither.
+          // stands between them and the next copy (TMA, the async proxy) into it. A release before the stores has
+          // neither.
           __syncwarp();
           if (lane == 0) {
             bar_arrive(fulls + 8 * st);
@@ -1276,9 +1277,9 @@ __global__ void __launch_bounds__(TreeCfg<KVDT>::kThreads, 1)
           ++xchg;
         }
       }
-      // An infinite V of a committed token, which every row sees: 0 x Inf, of a lane that does not weigh its key (a copy's,
-      // the lo part of an exact weight, a half whose sum is nothing beside the other's), left NaN where the row's value
-      // is that infinity. Each lane looks through 4 dims of this part's committed V.
+      // An infinite V of a committed token, which every row sees: 0 x Inf, of a lane that does not weigh its key (a
+      // copy's, the lo part of an exact weight, a half whose sum is nothing beside the other's), left NaN where the
+      // row's value is that infinity. Each lane looks through 4 dims of this part's committed V.
       if (!C::kFP8 && __any_sync(0xffffffffu, valid && odd && Lsum == Lsum)) {
         auto kind_of = [](float v) -> uint32_t { return v != v ? 4u : v == INFINITY ? 1u : v == -INFINITY ? 2u : 0u; };
         uint32_t kinds = 0;

@@ -140,8 +140,8 @@ def test_fp8_rows_survive_rejected_nodes_bit_for_bit(cuda_device, size, rope):
         x[::2] *= size
         x = x.bfloat16()
         if rope:
-            c.append_tree_rope(l, x[:, :4], x[:, 4:6], x[:, 6:], torch.zeros(T, dtype=torch.int32, device=dev), axis, cu,
-                               ctx_d, freq)
+            pos = torch.zeros(T, dtype=torch.int32, device=dev)
+            c.append_tree_rope(l, x[:, :4], x[:, 4:6], x[:, 6:], pos, axis, cu, ctx_d, freq)
         else:
             c.append_tree(l, x[:, 4:6].contiguous(), x[:, 6:].contiguous(), cu, ctx_d)
     none = torch.zeros(len(n), dtype=torch.int32, device=dev)
@@ -181,8 +181,8 @@ def test_fp8_commit_equals_an_append_of_the_accepted_rows(cuda_device, src, rope
         k, v = x[:, 4:6], x[:, 6:]
         if rope:
             a.append_tree_rope(l, x[:, :4], k, v, pos, axis, cu, ctx_d, freq)
-            b.pool.append_rope_axes(l, x[rows, :4], k[rows], v[rows], pos[rows], axis, kcu, ctx_d, b.block_table[:len(n)],
-                                    freq)
+            b.pool.append_rope_axes(l, x[rows, :4], k[rows], v[rows], pos[rows], axis, kcu, ctx_d,
+                                    b.block_table[:len(n)], freq)
         else:
             a.append_tree(l, k.contiguous(), v.contiguous(), cu, ctx_d)
             b.pool.append(k[rows], v[rows], kcu, ctx_d, b.block_table[:len(n)], layer0=l)
@@ -231,7 +231,8 @@ def test_fp8_step_captured_after_an_eager_call(cuda_device):
             c.append_tree(l, buf, buf, cu, ctx)
     buf.copy_(x)
     graph.replay()
-    c.commit_tree(torch.tensor([[0, 2]], dtype=torch.int32, device=dev), torch.tensor([2], dtype=torch.int32, device=dev), [2])
+    path = torch.tensor([[0, 2]], dtype=torch.int32, device=dev)
+    c.commit_tree(path, torch.tensor([2], dtype=torch.int32, device=dev), [2])
     c.check()
     torch.cuda.synchronize()
     for got in c.gather(0, torch.float32):
@@ -250,8 +251,8 @@ def test_fp8_step_refuses_fewer_rows_than_nodes(cuda_device):
     with pytest.raises(ValueError):
         c.append_tree(0, x[:, 4:6].contiguous(), x[:, 6:].contiguous(), cu, ctx)
     with pytest.raises(ValueError):
-        c.append_tree_rope(0, x[:, :4], x[:, 4:6], x[:, 6:], torch.zeros(9, dtype=torch.int32, device=dev), axis, cu, ctx,
-                           rope_inv_freq(1e4, D, dev))
+        pos = torch.zeros(9, dtype=torch.int32, device=dev)
+        c.append_tree_rope(0, x[:, :4], x[:, 4:6], x[:, 6:], pos, axis, cu, ctx, rope_inv_freq(1e4, D, dev))
     none = torch.zeros(2, dtype=torch.int32, device=dev)
     c.commit_tree(none[:, None], none, [0, 0])
     c.check()
